@@ -25,7 +25,8 @@ BENCH_SOURCES = ["bench_read.hip", "check_bf16.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["abi_v1.cpp", "linear_api.cpp", "safetensors.cpp", "evidence.hip", "noalloc.hip", "weights.hip",
-           "gemv.hip", "gemm_wq.hip", "gemm_fp8.hip"]
+           "gemv.hip", "gemm_wq.hip", "gemm_fp8.hip", "kv_api.cpp", "kv_store.hip",
+           "kv_attend.hip"]
 
 COMMON = [
     "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden",

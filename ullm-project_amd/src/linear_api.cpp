@@ -18,6 +18,7 @@
 #include <vector>
 
 #include "abi_common.hpp"
+#include "host_common.hpp"
 #include "kernels.hpp"
 #include "layout.hpp"
 #include "ullm/linear.h"
@@ -34,26 +35,13 @@ hipError_t launch_fp8_gemm(const uint8_t *xq, const float *xs, uint64_t ldxq,
 
 namespace {
 
-using ullm::write_error;
-using ullm::write_errorf;
-
-constexpr uint64_t kMaxDim = (uint64_t(1) << 31) - 1;
-
-std::mutex g_registry_mutex;
-std::unordered_set<const ullm_linear_weight_t *> g_registry;
-
-bool registered(const ullm_linear_weight_t *w) {
-  std::lock_guard<std::mutex> lock(g_registry_mutex);
-  return g_registry.count(w) != 0;
-}
-
 // Library-owned workspaces, one per (device, stream, kind) and grown on
-// demand: the prefill path's quantized activations, and the decode path's
-// split-K scratch (its counter words are zero on allocation and every launch
-// leaves them zero).  Calls on one stream are ordered, so they may share a
-// buffer; calls on different streams get different buffers.  A buffer that
-// is outgrown is retired, not freed: a HIP graph captured earlier may still
-// hold its address, and stays valid.
+// demand.  Two kinds: the linear layer's scratch, whose split-K counter words
+// are zero on allocation and left zero by every launch (zeroed), and the
+// scratch of cache attention, which starts with no value.  Calls on one
+// stream are ordered, so they may share a buffer; calls on different streams
+// get different buffers.  A buffer that is outgrown is retired, not freed: a
+// HIP graph captured earlier may still hold its address, and stays valid.
 struct Workspace {
   void *ptr = nullptr;
   uint64_t bytes = 0;
@@ -61,73 +49,35 @@ struct Workspace {
 struct WorkspaceKey {
   int device;
   const void *stream;
-  bool split;
+  bool zeroed;
   bool operator==(const WorkspaceKey &o) const {
-    return device == o.device && stream == o.stream && split == o.split;
+    return device == o.device && stream == o.stream && zeroed == o.zeroed;
   }
 };
 struct WorkspaceKeyHash {
   size_t operator()(const WorkspaceKey &k) const {
     return std::hash<const void *>()(k.stream) ^ (size_t(k.device) << 1) ^
-           size_t(k.split);
+           size_t(k.zeroed);
   }
 };
 std::mutex g_ws_mutex;
 std::unordered_map<WorkspaceKey, Workspace, WorkspaceKeyHash> g_ws;
 std::vector<std::pair<int, void *>> g_ws_retired;  // (device, buffer)
 
+}  // namespace
 
-// Makes `device` current for the scope and restores the caller's device.
-class DeviceScope {
- public:
-  explicit DeviceScope(int device) {
-    if (hipGetDevice(&prev_) != hipSuccess) {
-      prev_ = -1;
-    }
-    err_ = prev_ == device ? hipSuccess : hipSetDevice(device);
-    if (prev_ == device) {
-      prev_ = -1;  // nothing to restore
-    }
-  }
-  ~DeviceScope() {
-    if (prev_ >= 0) {
-      (void)hipSetDevice(prev_);
-    }
-  }
-  hipError_t error() const { return err_; }
-
- private:
-  int prev_ = -1;
-  hipError_t err_ = hipSuccess;
-};
-
-ullm_status_t hip_fail(ullm_error_sink_t *sink, const char *what,
-                       hipError_t err) {
-  const ullm_status_t st = err == hipErrorOutOfMemory
-                               ? ULLM_STATUS_OUT_OF_MEMORY
-                               : ULLM_STATUS_HIP_RUNTIME_ERROR;
-  return write_errorf(sink, st,
-                      std::string(what) + ": " + hipGetErrorName(err));
-}
-
-#define HIP_TRY(sink, what, expr)              \
-  do {                                         \
-    const hipError_t e_ = (expr);              \
-    if (e_ != hipSuccess) {                    \
-      return hip_fail(sink, what, e_);         \
-    }                                          \
-  } while (0)
+namespace ullm {
 
 // The library-owned workspace of at least `need` bytes for this call
-// (zeroed when first allocated, for the split-K counters).  Allocates, so a
-// call that needs a larger buffer is refused under stream capture.  The
-// zeroing is queued on the call's own stream, so the kernel that follows is
-// ordered after it even on a non-blocking stream.
-ullm_status_t library_workspace(int device, const void *stream, bool split,
+// (`zeroed`: filled with zeros when first allocated, for the split-K
+// counters).  Allocates, so a call that needs a larger buffer is refused
+// under stream capture.  The zeroing is queued on the call's own stream, so
+// the kernel that follows is ordered after it even on a non-blocking stream.
+ullm_status_t library_workspace(int device, const void *stream, bool zeroed,
                                 uint64_t need, void **out,
                                 ullm_error_sink_t *error_sink) {
   std::lock_guard<std::mutex> lock(g_ws_mutex);
-  Workspace &cache = g_ws[WorkspaceKey{device, stream, split}];
+  Workspace &cache = g_ws[WorkspaceKey{device, stream, zeroed}];
   if (cache.bytes < need) {
     const hipStream_t s = static_cast<hipStream_t>(const_cast<void *>(stream));
     hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
@@ -139,7 +89,7 @@ ullm_status_t library_workspace(int device, const void *stream, bool split,
     }
     void *p = nullptr;
     HIP_TRY(error_sink, "hipMalloc (workspace)", hipMalloc(&p, need));
-    if (split) {
+    if (zeroed) {
       const hipError_t e = hipMemsetAsync(p, 0, need, s);
       if (e != hipSuccess) {
         (void)hipFree(p);
@@ -156,25 +106,24 @@ ullm_status_t library_workspace(int device, const void *stream, bool split,
   return ULLM_STATUS_OK;
 }
 
-ullm_status_t check_device(int device, ullm_error_sink_t *sink) {
-  int count = 0;
-  const hipError_t err = hipGetDeviceCount(&count);
-  if (err != hipSuccess || count == 0) {
-    return write_error(sink, ULLM_STATUS_HIP_UNAVAILABLE,
-                       "no HIP device is visible");
-  }
-  if (device < 0 || device >= count) {
-    return write_error(sink, ULLM_STATUS_INVALID_ARGUMENT,
-                       "device ordinal is out of range");
-  }
-  hipDeviceProp_t prop;
-  HIP_TRY(sink, "hipGetDeviceProperties", hipGetDeviceProperties(&prop, device));
-  if (std::strncmp(prop.gcnArchName, "gfx950", 6) != 0) {
-    return write_errorf(sink, ULLM_STATUS_UNSUPPORTED,
-                        std::string("device architecture ") + prop.gcnArchName +
-                            " is not gfx950");
-  }
-  return ULLM_STATUS_OK;
+}  // namespace ullm
+
+namespace {
+
+using ullm::check_device;
+using ullm::DeviceScope;
+using ullm::hip_fail;
+using ullm::write_error;
+using ullm::write_errorf;
+
+constexpr uint64_t kMaxDim = (uint64_t(1) << 31) - 1;
+
+std::mutex g_registry_mutex;
+std::unordered_set<const ullm_linear_weight_t *> g_registry;
+
+bool registered(const ullm_linear_weight_t *w) {
+  std::lock_guard<std::mutex> lock(g_registry_mutex);
+  return g_registry.count(w) != 0;
 }
 
 // Owns device allocations until released (exception/early-return safe).
@@ -883,7 +832,7 @@ ullm_status_t forward_dispatch(const ullm_linear_forward_desc_t *desc,
           }
         } else {
           const ullm_status_t st =
-              library_workspace(w->device, desc->stream, true, need, &ws, error_sink);
+              ullm::library_workspace(w->device, desc->stream, true, need, &ws, error_sink);
           if (st != ULLM_STATUS_OK) {
             return st;
           }
@@ -934,7 +883,7 @@ ullm_status_t forward_dispatch(const ullm_linear_forward_desc_t *desc,
         }
       } else {
         const ullm_status_t st =
-            library_workspace(w->device, desc->stream, true, need, &buf, error_sink);
+            ullm::library_workspace(w->device, desc->stream, true, need, &buf, error_sink);
         if (st != ULLM_STATUS_OK) {
           return st;
         }

@@ -10,7 +10,9 @@ Mirrors the reference's Rust layering:
   * ``LinearWeight`` / ``linear_forward`` / ``quantize_activations`` wrap the
     linear-layer extension of include/ullm/linear.h, the calls a future
     ``HipBackend::execute`` (reference crates/ullm-hip/src/lib.rs:487-513)
-    would make for a Matmul with a quantized weight.
+    would make for a Matmul with a quantized weight;
+  * ``KvCache`` wraps the 8-bit key/value cache and its attention of
+    include/ullm/kv_cache.h.
 
 PyTorch is used only to hold device memory and to name streams.  There is no
 fallback: if the native library is missing, loading raises.
@@ -82,6 +84,10 @@ GEMV_MULTI_STRIPE = 3
 GEMV_REGISTER_STAGED = 4
 GEMV_SPLIT_K = 5
 BACKEND_HIP = 1
+KV_CACHE_TRACK_WEIGHTS = 1
+KV_ATTEND_ACCUMULATE = 1
+KV_KERNEL_FEW_ROWS = 1
+KV_KERNEL_MANY_ROWS = 2
 
 # ------------------------------------------------------------------- structs
 _u32 = ctypes.c_uint32
@@ -210,7 +216,65 @@ class WeightsSaveDesc(ctypes.Structure):
                 ("metadata_count", _u64), ("reserved", _u64 * 4)]
 
 
+class KvCacheDesc(ctypes.Structure):
+    _fields_ = [("struct_size", _u32), ("abi_version", _u32), ("blocks", _u64),
+                ("block_tokens", _u32), ("kv_heads", _u32), ("head_dim", _u32),
+                ("flags", _u32), ("device", _i32), ("reserved0", _u32),
+                ("reserved", _u64 * 4)]
+
+
+class KvCacheInfo(ctypes.Structure):
+    _fields_ = [("struct_size", _u32), ("abi_version", _u32), ("blocks", _u64),
+                ("block_tokens", _u32), ("kv_heads", _u32), ("head_dim", _u32),
+                ("flags", _u32), ("device", _i32), ("reserved0", _u32),
+                ("device_bytes", _u64), ("reserved", _u64 * 3)]
+
+
+class KvSequences(ctypes.Structure):
+    _fields_ = [("batch", _u64), ("rows", _u64), ("tables", _vp), ("table_stride", _u64),
+                ("max_blocks", _u64), ("lengths", _vp), ("starts", _vp)]
+
+
+class KvAppendDesc(ctypes.Structure):
+    _fields_ = [("struct_size", _u32), ("abi_version", _u32), ("cache", _vp),
+                ("seqs", KvSequences), ("k", _vp), ("k_row_stride", _u64),
+                ("k_head_stride", _u64), ("v", _vp), ("v_row_stride", _u64),
+                ("v_head_stride", _u64), ("weights", _vp), ("stream", _vp),
+                ("reserved", _u64 * 4)]
+
+
+class KvGatherDesc(ctypes.Structure):
+    _fields_ = [("struct_size", _u32), ("abi_version", _u32), ("cache", _vp),
+                ("seqs", KvSequences), ("k", _vp), ("v", _vp), ("weights", _vp),
+                ("stream", _vp), ("reserved", _u64 * 4)]
+
+
+class KvAttendDesc(ctypes.Structure):
+    _fields_ = [("struct_size", _u32), ("abi_version", _u32), ("cache", _vp),
+                ("seqs", KvSequences), ("q", _vp), ("q_row_stride", _u64),
+                ("q_head_stride", _u64), ("out", _vp), ("out_row_stride", _u64),
+                ("out_head_stride", _u64), ("lse", _vp), ("heads", _u32),
+                ("window", _u32), ("scale", ctypes.c_float), ("flags", _u32),
+                ("stream", _vp), ("workspace", _vp), ("workspace_size", _u64),
+                ("reserved", _u64 * 4)]
+
+
+class KvAttendPlan(ctypes.Structure):
+    _fields_ = [("struct_size", _u32), ("abi_version", _u32), ("kernel", _u32),
+                ("row_tile", _u32), ("parts", _u32), ("part_tokens", _u32),
+                ("grid", _u64), ("workspace_bytes", _u64), ("reserved", _u64 * 2)]
+
+
+class KvEvictDesc(ctypes.Structure):
+    _fields_ = [("struct_size", _u32), ("abi_version", _u32), ("cache", _vp),
+                ("seqs", KvSequences), ("new_tables", _vp), ("new_table_stride", _u64),
+                ("new_lengths", _vp), ("kept", _vp), ("keep", _u64), ("sink", _u64),
+                ("recent", _u64), ("stream", _vp), ("reserved", _u64 * 4)]
+
+
 _FORWARD_SIZE = ctypes.sizeof(ForwardDesc)
+_KV_APPEND_SIZE = ctypes.sizeof(KvAppendDesc)
+_KV_ATTEND_SIZE = ctypes.sizeof(KvAttendDesc)
 
 # safetensors dtype strings by ULLM_ST_DTYPE_* value
 ST_DTYPES = {1: "BOOL", 2: "U8", 3: "I8", 4: "F8_E4M3", 5: "F8_E5M2", 6: "U16",
@@ -275,6 +339,16 @@ _SIGNATURES = {
                                 ctypes.POINTER(ErrorSink)],
     "ullm_linear_weights_save": [ctypes.POINTER(WeightsSaveDesc), ctypes.c_char_p,
                                  ctypes.POINTER(ErrorSink)],
+    "ullm_kv_cache_create": [ctypes.POINTER(KvCacheDesc), ctypes.POINTER(_vp),
+                             ctypes.POINTER(ErrorSink)],
+    "ullm_kv_cache_destroy": [ctypes.POINTER(_vp), ctypes.POINTER(ErrorSink)],
+    "ullm_kv_cache_query": [_vp, ctypes.POINTER(KvCacheInfo), ctypes.POINTER(ErrorSink)],
+    "ullm_kv_cache_append": [ctypes.POINTER(KvAppendDesc), ctypes.POINTER(ErrorSink)],
+    "ullm_kv_cache_gather": [ctypes.POINTER(KvGatherDesc), ctypes.POINTER(ErrorSink)],
+    "ullm_kv_cache_attend": [ctypes.POINTER(KvAttendDesc), ctypes.POINTER(ErrorSink)],
+    "ullm_kv_cache_attend_plan": [ctypes.POINTER(KvAttendDesc), ctypes.POINTER(KvAttendPlan),
+                                  ctypes.POINTER(ErrorSink)],
+    "ullm_kv_cache_evict": [ctypes.POINTER(KvEvictDesc), ctypes.POINTER(ErrorSink)],
 }
 
 _lib = None
@@ -603,6 +677,207 @@ def release_workspaces(device: int = 0) -> None:
     (ullm_linear_release_workspaces)."""
     s = _Sink()
     _check(lib().ullm_linear_release_workspaces(device, s.ref), s)
+
+
+# --------------------------------------------------------- key/value cache
+
+def _strides3(t, name, heads, dim):
+    """(row, head) strides of a bf16 [rows][heads][dim] tensor."""
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim \
+            or t.dtype is not _torch().bfloat16:
+        raise ValueError(f"{name} must be bfloat16 [rows][{heads}][{dim}]")
+    row, head, one = t.stride()
+    # The stride of an axis of one is never used.
+    row = row if t.shape[0] > 1 else max(row, dim)
+    head = head if heads > 1 else dim
+    if one != 1 or row < dim or head < dim:
+        raise ValueError(f"{name} must have contiguous heads that do not overlap")
+    return row, head
+
+
+class KvCache:
+    """Keys and values in 8 bits (E4M3) with a power-of-two scale for each
+    block of tokens and head (opaque native handle; ullm/kv_cache.h).
+
+    A call takes the rows of all its sequences in one tensor: sequence b owns
+    rows ``starts[b]`` to ``starts[b + 1] - 1`` (``starts`` int32 [batch + 1]
+    on the device; None: the same number each).  ``lengths`` (int32 [batch])
+    counts its tokens with the new ones, ``tables`` (int32 [batch][columns])
+    names its blocks.  ``track_weights`` keeps the attention weight that each
+    token has received, for ``attend(accumulate=True)`` and ``evict``."""
+
+    def __init__(self, blocks, kv_heads, head_dim, block_tokens=64, track_weights=False,
+                 device=0):
+        self.handle = None
+        s = _Sink()
+        d = new(KvCacheDesc, blocks=blocks, block_tokens=block_tokens, kv_heads=kv_heads,
+                head_dim=head_dim, flags=KV_CACHE_TRACK_WEIGHTS if track_weights else 0,
+                device=device)
+        h = _vp()
+        _check(lib().ullm_kv_cache_create(ctypes.byref(d), ctypes.byref(h), s.ref), s)
+        self.handle = h.value
+        self.blocks, self.block_tokens = blocks, block_tokens
+        self.kv_heads, self.head_dim = kv_heads, head_dim
+        self.track_weights, self.device = track_weights, device
+
+    # -- lifetime ----------------------------------------------------------
+    def destroy(self):
+        if self.handle:
+            s = _Sink()
+            h = _vp(self.handle)
+            self.handle = None
+            _check(lib().ullm_kv_cache_destroy(ctypes.byref(h), s.ref), s)
+
+    def __del__(self):
+        try:
+            self.destroy()
+        except Exception:
+            pass
+
+    def info(self) -> KvCacheInfo:
+        s = _Sink()
+        i = new(KvCacheInfo)
+        _check(lib().ullm_kv_cache_query(self.handle, ctypes.byref(i), s.ref), s)
+        return i
+
+    # -- calls -------------------------------------------------------------
+    def _seqs(self, lengths, tables, rows, starts):
+        i32 = _torch().int32
+        batch, columns = tables.shape
+        stride, one = tables.stride()
+        if tables.dtype is not i32 or lengths.dtype is not i32 or lengths.dim() != 1 \
+                or lengths.shape[0] != batch or (batch > 1 and lengths.stride(0) != 1):
+            raise ValueError("tables must be int32 [batch][columns] and lengths int32 [batch]")
+        if (columns > 1 and one != 1) or (batch > 1 and stride < columns):
+            raise ValueError("rows of tables must be contiguous and must not overlap")
+        if starts is not None and (starts.dtype is not i32 or tuple(starts.shape) != (batch + 1,)
+                                   or not starts.is_contiguous()):
+            raise ValueError("starts must be int32 [batch + 1]")
+        return KvSequences(batch, rows, tables.data_ptr(), stride if batch > 1 else columns,
+                           columns, lengths.data_ptr(),
+                           None if starts is None else starts.data_ptr())
+
+    def append(self, k, v, lengths, tables, starts=None, weights=None, stream=None):
+        """Quantize and store new tokens: k, v bf16 [rows][kv_heads][head_dim]
+        (row and head strides honoured).  ``weights`` (f32 [rows][kv_heads])
+        restores weights read by ``gather_weights``; without it they are 0."""
+        ks = _strides3(k, "k", self.kv_heads, self.head_dim)
+        vs = _strides3(v, "v", self.kv_heads, self.head_dim)
+        rows = k.shape[0]
+        if v.shape[0] != rows:
+            raise ValueError("k and v must have the same number of rows")
+        if weights is not None and (tuple(weights.shape) != (rows, self.kv_heads)
+                                    or weights.dtype is not _torch().float32
+                                    or not weights.is_contiguous()):
+            raise ValueError("weights must be a contiguous float32 [rows][kv_heads] tensor")
+        d = KvAppendDesc(_KV_APPEND_SIZE, ABI_VERSION, self.handle,
+                         self._seqs(lengths, tables, rows, starts), k.data_ptr(), *ks,
+                         v.data_ptr(), *vs, _ptr(weights), _stream(stream))
+        s = _thread_sink()
+        st = lib().ullm_kv_cache_append(ctypes.byref(d), s.ref)
+        if st:
+            raise HipError(st, s.text())
+
+    def _gather(self, lengths, tables, rows, starts, k, v, weights, stream):
+        d = KvGatherDesc(ctypes.sizeof(KvGatherDesc), ABI_VERSION, self.handle,
+                         self._seqs(lengths, tables, rows, starts), _ptr(k), _ptr(v),
+                         _ptr(weights), _stream(stream))
+        s = _thread_sink()
+        st = lib().ullm_kv_cache_gather(ctypes.byref(d), s.ref)
+        if st:
+            raise HipError(st, s.text())
+
+    def gather(self, lengths, tables, rows, starts=None, stream=None):
+        """Keys and values of each sequence's last rows (``rows`` in all), bf16
+        [rows][kv_heads][head_dim] and exact: appending them again stores the
+        same values.  Rows that name no token are zero."""
+        torch = _torch()
+        k, v = (torch.empty((rows, self.kv_heads, self.head_dim), dtype=torch.bfloat16,
+                            device=tables.device) for _ in range(2))
+        self._gather(lengths, tables, rows, starts, k, v, None, stream)
+        return k, v
+
+    def gather_weights(self, lengths, tables, rows, starts=None, stream=None):
+        """The weights of each sequence's last rows, f32 [rows][kv_heads]."""
+        torch = _torch()
+        w = torch.empty((rows, self.kv_heads), dtype=torch.float32, device=tables.device)
+        self._gather(lengths, tables, rows, starts, None, None, w, stream)
+        return w
+
+    def _attend_desc(self, q, lengths, tables, starts, out, lse, scale, window, accumulate,
+                     stream, workspace):
+        heads, dim = q.shape[1], self.head_dim
+        qs = _strides3(q, "q", heads, dim)
+        os = _strides3(out, "out", heads, dim)
+        rows = q.shape[0]
+        if out.shape[0] != rows:
+            raise ValueError("q and out must have the same number of rows")
+        if lse is not None and (tuple(lse.shape) != (rows, heads) or not lse.is_contiguous()
+                                or lse.dtype is not _torch().float32):
+            raise ValueError("lse must be a contiguous float32 [rows][heads] tensor")
+        ws, wb = (None, 0) if workspace is None else \
+            (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+        return KvAttendDesc(_KV_ATTEND_SIZE, ABI_VERSION, self.handle,
+                            self._seqs(lengths, tables, rows, starts), q.data_ptr(), *qs,
+                            out.data_ptr(), *os, _ptr(lse), heads, window,
+                            dim ** -0.5 if scale is None else scale,
+                            KV_ATTEND_ACCUMULATE if accumulate else 0, _stream(stream), ws, wb)
+
+    def attend(self, q, lengths, tables, starts=None, out=None, lse=None, scale=None, window=0,
+               accumulate=False, stream=None, workspace=None):
+        """Causal attention of q (bf16 [rows][heads][head_dim], row and head
+        strides honoured) over the cached tokens: bf16 like q.  ``scale``
+        defaults to 1 / sqrt(head_dim); with ``window`` a query sees that many
+        tokens; ``lse`` (f32 [rows][heads]) receives the log of each row's sum;
+        ``accumulate`` adds to the weights of the tokens.  A query that sees
+        no token gives zeros."""
+        if out is None:
+            torch = _torch()
+            out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+        d = self._attend_desc(q, lengths, tables, starts, out, lse, scale, window, accumulate,
+                              stream, workspace)
+        s = _thread_sink()
+        st = lib().ullm_kv_cache_attend(ctypes.byref(d), s.ref)
+        if st:
+            raise HipError(st, s.text())
+        return out
+
+    def attend_plan(self, q, lengths, tables, starts=None, out=None, lse=None, scale=None,
+                    window=0, accumulate=False, stream=None, workspace=None) -> KvAttendPlan:
+        """The launch and the workspace of attend() with these arguments
+        (ullm_kv_cache_attend_plan); launches nothing."""
+        d = self._attend_desc(q, lengths, tables, starts, q if out is None else out, lse, scale,
+                              window, accumulate, stream, workspace)
+        p = new(KvAttendPlan)
+        s = _Sink()
+        _check(lib().ullm_kv_cache_attend_plan(ctypes.byref(d), ctypes.byref(p), s.ref), s)
+        return p
+
+    def evict(self, lengths, tables, new_tables, keep, sink=0, recent=0, stream=None):
+        """Cut each sequence to its ``keep`` heaviest tokens per head, among
+        them its first ``sink`` and last ``recent``, into the blocks of
+        ``new_tables``.  Returns (lengths int32 [batch], positions that stay
+        int32 [batch][kv_heads][keep], ascending, then -1)."""
+        torch = _torch()
+        batch = tables.shape[0]
+        columns = -(-keep // self.block_tokens)
+        if new_tables.dtype is not torch.int32 or new_tables.dim() != 2 \
+                or new_tables.shape[0] != batch or new_tables.shape[1] < columns \
+                or (columns > 1 and new_tables.stride(1) != 1) \
+                or (batch > 1 and new_tables.stride(0) < columns):
+            raise ValueError(f"new_tables must be int32 [batch][{columns} or more]")
+        lens = torch.empty((batch,), dtype=torch.int32, device=tables.device)
+        kept = torch.empty((batch, self.kv_heads, max(keep, 0)), dtype=torch.int32,
+                           device=tables.device)
+        d = KvEvictDesc(ctypes.sizeof(KvEvictDesc), ABI_VERSION, self.handle,
+                        self._seqs(lengths, tables, 0, None), new_tables.data_ptr(),
+                        new_tables.stride(0) if batch > 1 else columns, lens.data_ptr(),
+                        kept.data_ptr(), keep, sink, recent, _stream(stream))
+        s = _thread_sink()
+        st = lib().ullm_kv_cache_evict(ctypes.byref(d), s.ref)
+        if st:
+            raise HipError(st, s.text())
+        return lens, kept
 
 
 # ------------------------------------------------------------------ evidence
