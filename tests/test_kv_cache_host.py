@@ -50,6 +50,25 @@ def test_python_mirrors_the_header(uh, tmp_path):
         assert got == int(value), line
 
 
+def test_packed_descriptors_equal_ctypes_ones(uh):
+    """Every field of a descriptor filled by one pack, by its name."""
+    for cls in (uh.KvAppendDesc, uh.KvGatherDesc, uh.KvAttendDesc, uh.KvEvictDesc):
+        p = uh._Packed(cls)
+        count = len(p.format.unpack(bytes(p.format.size))) - 2
+        p.fill(*range(3, 3 + count))
+        assert (p.desc.struct_size, p.desc.abi_version) == (ctypes.sizeof(cls), 1)
+        got = []
+        for name, t in cls._fields_[2:]:
+            v = getattr(p.desc, name)
+            if name == "seqs":
+                got += [getattr(v, f) for f, _ in t._fields_]
+            elif name == "reserved":
+                assert list(v) == [0] * 4
+            else:
+                got.append(v)
+        assert got == list(range(3, 3 + count)), cls
+
+
 def _call(uh, fn, *args):
     s = uh._Sink()
     return uh.Status(fn(*args, s.ref)), s.text()
@@ -129,8 +148,9 @@ def test_python_checks_tensors(uh):
     import torch
     bf = torch.bfloat16
     x = torch.zeros((4, 2, 128), dtype=bf)
-    assert uh._strides3(x, "x", 2, 128) == (256, 128)
-    assert uh._strides3(x.transpose(0, 1).contiguous().transpose(0, 1), "x", 2, 128) == (128, 512)
+    assert uh._strides3(x, "x", 2, 128) == (4, 256, 128)
+    assert uh._strides3(x.transpose(0, 1).contiguous().transpose(0, 1), "x", 2, 128) == \
+        (4, 128, 512)
     for bad in (x.float(), x[0], x[:, :1], x[:, :, ::2], x[:1].expand(4, 2, 128),
                 x[:, :1].expand(4, 2, 128)):
         with pytest.raises(ValueError):
@@ -138,9 +158,8 @@ def test_python_checks_tensors(uh):
     c = uh.KvCache.__new__(uh.KvCache)
     c.handle, c.kv_heads, c.head_dim, c.block_tokens = None, 2, 128, 64
     n, t = torch.zeros(2, dtype=torch.int32), torch.zeros((2, 3), dtype=torch.int32)
-    s = c._seqs(n, t, 4, None)
-    assert (s.batch, s.rows, s.table_stride, s.max_blocks) == (2, 4, 3, 3)
-    assert c._seqs(n, t[:, :2], 4, None).table_stride == 3
+    assert c._seqs(n, t, 4, None) == (2, 4, t.data_ptr(), 3, 3, n.data_ptr(), 0)
+    assert c._seqs(n, t[:, :2], 4, None)[3:5] == (3, 2)
     for lens, tab, st in ((n.long(), t, None), (n, t.long(), None), (n[:1], t, None),
                           (n, t.t().contiguous().t(), None), (n, t[:1].expand(2, 3), None),
                           (n, t, torch.zeros(2, dtype=torch.int32)),

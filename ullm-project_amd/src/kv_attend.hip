@@ -26,6 +26,10 @@
 // down instead (kept exact in the sum, which is f32), one further above raises
 // the accumulator's exponent: blocks of any exponents meet in one product with
 // an error below 2^-60 of the largest value.
+#include <algorithm>
+#include <cstdlib>
+
+#include "kernels.hpp"
 #include "kv_cache.hpp"
 
 namespace ullm {
@@ -106,17 +110,25 @@ __device__ __forceinline__ f16x8 codes_to_f16(uint32_t a, uint32_t b, float powe
   return __builtin_bit_cast(f16x8, r);
 }
 
+// Codes that one workgroup alone reads pass the caches by (nontemporal: 47
+// against 53 us for 131072 tokens of 8 heads); with several tiles of rows to a
+// sequence the later ones find them there.
+template <bool NT>
+__device__ __forceinline__ u32x4 load_codes(const u32x4 *p) {
+  return NT ? __builtin_nontemporal_load(p) : *p;
+}
+
 // The codes of 16 keys: tile `tile` (of 16 tokens) of a block and head.
 template <int D>
 struct Keys {
   u32x4 w[D / 64];
 };
-template <int D>
+template <int D, bool NT>
 __device__ __forceinline__ Keys<D> load_keys(const uint8_t *keys, uint32_t tile, uint32_t lane) {
   Keys<D> r;
 #pragma unroll
   for (int c = 0; c < D / 64; ++c) {
-    r.w[c] = reinterpret_cast<const u32x4 *>(keys + tile * (D * 16))[c * 64 + lane];
+    r.w[c] = load_codes<NT>(reinterpret_cast<const u32x4 *>(keys + tile * (D * 16)) + c * 64 + lane);
   }
   return r;
 }
@@ -141,244 +153,545 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
 
 // Rows of a tile: positions of the queries, the tokens they can see.
 struct Tile {
-  uint32_t seq, length, first_row, live;  // live rows of the tile
-  uint32_t r0;                            // first row's index in the sequence's list
-  int64_t origin;                         // position of the sequence's first query
-  int64_t low, high;                      // positions of the tile's first and last query
-  uint32_t begin, end;                    // tokens that some row sees
+  uint32_t seq, length, first_row, count;  // the sequence, its rows
+  uint32_t r0, live;                       // the tile's rows in the sequence's list
+  int64_t origin;                          // position of the sequence's first query
+  int64_t low, high;                       // positions of the tile's first and last query
+  uint32_t begin, end;                     // tokens that some row sees
 };
 
-__device__ __forceinline__ bool make_tile(const KvAttendArgs &a, uint32_t id, uint32_t rows,
+// The rows of tile `id`; false if it has none.
+__device__ __forceinline__ bool tile_rows(const KvAttendArgs &a, uint32_t id, uint32_t rows,
                                           uint32_t each_slots, Tile *t) {
   const KvSlot slot = kv_find_slot(a.seqs, id, a.group, rows, 1, each_slots);
-  if (slot.seq >= a.seqs.batch) {
-    return false;
-  }
-  const KvRows r = kv_rows(a.seqs, slot.seq);
+  const uint32_t all = slot.rows.count * a.group;
   t->seq = slot.seq;
-  t->first_row = r.first;
+  t->first_row = slot.rows.first;
+  t->count = slot.rows.count;
   t->r0 = slot.local * rows;
-  const uint32_t all = r.count * a.group;
-  if (t->r0 >= all) {
-    return false;
-  }
   t->live = all - t->r0 < rows ? all - t->r0 : rows;
-  t->length = kv_length(a.seqs, a.pool.shift, slot.seq);
-  t->origin = int64_t(t->length) - r.count;
+  return slot.seq < a.seqs.batch && t->r0 < all;
+}
+// Their positions, from the sequence's length.
+__device__ __forceinline__ void tile_tokens(const KvAttendArgs &a, uint32_t length, Tile *t) {
+  t->length = length;
+  t->origin = int64_t(length) - t->count;
   t->low = t->origin + t->r0 / a.group;
   t->high = t->origin + (t->r0 + t->live - 1) / a.group;
   const int64_t begin = a.window != 0 ? t->low - int64_t(a.window) + 1 : 0;
   t->begin = begin > 0 ? uint32_t(begin) : 0u;
   t->end = t->high >= 0 ? uint32_t(t->high + 1) : 0u;
-  return true;
 }
 
-// One workgroup owns a tile of 16 rows of one key/value head; its waves take
-// the 32-token groups in turn, each with a softmax of its own, and join them
-// at the end.
+// The 32 tokens of a group: keys and values of one head, 16 bytes per lane
+// and load.
 template <int D>
-__global__ __launch_bounds__(kWaves * kWave) void few_rows_kernel(KvAttendArgs a,
-                                                                 RowStats *stats,
-                                                                 uint32_t each_slots) {
-  __shared__ float part_o[kWaves][kRows][D + 4];
-  __shared__ float part_m[kWaves][kRows], part_l[kWaves][kRows];
-  Tile t;
-  if (!make_tile(a, blockIdx.x / a.pool.heads, kRows, each_slots, &t)) {
+struct Group {
+  Keys<D> k[2];
+  u32x4 v[D / 32];
+};
+template <int D, bool NT>
+__device__ __forceinline__ void load_group_keys(Group<D> &x, const uint8_t *unit,
+                                                uint32_t in_block, uint32_t lane) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    x.k[i] = load_keys<D, NT>(unit, in_block / 16 + i, lane);
+  }
+}
+template <int D, bool NT>
+__device__ __forceinline__ void load_group_values(Group<D> &x, const uint8_t *unit,
+                                                  uint32_t shift, uint32_t in_block,
+                                                  uint32_t lane) {
+  const u32x4 *p = reinterpret_cast<const u32x4 *>(unit + (uint64_t(D) << shift) +
+                                                   in_block / 32 * (D * 32)) + lane;
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+    x.v[c] = load_codes<NT>(p + c * 64);
+  }
+}
+
+// What a row has met so far: the running maximum and the sum of 2^kOff
+// exp2(score - m) (this lane's part of it), and its accumulators, which hold
+// sums over 2^acc_exp.
+template <int D>
+struct RowState {
+  float m, l;
+  int acc_exp;
+  f32x4 o[D / 16];
+};
+
+// Where a group lies and which of its tokens the lane's row sees.
+struct Place {
+  int32_t pos, oldest;  // the row's query, and the newest token that it no longer sees
+  int32_t low;          // first query of the tile
+  int32_t hidden;       // newest token that the tile's last query no longer sees
+};
+
+// The newest token that a query at `pos` no longer sees, -1 if it sees all.
+__device__ __forceinline__ int32_t oldest_hidden(int64_t pos, uint32_t window) {
+  const int64_t t = window != 0 ? pos - int64_t(window) : -1;
+  return t > -1 ? int32_t(t) : -1;
+}
+
+// Maximum over the four lane groups of a column.
+__device__ __forceinline__ float max_groups(float v) {
+  const auto half = __builtin_amdgcn_permlane32_swap(f32_bits(v), f32_bits(v), false, false);
+  v = fmaxf(bits_f32(half[0]), bits_f32(half[1]));
+  const auto row = __builtin_amdgcn_permlane16_swap(f32_bits(v), f32_bits(v), false, false);
+  return fmaxf(bits_f32(row[0]), bits_f32(row[1]));
+}
+
+// A NaN in a token that some rows do not see must not reach them through a
+// weight of zero: it is taken out of the group's values, and the rows that do
+// see it become NaN.  Bit i of `seen`: the lane's row sees its i-th token.
+template <int D>
+__device__ __forceinline__ void confine_nan(RowState<D> &st, Group<D> &x, uint32_t seen) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) {
+    any |= nan_bytes(x.v[i / 4][i % 4]);
+  }
+  if (!__any(any)) {
     return;
   }
+  u32x4 sv;
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    sv[h] = (seen >> (2 * h) & 1u ? 0x3c00u : 0u) | (seen >> (2 * h + 1) & 1u ? 0x3c000000u : 0u);
+  }
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    u32x4 nv;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t w = x.v[i / 2][i % 2 * 2 + h], bad = nan_bytes(w);
+      x.v[i / 2][i % 2 * 2 + h] = w & ~(bad | (bad - (bad >> 7)));
+      nv[2 * h] = (bad & 0x80u ? 0x3c00u : 0u) | (bad & 0x8000u ? 0x3c000000u : 0u);
+      nv[2 * h + 1] = (bad & 0x800000u ? 0x3c00u : 0u) | (bad >> 31 ? 0x3c000000u : 0u);
+    }
+    const f32x4 hit = mfma_f16(__builtin_bit_cast(f16x8, nv), __builtin_bit_cast(f16x8, sv),
+                               f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      st.o[i][j] = hit[j] > 0.f ? __builtin_nanf("") : st.o[i][j];
+    }
+  }
+}
+
+// One group for the 16 rows of a wave.  `scores_to`: where the scores of the
+// lane's row start (token 0; SCORES).  `more_keys` and `more_values`
+// issue the next group's loads as soon as the registers of this one are used.
+template <int D, bool SCORES, typename FK, typename FV>
+__device__ __forceinline__ void attend_group(RowState<D> &st, Group<D> &x, const Query<D> &q,
+                                             const Place &at, uint32_t t0, bool present, float pk,
+                                             int ev, float scale_log2, uint32_t g,
+                                             float *scores_to, FK more_keys, FV more_values) {
+  f32x4 s[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    s[i] = products(x.k[i], pk, q) * scale_log2;
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  more_keys();
+  __builtin_amdgcn_sched_barrier(0);
+  const bool edge = !present || int32_t(t0) + 31 > at.low || int32_t(t0) <= at.hidden;
+  if (edge) {
+    uint32_t seen = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int32_t tok = int32_t(t0 + 16 * (i / 4) + 4 * g + i % 4);
+      const bool see = present && tok <= at.pos && tok > at.oldest;
+      seen |= see ? 1u << i : 0u;
+      s[i / 4][i % 4] = see ? s[i / 4][i % 4] : -INFINITY;
+    }
+    confine_nan(st, x, seen);
+  }
+  if constexpr (SCORES) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      *reinterpret_cast<f32x4 *>(scores_to + t0 + 16 * i + 4 * g) = s[i];
+    }
+  }
+  if (ev > st.acc_exp + kUp) {
+    const float f = exp2_int(max(st.acc_exp - ev, -126));
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      st.o[i] *= f;
+    }
+    st.acc_exp = ev;
+  }
+  const int d = ev - st.acc_exp;
+  const float pv = exp2_int(d < kDown ? kDown : d);
+  const int shift = d < kDown ? max(d - kDown, -100) : 0;
+  float top = s[0][0];  // fmaxf passes NaN over: it makes the sum below NaN
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    top = fmaxf(top, s[i / 4][i % 4]);
+  }
+  top = max_groups(top);
+  if (__any(top > st.m)) {  // rare once a row has met its largest scores
+    const float now = fmaxf(st.m, top);
+    const float keep = now == -INFINITY ? 1.f : exp2_fast(st.m - now);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      st.o[i] *= keep;
+    }
+    st.l *= keep;
+    st.m = now;
+  }
+  const float ref = st.m == -INFINITY ? 0.f : st.m;
+  float p[8], sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    p[i] = exp2_fast(s[i / 4][i % 4] - (ref - float(kOff + shift)));
+    sum += p[i];
+  }
+  st.l += sum * exp2_int(-shift);
+  u32x4 pw;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    pw[i] = f32x2_to_f16x2(p[2 * i], p[2 * i + 1]);
+  }
+  const f16x8 pb = __builtin_bit_cast(f16x8, pw);
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    const u32x4 &w = x.v[i / 2];
+    st.o[i] = mfma_f16(codes_to_f16(w[i % 2 * 2], w[i % 2 * 2 + 1], pv), pb, st.o[i]);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  more_values();
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// Results of a part of a row's tokens: the mean of the values by weight, and
+// what joins it with the other parts.
+struct PartSum {
+  float m, l;
+};
+
+// Scratch of a call: partial results [row][head][part], row statistics
+// [row][head] and scores [row][head][token].
+struct Scratch {
+  float *part_o;
+  PartSum *part_s;
+  RowStats *stats;
+  float *scores;
+  uint64_t score_stride;
+  uint32_t parts, part_tokens;
+};
+
+__device__ __forceinline__ uint32_t part_count(const Tile &t, uint32_t part_tokens) {
+  const uint32_t from = t.begin / 32 * 32;
+  return t.end > from ? (t.end - from + part_tokens - 1) / part_tokens : 0u;
+}
+
+// Final results of a row: `n` elements of the output from dim d0 on, log-sum
+// and statistics.
+template <int N>
+__device__ __forceinline__ void store_row(const KvAttendArgs &a, const Scratch &x, uint64_t row,
+                                          uint32_t head, uint32_t d0, const float (&v)[N],
+                                          float top, float sum) {
+  const float join = sum == 0.f ? 0.f : 1.0f / sum;
+  uint16_t *to = a.out + row * a.out_row + head * a.out_head + d0;
+  uint32_t packed[N / 2];
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    packed[i] = f32x2_to_bf16x2(v[2 * i] * join, v[2 * i + 1] * join);
+  }
+  if (N % 4 == 0 && a.out_vec) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      reinterpret_cast<u32x2 *>(to)[i] = u32x2{packed[2 * i], packed[2 * i + 1]};
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      to[2 * i] = uint16_t(packed[i]);
+      to[2 * i + 1] = uint16_t(packed[i] >> 16);
+    }
+  }
+  if (d0 == 0) {
+    const uint64_t at = row * a.heads + head;
+    if (a.lse != nullptr) {
+      a.lse[at] = sum == 0.f ? -INFINITY : (top + (log2f(sum) - float(kOff))) * kLn2;
+    }
+    if (x.stats != nullptr) {
+      x.stats[at] = RowStats{(top == -INFINITY ? 0.f : top) - float(kOff), join};
+    }
+  }
+}
+
+// One workgroup owns a part of the tokens of a tile of 16 rows of one
+// key/value head.  Its waves take the 32-token groups in turn, each with a
+// softmax of its own, and join them at the end.  Block numbers and exponents
+// of the part's blocks are fetched by one load of the wave, so that a group
+// costs no dependent load; the next group's codes are under way while one is
+// computed.
+template <int D, int W, bool NT, bool SCORES>
+__global__ __launch_bounds__(W * kWave, 3) void few_rows_kernel(KvAttendArgs a, Scratch x,
+                                                             uint32_t each_slots) {
+  __shared__ float part_o[W][kRows][D + 4];
+  __shared__ float part_m[W][kRows], part_l[W][kRows];
   const uint32_t kvh = blockIdx.x % a.pool.heads;
-  const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const uint32_t part = blockIdx.x / a.pool.heads % x.parts;
+  Tile t;
+  if (!tile_rows(a, blockIdx.x / a.pool.heads / x.parts, kRows, each_slots, &t)) {
+    return;
+  }
+  const uint32_t lane = threadIdx.x % kWave;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const uint32_t g = lane / 16, col = lane % 16;
   // Rows past the end see what the last one does; their results are not stored.
   const uint32_t r = t.r0 + (col < t.live ? col : t.live - 1);
   const uint32_t head = kvh * a.group + r % a.group;
   const uint64_t row = t.first_row + r / a.group;
-  const int64_t pos = t.origin + r / a.group;
-  const int64_t oldest = a.window != 0 ? pos - int64_t(a.window) : -1;  // not seen
+  // Three loads that wait for none: the query, the block numbers of the part
+  // (with a window they depend on the length) and the length.  Lane i: block i
+  // of the part, which spans at most 64.
   const Query<D> q = load_query<D>(a.q + row * a.q_row + head * a.q_head, a.vec, g);
   const int32_t *table = a.seqs.tables + t.seq * a.seqs.stride;
+  uint32_t block0 = part * x.part_tokens >> a.pool.shift;
+  int32_t mine = a.window == 0 ? kv_block(table, a.seqs, a.pool.blocks, block0 + lane) : -1;
+  tile_tokens(a, kv_length(a.seqs, a.pool.shift, t.seq), &t);
+  const uint32_t parts = part_count(t, x.part_tokens);
+  if (part != 0 && part >= parts) {
+    return;
+  }
+  Place at;
+  at.pos = int32_t(t.origin + r / a.group);
+  at.oldest = oldest_hidden(at.pos, a.window);
+  at.low = int32_t(t.low);
+  at.hidden = oldest_hidden(t.high, a.window);
+  float *scores_to = SCORES ? x.scores + (row * a.heads + head) * x.score_stride : nullptr;
 
-  float m = -INFINITY, l = 0.f;  // running maximum; sum of 2^kOff exp2(score - m)
-  int acc_exp = kKvExpMin;       // o holds sums over 2^(acc_exp)
-  f32x4 o[D / 16];
+  RowState<D> st;
+  st.m = -INFINITY;
+  st.l = 0.f;
+  st.acc_exp = kKvExpMin;
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
-    o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    st.o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  for (uint32_t grp = t.begin / 32 + wave; grp < (t.end + 31) / 32; grp += kWaves) {
-    const uint32_t t0 = grp * 32;
-    const int32_t id = kv_block(table, a.seqs, a.pool.blocks, t0 >> a.pool.shift);
-    if (id < 0) {
-      continue;
+  const uint32_t from = t.begin / 32 + part * (x.part_tokens / 32);
+  const uint32_t all = (t.end + 31) / 32;
+  const uint32_t to = __builtin_amdgcn_readfirstlane(
+      all < from + x.part_tokens / 32 ? all : from + x.part_tokens / 32);
+  uint32_t grp = __builtin_amdgcn_readfirstlane(from + wave);
+  if (grp < to) {
+    if (a.window != 0) {
+      block0 = from * 32 >> a.pool.shift;
+      mine = kv_block(table, a.seqs, a.pool.blocks, block0 + lane);
     }
-    const uint64_t unit = uint64_t(id) * a.pool.heads + kvh;
-    const uint8_t *keys = a.pool.codes + unit * (uint64_t(2 * D) << a.pool.shift);
-    const uint8_t *values = keys + (uint64_t(D) << a.pool.shift);
-    const uint32_t in_block = t0 & ((1u << a.pool.shift) - 1);
-    const float pk = exp2_int(a.pool.exps[unit * 2]);
-    const int ev = a.pool.exps[unit * 2 + 1];
-    if (ev > acc_exp + kUp) {
-      const float f = exp2_int(max(acc_exp - ev, -126));
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        o[i] *= f;
-      }
-      acc_exp = ev;
-    }
-    const int d = ev - acc_exp;
-    const float pv = exp2_int(d < kDown ? kDown : d);
-    const int shift = d < kDown ? max(d - kDown, -100) : 0;
-    f32x4 s[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      s[i] = products(load_keys<D>(keys, in_block / 16 + i, lane), pk, q) * a.scale_log2;
-    }
-    const bool edge = int64_t(t0) + 31 > t.low ||
-                      (a.window != 0 && int64_t(t0) <= t.high - int64_t(a.window));
-    uint32_t seen = 0xffu;
-    if (edge) {
-      seen = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int64_t tok = int64_t(t0) + 16 * (i / 4) + 4 * g + i % 4;
-        const bool see = tok <= pos && tok > oldest;
-        seen |= see ? 1u << i : 0u;
-        s[i / 4][i % 4] = see ? s[i / 4][i % 4] : -INFINITY;
-      }
-    }
-    float top = s[0][0];  // fmaxf passes NaN over: it makes the sum below NaN
-#pragma unroll
-    for (int i = 1; i < 8; ++i) {
-      top = fmaxf(top, s[i / 4][i % 4]);
-    }
-    top = fmaxf(top, __shfl_xor(top, 16, kWave));
-    top = fmaxf(top, __shfl_xor(top, 32, kWave));
-    const float now = fmaxf(m, top);
-    const float ref = now == -INFINITY ? 0.f : now;
-    const float keep = exp2_fast(m - ref);
-    m = now;
-    float p[8], sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      p[i] = exp2_fast(s[i / 4][i % 4] - (ref - float(kOff + shift)));
-      sum += p[i];
-    }
-    l = l * keep + sum * exp2_int(-shift);
-    u32x4 pw;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      pw[i] = f32x2_to_f16x2(p[2 * i], p[2 * i + 1]);
-    }
-    const f16x8 pb = __builtin_bit_cast(f16x8, pw);
-    const u32x4 *vt =
-        reinterpret_cast<const u32x4 *>(values + in_block / 32 * (D * 32)) + lane;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
-      u32x4 w = vt[c * 64];
-      u32x4 bad_v = {0u, 0u, 0u, 0u};
-      if (edge) {
-        // A NaN in a token that some rows do not see must not reach them
-        // through a weight of zero: it is taken out of the product, and the
-        // rows that see it become NaN.
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          bad_v[i] = nan_bytes(w[i]);
-          w[i] &= ~(bad_v[i] | (bad_v[i] - (bad_v[i] >> 7)));
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        f32x4 &acc = o[2 * c + h];
-        acc = mfma_f16(codes_to_f16(w[2 * h], w[2 * h + 1], pv), pb, acc * keep);
-        if (edge && __any(bad_v[2 * h] | bad_v[2 * h + 1])) {
-          u32x4 nv, sv;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t two = bad_v[2 * h + i / 2] >> (16 * (i % 2));
-            nv[i] = (two & 0x80u ? 0x3c00u : 0u) | (two & 0x8000u ? 0x3c000000u : 0u);
-            sv[i] = (seen >> (2 * i) & 1u ? 0x3c00u : 0u) |
-                    (seen >> (2 * i + 1) & 1u ? 0x3c000000u : 0u);
-          }
-          const f32x4 hit =
-              mfma_f16(__builtin_bit_cast(f16x8, nv), __builtin_bit_cast(f16x8, sv),
-                       f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            acc[i] = hit[i] > 0.f ? __builtin_nanf("") : acc[i];
-          }
-        }
-      }
+    block0 = __builtin_amdgcn_readfirstlane(block0);
+    const uint64_t my_unit = uint64_t(mine < 0 ? 0 : mine) * a.pool.heads + kvh;
+    const int my_exps = *reinterpret_cast<const uint16_t *>(a.pool.exps + my_unit * 2);
+    const auto unit_of = [&](uint32_t group) {
+      const int id = __builtin_amdgcn_readlane(mine, (group * 32 >> a.pool.shift) - block0);
+      return a.pool.codes + (uint64_t(id < 0 ? 0 : id) * a.pool.heads + kvh) *
+                                (uint64_t(2 * D) << a.pool.shift);
+    };
+    const uint32_t in_mask = (1u << a.pool.shift) - 1;
+    Group<D> x32;
+    // Keys first, as in the loop: a wait for them then leaves the values' loads
+    // in flight.
+    load_group_keys<D, NT>(x32, unit_of(grp), grp * 32 & in_mask, lane);
+    __builtin_amdgcn_sched_barrier(0);
+    load_group_values<D, NT>(x32, unit_of(grp), a.pool.shift, grp * 32 & in_mask, lane);
+    __builtin_amdgcn_sched_barrier(0);
+    while (grp < to) {
+      // The last group is loaded again past the end: no load is conditional.
+      const uint32_t ahead = grp + W < to ? grp + W : grp;
+      const uint32_t i = (grp * 32 >> a.pool.shift) - block0;
+      const int exps = __builtin_amdgcn_readlane(my_exps, i);
+      attend_group<D, SCORES>(
+          st, x32, q, at, grp * 32, __builtin_amdgcn_readlane(mine, i) >= 0, exp2_int(int8_t(exps)),
+          int8_t(exps >> 8), a.scale_log2, g, scores_to,
+          [&] { load_group_keys<D, NT>(x32, unit_of(ahead), ahead * 32 & in_mask, lane); },
+          [&] { load_group_values<D, NT>(x32, unit_of(ahead), a.pool.shift, ahead * 32 & in_mask, lane); });
+      grp += W;
     }
   }
-  l += __shfl_xor(l, 16, kWave);
+  float l = st.l + __shfl_xor(st.l, 16, kWave);
   l += __shfl_xor(l, 32, kWave);
   if (g == 0) {
-    part_m[wave][col] = m;
+    part_m[wave][col] = st.m;
     part_l[wave][col] = l;
   }
   // Means of the wave's tokens, to be joined by their sums.
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  const float power = exp2_int(acc_exp);
+  const float power = exp2_int(st.acc_exp);
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
-    *reinterpret_cast<f32x4 *>(&part_o[wave][col][16 * i + 4 * g]) = o[i] * inv * power;
+    *reinterpret_cast<f32x4 *>(&part_o[wave][col][16 * i + 4 * g]) = st.o[i] * inv * power;
   }
   __syncthreads();
-  // 16 threads to a row, D / 16 dims each.
-  const uint32_t mine = threadIdx.x / 16;
-  if (mine >= t.live) {
+  constexpr int kPer = D / (4 * W);  // dims of a thread: 4 W threads to a row
+  const uint32_t own = threadIdx.x / (4 * W);
+  if (own >= t.live) {
     return;
   }
-  const uint32_t rr = t.r0 + mine;
+  const uint32_t rr = t.r0 + own;
   const uint64_t out_row = t.first_row + rr / a.group;
   const uint32_t out_head = kvh * a.group + rr % a.group;
-  float top = part_m[0][mine];
+  float top = part_m[0][own];
 #pragma unroll
-  for (uint32_t w = 1; w < kWaves; ++w) {
-    top = fmaxf(top, part_m[w][mine]);
+  for (int w = 1; w < W; ++w) {
+    top = fmaxf(top, part_m[w][own]);
   }
   const float ref = top == -INFINITY ? 0.f : top;
-  float sum = 0.f, f[kWaves];
+  float sum = 0.f, f[W];
 #pragma unroll
-  for (uint32_t w = 0; w < kWaves; ++w) {
-    f[w] = exp2_fast(part_m[w][mine] - ref) * part_l[w][mine];
+  for (int w = 0; w < W; ++w) {
+    f[w] = exp2_fast(part_m[w][own] - ref) * part_l[w][own];
     sum += f[w];
   }
+  const uint32_t d0 = threadIdx.x % (4 * W) * kPer;
+  float v[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    v[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      v[i] += part_o[w][own][d0 + i] * f[w];
+    }
+  }
+  if (parts <= 1) {
+    store_row(a, x, out_row, out_head, d0, v, top, sum);
+    return;
+  }
+  const uint64_t slot = (out_row * a.heads + out_head) * x.parts + part;
   const float join = sum == 0.f ? 0.f : 1.0f / sum;
-  const uint32_t d0 = threadIdx.x % 16 * (D / 16);
-  uint32_t packed[D / 32];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-    float v[2] = {0.f, 0.f};
-#pragma unroll
-    for (uint32_t w = 0; w < kWaves; ++w) {
-      v[0] += part_o[w][mine][d0 + 2 * i] * f[w];
-      v[1] += part_o[w][mine][d0 + 2 * i + 1] * f[w];
-    }
-    packed[i] = f32x2_to_bf16x2(v[0] * join, v[1] * join);
+  for (int i = 0; i < kPer; ++i) {
+    x.part_o[slot * D + d0 + i] = v[i] * join;
   }
-  uint16_t *to = a.out + out_row * a.out_row + out_head * a.out_head + d0;
-  if (a.out_vec) {
+  if (d0 == 0) {
+    x.part_s[slot] = PartSum{top, sum};
+  }
+}
+
+// Joins the parts of a row: one workgroup of J waves, which take the parts in
+// turn, kJoinAhead of them under way at once (the sums of a part are small:
+// the time goes into waiting for them).
+constexpr uint32_t kJoinAhead = 4;
+template <int D, uint32_t J>
+__global__ __launch_bounds__(J * kWave) void join_parts_kernel(KvAttendArgs a, Scratch x,
+                                                               uint32_t rows_of_tile,
+                                                               uint32_t each_slots) {
+  __shared__ float part_o[J][D];
+  __shared__ float part_m[J], part_l[J];
+  constexpr int kPer = D / kWave;
+  Tile t;
+  const uint32_t index = blockIdx.x / rows_of_tile;
+  if (!tile_rows(a, index / a.pool.heads, kRows, each_slots, &t) ||
+      blockIdx.x % rows_of_tile >= t.live) {
+    return;
+  }
+  tile_tokens(a, kv_length(a.seqs, a.pool.shift, t.seq), &t);
+  const uint32_t parts = part_count(t, x.part_tokens), r = t.r0 + blockIdx.x % rows_of_tile;
+  if (parts <= 1) {
+    return;
+  }
+  const uint64_t row = t.first_row + r / a.group;
+  const uint32_t head = index % a.pool.heads * a.group + r % a.group;
+  const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const uint64_t slot = (row * a.heads + head) * x.parts;
+  float m = -INFINITY, l = 0.f, v[kPer] = {};
+  for (uint32_t p0 = wave; p0 < parts; p0 += J * kJoinAhead) {
+    PartSum s[kJoinAhead];
+    float o[kJoinAhead][kPer];
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-      reinterpret_cast<u32x2 *>(to)[i] = u32x2{packed[2 * i], packed[2 * i + 1]};
+    for (uint32_t j = 0; j < kJoinAhead; ++j) {
+      const uint32_t p = p0 + j * J;
+      const uint64_t at = slot + (p < parts ? p : p0);
+      s[j] = x.part_s[at];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        o[j][i] = x.part_o[at * D + lane * kPer + i];
+      }
+      s[j].l = p < parts ? s[j].l : 0.f;
     }
-  } else {
+    float now = m;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      to[2 * i] = uint16_t(packed[i]);
-      to[2 * i + 1] = uint16_t(packed[i] >> 16);
+    for (uint32_t j = 0; j < kJoinAhead; ++j) {
+      now = fmaxf(now, s[j].m);
+    }
+    const float ref = now == -INFINITY ? 0.f : now, keep = exp2_fast(m - ref);
+    m = now;
+    l *= keep;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      v[i] *= keep;
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kJoinAhead; ++j) {
+      const float f = exp2_fast(s[j].m - ref) * s[j].l;
+      const bool none = p0 + j * J >= parts;
+      l += f;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        v[i] += none ? 0.f : o[j][i] * f;
+      }
     }
   }
-  if (threadIdx.x % 16 == 0) {
-    const uint64_t at = out_row * a.heads + out_head;
-    if (a.lse != nullptr) {
-      a.lse[at] = sum == 0.f ? -INFINITY : (top + (log2f(sum) - float(kOff))) * kLn2;
-    }
-    if (stats != nullptr) {
-      stats[at] = RowStats{ref - float(kOff), join};
+  if (lane == 0) {
+    part_m[wave] = m;
+    part_l[wave] = l;
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    part_o[wave][lane * kPer + i] = v[i];
+  }
+  __syncthreads();
+  if (threadIdx.x * 2 >= D) {
+    return;
+  }
+  float top = part_m[0], sum = 0.f, out[2] = {0.f, 0.f};
+#pragma unroll
+  for (uint32_t w = 1; w < J; ++w) {
+    top = fmaxf(top, part_m[w]);
+  }
+  const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (uint32_t w = 0; w < J; ++w) {
+    const float f = exp2_fast(part_m[w] - ref);
+    sum += part_l[w] * f;
+    out[0] += part_o[w][threadIdx.x * 2] * f;
+    out[1] += part_o[w][threadIdx.x * 2 + 1] * f;
+  }
+  store_row(a, x, row, head, threadIdx.x * 2, out, top, sum);
+}
+
+// Adds each token's weights from the scores that few_rows_kernel stored: a
+// thread owns a token and sums its rows in order.
+__global__ __launch_bounds__(256) void add_scores_kernel(KvAttendArgs a, Scratch x) {
+  const uint32_t kvh = blockIdx.y, b = blockIdx.z;
+  const uint32_t t = blockIdx.x * 256 + threadIdx.x;
+  const uint32_t length = kv_length(a.seqs, a.pool.shift, b);
+  if (t >= length) {
+    return;
+  }
+  const int32_t id = kv_block(a.seqs.tables + b * a.seqs.stride, a.seqs, a.pool.blocks,
+                              t >> a.pool.shift);
+  if (id < 0) {
+    return;
+  }
+  const KvRows rows = kv_rows(a.seqs, b);
+  const int64_t origin = int64_t(length) - rows.count;
+  const int64_t from = int64_t(t) - origin;  // the first query that sees the token
+  uint32_t i = from > 0 ? uint32_t(from) : 0u;
+  const int64_t past = a.window != 0 ? from + int64_t(a.window) : int64_t(rows.count);
+  const uint32_t end = past < int64_t(rows.count) ? uint32_t(past < 0 ? 0 : past) : rows.count;
+  float sum = 0.f;
+  for (; i < end; ++i) {
+    const uint64_t at = uint64_t(rows.first + i) * a.heads + kvh * a.group;
+    for (uint32_t h = 0; h < a.group; ++h) {
+      const RowStats st = x.stats[at + h];
+      sum += exp2_fast(x.scores[(at + h) * x.score_stride + t] - st.top) * st.inv_sum;
     }
   }
+  const uint64_t unit = uint64_t(id) * a.pool.heads + kvh;
+  unsafeAtomicAdd(&a.pool.weights[(unit << a.pool.shift) + (t & ((1u << a.pool.shift) - 1))], sum);
 }
 
 // Adds the weights that the tokens of a 32-token group receive from all rows
@@ -408,7 +721,7 @@ __global__ __launch_bounds__(kWaves * kWave) void add_weights_kernel(KvAttendArg
   Keys<D> k[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    k[i] = load_keys<D>(keys, in_block / 16 + i, lane);
+    k[i] = load_keys<D, false>(keys, in_block / 16 + i, lane);
   }
   const int64_t origin = int64_t(length) - rows.count;
   const uint32_t all = rows.count * a.group;
@@ -463,6 +776,46 @@ __global__ __launch_bounds__(kWaves * kWave) void add_weights_kernel(KvAttendArg
 
 }  // namespace
 
+// Scratch of a plan in its order: partial results, row statistics, scores.
+static Scratch scratch_of(const KvAttendArgs &a, uint32_t dim, const KvAttendPlan &p, void *ws,
+                          uint64_t *bytes) {
+  Scratch x{};
+  x.parts = p.parts;
+  x.part_tokens = p.part_tokens;
+  const uint64_t rows = uint64_t(a.seqs.rows) * a.heads;
+  uint64_t at = 0;
+  const auto take = [&](uint64_t n) {
+    char *r = ws == nullptr ? nullptr : static_cast<char *>(ws) + at;
+    at += (n + 255) / 256 * 256;
+    return r;
+  };
+  if (p.parts > 1) {
+    x.part_o = reinterpret_cast<float *>(take(rows * p.parts * dim * sizeof(float)));
+    x.part_s = reinterpret_cast<PartSum *>(take(rows * p.parts * sizeof(PartSum)));
+  }
+  if (a.accumulate) {
+    x.stats = reinterpret_cast<RowStats *>(take(rows * sizeof(RowStats)));
+    if (p.keep_scores) {
+      x.score_stride = uint64_t(a.seqs.max_blocks) << a.pool.shift;
+      x.scores = reinterpret_cast<float *>(take(rows * x.score_stride * sizeof(float)));
+    }
+  }
+  *bytes = at;
+  return x;
+}
+
+static uint64_t each_tiles(const KvAttendArgs &a, uint32_t rows) {
+  return (uint64_t(a.seqs.each) * a.group + rows - 1) / rows;
+}
+
+// Tokens are split where the tiles alone leave compute units idle, into parts
+// that together give each a workgroup: more and smaller parts cost their
+// start and the join (131072 tokens of 8 heads: 32 parts each 46.7 us, 64
+// 50.1, 128 53.2).  A part has at least kPartLeast tokens (333 tokens of 8
+// heads: whole 5.7 us, in two parts 7.8) and at most 64 blocks, what a wave
+// looks up with one load.
+constexpr uint32_t kPartLeast = 512;
+
 KvAttendPlan plan_kv_attend(const KvAttendArgs &a, uint32_t dim) {
   KvAttendPlan p;
   if (a.seqs.rows == 0 || a.seqs.batch == 0) {
@@ -470,26 +823,70 @@ KvAttendPlan plan_kv_attend(const KvAttendArgs &a, uint32_t dim) {
   }
   p.kernel = ULLM_KV_KERNEL_FEW_ROWS;
   p.row_tile = kRows;
-  p.part_tokens = a.seqs.max_blocks << a.pool.shift;
-  const uint64_t each = (uint64_t(a.seqs.each) * a.group + kRows - 1) / kRows;
-  p.grid = kv_slots(a.seqs, a.group, kRows, 1, each) * a.pool.heads;
-  if (a.accumulate) {
-    p.workspace = uint64_t(a.seqs.rows) * a.heads * sizeof(RowStats);
+  const uint64_t tiles = kv_slots(a.seqs, a.group, kRows, 1, each_tiles(a, kRows)) * a.pool.heads;
+  // The most tokens that a tile's rows see, from the start of a 32-token group.
+  uint64_t span = uint64_t(a.seqs.max_blocks) << a.pool.shift;
+  if (a.window != 0) {
+    span = std::min<uint64_t>(span, uint64_t(a.window) + kRows / a.group + 32);
   }
+  const uint32_t cus = device_cu_count();
+  const uint64_t split = std::max<uint64_t>(cus / tiles, 1);
+  const uint64_t part = std::max<uint64_t>((span + split - 1) / split, kPartLeast);
+  p.part_tokens = uint32_t(std::min<uint64_t>((part + 31) / 32 * 32, 64u << a.pool.shift));
+  p.parts = uint32_t((span + p.part_tokens - 1) / p.part_tokens);
+  // Scores cost 8 bytes for each row and token, a second pass over the keys
+  // `dim` bytes for each token.
+  const uint64_t rows_of_head = uint64_t(a.seqs.rows) * a.group;
+  p.keep_scores = a.accumulate && rows_of_head <= uint64_t(dim) / 8 * a.seqs.batch;
+  p.one_tile = rows_of_head <= uint64_t(kRows) * a.seqs.batch;
+  p.grid = tiles * p.parts;
+  // Eight waves shorten the walk of a lone workgroup (333 tokens: 5.7 against
+  // 6.2 us), four have less to join where all units are busy.
+  p.waves = p.grid <= cus / 2 ? 8 : 4;
+  scratch_of(a, dim, p, nullptr, &p.workspace);
   return p;
 }
 
 template <int D>
 static hipError_t launch_attend(const KvAttendArgs &a, const KvAttendPlan &p, void *workspace,
                                 hipStream_t s) {
-  RowStats *stats = a.accumulate ? static_cast<RowStats *>(workspace) : nullptr;
-  const uint32_t each = (a.seqs.each * a.group + kRows - 1) / kRows;
-  few_rows_kernel<D><<<uint32_t(p.grid), kWaves * kWave, 0, s>>>(a, stats, each);
+  uint64_t bytes = 0;
+  const Scratch x = scratch_of(a, D, p, workspace, &bytes);
+  const uint32_t each = uint32_t(each_tiles(a, kRows));
+  const auto few = [&](auto kernel8, auto kernel4) {
+    if (p.waves == 8) {
+      kernel8<<<uint32_t(p.grid), 8 * kWave, 0, s>>>(a, x, each);
+    } else {
+      kernel4<<<uint32_t(p.grid), 4 * kWave, 0, s>>>(a, x, each);
+    }
+  };
+  if (x.scores != nullptr) {
+    few(few_rows_kernel<D, 8, true, true>, few_rows_kernel<D, 4, true, true>);
+  } else if (p.one_tile) {
+    few(few_rows_kernel<D, 8, true, false>, few_rows_kernel<D, 4, true, false>);
+  } else {
+    few(few_rows_kernel<D, 8, false, false>, few_rows_kernel<D, 4, false, false>);
+  }
+  if (p.parts > 1) {
+    const uint32_t rows =
+        a.seqs.starts == nullptr ? std::min(a.seqs.each * a.group, kRows) : kRows;
+    const uint32_t grid = uint32_t(p.grid / p.parts) * rows;
+    if (p.parts > 2 * kJoinAhead) {
+      join_parts_kernel<D, 8><<<grid, 8 * kWave, 0, s>>>(a, x, rows, each);
+    } else {
+      join_parts_kernel<D, 1><<<grid, kWave, 0, s>>>(a, x, rows, each);
+    }
+  }
   if (a.accumulate) {
     const uint64_t tokens = uint64_t(a.seqs.max_blocks) << a.pool.shift;
-    const dim3 grid(uint32_t((tokens + 32 * kWaves - 1) / (32 * kWaves)), a.pool.heads,
-                    a.seqs.batch);
-    add_weights_kernel<D><<<grid, kWaves * kWave, 0, s>>>(a, stats);
+    if (x.scores != nullptr) {
+      add_scores_kernel<<<dim3(uint32_t((tokens + 255) / 256), a.pool.heads, a.seqs.batch), 256, 0,
+                          s>>>(a, x);
+    } else {
+      const dim3 grid(uint32_t((tokens + 32 * kWaves - 1) / (32 * kWaves)), a.pool.heads,
+                      a.seqs.batch);
+      add_weights_kernel<D><<<grid, kWaves * kWave, 0, s>>>(a, x.stats);
+    }
   }
   return hipGetLastError();
 }

@@ -95,6 +95,9 @@ struct KvAttendArgs {
 };
 struct KvAttendPlan {
   uint32_t kernel = 0, row_tile = 0, parts = 1, part_tokens = 0;
+  uint32_t waves = 4;
+  bool keep_scores = false;  // weights from stored scores
+  bool one_tile = false;     // sequences have one tile of rows, on average
   uint64_t grid = 0, workspace = 0;
 };
 
@@ -155,33 +158,40 @@ __device__ __forceinline__ int32_t kv_block(const int32_t *table, const KvSeqs &
 // owns the slots from starts[b] * mult / tile + extra * b on.  Since
 // floor(x + y) + 1 >= floor(x) + ceil(y), `extra` = 1 leaves it room for
 // ceil(count * mult / tile) slots.  Returns the sequence of slot `id` (every
-// lane of a wave calls it) and its first slot, or batch when there is none.
+// lane of a wave calls it with the same one), its rows and the slot's number
+// within it; seq >= batch when there is none.  64 offsets are looked at with
+// one load.
 struct KvSlot {
   uint32_t seq, local;
+  KvRows rows;
 };
 __device__ __forceinline__ KvSlot kv_find_slot(const KvSeqs &s, uint32_t id, uint32_t mult,
                                                uint32_t tile, uint32_t extra,
                                                uint32_t each_slots) {
   if (s.starts == nullptr) {
-    return {id / each_slots, id % each_slots};
+    const uint32_t b = id / each_slots;
+    return {b, id % each_slots, {b * s.each, s.each}};
   }
   const uint32_t lane = threadIdx.x % kWave;
-  uint32_t owned = 0;
+  KvSlot r{s.batch, 0, {0, 0}};
   for (uint32_t c = 0; c < s.batch; c += kWave) {
     const uint32_t b = c + lane;
-    const bool mine =
-        b < s.batch && uint64_t(kv_start(s, b)) * mult / tile + uint64_t(extra) * b <= id;
-    const uint32_t n = uint32_t(__popcll(__ballot(mine)));
-    owned += n;
+    const uint32_t at = kv_start(s, b < s.batch ? b : s.batch);
+    const uint64_t slot0 = uint64_t(at) * mult / tile + uint64_t(extra) * b;
+    const uint32_t n = uint32_t(__popcll(__ballot(b < s.batch && slot0 <= id)));
+    if (n != 0) {
+      r.seq = c + n - 1;
+      r.local = id - uint32_t(__builtin_amdgcn_readlane(int(slot0), n - 1));
+      r.rows.first = uint32_t(__builtin_amdgcn_readlane(int(at), n - 1));
+      const uint32_t next = n < kWave ? uint32_t(__builtin_amdgcn_readlane(int(at), n & 63))
+                                      : kv_start(s, c + kWave);
+      r.rows.count = next > r.rows.first ? next - r.rows.first : 0u;
+    }
     if (n < kWave) {
       break;
     }
   }
-  if (owned == 0) {
-    return {s.batch, 0};
-  }
-  const uint32_t b = owned - 1;
-  return {b, id - uint32_t(uint64_t(kv_start(s, b)) * mult / tile + uint64_t(extra) * b)};
+  return r;
 }
 inline uint64_t kv_slots(const KvSeqs &s, uint64_t mult, uint64_t tile, uint64_t extra,
                          uint64_t each_slots) {

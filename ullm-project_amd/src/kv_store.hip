@@ -104,7 +104,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(KvAppendArgs a, uint32
   if (slot.seq >= a.seqs.batch) {
     return;
   }
-  const KvRows rows = kv_rows(a.seqs, slot.seq);
+  const KvRows rows = slot.rows;
   const uint32_t length = kv_length(a.seqs, a.pool.shift, slot.seq);
   const int64_t origin = int64_t(length) - rows.count;  // position of the first row
   const uint32_t first = origin < 0 ? 0u : uint32_t(origin);
@@ -226,7 +226,7 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(KvGatherArgs a) {
   if (slot.seq >= a.seqs.batch) {
     return;
   }
-  const KvRows rows = kv_rows(a.seqs, slot.seq);
+  const KvRows rows = slot.rows;
   if (slot.local >= rows.count) {
     return;
   }

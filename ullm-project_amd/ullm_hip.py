@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import ctypes
 import enum
+import struct
 import threading
 from pathlib import Path
 
@@ -273,8 +274,6 @@ class KvEvictDesc(ctypes.Structure):
 
 
 _FORWARD_SIZE = ctypes.sizeof(ForwardDesc)
-_KV_APPEND_SIZE = ctypes.sizeof(KvAppendDesc)
-_KV_ATTEND_SIZE = ctypes.sizeof(KvAttendDesc)
 
 # safetensors dtype strings by ULLM_ST_DTYPE_* value
 ST_DTYPES = {1: "BOOL", 2: "U8", 3: "I8", 4: "F8_E4M3", 5: "F8_E5M2", 6: "U16",
@@ -681,18 +680,59 @@ def release_workspaces(device: int = 0) -> None:
 
 # --------------------------------------------------------- key/value cache
 
+class _Packed:
+    """A descriptor filled in one pack of its flattened fields, header first
+    and reserved words left out (they stay zero): 0.6 us for the 25 fields of
+    an attend descriptor, 2.5 with ctypes constructors."""
+
+    def __init__(self, cls):
+        codes = {_u32: "I", _i32: "i", _u64: "Q", _vp: "Q", ctypes.c_float: "f"}
+
+        def flat(fields):
+            return "".join(flat(t._fields_) if hasattr(t, "_fields_") else codes[t]
+                           for _, t in fields if not hasattr(t, "_length_"))
+        self.format = struct.Struct("@" + flat(cls._fields_))
+        self.buffer = bytearray(ctypes.sizeof(cls))
+        self.desc = cls.from_buffer(self.buffer)
+        self.ref = ctypes.byref(self.desc)
+        self.header = (ctypes.sizeof(cls), ABI_VERSION)
+
+    def fill(self, *fields):
+        self.format.pack_into(self.buffer, 0, *self.header, *fields)
+        return self.ref
+
+
+def _packed(cls) -> _Packed:
+    """This thread's descriptor of a class (the library copies what it needs
+    before a call returns)."""
+    held = _thread.__dict__.get(cls)
+    if held is None:
+        held = _thread.__dict__[cls] = _Packed(cls)
+    return held
+
+
 def _strides3(t, name, heads, dim):
-    """(row, head) strides of a bf16 [rows][heads][dim] tensor."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim \
+    """(rows, row stride, head stride) of a bf16 [rows][heads][dim] tensor."""
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim \
             or t.dtype is not _torch().bfloat16:
         raise ValueError(f"{name} must be bfloat16 [rows][{heads}][{dim}]")
     row, head, one = t.stride()
     # The stride of an axis of one is never used.
-    row = row if t.shape[0] > 1 else max(row, dim)
-    head = head if heads > 1 else dim
+    if shape[0] <= 1:
+        row = max(row, dim)
+    if heads == 1:
+        head = dim
     if one != 1 or row < dim or head < dim:
         raise ValueError(f"{name} must have contiguous heads that do not overlap")
-    return row, head
+    return shape[0], row, head
+
+
+def _call(fn, ref):
+    s = _thread_sink()
+    st = fn(ref, s.ref)
+    if st:
+        raise HipError(st, s.text())
 
 
 class KvCache:
@@ -742,86 +782,85 @@ class KvCache:
 
     # -- calls -------------------------------------------------------------
     def _seqs(self, lengths, tables, rows, starts):
+        """The fields of a ullm_kv_sequences_t."""
         i32 = _torch().int32
         batch, columns = tables.shape
         stride, one = tables.stride()
-        if tables.dtype is not i32 or lengths.dtype is not i32 or lengths.dim() != 1 \
-                or lengths.shape[0] != batch or (batch > 1 and lengths.stride(0) != 1):
+        if tables.dtype is not i32 or lengths.dtype is not i32 or lengths.shape != (batch,) \
+                or (batch > 1 and lengths.stride(0) != 1):
             raise ValueError("tables must be int32 [batch][columns] and lengths int32 [batch]")
-        if (columns > 1 and one != 1) or (batch > 1 and stride < columns):
+        if batch == 1:
+            stride = columns
+        if (columns > 1 and one != 1) or stride < columns:
             raise ValueError("rows of tables must be contiguous and must not overlap")
-        if starts is not None and (starts.dtype is not i32 or tuple(starts.shape) != (batch + 1,)
-                                   or not starts.is_contiguous()):
+        if starts is None:
+            at = 0
+        elif starts.dtype is not i32 or starts.shape != (batch + 1,) \
+                or not starts.is_contiguous():
             raise ValueError("starts must be int32 [batch + 1]")
-        return KvSequences(batch, rows, tables.data_ptr(), stride if batch > 1 else columns,
-                           columns, lengths.data_ptr(),
-                           None if starts is None else starts.data_ptr())
+        else:
+            at = starts.data_ptr()
+        return batch, rows, tables.data_ptr(), stride, columns, lengths.data_ptr(), at
 
     def append(self, k, v, lengths, tables, starts=None, weights=None, stream=None):
         """Quantize and store new tokens: k, v bf16 [rows][kv_heads][head_dim]
         (row and head strides honoured).  ``weights`` (f32 [rows][kv_heads])
         restores weights read by ``gather_weights``; without it they are 0."""
-        ks = _strides3(k, "k", self.kv_heads, self.head_dim)
-        vs = _strides3(v, "v", self.kv_heads, self.head_dim)
-        rows = k.shape[0]
-        if v.shape[0] != rows:
+        heads, dim = self.kv_heads, self.head_dim
+        rows, k_row, k_head = _strides3(k, "k", heads, dim)
+        v_rows, v_row, v_head = _strides3(v, "v", heads, dim)
+        if v_rows != rows:
             raise ValueError("k and v must have the same number of rows")
-        if weights is not None and (tuple(weights.shape) != (rows, self.kv_heads)
+        if weights is not None and (weights.shape != (rows, heads)
                                     or weights.dtype is not _torch().float32
                                     or not weights.is_contiguous()):
             raise ValueError("weights must be a contiguous float32 [rows][kv_heads] tensor")
-        d = KvAppendDesc(_KV_APPEND_SIZE, ABI_VERSION, self.handle,
-                         self._seqs(lengths, tables, rows, starts), k.data_ptr(), *ks,
-                         v.data_ptr(), *vs, _ptr(weights), _stream(stream))
-        s = _thread_sink()
-        st = lib().ullm_kv_cache_append(ctypes.byref(d), s.ref)
-        if st:
-            raise HipError(st, s.text())
+        _call(lib().ullm_kv_cache_append, _packed(KvAppendDesc).fill(
+            self.handle or 0, *self._seqs(lengths, tables, rows, starts), k.data_ptr(), k_row,
+            k_head, v.data_ptr(), v_row, v_head, 0 if weights is None else weights.data_ptr(),
+            _stream(stream) or 0))
 
     def _gather(self, lengths, tables, rows, starts, k, v, weights, stream):
-        d = KvGatherDesc(ctypes.sizeof(KvGatherDesc), ABI_VERSION, self.handle,
-                         self._seqs(lengths, tables, rows, starts), _ptr(k), _ptr(v),
-                         _ptr(weights), _stream(stream))
-        s = _thread_sink()
-        st = lib().ullm_kv_cache_gather(ctypes.byref(d), s.ref)
-        if st:
-            raise HipError(st, s.text())
+        _call(lib().ullm_kv_cache_gather, _packed(KvGatherDesc).fill(
+            self.handle or 0, *self._seqs(lengths, tables, rows, starts), k, v, weights,
+            _stream(stream) or 0))
 
     def gather(self, lengths, tables, rows, starts=None, stream=None):
         """Keys and values of each sequence's last rows (``rows`` in all), bf16
         [rows][kv_heads][head_dim] and exact: appending them again stores the
         same values.  Rows that name no token are zero."""
-        torch = _torch()
-        k, v = (torch.empty((rows, self.kv_heads, self.head_dim), dtype=torch.bfloat16,
-                            device=tables.device) for _ in range(2))
-        self._gather(lengths, tables, rows, starts, k, v, None, stream)
-        return k, v
+        kv = tables.new_empty((2, rows, self.kv_heads, self.head_dim), dtype=_torch().bfloat16)
+        at = kv.data_ptr()
+        self._gather(lengths, tables, rows, starts, at,
+                     at + rows * self.kv_heads * self.head_dim * 2, 0, stream)
+        return kv.unbind(0)
 
     def gather_weights(self, lengths, tables, rows, starts=None, stream=None):
         """The weights of each sequence's last rows, f32 [rows][kv_heads]."""
-        torch = _torch()
-        w = torch.empty((rows, self.kv_heads), dtype=torch.float32, device=tables.device)
-        self._gather(lengths, tables, rows, starts, None, None, w, stream)
+        w = tables.new_empty((rows, self.kv_heads), dtype=_torch().float32)
+        self._gather(lengths, tables, rows, starts, 0, 0, w.data_ptr(), stream)
         return w
 
-    def _attend_desc(self, q, lengths, tables, starts, out, lse, scale, window, accumulate,
-                     stream, workspace):
+    def _attend_fields(self, q, lengths, tables, starts, out, lse, scale, window, accumulate,
+                       stream, workspace):
         heads, dim = q.shape[1], self.head_dim
-        qs = _strides3(q, "q", heads, dim)
-        os = _strides3(out, "out", heads, dim)
-        rows = q.shape[0]
-        if out.shape[0] != rows:
+        rows, q_row, q_head = _strides3(q, "q", heads, dim)
+        out_rows, out_row, out_head = _strides3(out, "out", heads, dim)
+        if out_rows != rows:
             raise ValueError("q and out must have the same number of rows")
-        if lse is not None and (tuple(lse.shape) != (rows, heads) or not lse.is_contiguous()
-                                or lse.dtype is not _torch().float32):
+        if lse is None:
+            lse_at = 0
+        elif lse.shape != (rows, heads) or not lse.is_contiguous() \
+                or lse.dtype is not _torch().float32:
             raise ValueError("lse must be a contiguous float32 [rows][heads] tensor")
-        ws, wb = (None, 0) if workspace is None else \
+        else:
+            lse_at = lse.data_ptr()
+        ws, wb = (0, 0) if workspace is None else \
             (workspace.data_ptr(), workspace.numel() * workspace.element_size())
-        return KvAttendDesc(_KV_ATTEND_SIZE, ABI_VERSION, self.handle,
-                            self._seqs(lengths, tables, rows, starts), q.data_ptr(), *qs,
-                            out.data_ptr(), *os, _ptr(lse), heads, window,
-                            dim ** -0.5 if scale is None else scale,
-                            KV_ATTEND_ACCUMULATE if accumulate else 0, _stream(stream), ws, wb)
+        return (self.handle or 0, *self._seqs(lengths, tables, rows, starts), q.data_ptr(), q_row,
+                q_head, out.data_ptr(), out_row, out_head, lse_at, heads, window,
+                dim ** -0.5 if scale is None else scale,
+                KV_ATTEND_ACCUMULATE if accumulate else 0, _stream(stream) or 0, ws, wb)
 
     def attend(self, q, lengths, tables, starts=None, out=None, lse=None, scale=None, window=0,
                accumulate=False, stream=None, workspace=None):
@@ -832,25 +871,21 @@ class KvCache:
         ``accumulate`` adds to the weights of the tokens.  A query that sees
         no token gives zeros."""
         if out is None:
-            torch = _torch()
-            out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-        d = self._attend_desc(q, lengths, tables, starts, out, lse, scale, window, accumulate,
-                              stream, workspace)
-        s = _thread_sink()
-        st = lib().ullm_kv_cache_attend(ctypes.byref(d), s.ref)
-        if st:
-            raise HipError(st, s.text())
+            out = _torch().empty_like(q)
+        _call(lib().ullm_kv_cache_attend, _packed(KvAttendDesc).fill(*self._attend_fields(
+            q, lengths, tables, starts, out, lse, scale, window, accumulate, stream, workspace)))
         return out
 
     def attend_plan(self, q, lengths, tables, starts=None, out=None, lse=None, scale=None,
                     window=0, accumulate=False, stream=None, workspace=None) -> KvAttendPlan:
         """The launch and the workspace of attend() with these arguments
         (ullm_kv_cache_attend_plan); launches nothing."""
-        d = self._attend_desc(q, lengths, tables, starts, q if out is None else out, lse, scale,
-                              window, accumulate, stream, workspace)
+        ref = _packed(KvAttendDesc).fill(*self._attend_fields(
+            q, lengths, tables, starts, q if out is None else out, lse, scale, window, accumulate,
+            stream, workspace))
         p = new(KvAttendPlan)
         s = _Sink()
-        _check(lib().ullm_kv_cache_attend_plan(ctypes.byref(d), ctypes.byref(p), s.ref), s)
+        _check(lib().ullm_kv_cache_attend_plan(ref, ctypes.byref(p), s.ref), s)
         return p
 
     def evict(self, lengths, tables, new_tables, keep, sink=0, recent=0, stream=None):
@@ -858,25 +893,20 @@ class KvCache:
         them its first ``sink`` and last ``recent``, into the blocks of
         ``new_tables``.  Returns (lengths int32 [batch], positions that stay
         int32 [batch][kv_heads][keep], ascending, then -1)."""
-        torch = _torch()
         batch = tables.shape[0]
         columns = -(-keep // self.block_tokens)
-        if new_tables.dtype is not torch.int32 or new_tables.dim() != 2 \
+        if new_tables.dtype is not _torch().int32 or new_tables.dim() != 2 \
                 or new_tables.shape[0] != batch or new_tables.shape[1] < columns \
                 or (columns > 1 and new_tables.stride(1) != 1) \
                 or (batch > 1 and new_tables.stride(0) < columns):
             raise ValueError(f"new_tables must be int32 [batch][{columns} or more]")
-        lens = torch.empty((batch,), dtype=torch.int32, device=tables.device)
-        kept = torch.empty((batch, self.kv_heads, max(keep, 0)), dtype=torch.int32,
-                           device=tables.device)
-        d = KvEvictDesc(ctypes.sizeof(KvEvictDesc), ABI_VERSION, self.handle,
-                        self._seqs(lengths, tables, 0, None), new_tables.data_ptr(),
-                        new_tables.stride(0) if batch > 1 else columns, lens.data_ptr(),
-                        kept.data_ptr(), keep, sink, recent, _stream(stream))
-        s = _thread_sink()
-        st = lib().ullm_kv_cache_evict(ctypes.byref(d), s.ref)
-        if st:
-            raise HipError(st, s.text())
+        seqs = self._seqs(lengths, tables, 0, None)
+        lens = tables.new_empty((batch,))
+        kept = tables.new_empty((batch, self.kv_heads, max(keep, 0)))
+        _call(lib().ullm_kv_cache_evict, _packed(KvEvictDesc).fill(
+            self.handle or 0, *seqs, new_tables.data_ptr(),
+            new_tables.stride(0) if batch > 1 else columns, lens.data_ptr(), kept.data_ptr(),
+            keep, sink, recent, _stream(stream) or 0))
         return lens, kept
 
 
