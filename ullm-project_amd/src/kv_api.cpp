@@ -7,6 +7,7 @@
 // their bounds.
 #include <hip/hip_runtime_api.h>
 
+#include <algorithm>
 #include <cmath>
 #include <mutex>
 #include <string>
@@ -213,7 +214,10 @@ ullm::KvAttendArgs attend_args(const ullm_kv_cache_attend_desc_t *d) {
   a.heads = d->heads;
   a.group = d->heads / c->kv_heads;
   a.window = d->window;
-  a.scale_log2 = float(double(d->scale) * 1.44269504088896340736);
+  // A scale of 0 becomes one that leaves every score at 0 but a token that is
+  // not seen at -infinity.
+  a.scale_log2 = std::max(std::fabs(float(double(d->scale) * 1.44269504088896340736)), 0x1p-120f);
+  a.q_sign = d->scale < 0.f ? 0x80008000u : 0u;
   a.accumulate = (d->flags & ULLM_KV_ATTEND_ACCUMULATE) != 0;
   return a;
 }

@@ -67,25 +67,28 @@ struct Query {
   bf16x8 q[D / 32];
 };
 
+// Eight elements of a query, negated if the scale is negative (so that scores
+// and products have one order and a maximum can be taken before scaling).
+__device__ __forceinline__ bf16x8 load_query8(const uint16_t *p, bool vec, uint32_t sign) {
+  u32x4 w;
+  if (vec) {
+    w = *reinterpret_cast<const u32x4 *>(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = p[2 * i] | uint32_t(p[2 * i + 1]) << 16;
+    }
+  }
+  return __builtin_bit_cast(bf16x8, u32x4{w.x ^ sign, w.y ^ sign, w.z ^ sign, w.w ^ sign});
+}
+
 template <int D>
-__device__ __forceinline__ Query<D> load_query(const uint16_t *row, bool vec, uint32_t g) {
+__device__ __forceinline__ Query<D> load_query(const uint16_t *row, bool vec, uint32_t sign,
+                                               uint32_t g) {
   Query<D> r;
 #pragma unroll
-  for (int c = 0; c < D / 64; ++c) {
-    const uint16_t *p = row + 64 * c + 16 * g;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (vec) {
-        r.q[2 * c + h] = reinterpret_cast<const bf16x8 *>(p)[h];
-      } else {
-        u32x4 w;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          w[i] = p[8 * h + 2 * i] | uint32_t(p[8 * h + 2 * i + 1]) << 16;
-        }
-        r.q[2 * c + h] = __builtin_bit_cast(bf16x8, w);
-      }
-    }
+  for (int c = 0; c < D / 32; ++c) {
+    r.q[c] = load_query8(row + 64 * (c / 2) + 16 * g + 8 * (c % 2), vec, sign);
   }
   return r;
 }
@@ -385,6 +388,19 @@ __device__ __forceinline__ uint32_t part_count(const Tile &t, uint32_t part_toke
   return t.end > from ? (t.end - from + part_tokens - 1) / part_tokens : 0u;
 }
 
+// Log-sum and statistics of a row.
+__device__ __forceinline__ void store_stats(const KvAttendArgs &a, const Scratch &x, uint64_t row,
+                                            uint32_t head, float top, float sum) {
+  const uint64_t at = row * a.heads + head;
+  if (a.lse != nullptr) {
+    a.lse[at] = sum == 0.f ? -INFINITY : (top + (log2f(sum) - float(kOff))) * kLn2;
+  }
+  if (x.stats != nullptr) {
+    x.stats[at] = RowStats{(top == -INFINITY ? 0.f : top) - float(kOff),
+                           sum == 0.f ? 0.f : 1.0f / sum};
+  }
+}
+
 // Final results of a row: `n` elements of the output from dim d0 on, log-sum
 // and statistics.
 template <int N>
@@ -411,13 +427,7 @@ __device__ __forceinline__ void store_row(const KvAttendArgs &a, const Scratch &
     }
   }
   if (d0 == 0) {
-    const uint64_t at = row * a.heads + head;
-    if (a.lse != nullptr) {
-      a.lse[at] = sum == 0.f ? -INFINITY : (top + (log2f(sum) - float(kOff))) * kLn2;
-    }
-    if (x.stats != nullptr) {
-      x.stats[at] = RowStats{(top == -INFINITY ? 0.f : top) - float(kOff), join};
-    }
+    store_stats(a, x, row, head, top, sum);
   }
 }
 
@@ -448,7 +458,7 @@ __global__ __launch_bounds__(W * kWave, 3) void few_rows_kernel(KvAttendArgs a, 
   // Three loads that wait for none: the query, the block numbers of the part
   // (with a window they depend on the length) and the length.  Lane i: block i
   // of the part, which spans at most 64.
-  const Query<D> q = load_query<D>(a.q + row * a.q_row + head * a.q_head, a.vec, g);
+  const Query<D> q = load_query<D>(a.q + row * a.q_row + head * a.q_head, a.vec, a.q_sign, g);
   const int32_t *table = a.seqs.tables + t.seq * a.seqs.stride;
   uint32_t block0 = part * x.part_tokens >> a.pool.shift;
   int32_t mine = a.window == 0 ? kv_block(table, a.seqs, a.pool.blocks, block0 + lane) : -1;
@@ -570,12 +580,396 @@ __global__ __launch_bounds__(W * kWave, 3) void few_rows_kernel(KvAttendArgs a, 
   }
 }
 
+// ------------------------------------------------------------- many rows
+//
+// 128 rows to a workgroup, 32 to a wave, in the same transposed form with
+// 32 x 32 x 16 products: each byte of a block serves 32 rows where the small
+// tiles serve 16, and a lane's column holds half of a row's scores.  Steps of
+// 64 tokens go through a ring of three stages in LDS, filled by copies that
+// no register waits for; every wave converts what it reads.
+//
+// Order of the operands (lane l, half h = l / 32, i = l % 32), all read with
+// 16 bytes to a lane, which 16 neighbours find in one row of banks:
+//   keys: row i of the product is token i with bits 3 and 4 exchanged, so that
+//     element e of a result is token {0, 16, 8, 24}[e / 4] + 4h + e % 4 and
+//     elements 8c .. 8c + 7 are the 8 tokens of pair 2c + h of a value tile;
+//   values: row i is dim 32 (i / 16) + i % 16 of 64 (first 8 bytes) or that
+//     plus 16 (last 8 bytes).
+constexpr uint32_t kManyRows = 128, kStep = 64, kStages = 3, kManyBlocks = 512;
+// A maximum may grow by this much before accumulators are scaled to it: the
+// weights then reach 2^(kOff + kSlack) = 2^15 in f16.
+constexpr float kSlack = 4.f;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16 mfma32_bf16(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32_f16(f16x8 a, f16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// 16 bytes per lane from memory into LDS at the wave's base.
+__device__ __forceinline__ void copy_to_lds(const uint8_t *from, uint8_t *to) {
+  __builtin_amdgcn_global_load_lds(
+      reinterpret_cast<const __attribute__((address_space(1))) void *>(
+          reinterpret_cast<uintptr_t>(from)),
+      (__attribute__((address_space(3))) void *)(to), 16, 0, 0);
+}
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  __builtin_amdgcn_s_waitcnt((N & 0xf) | ((N >> 4) << 14) | (0x7 << 4) | (0xf << 8));
+}
+// Workgroup barrier that waits for this wave's LDS reads only.
+__device__ __forceinline__ void step_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+template <int D>
+struct ManyState {
+  float m, l;
+  int acc_exp;
+  f32x16 o[D / 32];  // [2 pair + p]
+};
+
+// The values' 16 bytes of a lane for 64 dims and the tokens of pair 2c + h.
+__device__ __forceinline__ u32x4 value_unit(const uint8_t *values, uint32_t lane, uint32_t c,
+                                            uint32_t pair) {
+  const uint32_t i = lane % 32, h = lane / 32;
+  return *reinterpret_cast<const u32x4 *>(values + (2 * pair + i / 16) * 1024 +
+                                          (i % 16 + 16 * (2 * c + h)) * 16);
+}
+
+// O^T += V^T P^T for 32 tokens.
+template <int D>
+__device__ __forceinline__ void add_values(ManyState<D> &st, const uint8_t *values, uint32_t lane,
+                                           const u32x4 (&p)[2], float power) {
+#pragma unroll
+  for (uint32_t c = 0; c < 2; ++c) {
+#pragma unroll
+    for (uint32_t pair = 0; pair < D / 64; ++pair) {
+      const u32x4 w = value_unit(values, lane, c, pair);
+      f32x16 *acc = st.o + 2 * pair;
+      const f16x8 b = __builtin_bit_cast(f16x8, p[c]);
+      acc[0] = mfma32_f16(codes_to_f16(w.x, w.y, power), b, acc[0]);
+      acc[1] = mfma32_f16(codes_to_f16(w.z, w.w, power), b, acc[1]);
+    }
+  }
+}
+
+// A NaN value in a token that some rows do not see (confine_nan above): the
+// rows that see it become NaN, and `clean` receives the 32 tokens without it.
+template <int D>
+__device__ __forceinline__ void confine_values(ManyState<D> &st, const uint8_t *values,
+                                               uint8_t *clean, uint32_t lane, uint32_t seen) {
+  const auto one = [](uint32_t lo, uint32_t hi) {
+    return (lo ? 0x3c00u : 0u) | (hi ? 0x3c000000u : 0u);
+  };
+#pragma unroll
+  for (uint32_t c = 0; c < 2; ++c) {
+    u32x4 sv;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+      const uint32_t two = seen >> (8 * c + 2 * j);
+      sv[j] = one(two & 1u, two & 2u);
+    }
+#pragma unroll
+    for (uint32_t pair = 0; pair < D / 64; ++pair) {
+      const u32x4 w = value_unit(values, lane, c, pair);
+#pragma unroll
+      for (uint32_t k = 0; k < 2; ++k) {
+        const uint32_t b0 = nan_bytes(w[2 * k]), b1 = nan_bytes(w[2 * k + 1]);
+        const u32x4 nv = {one(b0 & 0x80u, b0 & 0x8000u), one(b0 & 0x800000u, b0 >> 31),
+                          one(b1 & 0x80u, b1 & 0x8000u), one(b1 & 0x800000u, b1 >> 31)};
+        const f32x16 hit = mfma32_f16(__builtin_bit_cast(f16x8, nv),
+                                      __builtin_bit_cast(f16x8, sv), f32x16{});
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          f32x16 &acc = st.o[2 * pair + k];
+          acc[j] = hit[j] > 0.f ? __builtin_nanf("") : acc[j];
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (uint32_t c = 0; c < D / 32; ++c) {
+    u32x4 w = reinterpret_cast<const u32x4 *>(values)[c * 64 + lane];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t bad = nan_bytes(w[j]);
+      w[j] &= ~(bad | (bad - (bad >> 7)));
+    }
+    reinterpret_cast<u32x4 *>(clean)[c * 64 + lane] = w;
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(kWaves * kWave, 2) void many_rows_kernel(KvAttendArgs a, Scratch x,
+                                                                      uint32_t each_slots) {
+  constexpr uint32_t kGroup = 64 * D;  // bytes of 32 tokens: keys, then values
+  // Dynamic, so that its reads are not taken to depend on every copy under way
+  // (as those of a static array are).
+  extern __shared__ __align__(1024) uint8_t many_ring[];
+  const auto ring = [](uint32_t stage) { return many_ring + stage * 2 * kGroup; };
+  __shared__ __align__(16) uint8_t clean[kWaves][32 * D];
+  __shared__ int32_t ids[kManyBlocks];
+  __shared__ uint16_t exps[kManyBlocks];
+  const uint32_t kvh = blockIdx.x % a.pool.heads;
+  const uint32_t rest = blockIdx.x / a.pool.heads, slots = gridDim.x / a.pool.heads / x.parts;
+  const uint32_t part = rest % x.parts;
+  Tile t;
+  // The last tiles see the most tokens: they start first.
+  if (!tile_rows(a, slots - 1 - rest / x.parts, kManyRows, each_slots, &t)) {
+    return;
+  }
+  tile_tokens(a, kv_length(a.seqs, a.pool.shift, t.seq), &t);
+  const uint32_t parts = part_count(t, x.part_tokens);
+  if (part != 0 && part >= parts) {
+    return;
+  }
+  const uint32_t lane = threadIdx.x % kWave;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const uint32_t h = lane / 32, i = lane % 32;
+  // The wave's rows; rows past the end see what the last one does.
+  const uint32_t last = t.live - 1;
+  const uint32_t w0 = min(32 * wave, last), w1 = min(32 * wave + 31, last);
+  const uint32_t r = t.r0 + min(32 * wave + i, last);
+  const uint32_t head = kvh * a.group + r % a.group;
+  const uint64_t row = t.first_row + r / a.group;
+  const int32_t pos = int32_t(t.origin + r / a.group), oldest = oldest_hidden(pos, a.window);
+  const int32_t low = int32_t(t.origin + (t.r0 + w0) / a.group);
+  const int32_t high = int32_t(t.origin + (t.r0 + w1) / a.group);
+  const int32_t hidden_low = oldest_hidden(low, a.window);
+  const int32_t hidden_high = oldest_hidden(high, a.window);
+  bf16x8 q[D / 16];
+#pragma unroll
+  for (int c = 0; c < D / 16; ++c) {
+    q[c] = load_query8(a.q + row * a.q_row + head * a.q_head + 16 * (2 * (c / 2) + h) + 8 * (c % 2),
+                       a.vec, a.q_sign);
+  }
+  const uint32_t from = t.begin / 32 + part * (x.part_tokens / 32);
+  const uint32_t all = (t.end + 31) / 32;
+  const uint32_t to = min(all, from + x.part_tokens / 32);
+  const uint32_t block0 = from * 32 >> a.pool.shift;
+  const uint32_t blocks = to > from ? ((to * 32 - 1) >> a.pool.shift) - block0 + 1 : 0;
+  const int32_t *table = a.seqs.tables + t.seq * a.seqs.stride;
+  for (uint32_t b = threadIdx.x; b < blocks; b += kWaves * kWave) {
+    const int32_t id = kv_block(table, a.seqs, a.pool.blocks, block0 + b);
+    const uint64_t unit = uint64_t(id < 0 ? 0 : id) * a.pool.heads + kvh;
+    ids[b] = id;
+    exps[b] = *reinterpret_cast<const uint16_t *>(a.pool.exps + unit * 2);
+  }
+  ManyState<D> st;
+  st.m = -INFINITY;
+  st.l = 0.f;
+  st.acc_exp = kKvExpMin;
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+    st.o[c] = f32x16{};
+  }
+  __syncthreads();
+
+  // Groups 2 step and 2 step + 1; one past the end is the last one again and
+  // counts as absent.
+  const uint32_t in_mask = (1u << a.pool.shift) - 1;
+  const auto block_of = [&](uint32_t grp) { return (grp * 32 >> a.pool.shift) - block0; };
+  const auto copy_step = [&](uint32_t grp0, uint8_t *stage) {
+#pragma unroll
+    for (uint32_t s = 0; s < 2; ++s) {
+      const uint32_t grp = min(grp0 + s, to - 1);
+      const int32_t id = __builtin_amdgcn_readfirstlane(ids[block_of(grp)]);
+      const uint8_t *unit = a.pool.codes + (uint64_t(id < 0 ? 0 : id) * a.pool.heads + kvh) *
+                                               (uint64_t(2 * D) << a.pool.shift);
+      const uint8_t *keys = unit + (grp * 32 & in_mask) * D;
+      const uint8_t *values = keys + (uint64_t(D) << a.pool.shift);
+      uint8_t *to_lds = stage + s * kGroup;
+      if (D == 128) {
+        copy_to_lds(keys + wave * 1024 + lane * 16, to_lds + wave * 1024);
+        copy_to_lds(values + wave * 1024 + lane * 16, to_lds + 32 * D + wave * 1024);
+      } else {
+        copy_to_lds((wave < 2 ? keys : values) + wave % 2 * 1024 + lane * 16,
+                    to_lds + wave * 1024);
+      }
+    }
+  };
+  const uint32_t steps = to > from ? (to - from + 1) / 2 : 0;
+  if (steps != 0) {
+    copy_step(from, ring(0));
+    copy_step(from + 2, ring(1));
+  }
+  // Lane's place in a key tile pair: token i with bits 3 and 4 exchanged.
+  const uint32_t tok = (i & 7) | (i & 8) << 1 | (i & 16) >> 1;
+  const uint32_t key_at = tok / 16 * (D / 64) * 1024 + tok % 16 * 16 + h * 256;
+  uint32_t rd = 0;
+  for (uint32_t step = 0; step < steps; ++step) {
+    wait_copies<D / 32>();  // this step's; the next one's stay under way
+    step_barrier();
+    copy_step(from + 2 * step + 4, ring(rd == 0 ? kStages - 1 : rd - 1));
+    const uint8_t *stage = ring(rd);
+    rd = rd + 1 == kStages ? 0 : rd + 1;
+    const uint32_t grp0 = from + 2 * step;
+    const int32_t t0 = int32_t(grp0 * 32);
+    if (t0 > high || t0 + 63 <= hidden_low) {
+      continue;  // none of the wave's rows sees it
+    }
+    int shift[2];
+    float power[2];
+    f32x16 s[2];
+    bool edge = t0 + 63 > low || t0 <= hidden_high;
+    bool present[2];
+#pragma unroll
+    for (uint32_t u = 0; u < 2; ++u) {
+      const uint32_t b = block_of(min(grp0 + u, to - 1));
+      present[u] = grp0 + u < to && __builtin_amdgcn_readfirstlane(ids[b]) >= 0;
+      edge = edge || !present[u];
+      const int e = __builtin_amdgcn_readfirstlane(exps[b]);
+      const float pk = exp2_int(int8_t(e));
+      const int ev = int8_t(e >> 8);
+      if (ev > st.acc_exp + kUp && present[u]) {
+        const float f = exp2_int(max(st.acc_exp - ev, -126));
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          st.o[c] *= f;
+        }
+        st.acc_exp = ev;
+      }
+      shift[u] = ev;
+      s[u] = f32x16{};
+      const uint8_t *keys = stage + u * kGroup + key_at;
+#pragma unroll
+      for (uint32_t c = 0; c < D / 32; ++c) {
+        const u32x4 w =
+            *reinterpret_cast<const u32x4 *>(keys + c / 2 * 1024 + c % 2 * 512);
+        s[u] = mfma32_bf16(codes_to_bf16(w.x, w.y, pk), q[2 * c], s[u]);
+        s[u] = mfma32_bf16(codes_to_bf16(w.z, w.w, pk), q[2 * c + 1], s[u]);
+      }
+    }
+    // Both exponents of the step are known to the accumulators now.
+#pragma unroll
+    for (uint32_t u = 0; u < 2; ++u) {
+      const int d = shift[u] - st.acc_exp;
+      power[u] = exp2_int(d < kDown ? kDown : d > kUp ? kUp : d);
+      shift[u] = d < kDown ? max(d - kDown, -100) : 0;
+    }
+    uint32_t seen[2] = {0xffffu, 0xffffu};
+    bool dirty = false;
+    if (edge) {
+      uint32_t any = 0;
+#pragma unroll
+      for (uint32_t u = 0; u < 2; ++u) {
+        seen[u] = 0;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int32_t at = t0 + int32_t(32 * u + (e / 4 % 2) * 16 + e / 8 * 8 + 4 * h + e % 4);
+          const bool see = present[u] && at <= pos && at > oldest;
+          seen[u] |= see ? 1u << e : 0u;
+          s[u][e] = see ? s[u][e] : -INFINITY;
+        }
+#pragma unroll
+        for (uint32_t c = 0; c < D / 32; ++c) {
+          const u32x4 w = reinterpret_cast<const u32x4 *>(stage + u * kGroup + 32 * D)[c * 64 + lane];
+          any |= nan_bytes(w.x) | nan_bytes(w.y) | nan_bytes(w.z) | nan_bytes(w.w);
+        }
+      }
+      dirty = __any(any);
+    }
+    float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int e = 1; e < 16; ++e) {
+      top = fmaxf(fmaxf(top, s[0][e]), s[1][e]);
+    }
+    const auto both = __builtin_amdgcn_permlane32_swap(f32_bits(top), f32_bits(top), false, false);
+    top = fmaxf(bits_f32(both[0]), bits_f32(both[1])) * a.scale_log2;
+    if (__any(top > st.m + kSlack)) {
+      const float now = fmaxf(st.m, top);
+      const float keep = now == -INFINITY ? 1.f : exp2_fast(st.m - now);
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        st.o[c] *= keep;
+      }
+      st.l *= keep;
+      st.m = now;
+    }
+    const float ref = st.m == -INFINITY ? 0.f : st.m;
+    u32x4 p[2][2];
+#pragma unroll
+    for (uint32_t u = 0; u < 2; ++u) {
+      const float bias = float(kOff + shift[u]) - ref;
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float p0 = exp2_fast(__builtin_fmaf(s[u][e], a.scale_log2, bias));
+        const float p1 = exp2_fast(__builtin_fmaf(s[u][e + 1], a.scale_log2, bias));
+        sum += p0;
+        sum += p1;
+        p[u][e / 8][e % 8 / 2] = f32x2_to_f16x2(p0, p1);
+      }
+      st.l += sum * exp2_int(-shift[u]);
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < 2; ++u) {
+      const uint8_t *values = stage + u * kGroup + 32 * D;
+      if (dirty) {
+        confine_values(st, values, clean[wave], lane, seen[u]);
+        values = clean[wave];
+      }
+      add_values(st, values, lane, p[u], power[u]);
+    }
+  }
+  wait_copies<0>();  // none may land after the workgroup has gone
+
+  const auto half = __builtin_amdgcn_permlane32_swap(f32_bits(st.l), f32_bits(st.l), false, false);
+  const float sum = bits_f32(half[0]) + bits_f32(half[1]);
+  if (32 * wave + i > last) {
+    return;
+  }
+  const float join = sum == 0.f ? 0.f : 1.0f / sum, power = exp2_int(st.acc_exp);
+  const uint64_t slot = (row * a.heads + head) * x.parts + part;
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t d0 = 64 * (c / 2) + 32 * (e / 2) + 16 * (c % 2) + 8 * (e % 2) + 4 * h;
+      f32x4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[j] = st.o[c][4 * e + j] * join * power;
+      }
+      if (parts > 1) {
+        *reinterpret_cast<f32x4 *>(x.part_o + slot * D + d0) = v;
+      } else {
+        uint16_t *to_out = a.out + row * a.out_row + head * a.out_head + d0;
+        const u32x2 w = {f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
+        if (a.out_vec) {
+          *reinterpret_cast<u32x2 *>(to_out) = w;
+        } else {
+          to_out[0] = uint16_t(w.x);
+          to_out[1] = uint16_t(w.x >> 16);
+          to_out[2] = uint16_t(w.y);
+          to_out[3] = uint16_t(w.y >> 16);
+        }
+      }
+    }
+  }
+  if (h == 0) {
+    if (parts > 1) {
+      x.part_s[slot] = PartSum{st.m, sum};
+    } else {
+      store_stats(a, x, row, head, st.m, sum);
+    }
+  }
+}
+
 // Joins the parts of a row: one workgroup of J waves, which take the parts in
 // turn, kJoinAhead of them under way at once (the sums of a part are small:
 // the time goes into waiting for them).
 constexpr uint32_t kJoinAhead = 4;
 template <int D, uint32_t J>
 __global__ __launch_bounds__(J * kWave) void join_parts_kernel(KvAttendArgs a, Scratch x,
+                                                               uint32_t tile,
                                                                uint32_t rows_of_tile,
                                                                uint32_t each_slots) {
   __shared__ float part_o[J][D];
@@ -583,7 +977,7 @@ __global__ __launch_bounds__(J * kWave) void join_parts_kernel(KvAttendArgs a, S
   constexpr int kPer = D / kWave;
   Tile t;
   const uint32_t index = blockIdx.x / rows_of_tile;
-  if (!tile_rows(a, index / a.pool.heads, kRows, each_slots, &t) ||
+  if (!tile_rows(a, index / a.pool.heads, tile, each_slots, &t) ||
       blockIdx.x % rows_of_tile >= t.live) {
     return;
   }
@@ -743,7 +1137,7 @@ __global__ __launch_bounds__(kWaves * kWave) void add_weights_kernel(KvAttendArg
     const uint64_t row = rows.first + (live ? r / a.group : 0u);
     const int64_t pos = origin + r / a.group;
     const int64_t oldest = a.window != 0 ? pos - int64_t(a.window) : -1;
-    const Query<D> q = load_query<D>(a.q + row * a.q_row + head * a.q_head, a.vec, g);
+    const Query<D> q = load_query<D>(a.q + row * a.q_row + head * a.q_head, a.vec, a.q_sign, g);
     const RowStats st = stats[row * a.heads + head];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -815,29 +1209,35 @@ static uint64_t each_tiles(const KvAttendArgs &a, uint32_t rows) {
 // heads: whole 5.7 us, in two parts 7.8) and at most 64 blocks, what a wave
 // looks up with one load.
 constexpr uint32_t kPartLeast = 512;
+// Rows of a sequence and key/value head, on average, up to which small tiles
+// serve.
+constexpr uint32_t kFewMost = 48;
 
 KvAttendPlan plan_kv_attend(const KvAttendArgs &a, uint32_t dim) {
   KvAttendPlan p;
   if (a.seqs.rows == 0 || a.seqs.batch == 0) {
     return p;
   }
-  p.kernel = ULLM_KV_KERNEL_FEW_ROWS;
-  p.row_tile = kRows;
-  const uint64_t tiles = kv_slots(a.seqs, a.group, kRows, 1, each_tiles(a, kRows)) * a.pool.heads;
+  const uint64_t rows_of_head = uint64_t(a.seqs.rows) * a.group;
+  const bool many = rows_of_head > uint64_t(kFewMost) * a.seqs.batch;
+  p.kernel = many ? ULLM_KV_KERNEL_MANY_ROWS : ULLM_KV_KERNEL_FEW_ROWS;
+  p.row_tile = many ? kManyRows : kRows;
+  const uint64_t tiles =
+      kv_slots(a.seqs, a.group, p.row_tile, 1, each_tiles(a, p.row_tile)) * a.pool.heads;
   // The most tokens that a tile's rows see, from the start of a 32-token group.
   uint64_t span = uint64_t(a.seqs.max_blocks) << a.pool.shift;
   if (a.window != 0) {
-    span = std::min<uint64_t>(span, uint64_t(a.window) + kRows / a.group + 32);
+    span = std::min<uint64_t>(span, uint64_t(a.window) + p.row_tile / a.group + 32);
   }
   const uint32_t cus = device_cu_count();
-  const uint64_t split = std::max<uint64_t>(cus / tiles, 1);
+  const uint64_t split = std::max<uint64_t>((many ? 2 : 1) * cus / tiles, 1);
   const uint64_t part = std::max<uint64_t>((span + split - 1) / split, kPartLeast);
-  p.part_tokens = uint32_t(std::min<uint64_t>((part + 31) / 32 * 32, 64u << a.pool.shift));
+  p.part_tokens = uint32_t(std::min<uint64_t>((part + kStep - 1) / kStep * kStep,
+                                              (many ? kManyBlocks : 64u) << a.pool.shift));
   p.parts = uint32_t((span + p.part_tokens - 1) / p.part_tokens);
   // Scores cost 8 bytes for each row and token, a second pass over the keys
   // `dim` bytes for each token.
-  const uint64_t rows_of_head = uint64_t(a.seqs.rows) * a.group;
-  p.keep_scores = a.accumulate && rows_of_head <= uint64_t(dim) / 8 * a.seqs.batch;
+  p.keep_scores = a.accumulate && !many && rows_of_head <= uint64_t(dim) / 8 * a.seqs.batch;
   p.one_tile = rows_of_head <= uint64_t(kRows) * a.seqs.batch;
   p.grid = tiles * p.parts;
   // Eight waves shorten the walk of a lone workgroup (333 tokens: 5.7 against
@@ -852,7 +1252,7 @@ static hipError_t launch_attend(const KvAttendArgs &a, const KvAttendPlan &p, vo
                                 hipStream_t s) {
   uint64_t bytes = 0;
   const Scratch x = scratch_of(a, D, p, workspace, &bytes);
-  const uint32_t each = uint32_t(each_tiles(a, kRows));
+  const uint32_t each = uint32_t(each_tiles(a, p.row_tile));
   const auto few = [&](auto kernel8, auto kernel4) {
     if (p.waves == 8) {
       kernel8<<<uint32_t(p.grid), 8 * kWave, 0, s>>>(a, x, each);
@@ -860,7 +1260,14 @@ static hipError_t launch_attend(const KvAttendArgs &a, const KvAttendPlan &p, vo
       kernel4<<<uint32_t(p.grid), 4 * kWave, 0, s>>>(a, x, each);
     }
   };
-  if (x.scores != nullptr) {
+  if (p.kernel == ULLM_KV_KERNEL_MANY_ROWS) {
+    constexpr uint32_t lds = kStages * 2 * 64 * D;
+    const hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(many_rows_kernel<D>), lds);
+    if (e != hipSuccess) {
+      return e;
+    }
+    many_rows_kernel<D><<<uint32_t(p.grid), kWaves * kWave, lds, s>>>(a, x, each);
+  } else if (x.scores != nullptr) {
     few(few_rows_kernel<D, 8, true, true>, few_rows_kernel<D, 4, true, true>);
   } else if (p.one_tile) {
     few(few_rows_kernel<D, 8, true, false>, few_rows_kernel<D, 4, true, false>);
@@ -869,12 +1276,12 @@ static hipError_t launch_attend(const KvAttendArgs &a, const KvAttendPlan &p, vo
   }
   if (p.parts > 1) {
     const uint32_t rows =
-        a.seqs.starts == nullptr ? std::min(a.seqs.each * a.group, kRows) : kRows;
+        a.seqs.starts == nullptr ? std::min(a.seqs.each * a.group, p.row_tile) : p.row_tile;
     const uint32_t grid = uint32_t(p.grid / p.parts) * rows;
     if (p.parts > 2 * kJoinAhead) {
-      join_parts_kernel<D, 8><<<grid, 8 * kWave, 0, s>>>(a, x, rows, each);
+      join_parts_kernel<D, 8><<<grid, 8 * kWave, 0, s>>>(a, x, p.row_tile, rows, each);
     } else {
-      join_parts_kernel<D, 1><<<grid, kWave, 0, s>>>(a, x, rows, each);
+      join_parts_kernel<D, 1><<<grid, kWave, 0, s>>>(a, x, p.row_tile, rows, each);
     }
   }
   if (a.accumulate) {

@@ -90,7 +90,8 @@ struct KvAttendArgs {
   float *lse;    // [rows][heads] or null
   uint32_t heads, group;
   uint32_t window;
-  float scale_log2;  // scale * log2(e)
+  float scale_log2;  // |scale| * log2(e), not 0
+  uint32_t q_sign;   // 0x80008000 if the scale is negative: two queries' signs
   bool accumulate;
 };
 struct KvAttendPlan {
