@@ -1088,82 +1088,182 @@ __global__ __launch_bounds__(256) void add_scores_kernel(KvAttendArgs a, Scratch
   unsafeAtomicAdd(&a.pool.weights[(unit << a.pool.shift) + (t & ((1u << a.pool.shift) - 1))], sum);
 }
 
-// Adds the weights that the tokens of a 32-token group receive from all rows
-// of their sequence: a wave owns the group, so its sums have a fixed order;
-// the addition is atomic for blocks that several sequences of a call share.
+// Adds the weights that tokens receive from all rows of their sequence, by a
+// second product of keys and queries: a wave owns 32 tokens, whose keys it
+// holds as operands, and the rows pass by in tiles of 64 that the workgroup
+// stages in LDS (chunk k of row r at place k ^ r, so that 8 neighbours read 8
+// groups of banks), the next tile on its way in registers meanwhile.  Each token's sum has a fixed order; the addition is
+// atomic for blocks that several sequences of a call share.
+constexpr uint32_t kWeightTokens = 32 * kWaves, kWeightRows = 64;
+
 template <int D>
 __global__ __launch_bounds__(kWaves * kWave) void add_weights_kernel(KvAttendArgs a,
-                                                                    const RowStats *stats) {
+                                                                     const RowStats *stats) {
+  constexpr uint32_t kChunks = D / 8;                          // 16-byte chunks of a row
+  constexpr uint32_t kMine = kWeightRows * kChunks / (kWaves * kWave);  // per thread
+  __shared__ __align__(16) uint8_t rows_lds[2][kWeightRows * D * 2];
+  __shared__ RowStats stats_lds[2][kWeightRows];
   const uint32_t kvh = blockIdx.y, b = blockIdx.z;
-  const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const uint32_t g = lane / 16, col = lane % 16;
-  const uint32_t t0 = (blockIdx.x * kWaves + wave) * 32;
+  const uint32_t lane = threadIdx.x % kWave;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const uint32_t h = lane / 32, i = lane % 32;
+  const uint32_t first = blockIdx.x * kWeightTokens;
   const uint32_t length = kv_length(a.seqs, a.pool.shift, b);
-  if (t0 >= length) {
-    return;
-  }
-  const int32_t id = kv_block(a.seqs.tables + b * a.seqs.stride, a.seqs, a.pool.blocks,
-                              t0 >> a.pool.shift);
-  if (id < 0) {
+  if (first >= length) {
     return;
   }
   const KvRows rows = kv_rows(a.seqs, b);
-  const uint64_t unit = uint64_t(id) * a.pool.heads + kvh;
-  const uint8_t *keys = a.pool.codes + unit * (uint64_t(2 * D) << a.pool.shift);
-  const uint32_t in_block = t0 & ((1u << a.pool.shift) - 1);
-  const float power = exp2_int(a.pool.exps[unit * 2]);
-  Keys<D> k[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    k[i] = load_keys<D, false>(keys, in_block / 16 + i, lane);
-  }
   const int64_t origin = int64_t(length) - rows.count;
   const uint32_t all = rows.count * a.group;
-  // Queries before the group's first token, or past its last one's window,
-  // see none of it.
-  const int64_t from = int64_t(t0) - origin;
-  uint32_t r0 = from <= 0 ? 0u
-                : from < int64_t(rows.count) ? uint32_t(from) * a.group / kRows * kRows
-                                             : all;
-  const int64_t past = a.window != 0 ? int64_t(t0) + 31 + a.window - origin : rows.count;
-  const uint32_t r1 = past <= 0 ? 0u
-                      : past < int64_t(rows.count) ? uint32_t(past) * a.group
-                                                   : all;
-  float sum[8] = {};
-  for (; r0 < r1; r0 += kRows) {
-    const uint32_t r = r0 + col;
-    const bool live = r < all;
-    const uint32_t head = kvh * a.group + (live ? r % a.group : 0u);
-    const uint64_t row = rows.first + (live ? r / a.group : 0u);
-    const int64_t pos = origin + r / a.group;
-    const int64_t oldest = a.window != 0 ? pos - int64_t(a.window) : -1;
-    const Query<D> q = load_query<D>(a.q + row * a.q_row + head * a.q_head, a.vec, a.q_sign, g);
-    const RowStats st = stats[row * a.heads + head];
+  // Queries before the first token, or past the last one's window, see none.
+  const int64_t from = int64_t(first) - origin;
+  const uint32_t begin = from <= 0 ? 0u
+                         : from < int64_t(rows.count) ? uint32_t(from) * a.group / kWeightRows * kWeightRows
+                                                      : all;
+  const int64_t past = a.window != 0 ? int64_t(first) + kWeightTokens - 1 + a.window - origin
+                                     : int64_t(rows.count);
+  const uint32_t end = past <= 0 ? 0u
+                       : past < int64_t(rows.count) ? uint32_t(past) * a.group
+                                                    : all;
+
+  const uint32_t t0 = first + 32 * wave;
+  const int32_t id = t0 < length ? kv_block(a.seqs.tables + b * a.seqs.stride, a.seqs,
+                                            a.pool.blocks, t0 >> a.pool.shift)
+                                 : -1;
+  const uint64_t unit = uint64_t(id < 0 ? 0 : id) * a.pool.heads + kvh;
+  const uint32_t in_block = t0 & ((1u << a.pool.shift) - 1);
+  const uint8_t *keys =
+      a.pool.codes + unit * (uint64_t(2 * D) << a.pool.shift) + uint64_t(in_block) * D;
+  const float power = exp2_int(a.pool.exps[unit * 2]);
+  bf16x8 k[D / 16];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const f32x4 s = products(k[i], power, q) * a.scale_log2;
+  for (int c = 0; c < D / 32; ++c) {
+    const u32x4 w = *reinterpret_cast<const u32x4 *>(
+        keys + (i / 16 * (D / 64) + c / 2) * 1024 + (i % 16 + 16 * (c % 2 * 2 + h)) * 16);
+    k[2 * c] = codes_to_bf16(w.x, w.y, power);
+    k[2 * c + 1] = codes_to_bf16(w.z, w.w, power);
+  }
+
+  // (query, head of the group) of a row, moved on by whole tiles without a
+  // division; rows past the end are the last one's.
+  struct RowAt {
+    uint32_t query, head;
+  };
+  const uint32_t tile_queries = kWeightRows / a.group,
+                 tile_heads = kWeightRows % a.group;
+  const auto row_at = [&](uint32_t r) { return RowAt{r / a.group, r % a.group}; };
+  const auto next_tile = [&](RowAt &r) {
+    r.head += tile_heads;
+    const bool carry = r.head >= a.group;
+    r.head -= carry ? a.group : 0u;
+    r.query += tile_queries + (carry ? 1u : 0u);
+  };
+  const auto clamped = [&](const RowAt &r) {
+    return r.query < rows.count ? r : RowAt{rows.count - 1, a.group - 1};
+  };
+  u32x4 held[kMine];
+  RowStats held_stats{0.f, 0.f};
+  RowAt mine[kMine], mine_stats = row_at(begin + threadIdx.x % kWeightRows), tile_at = row_at(begin);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t tok = int64_t(t0) + 16 * i + 4 * g + j;
-        const float p = exp2_fast(s[j] - st.top) * st.inv_sum;
-        sum[4 * i + j] += live && tok <= pos && tok > oldest ? p : 0.f;
+  for (uint32_t j = 0; j < kMine; ++j) {
+    mine[j] = row_at(begin + (threadIdx.x + j * kWaves * kWave) / kChunks);
+  }
+  const auto load_tile = [&]() {
+#pragma unroll
+    for (uint32_t j = 0; j < kMine; ++j) {
+      const RowAt r = clamped(mine[j]);
+      held[j] = __builtin_bit_cast(
+          u32x4, load_query8(a.q + uint64_t(rows.first + r.query) * a.q_row +
+                                 (kvh * a.group + r.head) * a.q_head +
+                                 threadIdx.x % kChunks * 8,
+                             a.vec, a.q_sign));
+      next_tile(mine[j]);
+    }
+    if (threadIdx.x < kWeightRows) {
+      const RowAt r = clamped(mine_stats);
+      held_stats = stats[uint64_t(rows.first + r.query) * a.heads + kvh * a.group + r.head];
+      next_tile(mine_stats);
+    }
+  };
+  const auto store_tile = [&](uint32_t stage) {
+#pragma unroll
+    for (uint32_t j = 0; j < kMine; ++j) {
+      const uint32_t at = threadIdx.x + j * kWaves * kWave;
+      const uint32_t r = at / kChunks, c = at % kChunks;
+      reinterpret_cast<u32x4 *>(rows_lds[stage])[r * kChunks + (c ^ r % kChunks)] = held[j];
+    }
+    if (threadIdx.x < kWeightRows) {
+      stats_lds[stage][threadIdx.x] = held_stats;
+    }
+  };
+  float sum[16] = {};
+  if (begin < end) {
+    load_tile();
+    store_tile(0);
+  }
+  __syncthreads();
+  uint32_t stage = 0;
+  for (uint32_t r0 = begin; r0 < end; r0 += kWeightRows, stage ^= 1) {
+    const bool more = r0 + kWeightRows < end;
+    if (more) {
+      load_tile();
+    }
+    const int32_t low = int32_t(origin + tile_at.query);
+    next_tile(tile_at);
+    const uint32_t last = min(r0 + kWeightRows - 1, all - 1);
+    // The tile's last query, or one that no row of it is past.
+    const int32_t high = int32_t(origin + min(tile_at.query, rows.count - 1));
+    if (id >= 0 && int32_t(t0) <= high) {
+      const bool edge = r0 + kWeightRows - 1 > last || int32_t(t0) + 31 > low ||
+                        int32_t(t0) <= oldest_hidden(high, a.window);
+      f32x16 s[2];
+#pragma unroll
+      for (uint32_t u = 0; u < 2; ++u) {
+        const u32x4 *tile =
+            reinterpret_cast<const u32x4 *>(rows_lds[stage]) + (32 * u + i) * kChunks;
+        s[u] = f32x16{};
+#pragma unroll
+        for (uint32_t c = 0; c < D / 16; ++c) {
+          const uint32_t chunk = 2 * (c / 2 * 2 + h) + c % 2;
+          s[u] = mfma32_bf16(k[c], __builtin_bit_cast(bf16x8, tile[chunk ^ i % kChunks]), s[u]);
+        }
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < 2; ++u) {
+        const RowStats st = stats_lds[stage][32 * u + i];
+        if (edge) {
+          const uint32_t r = r0 + 32 * u + i;
+          const int32_t pos = int32_t(origin + r / a.group);
+          const int32_t oldest = oldest_hidden(pos, a.window);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int32_t tok = int32_t(t0) + e / 4 * 8 + 4 * int32_t(h) + e % 4;
+            const float p = exp2_fast(__builtin_fmaf(s[u][e], a.scale_log2, -st.top)) * st.inv_sum;
+            sum[e] += r <= last && tok <= pos && tok > oldest ? p : 0.f;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            sum[e] = __builtin_fmaf(exp2_fast(__builtin_fmaf(s[u][e], a.scale_log2, -st.top)),
+                                    st.inv_sum, sum[e]);
+          }
+        }
       }
     }
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-#pragma unroll
-    for (int off = 1; off < 16; off <<= 1) {
-      sum[i] += __shfl_xor(sum[i], off, kWave);
+    if (more) {
+      store_tile(stage ^ 1);
     }
+    __syncthreads();
   }
-  if (col == 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t t = 16 * (i / 4) + 4 * g + i % 4;
-      if (t0 + t < length) {
-        unsafeAtomicAdd(&a.pool.weights[(unit << a.pool.shift) + in_block + t], sum[i]);
-      }
+  for (int e = 0; e < 16; ++e) {
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      sum[e] += __shfl_xor(sum[e], off, kWave);
+    }
+    const uint32_t t = e / 4 * 8 + 4 * h + e % 4;
+    if (i == uint32_t(e) && id >= 0 && t0 + t < length) {
+      unsafeAtomicAdd(&a.pool.weights[(unit << a.pool.shift) + in_block + t], sum[e]);
     }
   }
 }
@@ -1290,7 +1390,7 @@ static hipError_t launch_attend(const KvAttendArgs &a, const KvAttendPlan &p, vo
       add_scores_kernel<<<dim3(uint32_t((tokens + 255) / 256), a.pool.heads, a.seqs.batch), 256, 0,
                           s>>>(a, x);
     } else {
-      const dim3 grid(uint32_t((tokens + 32 * kWaves - 1) / (32 * kWaves)), a.pool.heads,
+      const dim3 grid(uint32_t((tokens + kWeightTokens - 1) / kWeightTokens), a.pool.heads,
                       a.seqs.batch);
       add_weights_kernel<D><<<grid, kWaves * kWave, 0, s>>>(a, x.stats);
     }
