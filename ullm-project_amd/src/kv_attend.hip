@@ -27,7 +27,6 @@
 // the accumulator's exponent: blocks of any exponents meet in one product with
 // an error below 2^-60 of the largest value.
 #include <algorithm>
-#include <cstdlib>
 
 #include "kernels.hpp"
 #include "kv_cache.hpp"
@@ -163,10 +162,9 @@ struct Tile {
   uint32_t begin, end;                     // tokens that some row sees
 };
 
-// The rows of tile `id`; false if it has none.
-__device__ __forceinline__ bool tile_rows(const KvAttendArgs &a, uint32_t id, uint32_t rows,
-                                          uint32_t each_slots, Tile *t) {
-  const KvSlot slot = kv_find_slot(a.seqs, id, a.group, rows, 1, each_slots);
+// The rows of a slot or of tile `id`; false if it has none.
+__device__ __forceinline__ bool slot_rows(const KvAttendArgs &a, const KvSlot &slot, uint32_t rows,
+                                          Tile *t) {
   const uint32_t all = slot.rows.count * a.group;
   t->seq = slot.seq;
   t->first_row = slot.rows.first;
@@ -174,6 +172,64 @@ __device__ __forceinline__ bool tile_rows(const KvAttendArgs &a, uint32_t id, ui
   t->r0 = slot.local * rows;
   t->live = all - t->r0 < rows ? all - t->r0 : rows;
   return slot.seq < a.seqs.batch && t->r0 < all;
+}
+__device__ __forceinline__ bool tile_rows(const KvAttendArgs &a, uint32_t id, uint32_t rows,
+                                          uint32_t each_slots, Tile *t) {
+  return slot_rows(a, kv_find_slot(a.seqs, id, a.group, rows, 1, each_slots), rows, t);
+}
+// The tiles of all sequences by their number in the sequence, highest first:
+// of prompts that see themselves the last tiles take longest, so they start
+// first (prompts of 4096 and 3001 tokens: @@ us; sequence by sequence 248).
+// Lane i looks at 64 numbers at once, one walk over the sequences for each
+// factor of 64 in the tiles; of more than 64 sequences none takes long, and
+// they are left in their order.  `slots`: ids in the grid.
+__device__ __forceinline__ bool tile_rows_last_first(const KvAttendArgs &a, uint32_t id,
+                                                     uint32_t slots, uint32_t rows,
+                                                     uint32_t each_slots, Tile *t) {
+  const uint32_t batch = a.seqs.batch;
+  if (a.seqs.starts == nullptr) {
+    const uint32_t b = id % batch;
+    return slot_rows(a, {b, each_slots - 1 - id / batch, {b * a.seqs.each, a.seqs.each}}, rows, t);
+  }
+  if (batch > kWave) {
+    return tile_rows(a, slots - 1 - id, rows, each_slots, t);
+  }
+  const uint32_t lane = threadIdx.x % kWave;
+  const KvRows mine = kv_rows(a.seqs, lane < batch ? lane : 0);
+  const uint32_t tiles =
+      lane < batch ? uint32_t((uint64_t(mine.count) * a.group + rows - 1) / rows) : 0u;
+  uint32_t step = 1;
+  while (__any(tiles > kWave * step)) {
+    step *= kWave;
+  }
+  // The lowest number that at most `id` tiles are above of lies in
+  // [number, number + 64 step): lane i looks at the end of its 64th of that.
+  uint32_t number = 0, above = 0;
+  for (; step != 0; step /= kWave) {
+    const uint32_t next = number + (lane + 1) * step;
+    uint32_t n = 0;
+    for (uint32_t b = 0; b < batch; ++b) {
+      const uint32_t of_b = uint32_t(__builtin_amdgcn_readlane(int(tiles), int(b)));
+      n += of_b > next ? of_b - next : 0u;
+    }
+    const uint32_t first = uint32_t(__builtin_ctzll(__ballot(n <= id)));
+    number += first * step;
+    above = uint32_t(__builtin_amdgcn_readlane(int(n), int(first)));
+  }
+  // Of the tiles of this number, the one of the (id - above)-th sequence.
+  const bool has = tiles > number;
+  const uint64_t with = __ballot(has);
+  const uint64_t mask = __ballot(
+      has && uint32_t(__popcll(with & ((uint64_t(1) << lane) - 1))) == id - above);
+  if (mask == 0) {
+    return false;
+  }
+  const uint32_t b = uint32_t(__builtin_ctzll(mask));
+  return slot_rows(a,
+                   {b, number,
+                    {uint32_t(__builtin_amdgcn_readlane(int(mine.first), int(b))),
+                     uint32_t(__builtin_amdgcn_readlane(int(mine.count), int(b)))}},
+                   rows, t);
 }
 // Their positions, from the sequence's length.
 __device__ __forceinline__ void tile_tokens(const KvAttendArgs &a, uint32_t length, Tile *t) {
@@ -585,7 +641,7 @@ __global__ __launch_bounds__(W * kWave, 3) void few_rows_kernel(KvAttendArgs a, 
 // 128 rows to a workgroup, 32 to a wave, in the same transposed form with
 // 32 x 32 x 16 products: each byte of a block serves 32 rows where the small
 // tiles serve 16, and a lane's column holds half of a row's scores.  Steps of
-// 64 tokens go through a ring of three stages in LDS, filled by copies that
+// 64 tokens go through a ring of two stages in LDS, filled by copies that
 // no register waits for; every wave converts what it reads.
 //
 // Order of the operands (lane l, half h = l / 32, i = l % 32), all read with
@@ -595,7 +651,7 @@ __global__ __launch_bounds__(W * kWave, 3) void few_rows_kernel(KvAttendArgs a, 
 //     elements 8c .. 8c + 7 are the 8 tokens of pair 2c + h of a value tile;
 //   values: row i is dim 32 (i / 16) + i % 16 of 64 (first 8 bytes) or that
 //     plus 16 (last 8 bytes).
-constexpr uint32_t kManyRows = 128, kStep = 64, kStages = 3, kManyBlocks = 512;
+constexpr uint32_t kManyRows = 128, kStep = 64, kStages = 2, kManyBlocks = 512;
 // A maximum may grow by this much before accumulators are scaled to it: the
 // weights then reach 2^(kOff + kSlack) = 2^15 in f16.
 constexpr float kSlack = 4.f;
@@ -631,9 +687,22 @@ __device__ __forceinline__ void step_barrier() {
 template <int D>
 struct ManyState {
   float m, l;
-  int acc_exp;
   f32x16 o[D / 32];  // [2 pair + p]
 };
+
+// A block of a workgroup's range, as LDS holds it: where its codes start, 2^e
+// of its keys, and the exponent of its values plus kExpCode; a block out of
+// the pool reads the first one's codes and has the bit kAbsent.
+struct BlockEntry {
+  uint64_t codes;
+  float power;
+  uint32_t exp_code;
+};
+constexpr uint32_t kExpCode = 256, kAbsent = 1u << 31;
+
+__device__ __forceinline__ uint32_t uniform(uint32_t v) {
+  return uint32_t(__builtin_amdgcn_readfirstlane(int(v)));
+}
 
 // The values' 16 bytes of a lane for 64 dims and the tokens of pair 2c + h.
 __device__ __forceinline__ u32x4 value_unit(const uint8_t *values, uint32_t lane, uint32_t c,
@@ -643,86 +712,75 @@ __device__ __forceinline__ u32x4 value_unit(const uint8_t *values, uint32_t lane
                                           (i % 16 + 16 * (2 * c + h)) * 16);
 }
 
-// O^T += V^T P^T for 32 tokens.
+// O^T += V^T P^T for 32 tokens.  The barriers keep later conversions out of the
+// registers that a third wave needs.
 template <int D>
-__device__ __forceinline__ void add_values(ManyState<D> &st, const uint8_t *values, uint32_t lane,
+__device__ __forceinline__ void add_values(ManyState<D> &st, const u32x4 (&v)[D / 32],
                                            const u32x4 (&p)[2], float power) {
 #pragma unroll
   for (uint32_t c = 0; c < 2; ++c) {
 #pragma unroll
     for (uint32_t pair = 0; pair < D / 64; ++pair) {
-      const u32x4 w = value_unit(values, lane, c, pair);
+      const u32x4 w = v[c * (D / 64) + pair];
       f32x16 *acc = st.o + 2 * pair;
       const f16x8 b = __builtin_bit_cast(f16x8, p[c]);
       acc[0] = mfma32_f16(codes_to_f16(w.x, w.y, power), b, acc[0]);
       acc[1] = mfma32_f16(codes_to_f16(w.z, w.w, power), b, acc[1]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 }
 
-// A NaN value in a token that some rows do not see (confine_nan above): the
-// rows that see it become NaN, and `clean` receives the 32 tokens without it.
-template <int D>
-__device__ __forceinline__ void confine_values(ManyState<D> &st, const uint8_t *values,
-                                               uint8_t *clean, uint32_t lane, uint32_t seen) {
-  const auto one = [](uint32_t lo, uint32_t hi) {
-    return (lo ? 0x3c00u : 0u) | (hi ? 0x3c000000u : 0u);
-  };
-#pragma unroll
-  for (uint32_t c = 0; c < 2; ++c) {
-    u32x4 sv;
-#pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) {
-      const uint32_t two = seen >> (8 * c + 2 * j);
-      sv[j] = one(two & 1u, two & 2u);
-    }
-#pragma unroll
-    for (uint32_t pair = 0; pair < D / 64; ++pair) {
-      const u32x4 w = value_unit(values, lane, c, pair);
-#pragma unroll
-      for (uint32_t k = 0; k < 2; ++k) {
-        const uint32_t b0 = nan_bytes(w[2 * k]), b1 = nan_bytes(w[2 * k + 1]);
-        const u32x4 nv = {one(b0 & 0x80u, b0 & 0x8000u), one(b0 & 0x800000u, b0 >> 31),
-                          one(b1 & 0x80u, b1 & 0x8000u), one(b1 & 0x800000u, b1 >> 31)};
-        const f32x16 hit = mfma32_f16(__builtin_bit_cast(f16x8, nv),
-                                      __builtin_bit_cast(f16x8, sv), f32x16{});
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          f32x16 &acc = st.o[2 * pair + k];
-          acc[j] = hit[j] > 0.f ? __builtin_nanf("") : acc[j];
-        }
-      }
-    }
+// Where a row's result goes: its part, or the output itself.
+struct RowSink {
+  uint64_t row;
+  uint32_t head;
+  bool live, whole;
+  uint64_t slot;
+};
+__device__ __forceinline__ void store4(const KvAttendArgs &a, const Scratch &x, const RowSink &to,
+                                       uint32_t dim, uint32_t d0, f32x4 v) {
+  if (!to.live) {
+    return;
   }
-#pragma unroll
-  for (uint32_t c = 0; c < D / 32; ++c) {
-    u32x4 w = reinterpret_cast<const u32x4 *>(values)[c * 64 + lane];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t bad = nan_bytes(w[j]);
-      w[j] &= ~(bad | (bad - (bad >> 7)));
-    }
-    reinterpret_cast<u32x4 *>(clean)[c * 64 + lane] = w;
+  if (!to.whole) {
+    *reinterpret_cast<f32x4 *>(x.part_o + to.slot * dim + d0) = v;
+    return;
+  }
+  uint16_t *p = a.out + to.row * a.out_row + to.head * a.out_head + d0;
+  const u32x2 w = {f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
+  if (a.out_vec) {
+    *reinterpret_cast<u32x2 *>(p) = w;
+  } else {
+    p[0] = uint16_t(w.x);
+    p[1] = uint16_t(w.x >> 16);
+    p[2] = uint16_t(w.y);
+    p[3] = uint16_t(w.y >> 16);
+  }
+}
+__device__ __forceinline__ void store_sums(const KvAttendArgs &a, const Scratch &x,
+                                           const RowSink &to, float top, float sum) {
+  if (to.live && to.whole) {
+    store_stats(a, x, to.row, to.head, top, sum);
+  } else if (to.live) {
+    x.part_s[to.slot] = PartSum{top, sum};
   }
 }
 
 template <int D>
-__global__ __launch_bounds__(kWaves * kWave, 2) void many_rows_kernel(KvAttendArgs a, Scratch x,
+__global__ __launch_bounds__(kWaves * kWave, 3) void many_rows_kernel(KvAttendArgs a, Scratch x,
                                                                       uint32_t each_slots) {
   constexpr uint32_t kGroup = 64 * D;  // bytes of 32 tokens: keys, then values
   // Dynamic, so that its reads are not taken to depend on every copy under way
   // (as those of a static array are).
   extern __shared__ __align__(1024) uint8_t many_ring[];
   const auto ring = [](uint32_t stage) { return many_ring + stage * 2 * kGroup; };
-  __shared__ __align__(16) uint8_t clean[kWaves][32 * D];
-  __shared__ int32_t ids[kManyBlocks];
-  __shared__ uint16_t exps[kManyBlocks];
+  __shared__ BlockEntry entries[kManyBlocks];
   const uint32_t kvh = blockIdx.x % a.pool.heads;
   const uint32_t rest = blockIdx.x / a.pool.heads, slots = gridDim.x / a.pool.heads / x.parts;
   const uint32_t part = rest % x.parts;
   Tile t;
-  // The last tiles see the most tokens: they start first.
-  if (!tile_rows(a, slots - 1 - rest / x.parts, kManyRows, each_slots, &t)) {
+  if (!tile_rows_last_first(a, rest / x.parts, slots, kManyRows, each_slots, &t)) {
     return;
   }
   tile_tokens(a, kv_length(a.seqs, a.pool.shift, t.seq), &t);
@@ -742,8 +800,6 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void many_rows_kernel(KvAttendAr
   const int32_t pos = int32_t(t.origin + r / a.group), oldest = oldest_hidden(pos, a.window);
   const int32_t low = int32_t(t.origin + (t.r0 + w0) / a.group);
   const int32_t high = int32_t(t.origin + (t.r0 + w1) / a.group);
-  const int32_t hidden_low = oldest_hidden(low, a.window);
-  const int32_t hidden_high = oldest_hidden(high, a.window);
   bf16x8 q[D / 16];
 #pragma unroll
   for (int c = 0; c < D / 16; ++c) {
@@ -759,206 +815,270 @@ __global__ __launch_bounds__(kWaves * kWave, 2) void many_rows_kernel(KvAttendAr
   for (uint32_t b = threadIdx.x; b < blocks; b += kWaves * kWave) {
     const int32_t id = kv_block(table, a.seqs, a.pool.blocks, block0 + b);
     const uint64_t unit = uint64_t(id < 0 ? 0 : id) * a.pool.heads + kvh;
-    ids[b] = id;
-    exps[b] = *reinterpret_cast<const uint16_t *>(a.pool.exps + unit * 2);
+    const int e = *reinterpret_cast<const uint16_t *>(a.pool.exps + unit * 2);
+    entries[b] = BlockEntry{
+        reinterpret_cast<uint64_t>(a.pool.codes) + unit * (uint64_t(2 * D) << a.pool.shift),
+        exp2_int(int8_t(e)), uint32_t(int8_t(e >> 8) + int(kExpCode)) | (id < 0 ? kAbsent : 0u)};
   }
   ManyState<D> st;
   st.m = -INFINITY;
   st.l = 0.f;
-  st.acc_exp = kKvExpMin;
 #pragma unroll
   for (int c = 0; c < D / 32; ++c) {
     st.o[c] = f32x16{};
   }
   __syncthreads();
 
-  // Groups 2 step and 2 step + 1; one past the end is the last one again and
-  // counts as absent.
+  // What a step needs of its two groups (one past the end is the last one
+  // again), looked up a step ahead.
+  struct Step {
+    float power[2];
+    uint32_t exp_code[2];
+  };
   const uint32_t in_mask = (1u << a.pool.shift) - 1;
-  const auto block_of = [&](uint32_t grp) { return (grp * 32 >> a.pool.shift) - block0; };
-  const auto copy_step = [&](uint32_t grp0, uint8_t *stage) {
+  const uint32_t copy_at = (D == 128 ? wave : wave % 2) * 1024 + lane * 16;
+  const auto start_step = [&](uint32_t grp0, uint8_t *stage) {
+    Step s;
 #pragma unroll
-    for (uint32_t s = 0; s < 2; ++s) {
-      const uint32_t grp = min(grp0 + s, to - 1);
-      const int32_t id = __builtin_amdgcn_readfirstlane(ids[block_of(grp)]);
-      const uint8_t *unit = a.pool.codes + (uint64_t(id < 0 ? 0 : id) * a.pool.heads + kvh) *
-                                               (uint64_t(2 * D) << a.pool.shift);
-      const uint8_t *keys = unit + (grp * 32 & in_mask) * D;
+    for (uint32_t u = 0; u < 2; ++u) {
+      const uint32_t tok = min(grp0 + u, to - 1) * 32;
+      const u32x4 e =
+          *reinterpret_cast<const u32x4 *>(&entries[(tok >> a.pool.shift) - block0]);
+      s.power[u] = bits_f32(uniform(e.z));
+      s.exp_code[u] = uniform(e.w);
+      const uint8_t *keys =
+          reinterpret_cast<const uint8_t *>(uint64_t(uniform(e.y)) << 32 | uniform(e.x)) +
+          (tok & in_mask) * D;
       const uint8_t *values = keys + (uint64_t(D) << a.pool.shift);
-      uint8_t *to_lds = stage + s * kGroup;
+      uint8_t *to_lds = stage + u * kGroup + wave * 1024;
       if (D == 128) {
-        copy_to_lds(keys + wave * 1024 + lane * 16, to_lds + wave * 1024);
-        copy_to_lds(values + wave * 1024 + lane * 16, to_lds + 32 * D + wave * 1024);
+        copy_to_lds(keys + copy_at, to_lds);
+        copy_to_lds(values + copy_at, to_lds + 32 * D);
       } else {
-        copy_to_lds((wave < 2 ? keys : values) + wave % 2 * 1024 + lane * 16,
-                    to_lds + wave * 1024);
+        copy_to_lds((wave < 2 ? keys : values) + copy_at, to_lds);
       }
     }
+    return s;
   };
+  // Groups that some of the wave's rows see, and of those the ones that every
+  // row sees whole: [first, first + count) each.
+  struct Range {
+    uint32_t first, count;
+  };
+  const auto range = [](int64_t first, int64_t end) {
+    return Range{uniform(uint32_t(first)), uniform(uint32_t(end > first ? end - first : 0))};
+  };
+  const Range some = range((int64_t(oldest_hidden(low, a.window)) + 1) / 32,
+                           high < 0 ? 0 : min(int64_t(high / 32 + 1), int64_t(to)));
+  const Range whole = range((int64_t(oldest_hidden(high, a.window)) + 1 + 31) / 32,
+                            low < 0 ? 0 : (int64_t(low) + 1) / 32);
   const uint32_t steps = to > from ? (to - from + 1) / 2 : 0;
+  Step next{};
   if (steps != 0) {
-    copy_step(from, ring(0));
-    copy_step(from + 2, ring(1));
+    next = start_step(from, ring(0));
   }
   // Lane's place in a key tile pair: token i with bits 3 and 4 exchanged.
   const uint32_t tok = (i & 7) | (i & 8) << 1 | (i & 16) >> 1;
   const uint32_t key_at = tok / 16 * (D / 64) * 1024 + tok % 16 * 16 + h * 256;
-  uint32_t rd = 0;
+  // The instructions of a group are what bounds this loop (a SIMD issues one
+  // in four cycles, whatever its kind): what changes rarely is kept ready and
+  // changed under a branch.  bias: kOff + shift - m, what a scaled score
+  // becomes a power of two with; limit: the unscaled score past which m grows;
+  // power, unshift: those of the last exponent code.
+  int acc_exp = kKvExpMin;
+  uint32_t code = ~0u;
+  float bias = 0.f, limit = -INFINITY, power = 1.f, unshift = 1.f;
+  int shift = 0;
+  const auto new_bias = [&] {
+    bias = float(kOff + shift) - (st.m == -INFINITY ? 0.f : st.m);
+  };
+  bool dirty = false;  // a NaN value in a group that some rows do not see
   for (uint32_t step = 0; step < steps; ++step) {
-    wait_copies<D / 32>();  // this step's; the next one's stay under way
+    wait_copies<0>();
     step_barrier();
-    copy_step(from + 2 * step + 4, ring(rd == 0 ? kStages - 1 : rd - 1));
-    const uint8_t *stage = ring(rd);
-    rd = rd + 1 == kStages ? 0 : rd + 1;
-    const uint32_t grp0 = from + 2 * step;
-    const int32_t t0 = int32_t(grp0 * 32);
-    if (t0 > high || t0 + 63 <= hidden_low) {
-      continue;  // none of the wave's rows sees it
+    const Step now = next;
+    const uint8_t *stage = ring(step % kStages);
+    if (step + 1 < steps) {
+      next = start_step(from + 2 * step + 2, ring((step + 1) % kStages));
     }
-    int shift[2];
-    float power[2];
-    f32x16 s[2];
-    bool edge = t0 + 63 > low || t0 <= hidden_high;
-    bool present[2];
 #pragma unroll
     for (uint32_t u = 0; u < 2; ++u) {
-      const uint32_t b = block_of(min(grp0 + u, to - 1));
-      present[u] = grp0 + u < to && __builtin_amdgcn_readfirstlane(ids[b]) >= 0;
-      edge = edge || !present[u];
-      const int e = __builtin_amdgcn_readfirstlane(exps[b]);
-      const float pk = exp2_int(int8_t(e));
-      const int ev = int8_t(e >> 8);
-      if (ev > st.acc_exp + kUp && present[u]) {
-        const float f = exp2_int(max(st.acc_exp - ev, -126));
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          st.o[c] *= f;
-        }
-        st.acc_exp = ev;
+      const uint32_t grp = from + 2 * step + u;
+      if (grp - some.first >= some.count) {
+        continue;
       }
-      shift[u] = ev;
-      s[u] = f32x16{};
-      const uint8_t *keys = stage + u * kGroup + key_at;
+      const uint8_t *keys = stage + u * kGroup + key_at, *values = stage + u * kGroup + 32 * D;
+      // All of a product's LDS reads are under way before its first use, those
+      // of the values during the softmax.
+      u32x4 units[D / 32];
 #pragma unroll
       for (uint32_t c = 0; c < D / 32; ++c) {
-        const u32x4 w =
-            *reinterpret_cast<const u32x4 *>(keys + c / 2 * 1024 + c % 2 * 512);
-        s[u] = mfma32_bf16(codes_to_bf16(w.x, w.y, pk), q[2 * c], s[u]);
-        s[u] = mfma32_bf16(codes_to_bf16(w.z, w.w, pk), q[2 * c + 1], s[u]);
+        units[c] = *reinterpret_cast<const u32x4 *>(keys + c / 2 * 1024 + c % 2 * 512);
       }
-    }
-    // Both exponents of the step are known to the accumulators now.
+      __builtin_amdgcn_sched_barrier(0);
+      f32x16 s = f32x16{};
 #pragma unroll
-    for (uint32_t u = 0; u < 2; ++u) {
-      const int d = shift[u] - st.acc_exp;
-      power[u] = exp2_int(d < kDown ? kDown : d > kUp ? kUp : d);
-      shift[u] = d < kDown ? max(d - kDown, -100) : 0;
-    }
-    uint32_t seen[2] = {0xffffu, 0xffffu};
-    bool dirty = false;
-    if (edge) {
-      uint32_t any = 0;
+      for (uint32_t c = 0; c < D / 32; ++c) {
+        const u32x4 w = units[c];
+        s = mfma32_bf16(codes_to_bf16(w.x, w.y, now.power[u]), q[2 * c], s);
+        s = mfma32_bf16(codes_to_bf16(w.z, w.w, now.power[u]), q[2 * c + 1], s);
+      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (uint32_t u = 0; u < 2; ++u) {
-        seen[u] = 0;
+      for (uint32_t c = 0; c < D / 32; ++c) {
+        units[c] = value_unit(values, lane, c / (D / 64), c % (D / 64));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (now.exp_code[u] != code) {
+        code = now.exp_code[u];
+        const int ev = int(code & 0xffffu) - int(kExpCode);
+        if (ev > acc_exp + kUp) {
+          const float f = exp2_int(max(acc_exp - ev, -126));
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            st.o[c] *= f;
+          }
+          acc_exp = ev;
+        }
+        const int d = ev - acc_exp;
+        power = exp2_int(d < kDown ? kDown : d);
+        shift = d < kDown ? max(d - kDown, -100) : 0;
+        unshift = exp2_int(-shift);
+        new_bias();
+      }
+      if (((grp - whole.first) | (code & kAbsent)) >= whole.count) {
+        const int32_t t0 = int32_t(grp * 32);
+        const bool present = (code & kAbsent) == 0;
+        uint32_t any = 0;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int32_t at = t0 + int32_t(32 * u + (e / 4 % 2) * 16 + e / 8 * 8 + 4 * h + e % 4);
-          const bool see = present[u] && at <= pos && at > oldest;
-          seen[u] |= see ? 1u << e : 0u;
-          s[u][e] = see ? s[u][e] : -INFINITY;
+          const int32_t at = t0 + int32_t((e / 4 % 2) * 16 + e / 8 * 8 + 4 * h + e % 4);
+          const bool see = present && at <= pos && at > oldest;
+          s[e] = see ? s[e] : -INFINITY;
         }
 #pragma unroll
         for (uint32_t c = 0; c < D / 32; ++c) {
-          const u32x4 w = reinterpret_cast<const u32x4 *>(stage + u * kGroup + 32 * D)[c * 64 + lane];
+          const u32x4 w = units[c];
           any |= nan_bytes(w.x) | nan_bytes(w.y) | nan_bytes(w.z) | nan_bytes(w.w);
         }
+        dirty = dirty || __any(any);
       }
-      dirty = __any(any);
-    }
-    float top = fmaxf(s[0][0], s[1][0]);
+      float top = s[0];
 #pragma unroll
-    for (int e = 1; e < 16; ++e) {
-      top = fmaxf(fmaxf(top, s[0][e]), s[1][e]);
-    }
-    const auto both = __builtin_amdgcn_permlane32_swap(f32_bits(top), f32_bits(top), false, false);
-    top = fmaxf(bits_f32(both[0]), bits_f32(both[1])) * a.scale_log2;
-    if (__any(top > st.m + kSlack)) {
-      const float now = fmaxf(st.m, top);
-      const float keep = now == -INFINITY ? 1.f : exp2_fast(st.m - now);
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        st.o[c] *= keep;
+      for (int e = 1; e < 16; ++e) {
+        top = fmaxf(top, s[e]);
       }
-      st.l *= keep;
-      st.m = now;
-    }
-    const float ref = st.m == -INFINITY ? 0.f : st.m;
-    u32x4 p[2][2];
+      if (__any(top > limit)) {
+        const auto both =
+            __builtin_amdgcn_permlane32_swap(f32_bits(top), f32_bits(top), false, false);
+        top = fmaxf(bits_f32(both[0]), bits_f32(both[1])) * a.scale_log2;
+        const float m = fmaxf(st.m, top);
+        const float keep = m == -INFINITY ? 1.f : exp2_fast(st.m - m);
 #pragma unroll
-    for (uint32_t u = 0; u < 2; ++u) {
-      const float bias = float(kOff + shift[u]) - ref;
+        for (int c = 0; c < D / 32; ++c) {
+          st.o[c] *= keep;
+        }
+        st.l *= keep;
+        st.m = m;
+        limit = (m + kSlack) / a.scale_log2;
+        new_bias();
+      }
       float sum = 0.f;
+      u32x4 p[2];
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
-        const float p0 = exp2_fast(__builtin_fmaf(s[u][e], a.scale_log2, bias));
-        const float p1 = exp2_fast(__builtin_fmaf(s[u][e + 1], a.scale_log2, bias));
+        const float p0 = exp2_fast(__builtin_fmaf(s[e], a.scale_log2, bias));
+        const float p1 = exp2_fast(__builtin_fmaf(s[e + 1], a.scale_log2, bias));
         sum += p0;
         sum += p1;
-        p[u][e / 8][e % 8 / 2] = f32x2_to_f16x2(p0, p1);
+        p[e / 8][e % 8 / 2] = f32x2_to_f16x2(p0, p1);
       }
-      st.l += sum * exp2_int(-shift[u]);
-    }
-#pragma unroll
-    for (uint32_t u = 0; u < 2; ++u) {
-      const uint8_t *values = stage + u * kGroup + 32 * D;
-      if (dirty) {
-        confine_values(st, values, clean[wave], lane, seen[u]);
-        values = clean[wave];
-      }
-      add_values(st, values, lane, p[u], power[u]);
+      st.l = __builtin_fmaf(sum, unshift, st.l);
+      add_values<D>(st, units, p, power);
     }
   }
   wait_copies<0>();  // none may land after the workgroup has gone
 
-  const auto half = __builtin_amdgcn_permlane32_swap(f32_bits(st.l), f32_bits(st.l), false, false);
-  const float sum = bits_f32(half[0]) + bits_f32(half[1]);
-  if (32 * wave + i > last) {
-    return;
-  }
-  const float join = sum == 0.f ? 0.f : 1.0f / sum, power = exp2_int(st.acc_exp);
-  const uint64_t slot = (row * a.heads + head) * x.parts + part;
+  const auto sink = [&](uint32_t r_of_tile) {
+    const uint32_t rr = t.r0 + min(r_of_tile, last);
+    RowSink to;
+    to.row = t.first_row + rr / a.group;
+    to.head = kvh * a.group + rr % a.group;
+    to.live = r_of_tile <= last;
+    to.whole = parts <= 1;
+    to.slot = (to.row * a.heads + to.head) * x.parts + part;
+    return to;
+  };
+  if (!dirty) {
+    const auto half =
+        __builtin_amdgcn_permlane32_swap(f32_bits(st.l), f32_bits(st.l), false, false);
+    const float sum = bits_f32(half[0]) + bits_f32(half[1]);
+    const float join = sum == 0.f ? 0.f : 1.0f / sum, unit = exp2_int(acc_exp);
+    const RowSink out = sink(32 * wave + i);
 #pragma unroll
-  for (int c = 0; c < D / 32; ++c) {
+    for (int c = 0; c < D / 32; ++c) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t d0 = 64 * (c / 2) + 32 * (e / 2) + 16 * (c % 2) + 8 * (e % 2) + 4 * h;
-      f32x4 v;
+      for (int e = 0; e < 4; ++e) {
+        f32x4 v;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[j] = st.o[c][4 * e + j] * join * power;
-      }
-      if (parts > 1) {
-        *reinterpret_cast<f32x4 *>(x.part_o + slot * D + d0) = v;
-      } else {
-        uint16_t *to_out = a.out + row * a.out_row + head * a.out_head + d0;
-        const u32x2 w = {f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
-        if (a.out_vec) {
-          *reinterpret_cast<u32x2 *>(to_out) = w;
-        } else {
-          to_out[0] = uint16_t(w.x);
-          to_out[1] = uint16_t(w.x >> 16);
-          to_out[2] = uint16_t(w.y);
-          to_out[3] = uint16_t(w.y >> 16);
+        for (int j = 0; j < 4; ++j) {
+          v[j] = st.o[c][4 * e + j] * join * unit;
         }
+        store4(a, x, out, D, 64 * (c / 2) + 32 * (e / 2) + 16 * (c % 2) + 8 * (e % 2) + 4 * h, v);
       }
     }
+    if (h == 0) {
+      store_sums(a, x, out, st.m, sum);
+    }
+    return;
   }
-  if (h == 0) {
-    if (parts > 1) {
-      x.part_s[slot] = PartSum{st.m, sum};
-    } else {
-      store_stats(a, x, row, head, st.m, sum);
+  // The NaN must reach the rows that see it and no others: the wave's rows go
+  // through the small tiles' code, which sees to that, 16 at a time.  (In the
+  // loop above it would cost the registers of a third wave.)
+  for (uint32_t part16 = 0; part16 < 2; ++part16) {
+    const uint32_t first = 32 * wave + 16 * part16, g = lane / 16;
+    if (first > last) {
+      return;
+    }
+    const RowSink out = sink(first + lane % 16);
+    Place at;
+    at.pos = int32_t(t.origin + (t.r0 + min(first + lane % 16, last)) / a.group);
+    at.oldest = oldest_hidden(at.pos, a.window);
+    at.low = int32_t(t.origin + (t.r0 + first) / a.group);
+    at.hidden =
+        oldest_hidden(t.origin + (t.r0 + min(first + 15, last)) / a.group, a.window);
+    const Query<D> q16 =
+        load_query<D>(a.q + out.row * a.q_row + out.head * a.q_head, a.vec, a.q_sign, g);
+    RowState<D> rs;
+    rs.m = -INFINITY;
+    rs.l = 0.f;
+    rs.acc_exp = kKvExpMin;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+      rs.o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (uint32_t grp = from; grp < to; ++grp) {
+      const uint32_t b = (grp * 32 >> a.pool.shift) - block0, in_block = grp * 32 & in_mask;
+      const u32x4 e = *reinterpret_cast<const u32x4 *>(&entries[b]);
+      const uint8_t *unit =
+          reinterpret_cast<const uint8_t *>(uint64_t(uniform(e.y)) << 32 | uniform(e.x));
+      const uint32_t exp_code = uniform(e.w);
+      Group<D> x32;
+      load_group_keys<D, false>(x32, unit, in_block, lane);
+      load_group_values<D, false>(x32, unit, a.pool.shift, in_block, lane);
+      attend_group<D, false>(
+          rs, x32, q16, at, grp * 32, (exp_code & kAbsent) == 0, bits_f32(uniform(e.z)),
+          int(exp_code & 0xffffu) - int(kExpCode), a.scale_log2, g, nullptr, [] {}, [] {});
+    }
+    float l = rs.l + __shfl_xor(rs.l, 16, kWave);
+    l += __shfl_xor(l, 32, kWave);
+    const float join = l == 0.f ? 0.f : 1.0f / l, power = exp2_int(rs.acc_exp);
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+      store4(a, x, out, D, 16 * c + 4 * g, rs.o[c] * join * power);
+    }
+    if (g == 0) {
+      store_sums(a, x, out, rs.m, l);
     }
   }
 }
@@ -1144,45 +1264,56 @@ __global__ __launch_bounds__(kWaves * kWave) void add_weights_kernel(KvAttendArg
     k[2 * c + 1] = codes_to_bf16(w.z, w.w, power);
   }
 
-  // (query, head of the group) of a row, moved on by whole tiles without a
-  // division; rows past the end are the last one's.
+  // A row's query, head of the group and an offset that goes with them, moved
+  // on by whole tiles without a division or product; rows past the end are
+  // the last one's.
+  const uint32_t tile_queries = kWeightRows / a.group, tile_heads = kWeightRows % a.group;
+  struct Strides {
+    uint64_t tile, wrap, last;
+  };
+  const auto strides = [&](uint64_t query, uint64_t head) {
+    return Strides{tile_queries * query + tile_heads * head, query - a.group * head,
+                   (rows.count - 1) * query + (a.group - 1) * head};
+  };
   struct RowAt {
     uint32_t query, head;
+    uint64_t offset;
   };
-  const uint32_t tile_queries = kWeightRows / a.group,
-                 tile_heads = kWeightRows % a.group;
-  const auto row_at = [&](uint32_t r) { return RowAt{r / a.group, r % a.group}; };
-  const auto next_tile = [&](RowAt &r) {
+  const Strides q_step = strides(a.q_row, a.q_head), stats_step = strides(a.heads, 1);
+  const auto row_at = [&](uint32_t r, uint64_t query, uint64_t head) {
+    return RowAt{r / a.group, r % a.group, r / a.group * query + r % a.group * head};
+  };
+  const auto next_tile = [&](RowAt &r, const Strides &by) {
     r.head += tile_heads;
     const bool carry = r.head >= a.group;
     r.head -= carry ? a.group : 0u;
     r.query += tile_queries + (carry ? 1u : 0u);
+    r.offset += by.tile + (carry ? by.wrap : 0u);
   };
-  const auto clamped = [&](const RowAt &r) {
-    return r.query < rows.count ? r : RowAt{rows.count - 1, a.group - 1};
+  const auto offset = [&](const RowAt &r, const Strides &by) {
+    return r.query < rows.count ? r.offset : by.last;
   };
   u32x4 held[kMine];
   RowStats held_stats{0.f, 0.f};
-  RowAt mine[kMine], mine_stats = row_at(begin + threadIdx.x % kWeightRows), tile_at = row_at(begin);
+  RowAt mine[kMine], mine_stats = row_at(begin + threadIdx.x % kWeightRows, a.heads, 1),
+                     tile_at = row_at(begin, 0, 0);
 #pragma unroll
   for (uint32_t j = 0; j < kMine; ++j) {
-    mine[j] = row_at(begin + (threadIdx.x + j * kWaves * kWave) / kChunks);
+    mine[j] = row_at(begin + (threadIdx.x + j * kWaves * kWave) / kChunks, a.q_row, a.q_head);
   }
+  const uint16_t *q_rows = a.q + uint64_t(rows.first) * a.q_row + uint64_t(kvh) * a.group * a.q_head +
+                           threadIdx.x % kChunks * 8;
+  const RowStats *stats_rows = stats + uint64_t(rows.first) * a.heads + kvh * a.group;
   const auto load_tile = [&]() {
 #pragma unroll
     for (uint32_t j = 0; j < kMine; ++j) {
-      const RowAt r = clamped(mine[j]);
       held[j] = __builtin_bit_cast(
-          u32x4, load_query8(a.q + uint64_t(rows.first + r.query) * a.q_row +
-                                 (kvh * a.group + r.head) * a.q_head +
-                                 threadIdx.x % kChunks * 8,
-                             a.vec, a.q_sign));
-      next_tile(mine[j]);
+          u32x4, load_query8(q_rows + offset(mine[j], q_step), a.vec, a.q_sign));
+      next_tile(mine[j], q_step);
     }
     if (threadIdx.x < kWeightRows) {
-      const RowAt r = clamped(mine_stats);
-      held_stats = stats[uint64_t(rows.first + r.query) * a.heads + kvh * a.group + r.head];
-      next_tile(mine_stats);
+      held_stats = stats_rows[offset(mine_stats, stats_step)];
+      next_tile(mine_stats, stats_step);
     }
   };
   const auto store_tile = [&](uint32_t stage) {
@@ -1209,7 +1340,7 @@ __global__ __launch_bounds__(kWaves * kWave) void add_weights_kernel(KvAttendArg
       load_tile();
     }
     const int32_t low = int32_t(origin + tile_at.query);
-    next_tile(tile_at);
+    next_tile(tile_at, Strides{0, 0, 0});
     const uint32_t last = min(r0 + kWeightRows - 1, all - 1);
     // The tile's last query, or one that no row of it is past.
     const int32_t high = int32_t(origin + min(tile_at.query, rows.count - 1));
