@@ -68,6 +68,10 @@ struct Query {
 
 // Eight elements of a query, negated if the scale is negative (so that scores
 // and products have one order and a maximum can be taken before scaling).
+__device__ __forceinline__ bf16x8 flip(bf16x8 v, uint32_t sign) {
+  const u32x4 w = __builtin_bit_cast(u32x4, v);
+  return __builtin_bit_cast(bf16x8, u32x4{w.x ^ sign, w.y ^ sign, w.z ^ sign, w.w ^ sign});
+}
 __device__ __forceinline__ bf16x8 load_query8(const uint16_t *p, bool vec, uint32_t sign) {
   u32x4 w;
   if (vec) {
@@ -78,7 +82,7 @@ __device__ __forceinline__ bf16x8 load_query8(const uint16_t *p, bool vec, uint3
       w[i] = p[2 * i] | uint32_t(p[2 * i + 1]) << 16;
     }
   }
-  return __builtin_bit_cast(bf16x8, u32x4{w.x ^ sign, w.y ^ sign, w.z ^ sign, w.w ^ sign});
+  return flip(__builtin_bit_cast(bf16x8, w), sign);
 }
 
 template <int D>
@@ -444,6 +448,12 @@ __device__ __forceinline__ uint32_t part_count(const Tile &t, uint32_t part_toke
   return t.end > from ? (t.end - from + part_tokens - 1) / part_tokens : 0u;
 }
 
+// Place of the first of a row's statistics for a key/value head: rows and the
+// heads of the group run on in the order of a tile's rows.
+__device__ __forceinline__ uint64_t stats_at(const KvAttendArgs &a, uint32_t kvh, uint64_t row) {
+  return (uint64_t(kvh) * a.seqs.rows + row) * a.group;
+}
+
 // Log-sum and statistics of a row.
 __device__ __forceinline__ void store_stats(const KvAttendArgs &a, const Scratch &x, uint64_t row,
                                             uint32_t head, float top, float sum) {
@@ -452,7 +462,7 @@ __device__ __forceinline__ void store_stats(const KvAttendArgs &a, const Scratch
     a.lse[at] = sum == 0.f ? -INFINITY : (top + (log2f(sum) - float(kOff))) * kLn2;
   }
   if (x.stats != nullptr) {
-    x.stats[at] = RowStats{(top == -INFINITY ? 0.f : top) - float(kOff),
+    x.stats[stats_at(a, head / a.group, row) + head % a.group] = RowStats{(top == -INFINITY ? 0.f : top) - float(kOff),
                            sum == 0.f ? 0.f : 1.0f / sum};
   }
 }
@@ -923,12 +933,10 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows_kernel(KvAttendAr
         s = mfma32_bf16(codes_to_bf16(w.x, w.y, now.power[u]), q[2 * c], s);
         s = mfma32_bf16(codes_to_bf16(w.z, w.w, now.power[u]), q[2 * c + 1], s);
       }
-      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (uint32_t c = 0; c < D / 32; ++c) {
         units[c] = value_unit(values, lane, c / (D / 64), c % (D / 64));
       }
-      __builtin_amdgcn_sched_barrier(0);
       if (now.exp_code[u] != code) {
         code = now.exp_code[u];
         const int ev = int(code & 0xffffu) - int(kExpCode);
@@ -1199,8 +1207,9 @@ __global__ __launch_bounds__(256) void add_scores_kernel(KvAttendArgs a, Scratch
   float sum = 0.f;
   for (; i < end; ++i) {
     const uint64_t at = uint64_t(rows.first + i) * a.heads + kvh * a.group;
+    const RowStats *stats = x.stats + stats_at(a, kvh, rows.first + i);
     for (uint32_t h = 0; h < a.group; ++h) {
-      const RowStats st = x.stats[at + h];
+      const RowStats st = stats[h];
       sum += exp2_fast(x.scores[(at + h) * x.score_stride + t] - st.top) * st.inv_sum;
     }
   }
@@ -1211,18 +1220,22 @@ __global__ __launch_bounds__(256) void add_scores_kernel(KvAttendArgs a, Scratch
 // Adds the weights that tokens receive from all rows of their sequence, by a
 // second product of keys and queries: a wave owns 32 tokens, whose keys it
 // holds as operands, and the rows pass by in tiles of 64 that the workgroup
-// stages in LDS (chunk k of row r at place k ^ r, so that 8 neighbours read 8
-// groups of banks), the next tile on its way in registers meanwhile.  Each token's sum has a fixed order; the addition is
-// atomic for blocks that several sequences of a call share.
+// stages in LDS, the next tile on its way meanwhile.  Each token's sum has a
+// fixed order; the addition is atomic for blocks that several sequences of a
+// call share.
+//
+// LDS holds a tile as D / 32 planes of 64 bytes of each row; 16-byte chunk k of
+// row r is at place k ^ r / 4 % 4 of the 64, so that 16 neighbours read 16
+// groups of banks and a wave copies 16 rows at once, a lane always the same.
 constexpr uint32_t kWeightTokens = 32 * kWaves, kWeightRows = 64;
 
 template <int D>
-__global__ __launch_bounds__(kWaves * kWave) void add_weights_kernel(KvAttendArgs a,
-                                                                     const RowStats *stats) {
-  constexpr uint32_t kChunks = D / 8;                          // 16-byte chunks of a row
-  constexpr uint32_t kMine = kWeightRows * kChunks / (kWaves * kWave);  // per thread
-  __shared__ __align__(16) uint8_t rows_lds[2][kWeightRows * D * 2];
-  __shared__ RowStats stats_lds[2][kWeightRows];
+__global__ __launch_bounds__(kWaves * kWave, 4) void add_weights_kernel(KvAttendArgs a,
+                                                                        const RowStats *stats) {
+  constexpr uint32_t kPlane = kWeightRows * 64;
+  static_assert(kWeightRows == 16 * kWaves, "a wave copies 16 rows of each plane");
+  extern __shared__ __align__(1024) uint8_t weight_rows[];
+  const auto rows_lds = [](uint32_t stage) { return weight_rows + stage * (D / 32 * kPlane); };
   const uint32_t kvh = blockIdx.y, b = blockIdx.z;
   const uint32_t lane = threadIdx.x % kWave;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -1260,131 +1273,116 @@ __global__ __launch_bounds__(kWaves * kWave) void add_weights_kernel(KvAttendArg
   for (int c = 0; c < D / 32; ++c) {
     const u32x4 w = *reinterpret_cast<const u32x4 *>(
         keys + (i / 16 * (D / 64) + c / 2) * 1024 + (i % 16 + 16 * (c % 2 * 2 + h)) * 16);
-    k[2 * c] = codes_to_bf16(w.x, w.y, power);
-    k[2 * c + 1] = codes_to_bf16(w.z, w.w, power);
+    k[2 * c] = flip(codes_to_bf16(w.x, w.y, power), a.q_sign);
+    k[2 * c + 1] = flip(codes_to_bf16(w.z, w.w, power), a.q_sign);
   }
 
-  // A row's query, head of the group and an offset that goes with them, moved
-  // on by whole tiles without a division or product; rows past the end are
-  // the last one's.
+  // A row's query, head of the group and offset, moved on by whole tiles
+  // without a division or product; rows past the end are the last one's.
   const uint32_t tile_queries = kWeightRows / a.group, tile_heads = kWeightRows % a.group;
-  struct Strides {
-    uint64_t tile, wrap, last;
-  };
-  const auto strides = [&](uint64_t query, uint64_t head) {
-    return Strides{tile_queries * query + tile_heads * head, query - a.group * head,
-                   (rows.count - 1) * query + (a.group - 1) * head};
-  };
+  const uint64_t tile_step = tile_queries * a.q_row + tile_heads * a.q_head;
+  const uint64_t wrap_step = a.q_row - a.group * a.q_head;
+  const uint64_t last_row = (rows.count - 1) * a.q_row + (a.group - 1) * a.q_head;
   struct RowAt {
     uint32_t query, head;
     uint64_t offset;
   };
-  const Strides q_step = strides(a.q_row, a.q_head), stats_step = strides(a.heads, 1);
-  const auto row_at = [&](uint32_t r, uint64_t query, uint64_t head) {
-    return RowAt{r / a.group, r % a.group, r / a.group * query + r % a.group * head};
+  const auto row_at = [&](uint32_t r) {
+    return RowAt{r / a.group, r % a.group, r / a.group * a.q_row + r % a.group * a.q_head};
   };
-  const auto next_tile = [&](RowAt &r, const Strides &by) {
+  const auto next_tile = [&](RowAt &r) {
     r.head += tile_heads;
     const bool carry = r.head >= a.group;
     r.head -= carry ? a.group : 0u;
     r.query += tile_queries + (carry ? 1u : 0u);
-    r.offset += by.tile + (carry ? by.wrap : 0u);
+    r.offset += tile_step + (carry ? wrap_step : 0u);
   };
-  const auto offset = [&](const RowAt &r, const Strides &by) {
-    return r.query < rows.count ? r.offset : by.last;
-  };
-  u32x4 held[kMine];
-  RowStats held_stats{0.f, 0.f};
-  RowAt mine[kMine], mine_stats = row_at(begin + threadIdx.x % kWeightRows, a.heads, 1),
-                     tile_at = row_at(begin, 0, 0);
+  RowAt mine = row_at(begin + 16 * wave + lane / 4), tile_at = row_at(begin);
+  const uint16_t *q_rows = a.q + rows.first * a.q_row + uint64_t(kvh) * a.group * a.q_head +
+                           (lane % 4 ^ lane / 16) * 8;
+  const auto start_tile = [&](uint8_t *to) {
+    const uint16_t *from = q_rows + (mine.query < rows.count ? mine.offset : last_row);
+    to += wave * 1024;
+    next_tile(mine);
+    if (a.vec) {
 #pragma unroll
-  for (uint32_t j = 0; j < kMine; ++j) {
-    mine[j] = row_at(begin + (threadIdx.x + j * kWaves * kWave) / kChunks, a.q_row, a.q_head);
-  }
-  const uint16_t *q_rows = a.q + uint64_t(rows.first) * a.q_row + uint64_t(kvh) * a.group * a.q_head +
-                           threadIdx.x % kChunks * 8;
-  const RowStats *stats_rows = stats + uint64_t(rows.first) * a.heads + kvh * a.group;
-  const auto load_tile = [&]() {
+      for (uint32_t c = 0; c < D / 32; ++c) {
+        copy_to_lds(reinterpret_cast<const uint8_t *>(from + c * 32), to + c * kPlane);
+      }
+    } else {
 #pragma unroll
-    for (uint32_t j = 0; j < kMine; ++j) {
-      held[j] = __builtin_bit_cast(
-          u32x4, load_query8(q_rows + offset(mine[j], q_step), a.vec, a.q_sign));
-      next_tile(mine[j], q_step);
-    }
-    if (threadIdx.x < kWeightRows) {
-      held_stats = stats_rows[offset(mine_stats, stats_step)];
-      next_tile(mine_stats, stats_step);
+      for (uint32_t c = 0; c < D / 32; ++c) {
+        *reinterpret_cast<bf16x8 *>(to + c * kPlane + lane * 16) =
+            load_query8(from + c * 32, false, 0);
+      }
     }
   };
-  const auto store_tile = [&](uint32_t stage) {
+  const RowStats *row_stats = stats + stats_at(a, kvh, rows.first);
+  RowStats next[2];
+  const auto load_stats = [&](uint32_t r0) {
 #pragma unroll
-    for (uint32_t j = 0; j < kMine; ++j) {
-      const uint32_t at = threadIdx.x + j * kWaves * kWave;
-      const uint32_t r = at / kChunks, c = at % kChunks;
-      reinterpret_cast<u32x4 *>(rows_lds[stage])[r * kChunks + (c ^ r % kChunks)] = held[j];
-    }
-    if (threadIdx.x < kWeightRows) {
-      stats_lds[stage][threadIdx.x] = held_stats;
+    for (uint32_t u = 0; u < 2; ++u) {
+      next[u] = row_stats[min(r0 + 32 * u + i, all - 1)];
     }
   };
   float sum[16] = {};
-  if (begin < end) {
-    load_tile();
-    store_tile(0);
-  }
-  __syncthreads();
   uint32_t stage = 0;
+  if (begin < end) {
+    load_stats(begin);
+    start_tile(rows_lds(0));
+  }
   for (uint32_t r0 = begin; r0 < end; r0 += kWeightRows, stage ^= 1) {
-    const bool more = r0 + kWeightRows < end;
-    if (more) {
-      load_tile();
+    wait_copies<0>();
+    step_barrier();
+    const RowStats now[2] = {next[0], next[1]};
+    if (r0 + kWeightRows < end) {
+      load_stats(r0 + kWeightRows);
+      start_tile(rows_lds(stage ^ 1));
     }
     const int32_t low = int32_t(origin + tile_at.query);
-    next_tile(tile_at, Strides{0, 0, 0});
-    const uint32_t last = min(r0 + kWeightRows - 1, all - 1);
+    next_tile(tile_at);
     // The tile's last query, or one that no row of it is past.
     const int32_t high = int32_t(origin + min(tile_at.query, rows.count - 1));
-    if (id >= 0 && int32_t(t0) <= high) {
-      const bool edge = r0 + kWeightRows - 1 > last || int32_t(t0) + 31 > low ||
-                        int32_t(t0) <= oldest_hidden(high, a.window);
-      f32x16 s[2];
+    if (id < 0 || int32_t(t0) > high) {
+      continue;
+    }
+    const bool edge = r0 + kWeightRows > all || int32_t(t0) + 31 > low ||
+                      int32_t(t0) <= oldest_hidden(high, a.window);
+    const uint8_t *tile = rows_lds(stage) + i * 64;
 #pragma unroll
-      for (uint32_t u = 0; u < 2; ++u) {
-        const u32x4 *tile =
-            reinterpret_cast<const u32x4 *>(rows_lds[stage]) + (32 * u + i) * kChunks;
-        s[u] = f32x16{};
+    for (uint32_t u = 0; u < 2; ++u) {
+      bf16x8 q[D / 16];
 #pragma unroll
-        for (uint32_t c = 0; c < D / 16; ++c) {
-          const uint32_t chunk = 2 * (c / 2 * 2 + h) + c % 2;
-          s[u] = mfma32_bf16(k[c], __builtin_bit_cast(bf16x8, tile[chunk ^ i % kChunks]), s[u]);
+      for (uint32_t c = 0; c < D / 16; ++c) {
+        const uint32_t place = (2 * h + c % 2) ^ i / 4 % 4;
+        q[c] = *reinterpret_cast<const bf16x8 *>(tile + c / 2 * kPlane + 32 * u * 64 + place * 16);
+      }
+      f32x16 s = f32x16{};
+#pragma unroll
+      for (uint32_t c = 0; c < D / 16; ++c) {
+        s = mfma32_bf16(k[c], q[c], s);
+      }
+      float inv_sum = now[u].inv_sum;
+      if (edge) {
+        // A row of NaN gives it to what it sees, and nothing to the rest.
+        const bool bad = inv_sum != inv_sum;
+        const float add = bad ? inv_sum : 0.f;
+        inv_sum = bad ? 1.f : inv_sum;
+        const uint32_t r = r0 + 32 * u + i;
+        const int32_t pos = int32_t(origin + r / a.group);
+        const int32_t oldest = oldest_hidden(pos, a.window);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int32_t tok = int32_t(t0) + e / 4 * 8 + 4 * int32_t(h) + e % 4;
+          s[e] = r < all && tok <= pos && tok > oldest ? s[e] + add : -INFINITY;
         }
       }
 #pragma unroll
-      for (uint32_t u = 0; u < 2; ++u) {
-        const RowStats st = stats_lds[stage][32 * u + i];
-        if (edge) {
-          const uint32_t r = r0 + 32 * u + i;
-          const int32_t pos = int32_t(origin + r / a.group);
-          const int32_t oldest = oldest_hidden(pos, a.window);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int32_t tok = int32_t(t0) + e / 4 * 8 + 4 * int32_t(h) + e % 4;
-            const float p = exp2_fast(__builtin_fmaf(s[u][e], a.scale_log2, -st.top)) * st.inv_sum;
-            sum[e] += r <= last && tok <= pos && tok > oldest ? p : 0.f;
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            sum[e] = __builtin_fmaf(exp2_fast(__builtin_fmaf(s[u][e], a.scale_log2, -st.top)),
-                                    st.inv_sum, sum[e]);
-          }
-        }
+      for (int e = 0; e < 16; ++e) {
+        sum[e] = __builtin_fmaf(exp2_fast(__builtin_fmaf(s[e], a.scale_log2, -now[u].top)),
+                                inv_sum, sum[e]);
       }
     }
-    if (more) {
-      store_tile(stage ^ 1);
-    }
-    __syncthreads();
   }
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
@@ -1461,7 +1459,7 @@ KvAttendPlan plan_kv_attend(const KvAttendArgs &a, uint32_t dim) {
     span = std::min<uint64_t>(span, uint64_t(a.window) + p.row_tile / a.group + 32);
   }
   const uint32_t cus = device_cu_count();
-  const uint64_t split = std::max<uint64_t>((many ? 2 : 1) * cus / tiles, 1);
+  const uint64_t split = std::max<uint64_t>((many ? 3 : 1) * cus / tiles, 1);
   const uint64_t part = std::max<uint64_t>((span + split - 1) / split, kPartLeast);
   p.part_tokens = uint32_t(std::min<uint64_t>((part + kStep - 1) / kStep * kStep,
                                               (many ? kManyBlocks : 64u) << a.pool.shift));
@@ -1523,7 +1521,8 @@ static hipError_t launch_attend(const KvAttendArgs &a, const KvAttendPlan &p, vo
     } else {
       const dim3 grid(uint32_t((tokens + kWeightTokens - 1) / kWeightTokens), a.pool.heads,
                       a.seqs.batch);
-      add_weights_kernel<D><<<grid, kWaves * kWave, 0, s>>>(a, x.stats);
+      add_weights_kernel<D>
+          <<<grid, kWaves * kWave, 2 * kWeightRows * D * 2, s>>>(a, x.stats);
     }
   }
   return hipGetLastError();
