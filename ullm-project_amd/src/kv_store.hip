@@ -52,14 +52,15 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
 __device__ __forceinline__ float scaled(uint16_t h, float inv) {
   return (h & 0x7f80u) == 0x7f80u ? __builtin_nanf("") : bf16_to_f32(h) * inv;
 }
-// Four codes times a power of two, rounded to codes again.
-__device__ __forceinline__ uint32_t rescale4(uint32_t w, float f) {
+// Four codes times powers of two, rounded to codes again.
+__device__ __forceinline__ uint32_t rescale4(uint32_t w, f32x4 f) {
   typedef float f2 __attribute__((ext_vector_type(2)));
   const f2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(int(w), false);
   const f2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(int(w), true);
-  return encode4(lo[0] * f, lo[1] * f, hi[0] * f, hi[1] * f);
+  return encode4(lo[0] * f[0], lo[1] * f[1], hi[0] * f[2], hi[1] * f[3]);
 }
-__device__ __forceinline__ u32x4 rescale16(u32x4 w, float f) {
+__device__ __forceinline__ u32x4 rescale16(u32x4 w, float by) {
+  const f32x4 f = {by, by, by, by};
   return u32x4{rescale4(w.x, f), rescale4(w.y, f), rescale4(w.z, f), rescale4(w.w, f)};
 }
 
@@ -293,17 +294,51 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (b & 0x80000000u) ? (b == 0x80000000u ? 0x80000000u : ~b) : (b | 0x80000000u);
 }
 
-constexpr uint32_t kSelectThreads = 1024;
+constexpr uint32_t kSelectThreads = 1024, kSelectWaves = kSelectThreads / kWave;
+constexpr uint32_t kSelectBins = 4096;
 
-// One workgroup selects the tokens of one sequence and head: the key that the
-// last selected token has, by its bytes from the highest (a histogram each),
-// then the selected positions in order.
+// Exclusive sums over the workgroup in the order of the threads; `sums`: one
+// per wave.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *sums) {
+  const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  uint32_t upto = v;
+#pragma unroll
+  for (uint32_t off = 1; off < kWave; off <<= 1) {
+    const uint32_t o = __shfl_up(upto, off, kWave);
+    upto += lane >= off ? o : 0u;
+  }
+  if (lane == kWave - 1) {
+    sums[wave] = upto;
+  }
+  __syncthreads();
+#pragma unroll
+  for (uint32_t w = 0; w < kSelectWaves; ++w) {
+    upto += w < wave ? sums[w] : 0u;
+  }
+  return upto - v;
+}
+
+// One workgroup selects the tokens of one sequence and head.  A thread holds K
+// keys in registers, 1024 K for the workgroup (longer sequences read theirs
+// again, as many at a time, in each pass), so that a pass costs no memory.
+//
+// First the key of the last token that stays: the range of the keys in
+// question, at first their smallest to their largest, is cut into 4096 bins,
+// and the bin that it falls into is the next range, until all keys of a bin
+// stay or they are equal.  Bins that follow the keys' own range keep the lanes
+// of a wave on different counters, which fixed digits do not (weights share
+// most of their exponent).  Then the positions, in order: a wave holds 64 K
+// tokens on end and counts its own, the waves' counts are joined once.
+//
+// Bound by the instructions of a lone workgroup per head.  (32768 tokens of 8
+// heads: 27 us; by bytes of the key, each pass reading the weights again, 128.)
+template <uint32_t K>
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(KvEvictArgs a) {
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t pick[2];
-  __shared__ uint32_t counts[2][kSelectThreads / kWave];
+  constexpr uint32_t kSpan = K * kSelectThreads;
+  __shared__ uint32_t hist[kSelectBins];
+  __shared__ uint32_t sums[kSelectWaves], ties[kSelectWaves], pick[3], range[2];
   const uint32_t b = blockIdx.y, head = blockIdx.x, tid = threadIdx.x;
-  const uint32_t lane = tid % kWave, wave = tid / kWave;
+  const uint32_t lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const uint32_t length = kv_length(a.seqs, a.pool.shift, b);
   int32_t *kept = a.kept + (uint64_t(b) * a.pool.heads + head) * a.keep;
   const uint32_t stay = length < a.keep ? length : a.keep;
@@ -316,90 +351,212 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(KvEvictArg
     }
     return;
   }
-  const int32_t *table = a.seqs.tables + b * a.seqs.stride;
-  const uint32_t mask = (1u << a.pool.shift) - 1;
-  const auto key_of = [&](uint32_t t) {
-    const int32_t id = kv_block(table, a.seqs, a.pool.blocks, t >> a.pool.shift);
-    return id < 0 ? 0u
-                  : weight_key(a.pool.weights[((uint64_t(id) * a.pool.heads + head)
-                                               << a.pool.shift) + (t & mask)]);
-  };
   const uint32_t lo = a.sink, hi = length - a.recent;  // candidates lo .. hi - 1
   uint32_t want = a.keep - a.sink - a.recent;
-  uint32_t prefix = 0;  // the bytes of the last selected key found so far
-  if (want != 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (uint32_t i = tid; i < 256; i += kSelectThreads) {
-        hist[i] = 0;
+  for (uint32_t i = tid; i < a.sink + a.recent; i += kSelectThreads) {
+    kept[i < lo ? i : i + want] = int32_t(i < lo ? i : i - lo + hi);
+  }
+  if (want == 0) {
+    return;
+  }
+  const int32_t *table = a.seqs.tables + b * a.seqs.stride;
+  const uint32_t mask = (1u << a.pool.shift) - 1;
+  const uint32_t spans = (length + kSpan - 1) / kSpan;
+  const uint32_t mine = wave * K * kWave + lane;  // this thread's first token of a span
+
+  uint32_t keys[K];
+  // Keys of a span: 0 is no candidate, 1 a token of no block, which is less
+  // than any weight.  Loads do not depend on what they find, so that two waits
+  // serve for all.
+  const auto load = [&](uint32_t span) __attribute__((always_inline)) {
+    const uint32_t t0 = span * kSpan + mine;
+    uint32_t id[K];
+    float w[K];
+#pragma unroll
+    for (uint32_t k = 0; k < K; ++k) {
+      id[k] = uint32_t(table[min((t0 + k * kWave) >> a.pool.shift, a.seqs.max_blocks - 1)]);
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < K; ++k) {
+      const uint64_t unit = uint64_t(id[k] < a.pool.blocks ? id[k] : 0u) * a.pool.heads + head;
+      w[k] = a.pool.weights[(unit << a.pool.shift) + ((t0 + k * kWave) & mask)];
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < K; ++k) {
+      const uint32_t t = t0 + k * kWave;
+      const uint32_t key = id[k] < a.pool.blocks ? weight_key(w[k]) : 1u;
+      keys[k] = t >= lo && t < hi ? key : 0u;
+    }
+  };
+  const auto each_span = [&](const auto &f) __attribute__((always_inline)) {
+    for (uint32_t span = 0; span < spans; ++span) {
+      if (spans > 1) {
+        load(span);
       }
-      __syncthreads();
-      for (uint32_t t = lo + tid; t < hi; t += kSelectThreads) {
-        const uint32_t key = key_of(t);
-        if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) {
-          atomicAdd(&hist[(key >> shift) & 255u], 1u);
+      f(span);
+    }
+  };
+  if (spans == 1) {
+    load(0);
+  }
+
+  if (tid == 0) {
+    range[0] = ~0u;
+    range[1] = 0u;
+  }
+  __syncthreads();
+  uint32_t least = ~0u, most = 0;
+  each_span([&](uint32_t) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t k = 0; k < K; ++k) {
+      least = min(least, keys[k] - 1u);  // no candidate: the largest
+      most = max(most, keys[k]);
+    }
+  });
+  least = ~wave_umax(~least);
+  most = wave_umax(most);
+  if (lane == 0) {
+    atomicMin(&range[0], least);
+    atomicMax(&range[1], most);
+  }
+  __syncthreads();
+  uint32_t from = range[0] + 1, width = range[1] - from;  // keys from .. from + width
+  uint32_t last;  // tokens of keys above it stay, and of this one `want`
+  for (;;) {
+    last = from;
+    if (width == 0) {
+      break;
+    }
+    for (uint32_t i = tid; i < kSelectBins; i += kSelectThreads) {
+      hist[i] = 0;
+    }
+    __syncthreads();
+    const uint32_t bits = 32 - __builtin_clz(width), shift = bits > 12 ? bits - 12 : 0;
+    each_span([&](uint32_t) __attribute__((always_inline)) {
+#pragma unroll
+      for (uint32_t k = 0; k < K; ++k) {
+        const uint32_t off = keys[k] - from;
+        if (off <= width) {
+          atomicAdd(&hist[kSelectBins - 1 - (off >> shift)], 1u);
         }
       }
-      __syncthreads();
-      if (tid == 0) {
-        uint32_t above = 0, bin = 255;
-        while (above + hist[bin] < want) {  // the bins hold at least `want` keys
-          above += hist[bin--];
-        }
-        pick[0] = bin;
-        pick[1] = above;
+    });
+    __syncthreads();
+    // The first bin, from the highest on, that reaches `want` keys.
+    constexpr uint32_t kMine = kSelectBins / kSelectThreads;
+    uint32_t n[kMine], sum = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kMine; ++i) {
+      n[i] = hist[tid * kMine + i];
+      sum += n[i];
+    }
+    uint32_t upto = block_scan(sum, sums);
+#pragma unroll
+    for (uint32_t i = 0; i < kMine; ++i) {
+      if (upto < want && upto + n[i] >= want) {
+        pick[0] = kSelectBins - 1 - (tid * kMine + i);
+        pick[1] = want - upto;
+        pick[2] = n[i];
       }
-      __syncthreads();
-      prefix |= pick[0] << shift;
-      want -= pick[1];
-      __syncthreads();
+      upto += n[i];
+    }
+    __syncthreads();
+    from += pick[0] << shift;
+    want = pick[1];
+    width = (1u << shift) - 1;
+    if (want == pick[2]) {
+      last = from - 1;
+      want = 0;
+      break;
     }
   }
-  // `want` tokens of key `prefix` stay, the lowest positions first.
-  const bool none = a.keep == a.sink + a.recent;
-  uint32_t done = 0, equal = 0;
-  for (uint32_t t0 = 0; t0 < length; t0 += kSelectThreads) {
-    const uint32_t t = t0 + tid;
-    const bool free = t >= lo && t < hi;
-    const uint32_t key = free && !none ? key_of(t) : 0u;
-    const bool tie = free && !none && key == prefix;
-    const uint64_t ties = __ballot(tie);
+
+  uint32_t at = a.sink, equal = 0;  // where the next goes, tokens of key `last` so far
+  each_span([&](uint32_t span) __attribute__((always_inline)) {
+    uint32_t n = 0, m = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < K; ++k) {
+      n += uint32_t(__popcll(__ballot(keys[k] > last)));
+      m += uint32_t(__popcll(__ballot(keys[k] == last)));
+    }
+    __syncthreads();  // the sums of the last span are read
+    if (lane == 0) {
+      sums[wave] = n;
+      ties[wave] = m;
+    }
+    __syncthreads();
+    uint32_t next = at, same = equal;
+#pragma unroll
+    for (uint32_t w = 0; w < kSelectWaves; ++w) {
+      next += w < wave ? sums[w] : 0u;
+      same += w < wave ? ties[w] : 0u;
+      at += sums[w];
+      equal += ties[w];
+    }
     const uint64_t below = (uint64_t(1) << lane) - 1;
-    if (lane == 0) {
-      counts[0][wave] = uint32_t(__popcll(ties));
+#pragma unroll
+    for (uint32_t k = 0; k < K; ++k) {
+      const uint64_t above = __ballot(keys[k] > last), tie = __ballot(keys[k] == last);
+      if ((above | tie) == 0) {
+        continue;
+      }
+      const uint32_t ties_before = same + uint32_t(__popcll(tie & below));
+      const uint32_t to = next + uint32_t(__popcll(above & below)) + min(ties_before, want);
+      if (keys[k] > last || (keys[k] == last && ties_before < want)) {
+        kept[to] = int32_t(span * kSpan + mine + k * kWave);
+      }
+      next += uint32_t(__popcll(above));
+      same += uint32_t(__popcll(tie));
     }
-    __syncthreads();
-    uint32_t rank = equal + uint32_t(__popcll(ties & below));
-    for (uint32_t i = 0; i < kSelectThreads / kWave; ++i) {
-      rank += i < wave ? counts[0][i] : 0u;
-      equal += counts[0][i];
-    }
-    const bool stays =
-        t < length && (!free || (!none && (key > prefix || (tie && rank < want))));
-    const uint64_t all = __ballot(stays);
-    if (lane == 0) {
-      counts[1][wave] = uint32_t(__popcll(all));
-    }
-    __syncthreads();
-    uint32_t at = done + uint32_t(__popcll(all & below));
-    for (uint32_t i = 0; i < kSelectThreads / kWave; ++i) {
-      at += i < wave ? counts[1][i] : 0u;
-      done += counts[1][i];
-    }
-    if (stays && at < a.keep) {
-      kept[at] = int32_t(t);
-    }
-  }
+  });
 }
 
-constexpr int kNoToken = -128;
+// Magnitudes of four codes without the sign, those of NaN as 0.
+__device__ __forceinline__ uint32_t finite_codes(uint32_t w) {
+  w &= 0x7f7f7f7fu;
+  const uint32_t nan = (w + 0x01010101u) & 0x80808080u;
+  return w & ~(nan - (nan >> 7));
+}
+// The largest of sixteen such magnitudes, two at a time.
+__device__ __forceinline__ uint32_t largest_code(u32x4 w) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 top = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t m = finite_codes(w[i]);
+    top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, m & 0x00ff00ffu));
+    top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, m >> 8 & 0x00ff00ffu));
+  }
+  return top[0] > top[1] ? top[0] : top[1];
+}
+// Factor of codes that go from one exponent to another.  Only codes of zero
+// and NaN meet a difference past the clamp upwards.
+__device__ __forceinline__ float code_factor(int from, int to) {
+  const int by = from - to;
+  return exp2_int(by < -126 ? -126 : by > 126 ? 126 : by);
+}
+
+constexpr uint32_t kMostBlock = 128;  // tokens of a block
 
 // One workgroup fills one block and head of the new tables with the tokens
-// that stay.
+// that stay.  All codes are read once: the keys' 16 bytes stay in registers,
+// and of the values' units, which a token shares with seven others, its two
+// bytes go to their new places in LDS.  Then the exponents are known, and
+// codes whose exponent does not change are written as they are.  Bound by the
+// values' units, eight bytes read for each that is kept (the cache lines serve
+// several tokens).  (16 sequences to 1536 tokens of 8 heads: 46 us; with loads
+// of single bytes, twice, 86.)
 template <int D>
 __global__ __launch_bounds__(kThreads) void evict_move_kernel(KvEvictArgs a) {
-  __shared__ uint64_t from[128];   // byte offset of the token's block and head
-  __shared__ uint32_t slot[128];   // its place in that block
-  __shared__ int power[2][128];    // the exponents there, kNoToken: no block
+  constexpr uint32_t kKeyUnits = kMostBlock * (D / 16) / kThreads;  // of a thread
+  constexpr uint32_t kLanes = D / 2;                                // of a token's values
+  constexpr uint32_t kTokens = kThreads / kLanes, kAhead = 8;
+  __shared__ __align__(16) uint8_t image[kMostBlock * D];  // the new block's values
+  __shared__ uint64_t from[kMostBlock];   // byte offset of the token's block and head
+  __shared__ uint32_t slot[kMostBlock];   // its place in that block, kNone: in none
+  __shared__ int power[2][kMostBlock];    // the exponents there
+  __shared__ __align__(16) float factor[kMostBlock];
+  constexpr uint32_t kNone = ~0u;
   const uint32_t bt = 1u << a.pool.shift, j = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
   const uint32_t tid = threadIdx.x;
   const uint32_t length = kv_length(a.seqs, a.pool.shift, b);
@@ -408,42 +565,80 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(KvEvictArgs a) {
   if (base >= stay) {
     return;
   }
-  const uint32_t n = stay - base < bt ? stay - base : bt;
+  const uint32_t n = stay - base < bt ? stay - base : bt, padded = (n + 31) / 32 * 32;
   const int32_t raw = a.new_tables[b * a.new_stride + j];
   if (raw < 0 || uint32_t(raw) >= a.pool.blocks) {
     return;
   }
   const uint64_t dst = uint64_t(raw) * a.pool.heads + head;
+  const uint64_t side = uint64_t(D) << a.pool.shift;
   const int32_t *kept = a.kept + (uint64_t(b) * a.pool.heads + head) * a.keep + base;
   const int32_t *table = a.seqs.tables + b * a.seqs.stride;
-  for (uint32_t i = tid; i < n; i += kThreads) {
-    const uint32_t t = uint32_t(kept[i]);
-    const int32_t id = kv_block(table, a.seqs, a.pool.blocks, t >> a.pool.shift);
+  if (tid < padded) {
+    const uint32_t t = tid < n ? uint32_t(kept[tid]) : 0u;
+    const int32_t id =
+        tid < n ? kv_block(table, a.seqs, a.pool.blocks, t >> a.pool.shift) : -1;
     const uint64_t src = uint64_t(id < 0 ? 0 : id) * a.pool.heads + head;
-    from[i] = src * (uint64_t(2 * D) << a.pool.shift);
-    slot[i] = t & (bt - 1);
-    power[0][i] = id < 0 ? kNoToken : int(a.pool.exps[src * 2]);
-    power[1][i] = id < 0 ? kNoToken : int(a.pool.exps[src * 2 + 1]);
-    if (a.pool.weights != nullptr) {
-      a.pool.weights[(dst << a.pool.shift) + i] =
-          id < 0 ? 0.f : a.pool.weights[(src << a.pool.shift) + slot[i]];
+    from[tid] = src * 2 * side;
+    slot[tid] = id < 0 ? kNone : t & (bt - 1);
+    power[0][tid] = a.pool.exps[src * 2];
+    power[1][tid] = a.pool.exps[src * 2 + 1];
+    if (a.pool.weights != nullptr && tid < n) {
+      a.pool.weights[(dst << a.pool.shift) + tid] =
+          id < 0 ? 0.f : a.pool.weights[(src << a.pool.shift) + (t & (bt - 1))];
     }
   }
   __syncthreads();
-  const uint64_t side = uint64_t(D) << a.pool.shift;
-  // A token of no block is moved as zeros.
-  const auto value = [](uint32_t code, int e) {
-    return e == kNoToken ? 0.f : __builtin_amdgcn_cvt_f32_fp8(int(code), 0) * exp2_int(e);
-  };
-  // Largest finite magnitudes, as f32 bits.
+
+  // Largest finite magnitudes, as f32 bits; a token of no block is zeros.
   uint32_t ak = 0, av = 0;
-  for (uint32_t u = tid; u < n * D; u += kThreads) {
-    const uint32_t i = u / D, d = u % D;
-    const uint8_t *src = a.pool.codes + from[i];
-    const uint32_t ck = src[kv_key_unit<D>(slot[i], d / 16) + d % 16] & 0x7fu;
-    const uint32_t cv = src[side + kv_value_byte<D>(slot[i], d)] & 0x7fu;
-    ak = max(ak, ck == 0x7fu ? 0u : f32_bits(value(ck, power[0][i])));
-    av = max(av, cv == 0x7fu ? 0u : f32_bits(value(cv, power[1][i])));
+  const auto magnitude = [](uint32_t code, int e) {
+    return f32_bits(__builtin_amdgcn_cvt_f32_fp8(int(code), 0) * exp2_int(e));
+  };
+  u32x4 keys[kKeyUnits];
+#pragma unroll
+  for (uint32_t r = 0; r < kKeyUnits; ++r) {
+    const uint32_t u = tid + r * kThreads, i = u / (D / 16), c = u % (D / 16);
+    keys[r] = u32x4{0u, 0u, 0u, 0u};
+    if (i < n && slot[i] != kNone) {
+      keys[r] = *reinterpret_cast<const u32x4 *>(a.pool.codes + from[i] +
+                                                 kv_key_unit<D>(slot[i], c));
+    }
+  }
+  const uint32_t vd = tid % kLanes / 16 * 32 + tid % 16;  // this lane's dims: vd, vd + 16
+  for (uint32_t i0 = 0; i0 < padded; i0 += kAhead * kTokens) {
+    u32x4 unit[kAhead];
+#pragma unroll
+    for (uint32_t r = 0; r < kAhead; ++r) {
+      const uint32_t i = i0 + r * kTokens + tid / kLanes;
+      unit[r] = u32x4{0u, 0u, 0u, 0u};
+      if (i < padded && slot[i] != kNone) {
+        unit[r] = *reinterpret_cast<const u32x4 *>(
+            a.pool.codes + from[i] + side + kv_value_byte<D>(slot[i], vd) / 16 * 16);
+      }
+    }
+#pragma unroll
+    for (uint32_t r = 0; r < kAhead; ++r) {
+      const uint32_t i = i0 + r * kTokens + tid / kLanes;
+      if (i < padded) {
+        const uint32_t byte = uint32_t(kv_value_byte<D>(slot[i] & (kMostBlock - 1), vd)) % 8;
+        const u32x4 w = unit[r];
+        const uint32_t x = (byte < 4 ? w.x : w.y) >> byte % 4 * 8 & 0xffu;
+        const uint32_t y = (byte < 4 ? w.z : w.w) >> byte % 4 * 8 & 0xffu;
+        uint8_t *to = image + kv_value_byte<D>(i, vd);
+        to[0] = uint8_t(x);
+        to[8] = uint8_t(y);
+        const uint32_t both = finite_codes(x | y << 8);
+        av = max(av, magnitude(max(both & 0xffu, both >> 8), power[1][i]));
+      }
+    }
+  }
+#pragma unroll
+  for (uint32_t r = 0; r < kKeyUnits; ++r) {
+    const uint32_t i = (tid + r * kThreads) / (D / 16);
+    if (i < n) {
+      ak = max(ak, magnitude(largest_code(keys[r]), power[0][i]));
+    }
   }
   block_umax2(ak, av);
   // Products of a code and a power of two are exact in bf16: their bits are
@@ -453,38 +648,38 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(KvEvictArgs a) {
     a.pool.exps[dst * 2] = int8_t(ek);
     a.pool.exps[dst * 2 + 1] = int8_t(ev);
   }
-  const float iv = exp2_int(-ev);
-  uint8_t *to = a.pool.codes + dst * 2 * side;
-  for (uint32_t u = tid; u < n * (D / 16); u += kThreads) {
-    const uint32_t i = u / (D / 16), c = u % (D / 16);
-    const u32x4 w = *reinterpret_cast<const u32x4 *>(a.pool.codes + from[i] +
-                                                     kv_key_unit<D>(slot[i], c));
-    // Only codes of zero and NaN meet a difference past the clamp upwards.
-    const int by = power[0][i] - ek;
-    const float f = exp2_int(by < -126 ? -126 : by > 126 ? 126 : by);
-    *reinterpret_cast<u32x4 *>(to + kv_key_unit<D>(i, c)) =
-        power[0][i] == kNoToken ? u32x4{0u, 0u, 0u, 0u} : rescale16(w, f);
+  if (tid < padded) {
+    factor[tid] = code_factor(power[1][tid], ev);
   }
-  for (uint32_t u = tid; u < (n + 31) / 32 * 4 * (D / 2); u += kThreads) {
-    const uint32_t set = u / (D / 2), r = u % (D / 2);
-    const uint32_t t32 = set / 4 * 32, g = set % 4, d = r / 16 * 32 + r % 16;
-    u32x4 w;
+  uint8_t *to = a.pool.codes + dst * 2 * side;
 #pragma unroll
-    for (uint32_t half = 0; half < 4; ++half) {
-      const uint32_t dd = d + 16 * (half / 2), i0 = 4 * (half % 2);
-      float x[4];
-#pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t t = t32 + value_token(g, i0 + i);
-        x[i] = 0.f;
-        if (t < n) {
-          const uint8_t code = a.pool.codes[from[t] + side + kv_value_byte<D>(slot[t], dd)];
-          x[i] = value(code, power[1][t]) * iv;
-        }
-      }
-      w[half] = encode4(x[0], x[1], x[2], x[3]);
+  for (uint32_t r = 0; r < kKeyUnits; ++r) {
+    const uint32_t u = tid + r * kThreads, i = u / (D / 16), c = u % (D / 16);
+    if (i < n) {
+      const float f = code_factor(power[0][i], ek);
+      *reinterpret_cast<u32x4 *>(to + kv_key_unit<D>(i, c)) =
+          f == 1.f ? keys[r] : rescale16(keys[r], f);
     }
-    *reinterpret_cast<u32x4 *>(to + side + kv_value_byte<D>(t32 + 4 * g, d)) = w;
+  }
+  __syncthreads();
+  for (uint32_t u = tid; u < padded * (D / 16); u += kThreads) {
+    // Unit u of the image: tokens t .. t + 3 and t + 16 .. t + 19.
+    const uint32_t t = u / (2 * D) * 32 + u % 64 / 16 * 4;
+    u32x4 w = reinterpret_cast<const u32x4 *>(image)[u];
+    const f32x4 f0 = *reinterpret_cast<const f32x4 *>(factor + t);
+    const f32x4 f1 = *reinterpret_cast<const f32x4 *>(factor + t + 16);
+    bool same = true;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      same = same && f0[i] == 1.f && f1[i] == 1.f;
+    }
+    if (!same) {
+      w.x = rescale4(w.x, f0);
+      w.y = rescale4(w.y, f1);
+      w.z = rescale4(w.z, f0);
+      w.w = rescale4(w.w, f1);
+    }
+    reinterpret_cast<u32x4 *>(to + side)[u] = w;
   }
 }
 
@@ -513,8 +708,15 @@ hipError_t launch_kv_gather(const KvGatherArgs &a, uint32_t dim, hipStream_t s) 
 }
 
 hipError_t launch_kv_evict(const KvEvictArgs &a, uint32_t dim, hipStream_t s) {
-  evict_select_kernel<<<dim3(a.pool.heads, a.seqs.batch), kSelectThreads, 0, s>>>(a);
   const uint32_t bt = 1u << a.pool.shift;
+  const dim3 units(a.pool.heads, a.seqs.batch);
+  // Keys of a thread: what the tables' size needs.  (16 sequences of up to
+  // 4500 tokens: 8 keys 11.4 us, 32 22.)
+  if (uint64_t(a.seqs.max_blocks) << a.pool.shift <= 8 * kSelectThreads) {
+    evict_select_kernel<8><<<units, kSelectThreads, 0, s>>>(a);
+  } else {
+    evict_select_kernel<32><<<units, kSelectThreads, 0, s>>>(a);
+  }
   const dim3 grid((a.keep + bt - 1) / bt, a.pool.heads, a.seqs.batch);
   if (dim == 64) {
     evict_move_kernel<64><<<grid, kThreads, 0, s>>>(a);
