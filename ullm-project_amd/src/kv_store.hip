@@ -52,6 +52,15 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
 __device__ __forceinline__ float scaled(uint16_t h, float inv) {
   return (h & 0x7f80u) == 0x7f80u ? __builtin_nanf("") : bf16_to_f32(h) * inv;
 }
+__device__ __forceinline__ u32x4 encode16(const Bf16x16 &x, float inv) {
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w[i] = encode4(scaled(x.v[4 * i], inv), scaled(x.v[4 * i + 1], inv),
+                   scaled(x.v[4 * i + 2], inv), scaled(x.v[4 * i + 3], inv));
+  }
+  return w;
+}
 // Four codes times powers of two, rounded to codes again.
 __device__ __forceinline__ uint32_t rescale4(uint32_t w, f32x4 f) {
   typedef float f2 __attribute__((ext_vector_type(2)));
@@ -94,12 +103,19 @@ __device__ __forceinline__ uint32_t value_token(uint32_t g, uint32_t j) {
   return 4 * g + j % 4 + 16 * (j / 4);
 }
 
-// One workgroup stores the new tokens of one block and head.  It reads the
-// new rows twice (the second time from L2): for the largest magnitude, then
-// to encode them.  Codes that were there are touched only when the exponent
-// grows, or where they share a 16-byte unit of values with a new one.
+constexpr uint32_t kMostBlock = 128;  // tokens of a block
+
+// One workgroup stores the new tokens of one block and head.  The new rows are
+// read once, into registers; with their largest magnitudes the exponents are
+// known.  Keys are written from there, values go through LDS, where a token's
+// bytes take their places among the others' of a 16-byte unit.  Codes that
+// were there are touched only when the exponent grows, or where they share a
+// unit with a new one.  (15760 tokens of 8 heads: @@ us; with rows read twice
+// and values two bytes at a time 33.)
 template <int D>
 __global__ __launch_bounds__(kThreads) void append_kernel(KvAppendArgs a, uint32_t each_slots) {
+  constexpr uint32_t kUnits = kMostBlock * (D / 16) / kThreads;  // of a thread
+  __shared__ __align__(16) uint8_t image[kMostBlock * D];        // the block's values
   const uint32_t bt = 1u << a.pool.shift, head = blockIdx.y, tid = threadIdx.x;
   const KvSlot slot = kv_find_slot(a.seqs, blockIdx.x, 1, bt, 2, each_slots);
   if (slot.seq >= a.seqs.batch) {
@@ -112,42 +128,51 @@ __global__ __launch_bounds__(kThreads) void append_kernel(KvAppendArgs a, uint32
   const uint32_t j = (first >> a.pool.shift) + slot.local;
   const uint32_t base = j << a.pool.shift;
   const uint32_t lo = first > base ? first - base : 0u;       // new tokens lo .. hi - 1
-  const uint32_t hi = length > base ? (length - base < bt ? length - base : bt) : 0u;
+  const uint32_t hi = uint32_t(min(max(int64_t(length) - base, int64_t(0)), int64_t(bt)));
   if (j >= a.seqs.max_blocks || lo >= hi) {
     return;
   }
   const int32_t id = kv_block(a.seqs.tables + slot.seq * a.seqs.stride, a.seqs, a.pool.blocks, j);
+  const uint64_t row0 = uint64_t(rows.first + (int64_t(base) - origin));  // row of token 0
+  const uint16_t *k = a.k + head * a.k_head, *v = a.v + head * a.v_head;
+  // Unit r of this thread: token t, dims 16c .. 16c + 15.
+  const auto token = [&](uint32_t r) { return lo + (tid + r * kThreads) / (D / 16); };
+  const uint32_t c = tid % (D / 16);
+  Bf16x16 x[kUnits], y[kUnits];
+#pragma unroll
+  for (uint32_t r = 0; r < kUnits; ++r) {
+    x[r] = Bf16x16{};
+    y[r] = Bf16x16{};
+    if (token(r) < hi) {
+      const uint64_t row = row0 + token(r);
+      x[r] = load16(k + row * a.k_row + c * 16, a.vec);
+      y[r] = load16(v + row * a.v_row + c * 16, a.vec);
+    }
+  }
   if (id < 0) {
     return;
   }
   const uint64_t unit = uint64_t(id) * a.pool.heads + head;
-  const uint64_t row0 = uint64_t(rows.first + (int64_t(base) - origin));  // row of token 0
-  const uint16_t *k = a.k + head * a.k_head, *v = a.v + head * a.v_head;
-
+  const int ek0 = a.pool.exps[unit * 2], ev0 = a.pool.exps[unit * 2 + 1];
   uint32_t ak = 0, av = 0;
-  for (uint32_t u = tid; u < (hi - lo) * (D / 16); u += kThreads) {
-    const uint64_t row = row0 + lo + u / (D / 16);
-    const uint32_t c = u % (D / 16) * 16;
-    const Bf16x16 x = load16(k + row * a.k_row + c, a.vec);
-    const Bf16x16 y = load16(v + row * a.v_row + c, a.vec);
+#pragma unroll
+  for (uint32_t r = 0; r < kUnits; ++r) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      ak = max(ak, finite_magnitude(x.v[i]));
-      av = max(av, finite_magnitude(y.v[i]));
+      ak = max(ak, finite_magnitude(x[r].v[i]));
+      av = max(av, finite_magnitude(y[r].v[i]));
     }
   }
   block_umax2(ak, av);
   int ek = exponent_for(ak), ev = exponent_for(av);
   float fk = 1.f, fv = 1.f;  // factor of the codes that were there
   if (lo > 0) {
-    const int ek0 = a.pool.exps[unit * 2], ev0 = a.pool.exps[unit * 2 + 1];
     ek = max(ek, ek0);
     ev = max(ev, ev0);
     fk = exp2_int(max(ek0 - ek, -126));
     fv = exp2_int(max(ev0 - ev, -126));
   }
-  __syncthreads();  // the old exponents are read
-  if (tid == 0) {
+  if (tid == 0) {  // all have read the old ones
     a.pool.exps[unit * 2] = int8_t(ek);
     a.pool.exps[unit * 2 + 1] = int8_t(ev);
   }
@@ -155,62 +180,54 @@ __global__ __launch_bounds__(kThreads) void append_kernel(KvAppendArgs a, uint32
   uint8_t *kc = a.pool.codes + unit * (uint64_t(2 * D) << a.pool.shift);
   uint8_t *vc = kc + (uint64_t(D) << a.pool.shift);
 
-  const uint32_t kfrom = fk != 1.f ? 0u : lo;
-  for (uint32_t u = tid; u < (hi - kfrom) * (D / 16); u += kThreads) {
-    const uint32_t t = kfrom + u / (D / 16), c = u % (D / 16);
-    u32x4 *at = reinterpret_cast<u32x4 *>(kc + kv_key_unit<D>(t, c));
-    if (t < lo) {
+  if (fk != 1.f) {
+    for (uint32_t u = tid; u < lo * (D / 16); u += kThreads) {
+      u32x4 *at = reinterpret_cast<u32x4 *>(kc + kv_key_unit<D>(u / (D / 16), c));
       *at = rescale16(*at, fk);
-    } else {
-      const Bf16x16 x = load16(k + (row0 + t) * a.k_row + c * 16, a.vec);
-      u32x4 w;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w[i] = encode4(scaled(x.v[4 * i], ik), scaled(x.v[4 * i + 1], ik),
-                       scaled(x.v[4 * i + 2], ik), scaled(x.v[4 * i + 3], ik));
-      }
-      *at = w;
     }
   }
-
-  // Units of 8 tokens x 2 dims, D / 2 of them for each lane group of 32 tokens.
-  const uint32_t vfrom = fv != 1.f ? 0u : lo;
-  const uint32_t s0 = vfrom / 32 * 4, s1 = (hi + 31) / 32 * 4;
-  for (uint32_t u = tid; u < (s1 - s0) * (D / 2); u += kThreads) {
-    const uint32_t set = s0 + u / (D / 2), r = u % (D / 2);
-    const uint32_t t32 = set / 4 * 32, g = set % 4, d = r / 16 * 32 + r % 16;
-    uint32_t fresh = 0;  // new tokens of the eight
-    bool kept = false;
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-      const uint32_t t = t32 + value_token(g, i);
-      fresh |= t >= lo && t < hi ? 1u << i : 0u;
-      kept = kept || t < lo;
+  for (uint32_t r = 0; r < kUnits; ++r) {
+    const uint32_t t = token(r);
+    if (t < hi) {
+      *reinterpret_cast<u32x4 *>(kc + kv_key_unit<D>(t, c)) = encode16(x[r], ik);
+      const u32x4 w = encode16(y[r], iv);
+      uint8_t *at = image + kv_value_byte<D>(t, c * 16);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        at[i * 16] = uint8_t(w[i / 4] >> (8 * (i % 4)));
+      }
     }
-    if (fresh == 0 && (fv == 1.f || !kept)) {
+  }
+  __syncthreads();
+  // Units of 8 tokens x 2 dims: unit u of the block's has tokens t .. t + 3 and
+  // t + 16 .. t + 19.
+  const uint32_t vfrom = fv != 1.f ? 0u : lo / 32 * 32;
+  for (uint32_t u = vfrom * (D / 16) + tid; u < (hi + 31) / 32 * (2 * D); u += kThreads) {
+    const uint32_t t = u / (2 * D) * 32 + u % 64 / 16 * 4;
+    // Bytes of the new ones among four tokens from t0 on.  (Signed differences:
+    // of an unsigned one that a condition guards the compiler has concluded
+    // that the condition always holds.)
+    const auto bytes = [&](uint32_t t0) {
+      const auto below = [&](uint32_t end) {
+        const int n = min(max(int(end) - int(t0), 0), 4);
+        return uint32_t((uint64_t(1) << (8 * n)) - 1);
+      };
+      return below(hi) & ~below(lo);
+    };
+    const uint32_t new0 = bytes(t), new1 = bytes(t + 16);
+    const bool kept = t < lo;
+    if ((new0 | new1) == 0 && (fv == 1.f || !kept)) {
       continue;
     }
-    u32x4 *at = reinterpret_cast<u32x4 *>(vc + kv_value_byte<D>(t32 + 4 * g, d));
+    u32x4 *at = reinterpret_cast<u32x4 *>(vc) + u;
+    const u32x4 now = reinterpret_cast<const u32x4 *>(image)[u];
     u32x4 w = {0u, 0u, 0u, 0u};
     if (kept) {
       w = fv != 1.f ? rescale16(*at, fv) : *at;
     }
-#pragma unroll
-    for (uint32_t half = 0; half < 4; ++half) {  // dim d or d + 16, tokens 0..3 or 4..7
-      const uint32_t dd = d + 16 * (half / 2), i0 = 4 * (half % 2);
-      float x[4];
-      uint32_t mask = 0;
-#pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) {
-        const bool is = (fresh >> (i0 + i)) & 1u;
-        const uint64_t row = row0 + t32 + value_token(g, i0 + i);
-        x[i] = is ? scaled(v[row * a.v_row + dd], iv) : 0.f;
-        mask |= is ? 0xffu << (8 * i) : 0u;
-      }
-      const uint32_t now = encode4(x[0], x[1], x[2], x[3]);
-      w[half] = (now & mask) | (w[half] & ~mask);
-    }
-    *at = w;
+    *at = u32x4{(now.x & new0) | (w.x & ~new0), (now.y & new1) | (w.y & ~new1),
+                (now.z & new0) | (w.z & ~new0), (now.w & new1) | (w.w & ~new1)};
   }
   if (a.pool.weights != nullptr) {
     for (uint32_t t = lo + tid; t < hi; t += kThreads) {
@@ -220,66 +237,102 @@ __global__ __launch_bounds__(kThreads) void append_kernel(KvAppendArgs a, uint32
   }
 }
 
-// One workgroup reads one row: all heads of a token.
+// Two times eight codes as bf16, times a power of two.
+__device__ __forceinline__ void store_decoded(uint16_t *to, u32x4 w, float f) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  u32x4 o[2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f2 x = __builtin_amdgcn_cvt_pk_f32_fp8(int(w[i]), false);
+    const f2 y = __builtin_amdgcn_cvt_pk_f32_fp8(int(w[i]), true);
+    o[i / 2][i % 2 * 2] = f32x2_to_bf16x2(x[0] * f, x[1] * f);
+    o[i / 2][i % 2 * 2 + 1] = f32x2_to_bf16x2(y[0] * f, y[1] * f);
+  }
+  reinterpret_cast<u32x4 *>(to)[0] = o[0];
+  reinterpret_cast<u32x4 *>(to)[1] = o[1];
+}
+
+// One workgroup reads 32 tokens of one head, from a multiple of 32 on: 16
+// bytes to a thread and load; values are brought into rows in LDS.  (15760
+// tokens of 8 heads: @@ us; a workgroup for each row, which fetches all it
+// needs to know for 4 KiB, 36.)
 template <int D>
-__global__ __launch_bounds__(kThreads) void gather_kernel(KvGatherArgs a) {
-  const KvSlot slot = kv_find_slot(a.seqs, blockIdx.x, 1, 1, 0, a.seqs.each);
+__global__ __launch_bounds__(kThreads) void gather_kernel(KvGatherArgs a, uint32_t each_slots) {
+  constexpr uint32_t kUnits = 32 * (D / 16);  // of a side
+  constexpr uint32_t kPitch = D + 16;
+  __shared__ __align__(16) uint8_t values[32 * kPitch];
+  const uint32_t head = blockIdx.y, tid = threadIdx.x;
+  const KvSlot slot = kv_find_slot(a.seqs, blockIdx.x, 1, 32, 2, each_slots);
   if (slot.seq >= a.seqs.batch) {
     return;
   }
   const KvRows rows = slot.rows;
-  if (slot.local >= rows.count) {
+  const uint32_t length = kv_length(a.seqs, a.pool.shift, slot.seq);
+  const int64_t origin = int64_t(length) - rows.count;  // position of the first row
+  const int64_t base = (origin >> 5) * 32 + int64_t(slot.local) * 32;
+  const uint32_t lo = origin > base ? uint32_t(origin - base) : 0u;  // tokens lo .. hi - 1
+  const uint32_t hi = uint32_t(min(max(length - base, int64_t(0)), int64_t(32)));
+  if (lo >= hi) {
     return;
   }
-  const uint64_t row = rows.first + slot.local;
-  const int64_t at =
-      int64_t(kv_length(a.seqs, a.pool.shift, slot.seq)) - rows.count + slot.local;
-  const uint32_t t = uint32_t(at) & ((1u << a.pool.shift) - 1);
-  const int32_t id = at < 0 ? -1
-                            : kv_block(a.seqs.tables + slot.seq * a.seqs.stride, a.seqs,
-                                       a.pool.blocks, uint32_t(at) >> a.pool.shift);
-  const uint32_t per = D / 16;
-  for (uint32_t u = threadIdx.x; u < a.pool.heads * per; u += kThreads) {
-    const uint32_t head = u / per, c = u % per;
-    const uint64_t unit = uint64_t(id < 0 ? 0 : id) * a.pool.heads + head;
-    const uint8_t *codes = a.pool.codes + unit * (uint64_t(2 * D) << a.pool.shift);
+  // Rows before the first position, and those of no block, are zeros.
+  const int32_t id = base < 0 ? -1
+                              : kv_block(a.seqs.tables + slot.seq * a.seqs.stride, a.seqs,
+                                         a.pool.blocks, uint32_t(base) >> a.pool.shift);
+  const uint32_t in_block = uint32_t(base) & ((1u << a.pool.shift) - 1);
+  const uint64_t unit = uint64_t(id < 0 ? 0 : id) * a.pool.heads + head;
+  const int64_t row0 = int64_t(rows.first) + (base - origin);
+  const uint8_t *keys =
+      a.pool.codes + unit * (uint64_t(2 * D) << a.pool.shift) + uint64_t(in_block) * D;
+  const uint8_t *side1 = keys + (uint64_t(D) << a.pool.shift);
+  const float fk = exp2_int(a.pool.exps[unit * 2]), fv = exp2_int(a.pool.exps[unit * 2 + 1]);
+  // Threads take the keys' units, then the values'.
+  constexpr uint32_t kTurns = 2 * kUnits / kThreads;
+  u32x4 w[kTurns];
 #pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      uint16_t *to = side == 0 ? a.k : a.v;
-      if (to == nullptr) {
-        continue;
-      }
-      u32x4 w = {0u, 0u, 0u, 0u};
-      float f = 1.f;
-      if (id >= 0) {
-        f = exp2_int(a.pool.exps[unit * 2 + side]);
-        if (side == 0) {
-          w = *reinterpret_cast<const u32x4 *>(codes + kv_key_unit<D>(t, c));
-        } else {
-          const uint8_t *vc = codes + (uint64_t(D) << a.pool.shift) + kv_value_byte<D>(t, c * 16);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            w[i / 4] |= uint32_t(vc[i * 16]) << (8 * (i % 4));
-          }
-        }
-      }
-      u32x4 o[2];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        typedef float f2 __attribute__((ext_vector_type(2)));
-        const f2 x = __builtin_amdgcn_cvt_pk_f32_fp8(int(w[i]), false);
-        const f2 y = __builtin_amdgcn_cvt_pk_f32_fp8(int(w[i]), true);
-        o[i / 2][i % 2 * 2] = f32x2_to_bf16x2(x[0] * f, x[1] * f);
-        o[i / 2][i % 2 * 2 + 1] = f32x2_to_bf16x2(y[0] * f, y[1] * f);
-      }
-      u32x4 *p = reinterpret_cast<u32x4 *>(to + (row * a.pool.heads + head) * D + c * 16);
-      p[0] = o[0];
-      p[1] = o[1];
+  for (uint32_t r = 0; r < kTurns; ++r) {
+    const uint32_t u = tid + r * kThreads;
+    w[r] = u32x4{0u, 0u, 0u, 0u};
+    if (id >= 0) {
+      w[r] = u < kUnits ? *reinterpret_cast<const u32x4 *>(
+                              keys + kv_key_unit<D>(u / (D / 16), u % (D / 16)))
+                        : reinterpret_cast<const u32x4 *>(side1)[u - kUnits];
     }
-    if (a.weights != nullptr && c == 0) {
-      a.weights[row * a.pool.heads + head] =
-          id < 0 ? 0.f : a.pool.weights[(unit << a.pool.shift) + t];
+  }
+  const auto row_of = [&](uint16_t *to, uint32_t u) {
+    return to + (uint64_t(row0 + u / (D / 16)) * a.pool.heads + head) * D + u % (D / 16) * 16;
+  };
+  const auto live = [&](uint32_t u) { return u / (D / 16) >= lo && u / (D / 16) < hi; };
+#pragma unroll
+  for (uint32_t r = 0; r < kTurns; ++r) {
+    const uint32_t u = tid + r * kThreads;
+    if (u < kUnits) {
+      if (a.k != nullptr && live(u)) {
+        store_decoded(row_of(a.k, u), w[r], fk);
+      }
+    } else {
+      const uint32_t l = (u - kUnits) % 64, d = (u - kUnits) / 64 * 32 + l % 16;
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i) {
+        values[value_token(l / 16, i % 8) * kPitch + d + 16 * (i / 8)] =
+            uint8_t(w[r][i / 4] >> (8 * (i % 4)));
+      }
     }
+  }
+  __syncthreads();
+  if (a.v != nullptr) {
+    for (uint32_t u = tid; u < kUnits; u += kThreads) {
+      if (live(u)) {
+        store_decoded(row_of(a.v, u),
+                      *reinterpret_cast<const u32x4 *>(values + u / (D / 16) * kPitch +
+                                                       u % (D / 16) * 16),
+                      fv);
+      }
+    }
+  }
+  if (a.weights != nullptr && tid >= lo && tid < hi) {
+    a.weights[uint64_t(row0 + tid) * a.pool.heads + head] =
+        id < 0 ? 0.f : a.pool.weights[(unit << a.pool.shift) + in_block + tid];
   }
 }
 
@@ -536,8 +589,6 @@ __device__ __forceinline__ float code_factor(int from, int to) {
   return exp2_int(by < -126 ? -126 : by > 126 ? 126 : by);
 }
 
-constexpr uint32_t kMostBlock = 128;  // tokens of a block
-
 // One workgroup fills one block and head of the new tables with the tokens
 // that stay.  All codes are read once: the keys' 16 bytes stay in registers,
 // and of the values' units, which a token shares with seven others, its two
@@ -699,10 +750,12 @@ hipError_t launch_kv_append(const KvAppendArgs &a, uint32_t dim, hipStream_t s) 
 }
 
 hipError_t launch_kv_gather(const KvGatherArgs &a, uint32_t dim, hipStream_t s) {
+  const uint32_t each = a.seqs.each == 0 ? 1 : (a.seqs.each + 30) / 32 + 1;
+  const dim3 grid(uint32_t(kv_slots(a.seqs, 1, 32, 2, each)), a.pool.heads);
   if (dim == 64) {
-    gather_kernel<64><<<a.seqs.rows, kThreads, 0, s>>>(a);
+    gather_kernel<64><<<grid, kThreads, 0, s>>>(a, each);
   } else {
-    gather_kernel<128><<<a.seqs.rows, kThreads, 0, s>>>(a);
+    gather_kernel<128><<<grid, kThreads, 0, s>>>(a, each);
   }
   return hipGetLastError();
 }
