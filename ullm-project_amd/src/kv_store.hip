@@ -110,13 +110,13 @@ constexpr uint32_t kMostBlock = 128;  // tokens of a block
 // known.  Keys are written from there, values go through LDS, where a token's
 // bytes take their places among the others' of a 16-byte unit.  Codes that
 // were there are touched only when the exponent grows, or where they share a
-// unit with a new one.  (15760 tokens of 8 heads: @@ us; with rows read twice
+// unit with a new one.  (15760 tokens of 8 heads: 21 us; with rows read twice
 // and values two bytes at a time 33.)
-template <int D>
+template <int D, uint32_t bt>
 __global__ __launch_bounds__(kThreads) void append_kernel(KvAppendArgs a, uint32_t each_slots) {
-  constexpr uint32_t kUnits = kMostBlock * (D / 16) / kThreads;  // of a thread
-  __shared__ __align__(16) uint8_t image[kMostBlock * D];        // the block's values
-  const uint32_t bt = 1u << a.pool.shift, head = blockIdx.y, tid = threadIdx.x;
+  constexpr uint32_t kUnits = (bt * (D / 16) + kThreads - 1) / kThreads;  // of a thread
+  __shared__ __align__(16) uint8_t image[bt * D];  // the block's values
+  const uint32_t head = blockIdx.y, tid = threadIdx.x;
   const KvSlot slot = kv_find_slot(a.seqs, blockIdx.x, 1, bt, 2, each_slots);
   if (slot.seq >= a.seqs.batch) {
     return;
@@ -254,7 +254,7 @@ __device__ __forceinline__ void store_decoded(uint16_t *to, u32x4 w, float f) {
 
 // One workgroup reads 32 tokens of one head, from a multiple of 32 on: 16
 // bytes to a thread and load; values are brought into rows in LDS.  (15760
-// tokens of 8 heads: @@ us; a workgroup for each row, which fetches all it
+// tokens of 8 heads: 15 us; a workgroup for each row, which fetches all it
 // needs to know for 4 KiB, 36.)
 template <int D>
 __global__ __launch_bounds__(kThreads) void gather_kernel(KvGatherArgs a, uint32_t each_slots) {
@@ -741,10 +741,13 @@ hipError_t launch_kv_append(const KvAppendArgs &a, uint32_t dim, hipStream_t s) 
   // A sequence's n rows touch at most (n + bt - 2) / bt + 1 blocks.
   const uint32_t each = a.seqs.each == 0 ? 1 : (a.seqs.each + bt - 2) / bt + 1;
   const dim3 grid(uint32_t(kv_slots(a.seqs, 1, bt, 2, each)), a.pool.heads);
+  const auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(a, each); };
   if (dim == 64) {
-    append_kernel<64><<<grid, kThreads, 0, s>>>(a, each);
+    launch(bt == 32 ? append_kernel<64, 32> : bt == 64 ? append_kernel<64, 64>
+                                                       : append_kernel<64, 128>);
   } else {
-    append_kernel<128><<<grid, kThreads, 0, s>>>(a, each);
+    launch(bt == 32 ? append_kernel<128, 32> : bt == 64 ? append_kernel<128, 64>
+                                                        : append_kernel<128, 128>);
   }
   return hipGetLastError();
 }
