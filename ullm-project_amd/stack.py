@@ -2,12 +2,19 @@
 
 BASELINE configuration #5: 32 decoder layers (hidden 4096, 32 q / 8 kv heads
 x 128, FFN 14336) plus the 128256-row lm_head, every weight AQ4 g128, batch 8
-single-token decode.  Only the linear layers are on the path; the reference
-defines no attention or norm numerics for it, so fixed stand-ins keep the
-chain well-defined and bounded:
+single-token decode.  The reference defines no attention or norm numerics for
+it, so fixed stand-ins keep the chain well-defined and bounded:
 
-  * attention output = the q slice (first 4096 columns) of the qkv output,
-    read in place as a strided view (x_row_stride = 6144);
+  * attention output, by default the q slice (first 4096 columns) of the qkv
+    output, read in place as a strided view (x_row_stride = 6144).  With
+    context=N it is attention over an 8-bit key/value cache of up to N tokens
+    for each sequence instead: prompt() takes the sequences' first rows,
+    step() one more each, and with evict_to=T evict() cuts each sequence to
+    the T tokens per head that received most of the weight.  Queries, keys
+    and values are the strided thirds of the qkv output.  Scores are not
+    scaled (scale = 1 instead of 1 / sqrt(128)): those of unit normal rows
+    are then far apart, and the output of a row stays near unit RMS however
+    many tokens it sees, as the missing norms would have it;
   * MLP activation, by default the pass-through stand-in: the gate half
     (first 14336 columns) of the gate_up output, read in place
     (x_row_stride = 28672).  With swiglu=True it is the real SwiGLU gate
@@ -27,8 +34,9 @@ chain well-defined and bounded:
     are available as ULLM_LINEAR_EPILOGUE_RESIDUAL_ADD; without the norms a
     residual stream is not bounded either, so the stand-in chain omits them.)
 
-Per step: 4 x 32 + 1 = 129 forward calls through the C ABI, all on one stream;
-the caller may capture them in a HIP graph.
+Per step: 4 x 32 + 1 = 129 forward calls through the C ABI (and, with a cache,
+an append and an attention call per layer), all on one stream; the caller may
+capture them in a HIP graph.
 """
 from __future__ import annotations
 
@@ -67,7 +75,7 @@ class DecodeStack:
 
     def __init__(self, uh, torch, device, batch=8, layers=LAYERS, hidden=HIDDEN,
                  qkv=QKV, ffn=FFN, vocab=VOCAB, seed=0, weights=None,
-                 swiglu=False):
+                 swiglu=False, context=0, head_dim=128, block_tokens=64, evict_to=0):
         self.uh, self.torch, self.dev = uh, torch, device
         self.m, self.layers = batch, layers
         self.hidden, self.qkv, self.ffn, self.vocab = hidden, qkv, ffn, vocab
@@ -112,21 +120,103 @@ class DecodeStack:
         self.alpha_h = 1.0 / (0.02 * math.sqrt(hidden))
         self.alpha_f = 1.0 / (0.02 * math.sqrt(ffn) * (SILU_RMS if swiglu else 1.0))
 
-    def step(self, stream=None):
-        """One decode step: self.h0 -> layers -> self.logits."""
+        self.caches = []
+        self.evict_to = evict_to
+        if context:
+            self._make_caches(context, head_dim, block_tokens)
+
+    def _make_caches(self, context, dim, block_tokens):
+        """One cache per layer; all share the tables, of which sequence b has
+        row b, and the blocks that evict() moves tokens into."""
+        torch = self.torch
+        self.head_dim, self.kv_heads = dim, (self.qkv - self.hidden) // (2 * dim)
+        columns = -(-context // block_tokens)
+        moved = -(-self.evict_to // block_tokens)
+        if moved > columns:
+            raise ValueError("evict_to must not exceed context")
+        ids = torch.arange(self.m * (columns + moved), dtype=torch.int32, device=self.dev)
+        self.tables = ids[:self.m * columns].view(self.m, columns)
+        self.spare = ids[self.m * columns:].view(self.m, moved)
+        self.lengths = torch.zeros((self.m,), dtype=torch.int32, device=self.dev)
+        self.caches = [self.uh.KvCache(ids.numel(), self.kv_heads, dim,
+                                       block_tokens=block_tokens,
+                                       track_weights=self.evict_to > 0,
+                                       device=torch.device(self.dev).index or 0)
+                       for _ in range(self.layers)]
+        self.attn = torch.empty((self.m, self.hidden), dtype=torch.bfloat16, device=self.dev)
+
+    def _attention(self, layer, qkv, out, starts, stream):
+        """Store the rows' keys and values, attend from their queries."""
+        if not self.caches:
+            return qkv[:, :self.hidden]
+        cache, dim = self.caches[layer], self.head_dim
+        rows, k0 = qkv.shape[0], self.hidden
+        v0 = k0 + self.kv_heads * dim
+        heads = [qkv[:, a:b].view(rows, -1, dim) for a, b in
+                 ((0, k0), (k0, v0), (v0, v0 + self.kv_heads * dim))]
+        cache.append(heads[1], heads[2], self.lengths, self.tables, starts=starts, stream=stream)
+        cache.attend(heads[0], self.lengths, self.tables, starts=starts,
+                     out=out.view(rows, -1, dim), scale=1.0,
+                     accumulate=self.evict_to > 0, stream=stream)
+        return out
+
+    def _layers(self, h0, h, qkv_out, attn, o_out, act, starts, stream):
         for i, ws in enumerate(self.weights):
-            ws["qkv"].forward(self.h0 if i == 0 else self.h, self.qkv_out,
-                              alpha=self.alpha_h, stream=stream)
-            ws["o"].forward(self.qkv_out[:, :self.hidden], self.o_out,
+            ws["qkv"].forward(h0 if i == 0 else h, qkv_out, alpha=self.alpha_h,
+                              stream=stream)
+            ws["o"].forward(self._attention(i, qkv_out, attn, starts, stream), o_out,
                             alpha=self.alpha_h, stream=stream)
-            ws["gate_up"].forward(self.o_out, self.act, alpha=self.alpha_h,
-                                  stream=stream)
-            ws["down"].forward(self.act[:, :self.ffn], self.h, alpha=self.alpha_f,
-                               stream=stream)
+            ws["gate_up"].forward(o_out, act, alpha=self.alpha_h, stream=stream)
+            ws["down"].forward(act[:, :self.ffn], h, alpha=self.alpha_f, stream=stream)
+
+    def step(self, stream=None):
+        """One decode step: self.h0 -> layers -> self.logits.  With a cache
+        every sequence grows by the step's token (on torch's current stream,
+        which `stream` must then be)."""
+        if self.caches:
+            self.lengths.add_(1)
+        self._layers(self.h0, self.h, self.qkv_out, self.attn if self.caches else None,
+                     self.o_out, self.act, None, stream)
         self.lm_head.forward(self.h, self.logits, alpha=self.alpha_h, stream=stream)
         return self.logits
 
+    def prompt(self, h, counts):
+        """The first (or next) counts[b] tokens of each sequence b, at least
+        one, as rows of h (bf16 [sum(counts)][hidden]) in the order of the
+        sequences: self.logits of their last ones."""
+        torch, rows = self.torch, h.shape[0]
+        if not self.caches or len(counts) != self.m or min(counts) < 1 or sum(counts) != rows:
+            raise ValueError("prompt needs a cache, and a count of rows for each sequence")
+        n = torch.tensor(counts, dtype=torch.int32, device=self.dev)
+        ends = n.cumsum(0, dtype=torch.int32)
+        starts = torch.cat([torch.zeros_like(ends[:1]), ends])
+        self.lengths.add_(n)
+        x, qkv, attn, o, act = (torch.empty((rows, c), dtype=torch.bfloat16, device=self.dev)
+                                for c in (self.hidden, self.qkv, self.hidden, self.hidden,
+                                          self.act.shape[1]))
+        self._layers(h, x, qkv, attn, o, act, starts, None)
+        self.h.copy_(x[(ends - 1).long()])
+        self.lm_head.forward(self.h, self.logits, alpha=self.alpha_h)
+        return self.logits
+
+    def evict(self, sink=4, recent=0):
+        """Cut every sequence to its evict_to tokens of most weight in each
+        head and layer, the first `sink` and last `recent` among them; the
+        blocks that they leave are the next call's to move into."""
+        if not self.evict_to:
+            raise ValueError("evict needs a stack with evict_to")
+        for cache in self.caches:
+            lengths, _ = cache.evict(self.lengths, self.tables, self.spare, self.evict_to,
+                                     sink=sink, recent=recent)
+        left = self.tables.clone()
+        moved = self.spare.shape[1]
+        self.tables[:, :moved] = self.spare
+        self.spare.copy_(left[:, :moved])
+        self.lengths.copy_(lengths)
+
     def destroy(self):
+        for cache in self.caches:
+            cache.destroy()
         for ws in self.weights:
             for w in ws.values():
                 w.destroy()
