@@ -293,7 +293,7 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(KvGatherArgs a, uint32
   for (uint32_t r = 0; r < kTurns; ++r) {
     const uint32_t u = tid + r * kThreads;
     w[r] = u32x4{0u, 0u, 0u, 0u};
-    if (id >= 0) {
+    if (id >= 0 && (u < kUnits ? a.k : a.v) != nullptr) {
       w[r] = u < kUnits ? *reinterpret_cast<const u32x4 *>(
                               keys + kv_key_unit<D>(u / (D / 16), u % (D / 16)))
                         : reinterpret_cast<const u32x4 *>(side1)[u - kUnits];
@@ -333,6 +333,38 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(KvGatherArgs a, uint32
   if (a.weights != nullptr && tid >= lo && tid < hi) {
     a.weights[uint64_t(row0 + tid) * a.pool.heads + head] =
         id < 0 ? 0.f : a.pool.weights[(unit << a.pool.shift) + in_block + tid];
+  }
+}
+
+constexpr uint32_t kWeightRows = 128;
+
+// Weights alone: one workgroup reads 128 rows of all heads.  (131072 tokens of
+// 8 heads: 4.4 us; by the kernel above, whose workgroups fetch all they need to
+// know for 128 bytes, 43.)
+__global__ __launch_bounds__(kThreads) void gather_weights_kernel(KvGatherArgs a,
+                                                                  uint32_t each_slots) {
+  const KvSlot slot = kv_find_slot(a.seqs, blockIdx.x, 1, kWeightRows, 1, each_slots);
+  if (slot.seq >= a.seqs.batch) {
+    return;
+  }
+  const KvRows rows = slot.rows;
+  const uint32_t first = slot.local * kWeightRows;
+  if (first >= rows.count) {
+    return;
+  }
+  const uint32_t n = min(rows.count - first, kWeightRows);
+  const int64_t at =
+      int64_t(kv_length(a.seqs, a.pool.shift, slot.seq)) - rows.count + first;
+  const int32_t *table = a.seqs.tables + slot.seq * a.seqs.stride;
+  float *to = a.weights + uint64_t(rows.first + first) * a.pool.heads;
+  for (uint32_t u = threadIdx.x; u < n * a.pool.heads; u += kThreads) {
+    const int64_t t = at + u / a.pool.heads;
+    const int32_t id =
+        t < 0 ? -1 : kv_block(table, a.seqs, a.pool.blocks, uint32_t(t) >> a.pool.shift);
+    const uint64_t unit = uint64_t(id < 0 ? 0 : id) * a.pool.heads + u % a.pool.heads;
+    const float w =
+        a.pool.weights[(unit << a.pool.shift) + (uint32_t(t) & ((1u << a.pool.shift) - 1))];
+    to[u] = id < 0 ? 0.f : w;
   }
 }
 
@@ -753,6 +785,12 @@ hipError_t launch_kv_append(const KvAppendArgs &a, uint32_t dim, hipStream_t s) 
 }
 
 hipError_t launch_kv_gather(const KvGatherArgs &a, uint32_t dim, hipStream_t s) {
+  if (a.k == nullptr && a.v == nullptr) {
+    const uint32_t each = (a.seqs.each + kWeightRows - 1) / kWeightRows;
+    gather_weights_kernel<<<uint32_t(kv_slots(a.seqs, 1, kWeightRows, 1, each)), kThreads, 0, s>>>(
+        a, each);
+    return hipGetLastError();
+  }
   const uint32_t each = a.seqs.each == 0 ? 1 : (a.seqs.each + 30) / 32 + 1;
   const dim3 grid(uint32_t(kv_slots(a.seqs, 1, 32, 2, each)), a.pool.heads);
   if (dim == 64) {

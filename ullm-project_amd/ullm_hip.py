@@ -845,9 +845,12 @@ class KvCache:
                        stream, workspace):
         heads, dim = q.shape[1], self.head_dim
         rows, q_row, q_head = _strides3(q, "q", heads, dim)
-        out_rows, out_row, out_head = _strides3(out, "out", heads, dim)
-        if out_rows != rows:
-            raise ValueError("q and out must have the same number of rows")
+        if out is None:
+            out, out_row, out_head = q.new_empty((rows, heads, dim)), 0, 0
+        else:
+            out_rows, out_row, out_head = _strides3(out, "out", heads, dim)
+            if out_rows != rows:
+                raise ValueError("q and out must have the same number of rows")
         if lse is None:
             lse_at = 0
         elif lse.shape != (rows, heads) or not lse.is_contiguous() \
@@ -857,32 +860,31 @@ class KvCache:
             lse_at = lse.data_ptr()
         ws, wb = (0, 0) if workspace is None else \
             (workspace.data_ptr(), workspace.numel() * workspace.element_size())
-        return (self.handle or 0, *self._seqs(lengths, tables, rows, starts), q.data_ptr(), q_row,
-                q_head, out.data_ptr(), out_row, out_head, lse_at, heads, window,
-                dim ** -0.5 if scale is None else scale,
-                KV_ATTEND_ACCUMULATE if accumulate else 0, _stream(stream) or 0, ws, wb)
+        return out, (self.handle or 0, *self._seqs(lengths, tables, rows, starts), q.data_ptr(),
+                     q_row, q_head, out.data_ptr(), out_row, out_head, lse_at, heads, window,
+                     dim ** -0.5 if scale is None else scale,
+                     KV_ATTEND_ACCUMULATE if accumulate else 0, _stream(stream) or 0, ws, wb)
 
     def attend(self, q, lengths, tables, starts=None, out=None, lse=None, scale=None, window=0,
                accumulate=False, stream=None, workspace=None):
         """Causal attention of q (bf16 [rows][heads][head_dim], row and head
-        strides honoured) over the cached tokens: bf16 like q.  ``scale``
+        strides honoured) over the cached tokens, bf16 [rows][heads][head_dim].  ``scale``
         defaults to 1 / sqrt(head_dim); with ``window`` a query sees that many
         tokens; ``lse`` (f32 [rows][heads]) receives the log of each row's sum;
         ``accumulate`` adds to the weights of the tokens.  A query that sees
         no token gives zeros."""
-        if out is None:
-            out = _torch().empty_like(q)
-        _call(lib().ullm_kv_cache_attend, _packed(KvAttendDesc).fill(*self._attend_fields(
-            q, lengths, tables, starts, out, lse, scale, window, accumulate, stream, workspace)))
+        out, fields = self._attend_fields(q, lengths, tables, starts, out, lse, scale, window,
+                                          accumulate, stream, workspace)
+        _call(lib().ullm_kv_cache_attend, _packed(KvAttendDesc).fill(*fields))
         return out
 
     def attend_plan(self, q, lengths, tables, starts=None, out=None, lse=None, scale=None,
                     window=0, accumulate=False, stream=None, workspace=None) -> KvAttendPlan:
         """The launch and the workspace of attend() with these arguments
         (ullm_kv_cache_attend_plan); launches nothing."""
-        ref = _packed(KvAttendDesc).fill(*self._attend_fields(
-            q, lengths, tables, starts, q if out is None else out, lse, scale, window, accumulate,
-            stream, workspace))
+        _, fields = self._attend_fields(q, lengths, tables, starts, q if out is None else out,
+                                        lse, scale, window, accumulate, stream, workspace)
+        ref = _packed(KvAttendDesc).fill(*fields)
         p = new(KvAttendPlan)
         s = _Sink()
         _check(lib().ullm_kv_cache_attend_plan(ref, ctypes.byref(p), s.ref), s)
