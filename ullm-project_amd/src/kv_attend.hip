@@ -1208,9 +1208,20 @@ __global__ __launch_bounds__(256) void add_scores_kernel(KvAttendArgs a, Scratch
   for (; i < end; ++i) {
     const uint64_t at = uint64_t(rows.first + i) * a.heads + kvh * a.group;
     const RowStats *stats = x.stats + stats_at(a, kvh, rows.first + i);
-    for (uint32_t h = 0; h < a.group; ++h) {
-      const RowStats st = stats[h];
-      sum += exp2_fast(x.scores[(at + h) * x.score_stride + t] - st.top) * st.inv_sum;
+    for (uint32_t h0 = 0; h0 < a.group; h0 += 4) {  // four on their way at once
+      float s[4];
+      RowStats st[4];
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        const uint32_t h = min(h0 + j, a.group - 1);
+        s[j] = x.scores[(at + h) * x.score_stride + t];
+        st[j] = stats[h];
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        const float p = exp2_fast(s[j] - st[j].top) * st[j].inv_sum;
+        sum += h0 + j < a.group ? p : 0.f;
+      }
     }
   }
   const uint64_t unit = uint64_t(id) * a.pool.heads + kvh;
