@@ -416,7 +416,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *sums) {
 // tokens on end and counts its own, the waves' counts are joined once.
 //
 // Bound by the instructions of a lone workgroup per head.  (32768 tokens of 8
-// heads: 27 us; by bytes of the key, each pass reading the weights again, 128.)
+// heads: 24 us; by bytes of the key, each pass reading the weights again, 128.)
 template <uint32_t K>
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(KvEvictArgs a) {
   constexpr uint32_t kSpan = K * kSelectThreads;
@@ -556,13 +556,23 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(KvEvictArg
     }
   }
 
+  // Lanes below this one among those of a mask, from `base` on.
+  const auto rank = [](uint64_t lanes, uint32_t base) {
+    return __builtin_amdgcn_mbcnt_hi(uint32_t(lanes >> 32),
+                                     __builtin_amdgcn_mbcnt_lo(uint32_t(lanes), base));
+  };
   uint32_t at = a.sink, equal = 0;  // where the next goes, tokens of key `last` so far
   each_span([&](uint32_t span) __attribute__((always_inline)) {
     uint32_t n = 0, m = 0;
 #pragma unroll
     for (uint32_t k = 0; k < K; ++k) {
       n += uint32_t(__popcll(__ballot(keys[k] > last)));
-      m += uint32_t(__popcll(__ballot(keys[k] == last)));
+    }
+    if (want != 0) {
+#pragma unroll
+      for (uint32_t k = 0; k < K; ++k) {
+        m += uint32_t(__popcll(__ballot(keys[k] == last)));
+      }
     }
     __syncthreads();  // the sums of the last span are read
     if (lane == 0) {
@@ -578,20 +588,27 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(KvEvictArg
       at += sums[w];
       equal += ties[w];
     }
-    const uint64_t below = (uint64_t(1) << lane) - 1;
+    const uint32_t t0 = span * kSpan + mine;
+    if (want == 0) {
 #pragma unroll
-    for (uint32_t k = 0; k < K; ++k) {
-      const uint64_t above = __ballot(keys[k] > last), tie = __ballot(keys[k] == last);
-      if ((above | tie) == 0) {
-        continue;
+      for (uint32_t k = 0; k < K; ++k) {
+        const uint64_t above = __ballot(keys[k] > last);
+        if (keys[k] > last) {
+          kept[rank(above, next)] = int32_t(t0 + k * kWave);
+        }
+        next += uint32_t(__popcll(above));
       }
-      const uint32_t ties_before = same + uint32_t(__popcll(tie & below));
-      const uint32_t to = next + uint32_t(__popcll(above & below)) + min(ties_before, want);
-      if (keys[k] > last || (keys[k] == last && ties_before < want)) {
-        kept[to] = int32_t(span * kSpan + mine + k * kWave);
+    } else {
+#pragma unroll
+      for (uint32_t k = 0; k < K; ++k) {
+        const uint64_t above = __ballot(keys[k] > last), tie = __ballot(keys[k] == last);
+        const uint32_t before = rank(tie, same);
+        if (keys[k] > last || (keys[k] == last && before < want)) {
+          kept[rank(above, next) + min(before, want)] = int32_t(t0 + k * kWave);
+        }
+        next += uint32_t(__popcll(above));
+        same += uint32_t(__popcll(tie));
       }
-      next += uint32_t(__popcll(above));
-      same += uint32_t(__popcll(tie));
     }
   });
 }
