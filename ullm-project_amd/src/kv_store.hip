@@ -103,8 +103,6 @@ __device__ __forceinline__ uint32_t value_token(uint32_t g, uint32_t j) {
   return 4 * g + j % 4 + 16 * (j / 4);
 }
 
-constexpr uint32_t kMostBlock = 128;  // tokens of a block
-
 // One workgroup stores the new tokens of one block and head.  The new rows are
 // read once, into registers; with their largest magnitudes the exponents are
 // known.  Keys are written from there, values go through LDS, where a token's
@@ -646,18 +644,18 @@ __device__ __forceinline__ float code_factor(int from, int to) {
 // values' units, eight bytes read for each that is kept (the cache lines serve
 // several tokens).  (16 sequences to 1536 tokens of 8 heads: 46 us; with loads
 // of single bytes, twice, 86.)
-template <int D>
+template <int D, uint32_t bt>
 __global__ __launch_bounds__(kThreads) void evict_move_kernel(KvEvictArgs a) {
-  constexpr uint32_t kKeyUnits = kMostBlock * (D / 16) / kThreads;  // of a thread
+  constexpr uint32_t kKeyUnits = (bt * (D / 16) + kThreads - 1) / kThreads;  // of a thread
   constexpr uint32_t kLanes = D / 2;                                // of a token's values
   constexpr uint32_t kTokens = kThreads / kLanes, kAhead = 8;
-  __shared__ __align__(16) uint8_t image[kMostBlock * D];  // the new block's values
-  __shared__ uint64_t from[kMostBlock];   // byte offset of the token's block and head
-  __shared__ uint32_t slot[kMostBlock];   // its place in that block, kNone: in none
-  __shared__ int power[2][kMostBlock];    // the exponents there
-  __shared__ __align__(16) float factor[kMostBlock];
+  __shared__ __align__(16) uint8_t image[bt * D];  // the new block's values
+  __shared__ uint64_t from[bt];   // byte offset of the token's block and head
+  __shared__ uint32_t slot[bt];   // its place in that block, kNone: in none
+  __shared__ int power[2][bt];    // the exponents there
+  __shared__ __align__(16) float factor[bt];
   constexpr uint32_t kNone = ~0u;
-  const uint32_t bt = 1u << a.pool.shift, j = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
+  const uint32_t j = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
   const uint32_t tid = threadIdx.x;
   const uint32_t length = kv_length(a.seqs, a.pool.shift, b);
   const uint32_t stay = length < a.keep ? length : a.keep;
@@ -721,7 +719,7 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(KvEvictArgs a) {
     for (uint32_t r = 0; r < kAhead; ++r) {
       const uint32_t i = i0 + r * kTokens + tid / kLanes;
       if (i < padded) {
-        const uint32_t byte = uint32_t(kv_value_byte<D>(slot[i] & (kMostBlock - 1), vd)) % 8;
+        const uint32_t byte = uint32_t(kv_value_byte<D>(slot[i] & (bt - 1), vd)) % 8;
         const u32x4 w = unit[r];
         const uint32_t x = (byte < 4 ? w.x : w.y) >> byte % 4 * 8 & 0xffu;
         const uint32_t y = (byte < 4 ? w.z : w.w) >> byte % 4 * 8 & 0xffu;
@@ -829,10 +827,13 @@ hipError_t launch_kv_evict(const KvEvictArgs &a, uint32_t dim, hipStream_t s) {
     evict_select_kernel<32><<<units, kSelectThreads, 0, s>>>(a);
   }
   const dim3 grid((a.keep + bt - 1) / bt, a.pool.heads, a.seqs.batch);
+  const auto move = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(a); };
   if (dim == 64) {
-    evict_move_kernel<64><<<grid, kThreads, 0, s>>>(a);
+    move(bt == 32 ? evict_move_kernel<64, 32> : bt == 64 ? evict_move_kernel<64, 64>
+                                                         : evict_move_kernel<64, 128>);
   } else {
-    evict_move_kernel<128><<<grid, kThreads, 0, s>>>(a);
+    move(bt == 32 ? evict_move_kernel<128, 32> : bt == 64 ? evict_move_kernel<128, 64>
+                                                          : evict_move_kernel<128, 128>);
   }
   return hipGetLastError();
 }
