@@ -1308,7 +1308,7 @@ __global__ __launch_bounds__(kWaves * kWave, 4) void add_weights_kernel(KvAttend
     r.query += tile_queries + (carry ? 1u : 0u);
     r.offset += tile_step + (carry ? wrap_step : 0u);
   };
-  RowAt mine = row_at(begin + 16 * wave + lane / 4), tile_at = row_at(begin);
+  RowAt mine = row_at(begin + 16 * wave + lane / 4);
   const uint16_t *q_rows = a.q + rows.first * a.q_row + uint64_t(kvh) * a.group * a.q_head +
                            (lane % 4 ^ lane / 16) * 8;
   const auto start_tile = [&](uint8_t *to) {
@@ -1336,6 +1336,17 @@ __global__ __launch_bounds__(kWaves * kWave, 4) void add_weights_kernel(KvAttend
       next[u] = row_stats[min(r0 + 32 * u + i, all - 1)];
     }
   };
+  // Rows that see some of the wave's tokens, and all of them.
+  struct Range {
+    uint32_t first, end;
+  };
+  const auto range = [&](int64_t from, int64_t past) {
+    const auto row = [&](int64_t query) {
+      return uint32_t(min(max(query - origin, int64_t(0)), int64_t(rows.count))) * a.group;
+    };
+    return Range{uniform(row(from)), a.window != 0 ? uniform(row(past + a.window)) : all};
+  };
+  const Range seen = range(t0, int64_t(t0) + 31), whole = range(int64_t(t0) + 31, t0);
   float sum[16] = {};
   uint32_t stage = 0;
   if (begin < end) {
@@ -1350,15 +1361,10 @@ __global__ __launch_bounds__(kWaves * kWave, 4) void add_weights_kernel(KvAttend
       load_stats(r0 + kWeightRows);
       start_tile(rows_lds(stage ^ 1));
     }
-    const int32_t low = int32_t(origin + tile_at.query);
-    next_tile(tile_at);
-    // The tile's last query, or one that no row of it is past.
-    const int32_t high = int32_t(origin + min(tile_at.query, rows.count - 1));
-    if (id < 0 || int32_t(t0) > high) {
+    if (id < 0 || r0 + kWeightRows <= seen.first || r0 >= seen.end) {
       continue;
     }
-    const bool edge = r0 + kWeightRows > all || int32_t(t0) + 31 > low ||
-                      int32_t(t0) <= oldest_hidden(high, a.window);
+    const bool edge = r0 < whole.first || r0 + kWeightRows > whole.end;
     const uint8_t *tile = rows_lds(stage) + i * 64;
 #pragma unroll
     for (uint32_t u = 0; u < 2; ++u) {
