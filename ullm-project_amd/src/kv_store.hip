@@ -642,7 +642,7 @@ __device__ __forceinline__ float code_factor(int from, int to) {
 // bytes go to their new places in LDS.  Then the exponents are known, and
 // codes whose exponent does not change are written as they are.  Bound by the
 // values' units, eight bytes read for each that is kept (the cache lines serve
-// several tokens).  (16 sequences to 1536 tokens of 8 heads: 46 us; with loads
+// several tokens).  (16 sequences to 1536 tokens of 8 heads: 44 us; with loads
 // of single bytes, twice, 86.)
 template <int D, uint32_t bt>
 __global__ __launch_bounds__(kThreads) void evict_move_kernel(KvEvictArgs a) {
@@ -650,11 +650,13 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(KvEvictArgs a) {
   constexpr uint32_t kLanes = D / 2;                                // of a token's values
   constexpr uint32_t kTokens = kThreads / kLanes, kAhead = 8;
   __shared__ __align__(16) uint8_t image[bt * D];  // the new block's values
-  __shared__ uint64_t from[bt];   // byte offset of the token's block and head
-  __shared__ uint32_t slot[bt];   // its place in that block, kNone: in none
-  __shared__ int power[2][bt];    // the exponents there
+  // Of each token: where its part of the keys' units starts (kNone: it has no
+  // block), where that of the values' does, with its byte of the eight in the
+  // low bits, and the exponents there.
+  __shared__ uint64_t key_from[bt], value_from[bt];
+  __shared__ int power[2][bt];
   __shared__ __align__(16) float factor[bt];
-  constexpr uint32_t kNone = ~0u;
+  constexpr uint64_t kNone = ~uint64_t(0);
   const uint32_t j = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
   const uint32_t tid = threadIdx.x;
   const uint32_t length = kv_length(a.seqs, a.pool.shift, b);
@@ -677,13 +679,14 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(KvEvictArgs a) {
     const int32_t id =
         tid < n ? kv_block(table, a.seqs, a.pool.blocks, t >> a.pool.shift) : -1;
     const uint64_t src = uint64_t(id < 0 ? 0 : id) * a.pool.heads + head;
-    from[tid] = src * 2 * side;
-    slot[tid] = id < 0 ? kNone : t & (bt - 1);
+    const uint32_t at = t & (bt - 1);
+    key_from[tid] = id < 0 ? kNone : src * 2 * side + kv_key_unit<D>(at, 0);
+    value_from[tid] = src * 2 * side + side + kv_value_byte<D>(at, 0);
     power[0][tid] = a.pool.exps[src * 2];
     power[1][tid] = a.pool.exps[src * 2 + 1];
     if (a.pool.weights != nullptr && tid < n) {
       a.pool.weights[(dst << a.pool.shift) + tid] =
-          id < 0 ? 0.f : a.pool.weights[(src << a.pool.shift) + (t & (bt - 1))];
+          id < 0 ? 0.f : a.pool.weights[(src << a.pool.shift) + at];
     }
   }
   __syncthreads();
@@ -698,9 +701,9 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(KvEvictArgs a) {
   for (uint32_t r = 0; r < kKeyUnits; ++r) {
     const uint32_t u = tid + r * kThreads, i = u / (D / 16), c = u % (D / 16);
     keys[r] = u32x4{0u, 0u, 0u, 0u};
-    if (i < n && slot[i] != kNone) {
-      keys[r] = *reinterpret_cast<const u32x4 *>(a.pool.codes + from[i] +
-                                                 kv_key_unit<D>(slot[i], c));
+    if (i < n && key_from[i] != kNone) {
+      keys[r] = *reinterpret_cast<const u32x4 *>(a.pool.codes + key_from[i] +
+                                                 kv_key_unit<D>(0, c));
     }
   }
   const uint32_t vd = tid % kLanes / 16 * 32 + tid % 16;  // this lane's dims: vd, vd + 16
@@ -710,19 +713,20 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(KvEvictArgs a) {
     for (uint32_t r = 0; r < kAhead; ++r) {
       const uint32_t i = i0 + r * kTokens + tid / kLanes;
       unit[r] = u32x4{0u, 0u, 0u, 0u};
-      if (i < padded && slot[i] != kNone) {
+      if (i < padded && key_from[i] != kNone) {
         unit[r] = *reinterpret_cast<const u32x4 *>(
-            a.pool.codes + from[i] + side + kv_value_byte<D>(slot[i], vd) / 16 * 16);
+            a.pool.codes + (value_from[i] & ~uint64_t(7)) + kv_value_byte<D>(0, vd));
       }
     }
 #pragma unroll
     for (uint32_t r = 0; r < kAhead; ++r) {
       const uint32_t i = i0 + r * kTokens + tid / kLanes;
       if (i < padded) {
-        const uint32_t byte = uint32_t(kv_value_byte<D>(slot[i] & (bt - 1), vd)) % 8;
+        // Its byte of each half, the others 0.
+        const uint32_t pick = 0x0c0c0c00u | (uint32_t(value_from[i]) & 7u);
         const u32x4 w = unit[r];
-        const uint32_t x = (byte < 4 ? w.x : w.y) >> byte % 4 * 8 & 0xffu;
-        const uint32_t y = (byte < 4 ? w.z : w.w) >> byte % 4 * 8 & 0xffu;
+        const uint32_t x = __builtin_amdgcn_perm(w.y, w.x, pick);
+        const uint32_t y = __builtin_amdgcn_perm(w.w, w.z, pick);
         uint8_t *to = image + kv_value_byte<D>(i, vd);
         to[0] = uint8_t(x);
         to[8] = uint8_t(y);
