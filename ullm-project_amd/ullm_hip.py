@@ -20,6 +20,7 @@ fallback: if the native library is missing, loading raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import enum
 import struct
 import threading
@@ -697,9 +698,21 @@ class _Packed:
         self.ref = ctypes.byref(self.desc)
         self.header = (ctypes.sizeof(cls), ABI_VERSION)
 
+        # The first arguments bound in C: a call unpacks only its own fields.
+        self.pack = functools.partial(self.format.pack_into, self.buffer, 0, *self.header)
+        self.sink = _thread_sink()
+        self.sink_ref = self.sink.ref
+
     def fill(self, *fields):
-        self.format.pack_into(self.buffer, 0, *self.header, *fields)
+        self.pack(*fields)
         return self.ref
+
+    def call(self, fn, *fields):
+        """fn(descriptor of these fields), its error raised."""
+        self.pack(*fields)
+        st = fn(self.ref, self.sink_ref)
+        if st:
+            raise HipError(st, self.sink.text())
 
 
 def _packed(cls) -> _Packed:
@@ -717,6 +730,8 @@ def _strides3(t, name, heads, dim):
     if len(shape) != 3 or shape[1] != heads or shape[2] != dim \
             or t.dtype is not _torch().bfloat16:
         raise ValueError(f"{name} must be bfloat16 [rows][{heads}][{dim}]")
+    if t.is_contiguous():
+        return shape[0], heads * dim, dim
     row, head, one = t.stride()
     # The stride of an axis of one is never used.
     if shape[0] <= 1:
@@ -726,13 +741,6 @@ def _strides3(t, name, heads, dim):
     if one != 1 or row < dim or head < dim:
         raise ValueError(f"{name} must have contiguous heads that do not overlap")
     return shape[0], row, head
-
-
-def _call(fn, ref):
-    s = _thread_sink()
-    st = fn(ref, s.ref)
-    if st:
-        raise HipError(st, s.text())
 
 
 class KvCache:
@@ -785,14 +793,17 @@ class KvCache:
         """The fields of a ullm_kv_sequences_t."""
         i32 = _torch().int32
         batch, columns = tables.shape
-        stride, one = tables.stride()
         if tables.dtype is not i32 or lengths.dtype is not i32 or lengths.shape != (batch,) \
-                or (batch > 1 and lengths.stride(0) != 1):
+                or not lengths.is_contiguous():
             raise ValueError("tables must be int32 [batch][columns] and lengths int32 [batch]")
-        if batch == 1:
+        if tables.is_contiguous():
             stride = columns
-        if (columns > 1 and one != 1) or stride < columns:
-            raise ValueError("rows of tables must be contiguous and must not overlap")
+        else:
+            stride, one = tables.stride()
+            if batch == 1:
+                stride = columns
+            if (columns > 1 and one != 1) or stride < columns:
+                raise ValueError("rows of tables must be contiguous and must not overlap")
         if starts is None:
             at = 0
         elif starts.dtype is not i32 or starts.shape != (batch + 1,) \
@@ -815,15 +826,17 @@ class KvCache:
                                     or weights.dtype is not _torch().float32
                                     or not weights.is_contiguous()):
             raise ValueError("weights must be a contiguous float32 [rows][kv_heads] tensor")
-        _call(lib().ullm_kv_cache_append, _packed(KvAppendDesc).fill(
+        _packed(KvAppendDesc).call(
+            lib().ullm_kv_cache_append,
             self.handle or 0, *self._seqs(lengths, tables, rows, starts), k.data_ptr(), k_row,
             k_head, v.data_ptr(), v_row, v_head, 0 if weights is None else weights.data_ptr(),
-            _stream(stream) or 0))
+            _stream(stream) or 0)
 
     def _gather(self, lengths, tables, rows, starts, k, v, weights, stream):
-        _call(lib().ullm_kv_cache_gather, _packed(KvGatherDesc).fill(
+        _packed(KvGatherDesc).call(
+            lib().ullm_kv_cache_gather,
             self.handle or 0, *self._seqs(lengths, tables, rows, starts), k, v, weights,
-            _stream(stream) or 0))
+            _stream(stream) or 0)
 
     def gather(self, lengths, tables, rows, starts=None, stream=None):
         """Keys and values of each sequence's last rows (``rows`` in all), bf16
@@ -875,7 +888,7 @@ class KvCache:
         no token gives zeros."""
         out, fields = self._attend_fields(q, lengths, tables, starts, out, lse, scale, window,
                                           accumulate, stream, workspace)
-        _call(lib().ullm_kv_cache_attend, _packed(KvAttendDesc).fill(*fields))
+        _packed(KvAttendDesc).call(lib().ullm_kv_cache_attend, *fields)
         return out
 
     def attend_plan(self, q, lengths, tables, starts=None, out=None, lse=None, scale=None,
@@ -905,10 +918,11 @@ class KvCache:
         seqs = self._seqs(lengths, tables, 0, None)
         lens = tables.new_empty((batch,))
         kept = tables.new_empty((batch, self.kv_heads, max(keep, 0)))
-        _call(lib().ullm_kv_cache_evict, _packed(KvEvictDesc).fill(
+        _packed(KvEvictDesc).call(
+            lib().ullm_kv_cache_evict,
             self.handle or 0, *seqs, new_tables.data_ptr(),
             new_tables.stride(0) if batch > 1 else columns, lens.data_ptr(), kept.data_ptr(),
-            keep, sink, recent, _stream(stream) or 0))
+            keep, sink, recent, _stream(stream) or 0)
         return lens, kept
 
 
