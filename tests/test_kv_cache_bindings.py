@@ -7,30 +7,37 @@ from pathlib import Path
 import abi_parse as A
 
 ROOT = Path(__file__).resolve().parent.parent
-HEADER = (ROOT / "include" / "ullm" / "kv_cache.h").read_text()
-RUST = (ROOT / "rust" / "ullm-hip-sys" / "src" / "kv_cache_bindings.rs").read_text()
-PATCH = (ROOT / "rust" / "patches" / "ullm-hip-sys.patch").read_text()
+
+
+def _header():
+    return (ROOT / "include" / "ullm" / "kv_cache.h").read_text()
+
+
+def _rust():
+    return (ROOT / "rust" / "ullm-hip-sys" / "src" / "kv_cache_bindings.rs").read_text()
 
 
 def test_constants():
-    assert A.rust_constants(RUST) == A.c_constants(HEADER)
+    assert A.rust_constants(_rust()) == A.c_constants(_header())
 
 
 def test_structs():
-    c, r = A.c_structs(HEADER, A.c_constants(HEADER)), A.rust_structs(RUST)
+    header, rust = _header(), _rust()
+    c, r = A.c_structs(header, A.c_constants(header)), A.rust_structs(rust)
     assert r.pop("ullm_kv_cache_t") == [("_private", ("array", "u8", 0))]
     assert r == c
-    sizes = re.findall(r"/// (\d+) bytes\.\n(?:#.*\n)+pub struct (\w+)", RUST)
+    sizes = re.findall(r"/// (\d+) bytes\.\n(?:#.*\n)+pub struct (\w+)", rust)
     assert {n: int(s) for s, n in sizes} == {n: A.size_align(n, c)[0] for n in c}
 
 
 def test_functions():
-    assert A.rust_functions(RUST) == A.c_functions(HEADER)
+    assert A.rust_functions(_rust()) == A.c_functions(_header())
 
 
 def test_the_patch_includes_the_module_and_counts_its_lines():
-    assert '+    include!("kv_cache_bindings.rs");\n' in PATCH
-    hunks = re.finditer(r"^(@@ .*)\n((?:[ +\-].*\n|\n)*?)(?=^@@|^--- |\Z)", PATCH, flags=re.M)
+    patch = (ROOT / "rust" / "patches" / "ullm-hip-sys.patch").read_text()
+    assert '+    include!("kv_cache_bindings.rs");\n' in patch
+    hunks = re.finditer(r"^(@@ .*)\n((?:[ +\-].*\n|\n)*?)(?=^@@|^--- |\Z)", patch, flags=re.M)
     for head, body in (m.groups() for m in hunks):
         old, new = map(int, re.search(r"-\d+,(\d+) \+\d+,(\d+)", head).groups())
         lines = body.split("\n")[:-1]
@@ -41,4 +48,4 @@ def test_the_patch_includes_the_module_and_counts_its_lines():
 def test_the_integration_guide_names_every_function():
     doc = (ROOT / "INTEGRATION.md").read_text()
     assert "rust/ullm-hip-sys/src/kv_cache_bindings.rs" in doc
-    assert not [f for f in A.c_functions(HEADER) if f not in doc]
+    assert not [f for f in A.c_functions(_header()) if f not in doc]
