@@ -370,11 +370,9 @@ __global__ __launch_bounds__(kThreads) void gather_weights_kernel(KvGatherArgs a
 
 // A weight as an unsigned key of the same order, NaN above all, -0 as 0.
 __device__ __forceinline__ uint32_t weight_key(float w) {
-  const uint32_t b = f32_bits(w);
-  if ((b & 0x7fffffffu) > 0x7f800000u) {
-    return 0xffffffffu;
-  }
-  return (b & 0x80000000u) ? (b == 0x80000000u ? 0x80000000u : ~b) : (b | 0x80000000u);
+  const uint32_t b = f32_bits(w + 0.f);  // -0 becomes 0
+  const uint32_t key = b ^ (uint32_t(int32_t(b) >> 31) | 0x80000000u);
+  return w != w ? 0xffffffffu : key;
 }
 
 constexpr uint32_t kSelectThreads = 1024, kSelectWaves = kSelectThreads / kWave;
@@ -402,8 +400,9 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *sums) {
 }
 
 // One workgroup selects the tokens of one sequence and head.  A thread holds K
-// keys in registers, 1024 K for the workgroup (longer sequences read theirs
-// again, as many at a time, in each pass), so that a pass costs no memory.
+// keys in registers, 1024 K for the workgroup, so that a pass costs no memory.
+// (ONE: the tables hold no more.  Longer sequences read theirs again, as many
+// at a time, in each pass.)
 //
 // First the key of the last token that stays: the range of the keys in
 // question, at first their smallest to their largest, is cut into 4096 bins,
@@ -414,8 +413,8 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *sums) {
 // tokens on end and counts its own, the waves' counts are joined once.
 //
 // Bound by the instructions of a lone workgroup per head.  (32768 tokens of 8
-// heads: 24 us; by bytes of the key, each pass reading the weights again, 128.)
-template <uint32_t K>
+// heads: 16 us; by bytes of the key, each pass reading the weights again, 128.)
+template <uint32_t K, bool ONE>
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(KvEvictArgs a) {
   constexpr uint32_t kSpan = K * kSelectThreads;
   __shared__ uint32_t hist[kSelectBins];
@@ -444,42 +443,60 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(KvEvictArg
   }
   const int32_t *table = a.seqs.tables + b * a.seqs.stride;
   const uint32_t mask = (1u << a.pool.shift) - 1;
-  const uint32_t spans = (length + kSpan - 1) / kSpan;
+  const uint32_t spans = ONE ? 1 : (length + kSpan - 1) / kSpan;
   const uint32_t mine = wave * K * kWave + lane;  // this thread's first token of a span
 
   uint32_t keys[K];
   // Keys of a span: 0 is no candidate, 1 a token of no block, which is less
-  // than any weight.  Loads do not depend on what they find, so that two waits
-  // serve for all.
+  // than any weight.  Lane i looks up where the wave's 32 tokens from 32 i on
+  // lie: two waits serve for all, and a key costs its load and little else.
   const auto load = [&](uint32_t span) __attribute__((always_inline)) {
-    const uint32_t t0 = span * kSpan + mine;
-    uint32_t id[K];
+    static_assert(2 * K <= kWave, "a lane for each 32 tokens");
+    const uint32_t first = span * kSpan + wave * K * kWave;
+    const uint32_t t32 = first + 32 * lane, block = t32 >> a.pool.shift;
+    const uint32_t id = uint32_t(table[min(block, a.seqs.max_blocks - 1)]);
+    const bool there = id < a.pool.blocks && block < a.seqs.max_blocks;
+    const uint64_t at = (((there ? id : 0u) * uint64_t(a.pool.heads) + head) << a.pool.shift) +
+                        (t32 & mask);
+    const auto at_lane = [&](uint32_t from) {
+      return uint64_t(uint32_t(__builtin_amdgcn_readlane(int(at >> 32), int(from)))) << 32 |
+             uint32_t(__builtin_amdgcn_readlane(int(at), int(from)));
+    };
     float w[K];
+    if (a.pool.shift >= 6) {  // 64 tokens of a block at a time
 #pragma unroll
-    for (uint32_t k = 0; k < K; ++k) {
-      id[k] = uint32_t(table[min((t0 + k * kWave) >> a.pool.shift, a.seqs.max_blocks - 1)]);
+      for (uint32_t k = 0; k < K; ++k) {
+        w[k] = a.pool.weights[at_lane(2 * k) + lane];
+      }
+    } else {
+#pragma unroll
+      for (uint32_t k = 0; k < K; ++k) {
+        const uint64_t low = at_lane(2 * k), high = at_lane(2 * k + 1);
+        w[k] = a.pool.weights[(lane < 32 ? low : high) + lane % 32];
+      }
     }
+    const uint32_t from_lo = first + lane - lo, candidates = hi - lo;
 #pragma unroll
     for (uint32_t k = 0; k < K; ++k) {
-      const uint64_t unit = uint64_t(id[k] < a.pool.blocks ? id[k] : 0u) * a.pool.heads + head;
-      w[k] = a.pool.weights[(unit << a.pool.shift) + ((t0 + k * kWave) & mask)];
+      keys[k] = from_lo + k * kWave < candidates ? weight_key(w[k]) : 0u;
     }
+    if (__any(!there && lane < 2 * K && t32 < hi)) {
 #pragma unroll
-    for (uint32_t k = 0; k < K; ++k) {
-      const uint32_t t = t0 + k * kWave;
-      const uint32_t key = id[k] < a.pool.blocks ? weight_key(w[k]) : 1u;
-      keys[k] = t >= lo && t < hi ? key : 0u;
+      for (uint32_t k = 0; k < K; ++k) {
+        const bool none = __shfl(int(there), int(2 * k + lane / 32), kWave) == 0;
+        keys[k] = none && keys[k] != 0u ? 1u : keys[k];
+      }
     }
   };
   const auto each_span = [&](const auto &f) __attribute__((always_inline)) {
     for (uint32_t span = 0; span < spans; ++span) {
-      if (spans > 1) {
+      if (!ONE) {
         load(span);
       }
       f(span);
     }
   };
-  if (spans == 1) {
+  if (ONE) {
     load(0);
   }
 
@@ -824,11 +841,15 @@ hipError_t launch_kv_evict(const KvEvictArgs &a, uint32_t dim, hipStream_t s) {
   const uint32_t bt = 1u << a.pool.shift;
   const dim3 units(a.pool.heads, a.seqs.batch);
   // Keys of a thread: what the tables' size needs.  (16 sequences of up to
-  // 4500 tokens: 8 keys 11.4 us, 32 22.)
-  if (uint64_t(a.seqs.max_blocks) << a.pool.shift <= 8 * kSelectThreads) {
-    evict_select_kernel<8><<<units, kSelectThreads, 0, s>>>(a);
+  // 4500 tokens: 8 keys 9.5 us, 32 16, 32 read in spans 32; one of 32768: 16,
+  // in spans 27.)
+  const uint64_t tokens = uint64_t(a.seqs.max_blocks) << a.pool.shift;
+  if (tokens <= 8 * kSelectThreads) {
+    evict_select_kernel<8, true><<<units, kSelectThreads, 0, s>>>(a);
+  } else if (tokens <= 32 * kSelectThreads) {
+    evict_select_kernel<32, true><<<units, kSelectThreads, 0, s>>>(a);
   } else {
-    evict_select_kernel<32><<<units, kSelectThreads, 0, s>>>(a);
+    evict_select_kernel<32, false><<<units, kSelectThreads, 0, s>>>(a);
   }
   const dim3 grid((a.keep + bt - 1) / bt, a.pool.heads, a.seqs.batch);
   const auto move = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(a); };
