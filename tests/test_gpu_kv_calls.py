@@ -111,6 +111,18 @@ def test_refusals(calls, name, over, status, word):
     assert st == status and word in text, (st, text)
 
 
+def test_attend_refuses_more_tiles_than_a_launch_has(calls, uh):
+    """2^31 - 1 rows of one head: 2^24 tiles of 128, by the checks on the host
+    alone (the pointers name a megabyte)."""
+    one = uh.KvCache(4, 1, 128)
+    d = uh.new(uh.KvAttendDesc, cache=one.handle, q=calls.at(2), out=calls.at(4), heads=1,
+               scale=1.0, seqs=uh.KvSequences(batch=1, rows=2 ** 31 - 1, tables=calls.at(0),
+                                              max_blocks=1, lengths=calls.at(1)))
+    s = uh._Sink()
+    st = uh.Status(uh.lib().ullm_kv_cache_attend(ctypes.byref(d), s.ref))
+    assert st == uh.Status.UNSUPPORTED and "tiles" in s.text()
+
+
 def test_evict_refuses_its_own_tables(calls):
     for over in ({"new_tables": calls.at(0)}, {"new_lengths": calls.at(1)}):
         st, text = calls.call("evict", **over)

@@ -478,6 +478,12 @@ extern "C" ULLM_HIP_API ullm_status_t ullm_kv_cache_attend(
     HIP_TRY(error_sink, "hipSetDevice", scope.error());
     const ullm::KvAttendArgs a = attend_args(desc);
     const ullm::KvAttendPlan p = ullm::plan_kv_attend(a, c->head_dim);
+    // A launch counts its threads in 32 bits; the join has a wave for each row.
+    if (p.grid > UINT32_MAX / 512 ||
+        (p.parts > 1 && p.grid / p.parts > UINT32_MAX / 512 / p.row_tile)) {
+      return write_error(error_sink, ULLM_STATUS_UNSUPPORTED,
+                         "too many tiles of rows for one launch");
+    }
     void *ws = desc->workspace;
     if (p.workspace != 0 && ws != nullptr) {
       if (desc->workspace_size < p.workspace) {

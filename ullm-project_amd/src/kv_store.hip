@@ -676,34 +676,34 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(KvEvictArgs a) {
   constexpr uint64_t kNone = ~uint64_t(0);
   const uint32_t j = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
   const uint32_t tid = threadIdx.x;
+  const uint32_t base = j << a.pool.shift;
+  // Loads that do not depend on each other first: the kernel is a chain of
+  // them (position, block, exponents beside codes).
+  const uint32_t place = base + tid < a.keep ? base + tid : base;
+  const uint32_t t = uint32_t(a.kept[(uint64_t(b) * a.pool.heads + head) * a.keep + place]);
+  const int32_t raw = a.new_tables[b * a.new_stride + j];
   const uint32_t length = kv_length(a.seqs, a.pool.shift, b);
   const uint32_t stay = length < a.keep ? length : a.keep;
-  const uint32_t base = j << a.pool.shift;
-  if (base >= stay) {
+  if (base >= stay || raw < 0 || uint32_t(raw) >= a.pool.blocks) {
     return;
   }
   const uint32_t n = stay - base < bt ? stay - base : bt, padded = (n + 31) / 32 * 32;
-  const int32_t raw = a.new_tables[b * a.new_stride + j];
-  if (raw < 0 || uint32_t(raw) >= a.pool.blocks) {
-    return;
-  }
   const uint64_t dst = uint64_t(raw) * a.pool.heads + head;
   const uint64_t side = uint64_t(D) << a.pool.shift;
-  const int32_t *kept = a.kept + (uint64_t(b) * a.pool.heads + head) * a.keep + base;
-  const int32_t *table = a.seqs.tables + b * a.seqs.stride;
+  int exp_key = 0, exp_value = 0;
+  float weight = 0.f;
   if (tid < padded) {
-    const uint32_t t = tid < n ? uint32_t(kept[tid]) : 0u;
-    const int32_t id =
-        tid < n ? kv_block(table, a.seqs, a.pool.blocks, t >> a.pool.shift) : -1;
+    const int32_t id = tid < n ? kv_block(a.seqs.tables + b * a.seqs.stride, a.seqs,
+                                          a.pool.blocks, t >> a.pool.shift)
+                               : -1;
     const uint64_t src = uint64_t(id < 0 ? 0 : id) * a.pool.heads + head;
     const uint32_t at = t & (bt - 1);
     key_from[tid] = id < 0 ? kNone : src * 2 * side + kv_key_unit<D>(at, 0);
     value_from[tid] = src * 2 * side + side + kv_value_byte<D>(at, 0);
-    power[0][tid] = a.pool.exps[src * 2];
-    power[1][tid] = a.pool.exps[src * 2 + 1];
-    if (a.pool.weights != nullptr && tid < n) {
-      a.pool.weights[(dst << a.pool.shift) + tid] =
-          id < 0 ? 0.f : a.pool.weights[(src << a.pool.shift) + at];
+    exp_key = a.pool.exps[src * 2];
+    exp_value = a.pool.exps[src * 2 + 1];
+    if (id >= 0) {
+      weight = a.pool.weights[(src << a.pool.shift) + at];
     }
   }
   __syncthreads();
@@ -724,8 +724,8 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(KvEvictArgs a) {
     }
   }
   const uint32_t vd = tid % kLanes / 16 * 32 + tid % 16;  // this lane's dims: vd, vd + 16
-  for (uint32_t i0 = 0; i0 < padded; i0 += kAhead * kTokens) {
-    u32x4 unit[kAhead];
+  u32x4 unit[kAhead];
+  const auto load_values = [&](uint32_t i0) {
 #pragma unroll
     for (uint32_t r = 0; r < kAhead; ++r) {
       const uint32_t i = i0 + r * kTokens + tid / kLanes;
@@ -734,6 +734,17 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(KvEvictArgs a) {
         unit[r] = *reinterpret_cast<const u32x4 *>(
             a.pool.codes + (value_from[i] & ~uint64_t(7)) + kv_value_byte<D>(0, vd));
       }
+    }
+  };
+  load_values(0);
+  if (tid < padded) {
+    power[0][tid] = exp_key;
+    power[1][tid] = exp_value;
+  }
+  __syncthreads();
+  for (uint32_t i0 = 0; i0 < padded; i0 += kAhead * kTokens) {
+    if (i0 != 0) {
+      load_values(i0);
     }
 #pragma unroll
     for (uint32_t r = 0; r < kAhead; ++r) {
@@ -769,6 +780,9 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(KvEvictArgs a) {
   }
   if (tid < padded) {
     factor[tid] = code_factor(power[1][tid], ev);
+  }
+  if (tid < n) {
+    a.pool.weights[(dst << a.pool.shift) + tid] = weight;
   }
   uint8_t *to = a.pool.codes + dst * 2 * side;
 #pragma unroll
