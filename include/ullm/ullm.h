@@ -1,5 +1,5 @@
 /* ullm/ullm.h -- umbrella header (reference include/ullm/ullm.h:1-6), extended
- * with the linear-layer, key/value-cache and weight-file entry points of this build. */
+ * with the linear-layer, key/value-cache and weight-file entry points of this library. */
 #ifndef ULLM_ULLM_H
 #define ULLM_ULLM_H
 

@@ -1,8 +1,7 @@
 // Bindings of the gfx950 library's key/value cache ABI
-// (include/ullm/kv_cache.h), for crates/ullm-hip-sys.  Not compiled in this
-// build's container (no Rust toolchain).  tests/test_kv_cache_bindings.py
-// checks every constant, struct layout and function signature here against
-// the C header.
+// (include/ullm/kv_cache.h), for crates/ullm-hip-sys.  Written without a Rust
+// toolchain: tests/test_kv_cache_bindings.py checks every constant, struct
+// layout and function signature here against the C header.
 //
 // Wiring (rust/patches/ullm-hip-sys.patch): `pub mod kv_cache {
 // include!("kv_cache_bindings.rs"); }` in crates/ullm-hip-sys/src/lib.rs,

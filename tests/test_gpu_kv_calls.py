@@ -195,6 +195,38 @@ def test_tiles_of_ragged_prompts(uh, gpu, counts):
     p.check_attend(counts, 4, kernel=uh.KV_KERNEL_MANY_ROWS, accumulate=True)
 
 
+@pytest.mark.parametrize("nan", [False, True])
+def test_long_prompt_of_small_blocks(uh, gpu, nan):
+    """A prompt whose tiles walk through more blocks than a workgroup holds,
+    against the same values in larger blocks: the stored values are equal
+    (read back from the larger blocks, whose exponents reach further), the
+    products and sums too, up to powers of two."""
+    n, rows = 20000, 12800
+    g = torch.Generator(device=gpu).manual_seed(5)
+    k, v = (torch.randn((n, 1, 64), generator=g, device=gpu).bfloat16() for _ in range(2))
+    q = torch.randn((rows, 4, 64), generator=g, device=gpu).bfloat16()
+    if nan:
+        v[19990, 0, 7] = float("nan")
+    length = torch.tensor([n], dtype=torch.int32, device=gpu)
+    got = []
+    for bt in (128, 32):
+        c = uh.KvCache(-(-n // bt), 1, 64, block_tokens=bt, track_weights=True)
+        table = torch.randperm(-(-n // bt), generator=g, device=gpu).int().view(1, -1)
+        c.append(k, v, length, table)
+        k, v = c.gather(length, table, n)
+        p = c.attend_plan(q, length, table)
+        assert p.kernel == uh.KV_KERNEL_MANY_ROWS and p.parts == 1
+        lse = torch.empty((rows, 4), device=gpu)
+        got.append((c.attend(q, length, table, lse=lse, accumulate=True), lse,
+                    c.gather_weights(length, table, n)))
+    for a, b in zip(*got):
+        assert torch.equal(a.isnan(), b.isnan())
+        assert torch.equal(a.nan_to_num(), b.nan_to_num())
+    out = got[1][0]
+    assert out[:-10].isfinite().all()
+    assert bool(out[-10:, :, 7].isnan().all()) == nan and out[-10:, :, :7].isfinite().all()
+
+
 @pytest.mark.parametrize("n,keep", [(9000, 700), (40000, 2500)])
 def test_evict_long_sequences(uh, gpu, n, keep):
     """More tokens than a thread holds keys of, and than a workgroup does."""

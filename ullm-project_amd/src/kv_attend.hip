@@ -787,7 +787,9 @@ __device__ __forceinline__ void store_sums(const KvAttendArgs &a, const Scratch 
   }
 }
 
-template <int D>
+// LONG: a part may have more blocks than LDS holds entries of, which are then
+// replaced on the way.  (Where it has not, that costs 229 against 221 us.)
+template <int D, bool LONG>
 __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows_kernel(KvAttendArgs a, Scratch x,
                                                                       uint32_t each_slots) {
   constexpr uint32_t kGroup = 64 * D;  // bytes of 32 tokens: keys, then values
@@ -829,17 +831,25 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows_kernel(KvAttendAr
   const uint32_t from = t.begin / 32 + part * (x.part_tokens / 32);
   const uint32_t all = (t.end + 31) / 32;
   const uint32_t to = min(all, from + x.part_tokens / 32);
-  const uint32_t block0 = from * 32 >> a.pool.shift;
-  const uint32_t blocks = to > from ? ((to * 32 - 1) >> a.pool.shift) - block0 + 1 : 0;
   const int32_t *table = a.seqs.tables + t.seq * a.seqs.stride;
-  for (uint32_t b = threadIdx.x; b < blocks; b += kWaves * kWave) {
-    const int32_t id = kv_block(table, a.seqs, a.pool.blocks, block0 + b);
+  const auto entry_of = [&](uint32_t block) {
+    const int32_t id = kv_block(table, a.seqs, a.pool.blocks, block);
     const uint64_t unit = uint64_t(id < 0 ? 0 : id) * a.pool.heads + kvh;
     const int e = *reinterpret_cast<const uint16_t *>(a.pool.exps + unit * 2);
-    entries[b] = BlockEntry{
+    return BlockEntry{
         reinterpret_cast<uint64_t>(a.pool.codes) + unit * (uint64_t(2 * D) << a.pool.shift),
         exp2_int(int8_t(e)), uint32_t(int8_t(e >> 8) + int(kExpCode)) | (id < 0 ? kAbsent : 0u)};
-  }
+  };
+  // LDS holds the blocks `held` .. held + kManyBlocks - 1 of the sequence, as
+  // far as the part goes.
+  uint32_t held = from * 32 >> a.pool.shift;
+  const auto hold_blocks = [&] {
+    const uint32_t end = to > from ? ((to * 32 - 1) >> a.pool.shift) + 1 : held;
+    for (uint32_t b = threadIdx.x; b < kManyBlocks && held + b < end; b += kWaves * kWave) {
+      entries[b] = entry_of(held + b);
+    }
+  };
+  hold_blocks();
   ManyState<D> st;
   st.m = -INFINITY;
   st.l = 0.f;
@@ -863,7 +873,7 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows_kernel(KvAttendAr
     for (uint32_t u = 0; u < 2; ++u) {
       const uint32_t tok = min(grp0 + u, to - 1) * 32;
       const u32x4 e =
-          *reinterpret_cast<const u32x4 *>(&entries[(tok >> a.pool.shift) - block0]);
+          *reinterpret_cast<const u32x4 *>(&entries[(tok >> a.pool.shift) - held]);
       s.power[u] = bits_f32(uniform(e.z));
       s.exp_code[u] = uniform(e.w);
       const uint8_t *keys =
@@ -919,7 +929,14 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows_kernel(KvAttendAr
     const Step now = next;
     const uint8_t *stage = ring(step % kStages);
     if (step + 1 < steps) {
-      next = start_step(from + 2 * step + 2, ring((step + 1) % kStages));
+      const uint32_t grp0 = from + 2 * step + 2;
+      if (LONG && (min(grp0 + 1, to - 1) * 32 >> a.pool.shift) - held >= kManyBlocks) {
+        // No wave is past this step's barrier without the entries it read.
+        held = grp0 * 32 >> a.pool.shift;
+        hold_blocks();
+        __syncthreads();
+      }
+      next = start_step(grp0, ring((step + 1) % kStages));
     }
 #pragma unroll
     for (uint32_t u = 0; u < 2; ++u) {
@@ -1076,16 +1093,15 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows_kernel(KvAttendAr
       rs.o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     for (uint32_t grp = from; grp < to; ++grp) {
-      const uint32_t b = (grp * 32 >> a.pool.shift) - block0, in_block = grp * 32 & in_mask;
-      const u32x4 e = *reinterpret_cast<const u32x4 *>(&entries[b]);
-      const uint8_t *unit =
-          reinterpret_cast<const uint8_t *>(uint64_t(uniform(e.y)) << 32 | uniform(e.x));
-      const uint32_t exp_code = uniform(e.w);
+      const uint32_t in_block = grp * 32 & in_mask;
+      const BlockEntry e = entry_of(grp * 32 >> a.pool.shift);
+      const uint8_t *unit = reinterpret_cast<const uint8_t *>(e.codes);
+      const uint32_t exp_code = uniform(e.exp_code);
       Group<D> x32;
       load_group_keys<D, false>(x32, unit, in_block, lane);
       load_group_values<D, false>(x32, unit, a.pool.shift, in_block, lane);
       attend_group<D, false>(
-          rs, x32, q16, at, grp * 32, (exp_code & kAbsent) == 0, bits_f32(uniform(e.z)),
+          rs, x32, q16, at, grp * 32, (exp_code & kAbsent) == 0, bits_f32(uniform(f32_bits(e.power))),
           int(exp_code & 0xffffu) - int(kExpCode), a.scale_log2, g, nullptr, [] {}, [] {});
     }
     float l = rs.l + __shfl_xor(rs.l, 16, kWave);
@@ -1466,8 +1482,8 @@ static uint64_t each_tiles(const KvAttendArgs &a, uint32_t rows) {
 // that together give each a workgroup: more and smaller parts cost their
 // start and the join (131072 tokens of 8 heads: 32 parts each 46.7 us, 64
 // 50.1, 128 53.2).  A part has at least kPartLeast tokens (333 tokens of 8
-// heads: whole 5.7 us, in two parts 7.8) and at most 64 blocks, what a wave
-// looks up with one load.
+// heads: whole 5.7 us, in two parts 7.8), with few rows at most 64 blocks,
+// what a wave looks up with one load.
 constexpr uint32_t kPartLeast = 512;
 // Rows of a sequence and key/value head, on average, up to which small tiles
 // serve.
@@ -1492,8 +1508,8 @@ KvAttendPlan plan_kv_attend(const KvAttendArgs &a, uint32_t dim) {
   const uint32_t cus = device_cu_count();
   const uint64_t split = std::max<uint64_t>((many ? 3 : 1) * cus / tiles, 1);
   const uint64_t part = std::max<uint64_t>((span + split - 1) / split, kPartLeast);
-  p.part_tokens = uint32_t(std::min<uint64_t>((part + kStep - 1) / kStep * kStep,
-                                              (many ? kManyBlocks : 64u) << a.pool.shift));
+  const uint64_t most = many ? uint64_t(1) << 31 : uint64_t(64) << a.pool.shift;
+  p.part_tokens = uint32_t(std::min<uint64_t>((part + kStep - 1) / kStep * kStep, most));
   p.parts = uint32_t((span + p.part_tokens - 1) / p.part_tokens);
   // Scores cost 8 bytes for each row and token, a second pass over the keys
   // `dim` bytes for each token.
@@ -1522,11 +1538,18 @@ static hipError_t launch_attend(const KvAttendArgs &a, const KvAttendPlan &p, vo
   };
   if (p.kernel == ULLM_KV_KERNEL_MANY_ROWS) {
     constexpr uint32_t lds = kStages * 2 * 64 * D;
-    const hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(many_rows_kernel<D>), lds);
+    const auto many = [&](auto kernel) {
+      const hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kernel), lds);
+      if (e == hipSuccess) {
+        kernel<<<uint32_t(p.grid), kWaves * kWave, lds, s>>>(a, x, each);
+      }
+      return e;
+    };
+    const bool longer = p.part_tokens > uint64_t(kManyBlocks) << a.pool.shift;
+    const hipError_t e = longer ? many(many_rows_kernel<D, true>) : many(many_rows_kernel<D, false>);
     if (e != hipSuccess) {
       return e;
     }
-    many_rows_kernel<D><<<uint32_t(p.grid), kWaves * kWave, lds, s>>>(a, x, each);
   } else if (x.scores != nullptr) {
     few(few_rows_kernel<D, 8, true, true>, few_rows_kernel<D, 4, true, true>);
   } else if (p.one_tile) {
