@@ -859,7 +859,10 @@ class KvCache:
         heads, dim = q.shape[1], self.head_dim
         rows, q_row, q_head = _strides3(q, "q", heads, dim)
         if out is None:
-            out, out_row, out_head = q.new_empty((rows, heads, dim)), 0, 0
+            # empty_like costs 0.6 us, new_empty 1.5.
+            out = _torch().empty_like(q) if q.is_contiguous() else \
+                q.new_empty((rows, heads, dim))
+            out_row, out_head = 0, 0
         else:
             out_rows, out_row, out_head = _strides3(out, "out", heads, dim)
             if out_rows != rows:
