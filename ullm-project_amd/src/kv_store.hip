@@ -7,29 +7,58 @@ namespace {
 
 constexpr uint32_t kThreads = 256;
 
-// 16 bf16 of a row (two 16-byte loads, or 16 loads where rows are unaligned).
-struct alignas(16) Bf16x16 {
-  uint16_t v[16];
+// 16 bf16 of a row, two to a word (two 16-byte loads, or 16 loads where rows
+// are unaligned).
+struct Bf16x16 {
+  u32x4 w[2];
 };
 __device__ __forceinline__ Bf16x16 load16(const uint16_t *p, bool vec) {
   Bf16x16 r;
   if (vec) {
-    u32x4 *o = reinterpret_cast<u32x4 *>(&r);
-    o[0] = reinterpret_cast<const u32x4 *>(p)[0];
-    o[1] = reinterpret_cast<const u32x4 *>(p)[1];
+    r.w[0] = reinterpret_cast<const u32x4 *>(p)[0];
+    r.w[1] = reinterpret_cast<const u32x4 *>(p)[1];
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      r.v[i] = p[i];
+    for (int i = 0; i < 8; ++i) {
+      r.w[i / 4][i % 4] = p[2 * i] | uint32_t(p[2 * i + 1]) << 16;
     }
   }
   return r;
 }
 
-// Magnitude bits of a bf16, 0 for infinities and NaN.
-__device__ __forceinline__ uint32_t finite_magnitude(uint16_t h) {
-  const uint32_t a = h & 0x7fffu;
-  return a < 0x7f80u ? a : 0u;
+// The larger magnitude bits in each half of a word, of what was found so far
+// and two bf16.
+__device__ __forceinline__ uint32_t max_magnitudes(uint32_t top, uint32_t w) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t,
+                            __builtin_elementwise_max(__builtin_bit_cast(u16x2, top),
+                                                      __builtin_bit_cast(u16x2, w & 0x7fff7fffu)));
+}
+// Two bf16 with infinities and NaN as 0, or with magnitudes past 448 * 2^119
+// as that.
+__device__ __forceinline__ uint32_t each_half(uint32_t w, bool finite) {
+  const auto one = [&](uint32_t h) {
+    const uint32_t m = h & 0x7fffu;
+    return finite ? (m < 0x7f80u ? h : 0u) : (m > 0x7f60u && m < 0x7f80u ? h - m + 0x7f60u : h);
+  };
+  return one(w & 0xffffu) | one(w >> 16) << 16;
+}
+// Magnitude bits of the largest finite one of N rows' pieces.
+template <uint32_t N>
+__device__ __forceinline__ uint32_t largest_magnitude(const Bf16x16 (&x)[N]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < 8 * N; ++i) {
+    top = max_magnitudes(top, x[i / 8].w[i / 4 % 2][i % 4]);
+  }
+  if (max(top & 0xffffu, top >> 16) >= 0x7f80u) {  // once more, past infinities and NaN
+    top = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 8 * N; ++i) {
+      top = max_magnitudes(top, each_half(x[i / 8].w[i / 4 % 2][i % 4], true));
+    }
+  }
+  return max(top & 0xffffu, top >> 16);
 }
 // Smallest exponent e with a <= 448 * 2^e = 1.75 * 2^(e + 8), clamped, of
 // magnitude bits of a bf16.
@@ -48,16 +77,29 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
   r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, clip(c), clip(d), 1.0f, true);
   return __builtin_bit_cast(uint32_t, r);
 }
-// A bf16 to encode, over 2^e: infinities become NaN.
-__device__ __forceinline__ float scaled(uint16_t h, float inv) {
-  return (h & 0x7f80u) == 0x7f80u ? __builtin_nanf("") : bf16_to_f32(h) * inv;
-}
-__device__ __forceinline__ u32x4 encode16(const Bf16x16 &x, float inv) {
+// Codes of 16 bf16 over 2^e, of magnitudes that 448 * 2^e reaches: rounded to
+// nearest even, infinities and NaN to NaN (checked for every bf16).  Only the
+// largest exponent leaves finite elements past its reach.
+__device__ __forceinline__ u32x4 encode16(Bf16x16 x, int e) {
+  typedef short s16x2v __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  if (e == kKvExpMax) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x.w[i / 4][i % 4] = each_half(x.w[i / 4][i % 4], false);
+    }
+  }
+  const float power = exp2_int(e);
   u32x4 w;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    w[i] = encode4(scaled(x.v[4 * i], inv), scaled(x.v[4 * i + 1], inv),
-                   scaled(x.v[4 * i + 2], inv), scaled(x.v[4 * i + 3], inv));
+    const auto pair = [&](int j) {
+      return __builtin_bit_cast(bf16x2, uint32_t(x.w[i / 2][i % 2 * 2 + j]));
+    };
+    s16x2v r = {0, 0};
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, pair(0), power, false);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, pair(1), power, true);
+    w[i] = __builtin_bit_cast(uint32_t, r);
   }
   return w;
 }
@@ -108,8 +150,10 @@ __device__ __forceinline__ uint32_t value_token(uint32_t g, uint32_t j) {
 // known.  Keys are written from there, values go through LDS, where a token's
 // bytes take their places among the others' of a 16-byte unit.  Codes that
 // were there are touched only when the exponent grows, or where they share a
-// unit with a new one.  (15760 tokens of 8 heads: 21 us; with rows read twice
-// and values two bytes at a time 33.)
+// unit with a new one.  Bound by reading and writing: 12000 tokens of 8 heads
+// 16 us, 4.6 TB/s (with 32-token blocks, whose workgroups have half the work
+// for the same start, 18.6; a token encoded with 18 vector instructions per
+// element instead of 4: 21; rows read twice and values two bytes at a time 33).
 template <int D, uint32_t bt>
 __global__ __launch_bounds__(kThreads) void append_kernel(KvAppendArgs a, uint32_t each_slots) {
   constexpr uint32_t kUnits = (bt * (D / 16) + kThreads - 1) / kThreads;  // of a thread
@@ -152,15 +196,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(KvAppendArgs a, uint32
   }
   const uint64_t unit = uint64_t(id) * a.pool.heads + head;
   const int ek0 = a.pool.exps[unit * 2], ev0 = a.pool.exps[unit * 2 + 1];
-  uint32_t ak = 0, av = 0;
-#pragma unroll
-  for (uint32_t r = 0; r < kUnits; ++r) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      ak = max(ak, finite_magnitude(x[r].v[i]));
-      av = max(av, finite_magnitude(y[r].v[i]));
-    }
-  }
+  uint32_t ak = largest_magnitude(x), av = largest_magnitude(y);
   block_umax2(ak, av);
   int ek = exponent_for(ak), ev = exponent_for(av);
   float fk = 1.f, fv = 1.f;  // factor of the codes that were there
@@ -174,7 +210,6 @@ __global__ __launch_bounds__(kThreads) void append_kernel(KvAppendArgs a, uint32
     a.pool.exps[unit * 2] = int8_t(ek);
     a.pool.exps[unit * 2 + 1] = int8_t(ev);
   }
-  const float ik = exp2_int(-ek), iv = exp2_int(-ev);
   uint8_t *kc = a.pool.codes + unit * (uint64_t(2 * D) << a.pool.shift);
   uint8_t *vc = kc + (uint64_t(D) << a.pool.shift);
 
@@ -188,8 +223,8 @@ __global__ __launch_bounds__(kThreads) void append_kernel(KvAppendArgs a, uint32
   for (uint32_t r = 0; r < kUnits; ++r) {
     const uint32_t t = token(r);
     if (t < hi) {
-      *reinterpret_cast<u32x4 *>(kc + kv_key_unit<D>(t, c)) = encode16(x[r], ik);
-      const u32x4 w = encode16(y[r], iv);
+      *reinterpret_cast<u32x4 *>(kc + kv_key_unit<D>(t, c)) = encode16(x[r], ek);
+      const u32x4 w = encode16(y[r], ev);
       uint8_t *at = image + kv_value_byte<D>(t, c * 16);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -235,24 +270,23 @@ __global__ __launch_bounds__(kThreads) void append_kernel(KvAppendArgs a, uint32
   }
 }
 
-// Two times eight codes as bf16, times a power of two.
+// 16 codes as bf16, times a power of two: exact.
 __device__ __forceinline__ void store_decoded(uint16_t *to, u32x4 w, float f) {
-  typedef float f2 __attribute__((ext_vector_type(2)));
   u32x4 o[2];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const f2 x = __builtin_amdgcn_cvt_pk_f32_fp8(int(w[i]), false);
-    const f2 y = __builtin_amdgcn_cvt_pk_f32_fp8(int(w[i]), true);
-    o[i / 2][i % 2 * 2] = f32x2_to_bf16x2(x[0] * f, x[1] * f);
-    o[i / 2][i % 2 * 2 + 1] = f32x2_to_bf16x2(y[0] * f, y[1] * f);
+    o[i / 2][i % 2 * 2] = __builtin_bit_cast(
+        uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], f, false));
+    o[i / 2][i % 2 * 2 + 1] = __builtin_bit_cast(
+        uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], f, true));
   }
   reinterpret_cast<u32x4 *>(to)[0] = o[0];
   reinterpret_cast<u32x4 *>(to)[1] = o[1];
 }
 
 // One workgroup reads 32 tokens of one head, from a multiple of 32 on: 16
-// bytes to a thread and load; values are brought into rows in LDS.  (15760
-// tokens of 8 heads: 15 us; a workgroup for each row, which fetches all it
+// bytes to a thread and load; values are brought into rows in LDS.  (12000
+// tokens of 8 heads: 15 us, 4.9 TB/s; a workgroup for each row, which fetches all it
 // needs to know for 4 KiB, 36.)
 template <int D>
 __global__ __launch_bounds__(kThreads) void gather_kernel(KvGatherArgs a, uint32_t each_slots) {
@@ -659,7 +693,7 @@ __device__ __forceinline__ float code_factor(int from, int to) {
 // bytes go to their new places in LDS.  Then the exponents are known, and
 // codes whose exponent does not change are written as they are.  Bound by the
 // values' units, eight bytes read for each that is kept (the cache lines serve
-// several tokens).  (16 sequences to 1536 tokens of 8 heads: 44 us; with loads
+// several tokens).  (16 sequences to 1536 tokens of 8 heads: 42 us; with loads
 // of single bytes, twice, 86.)
 template <int D, uint32_t bt>
 __global__ __launch_bounds__(kThreads) void evict_move_kernel(KvEvictArgs a) {
