@@ -132,7 +132,9 @@ typedef struct ullm_kv_cache_gather_desc_t {
  *   lse = log(sum_t exp(scale * q.k_t));
  * a query that sees no token gives zeros and lse = -infinity.  Query head h
  * reads key/value head h / (heads / kv_heads).  Scores, sums and accumulators
- * are f32, the softmax weights enter the product with V in f16. */
+ * are f32, the softmax weights enter the product with V in f16, 2^11 for the
+ * largest of a row: each with a relative error of 2^-11, and those below 2^-25
+ * of the largest with an absolute one of 2^-36 of it. */
 typedef struct ullm_kv_cache_attend_desc_t {
   uint32_t struct_size;
   uint32_t abi_version;
