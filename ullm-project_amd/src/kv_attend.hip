@@ -1517,8 +1517,11 @@ KvAttendPlan plan_kv_attend(const KvAttendArgs &a, uint32_t dim) {
   p.one_tile = rows_of_head <= uint64_t(kRows) * a.seqs.batch;
   p.grid = tiles * p.parts;
   // Eight waves shorten the walk of a lone workgroup (333 tokens: 5.7 against
-  // 6.2 us), four have less to join where all units are busy.
-  p.waves = p.grid <= cus / 2 ? 8 : 4;
+  // 6.2 us) and keep enough bytes on their way where a workgroup has a unit to
+  // itself and 64 dims (131072 tokens of 8 heads: 27.4 against 32.2 us); four
+  // have less to join and do better beyond that (128 dims, 32 sequences of 2000
+  // tokens: 24.4 against 26.4; 64 dims, 64 of them: 24.5 against 27.1).
+  p.waves = p.grid <= uint64_t(cus) * 64 / dim ? 8 : 4;
   scratch_of(a, dim, p, nullptr, &p.workspace);
   return p;
 }
