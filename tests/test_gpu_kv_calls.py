@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from kv_reference import encode, exponent
+import test_gpu_kv_cache as T
 from test_gpu_kv_cache import Pair, f64
 
 pytestmark = pytest.mark.gpu
@@ -156,13 +157,17 @@ def test_calls_without_work(calls, uh, gpu):
 
 # --------------------------------------------------------------------- plans
 
+WIDE = 4160  # tokens of tables that the large tiles are chosen for
+
+
 @pytest.mark.parametrize("counts,heads,lengths,few,parts", [
     ([1], 8, [333], True, 1),
     ([1], 8, [5000], True, 2),
-    ([12, 12], 8, [400, 90], True, 1),       # 48 rows for each sequence and head
-    ([13, 12], 8, [400, 90], False, 1),
-    ([13, 13], 8, [400, 90], False, 1),
-    ([150], 8, [3000], False, 2)])
+    ([16], 8, [5000], True, 2),              # 64 rows for each sequence and head
+    ([17], 8, [5000], False, 2),
+    ([150, 12], 8, [400, 90], True, 1),      # few tokens
+    ([150], 8, [5000], False, 2),
+    ([1500, 700], 16, [1500, 700], False, 1)])
 def test_plans_and_their_results(uh, gpu, counts, heads, lengths, few, parts):
     p = Pair(uh, gpu, lengths, heads=2, seed=sum(counts))
     p.fill()
@@ -182,7 +187,7 @@ def test_tiles_of_many_sequences(uh, gpu):
     counts = [int(n) for n in rs.integers(0, 60, 70)]
     counts[5], counts[69] = 0, 200
     lengths = [n + int(m) for n, m in zip(counts, rs.integers(0, 40, 70))]
-    p = Pair(uh, gpu, lengths, heads=1, bt=32, dim=64, seed=4)
+    p = Pair(uh, gpu, lengths, heads=1, bt=32, dim=64, seed=4, spare=WIDE // 32)
     p.fill()
     p.check_attend(counts, 4, kernel=uh.KV_KERNEL_MANY_ROWS, accumulate=True)
 
@@ -190,9 +195,56 @@ def test_tiles_of_many_sequences(uh, gpu):
 @pytest.mark.parametrize("counts", [[1, 300, 0, 129, 40], [300, 1], [0, 0, 500], [128, 128]])
 def test_tiles_of_ragged_prompts(uh, gpu, counts):
     lengths = [n + 7 * i for i, n in enumerate(counts)]
-    p = Pair(uh, gpu, lengths, heads=2, seed=5)
+    p = Pair(uh, gpu, lengths, heads=2, seed=5, spare=WIDE // 64)
     p.fill()
     p.check_attend(counts, 4, kernel=uh.KV_KERNEL_MANY_ROWS, accumulate=True)
+
+
+@pytest.mark.parametrize("case", [
+    lambda *g: T.test_ragged_rows(*g, 128, 8, 2, 0, True),
+    lambda *g: T.test_ragged_rows(*g, 64, 7, 1, 0, False),
+    lambda *g: T.test_prompts_and_chunks(*g, 700, 700, 128, 8, 2, 0),
+    lambda *g: T.test_prompts_and_chunks(*g, 1500, 130, 64, 14, 2, 0),
+    lambda *g: T.test_values_of_very_different_blocks(*g),
+    lambda *g: T.test_nan_and_infinity_stay_with_the_rows_that_see_them(*g, 100),
+    lambda *g: T.test_stale_tokens_are_not_seen(*g),
+    lambda *g: T.test_blocks_out_of_the_pool_are_not_seen(*g),
+    lambda *g: T.test_query_and_output_strides(*g, 150),
+    lambda *g: T.test_repeated_calls_give_the_same_bits(*g),
+    lambda *g: T.test_other_streams_and_workspaces(*g)])
+def test_with_wide_tables(uh, gpu, monkeypatch, case):
+    """Tests of small tiles with tables that the large ones are chosen for."""
+    init, attend, kernels = Pair.__init__, uh.KvCache.attend, set()
+
+    def wide(self, uh, gpu, lengths, bt=64, spare=0, **kw):
+        init(self, uh, gpu, lengths, bt=bt, spare=spare + WIDE // bt, **kw)
+
+    def watched(self, q, lengths, tables, out=None, lse=None, workspace=None, **kw):
+        kernels.add(self.attend_plan(q, lengths, tables, **kw).kernel)
+        return attend(self, q, lengths, tables, out=out, lse=lse, workspace=workspace, **kw)
+
+    monkeypatch.setattr(Pair, "__init__", wide)
+    monkeypatch.setattr(uh.KvCache, "attend", watched)
+    case(uh, gpu)
+    assert uh.KV_KERNEL_MANY_ROWS in kernels
+
+
+@pytest.mark.parametrize("dim,group,rows", [(128, 4, 520), (64, 7, 300), (128, 1, 2100)])
+@pytest.mark.parametrize("window", [0, 1, 17, 300])
+def test_windows_of_large_tiles(uh, gpu, dim, group, rows, window):
+    p = Pair(uh, gpu, [rows + 90, 80], heads=8, dim=dim, bt=32, seed=window)
+    p.fill()
+    p.check_attend([rows, 1], 8 * group, window=window, accumulate=True,
+                   kernel=uh.KV_KERNEL_MANY_ROWS)
+
+
+def test_large_scores_of_large_tiles(uh, gpu):
+    """Maxima that grow all along, scores of both signs, scales of all kinds."""
+    p = Pair(uh, gpu, [900], heads=2, seed=12, spare=WIDE // 64)
+    ramp = torch.arange(900, device=gpu).view(900, 1, 1) / 60
+    p.append([900], k=p.random(900, 2).float().mul(ramp).bfloat16())
+    for scale in (None, 1.0, -0.3, 0.0, 1e-30, 50.0):
+        p.check_attend([120], 8, scale=scale, kernel=uh.KV_KERNEL_MANY_ROWS)
 
 
 @pytest.mark.parametrize("nan", [False, True])
@@ -201,12 +253,12 @@ def test_long_prompt_of_small_blocks(uh, gpu, nan):
     against the same values in larger blocks: the stored values are equal
     (read back from the larger blocks, whose exponents reach further), the
     products and sums too, up to powers of two."""
-    n, rows = 20000, 12800
+    n, rows = 40064, 12800
     g = torch.Generator(device=gpu).manual_seed(5)
     k, v = (torch.randn((n, 1, 64), generator=g, device=gpu).bfloat16() for _ in range(2))
     q = torch.randn((rows, 4, 64), generator=g, device=gpu).bfloat16()
     if nan:
-        v[19990, 0, 7] = float("nan")
+        v[n - 10, 0, 7] = float("nan")
     length = torch.tensor([n], dtype=torch.int32, device=gpu)
     got = []
     for bt in (128, 32):
@@ -215,7 +267,7 @@ def test_long_prompt_of_small_blocks(uh, gpu, nan):
         c.append(k, v, length, table)
         k, v = c.gather(length, table, n)
         p = c.attend_plan(q, length, table)
-        assert p.kernel == uh.KV_KERNEL_MANY_ROWS and p.parts == 1
+        assert p.kernel == uh.KV_KERNEL_MANY_ROWS and p.parts == 2 and p.part_tokens > 512 * 32
         lse = torch.empty((rows, 4), device=gpu)
         got.append((c.attend(q, length, table, lse=lse, accumulate=True), lse,
                     c.gather_weights(length, table, n)))

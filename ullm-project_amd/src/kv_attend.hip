@@ -1479,34 +1479,50 @@ static uint64_t each_tiles(const KvAttendArgs &a, uint32_t rows) {
 }
 
 // Tokens are split where the tiles alone leave compute units idle, into parts
-// that together give each a workgroup: more and smaller parts cost their
-// start and the join (131072 tokens of 8 heads: 32 parts each 46.7 us, 64
-// 50.1, 128 53.2).  A part has at least kPartLeast tokens (333 tokens of 8
-// heads: whole 5.7 us, in two parts 7.8), with few rows at most 64 blocks,
-// what a wave looks up with one load.
-constexpr uint32_t kPartLeast = 512;
-// Rows of a sequence and key/value head, on average, up to which small tiles
-// serve.
-constexpr uint32_t kFewMost = 48;
+// that together give each a workgroup: more and smaller parts cost their start
+// and the join (131072 tokens of 8 heads: 32 parts each 46.7 us, 64 50.1, 128
+// 53.2).  With many rows two of them, three at 64 dims, run at once (twice 128
+// queries at 8000 tokens 56 us, three 76; 64 dims, 28 heads over 4, 500 queries
+// at 8000: 70, three 68).  Many rows that fill the units by themselves are
+// split in two if they are long (8 times 128 queries at 16000 tokens: 327 us,
+// whole 343; 4 times 300: 406, whole 488), and not if they are short (16 times
+// 64 at 2000: 51, in three 64; 1024 at 1024: 30, in two 45).  A part has at least kPartLeast
+// tokens (333 tokens of 8 heads: whole 5.7 us, in two parts 7.8), with few rows
+// at most 64 blocks, what a wave looks up with one load.
+constexpr uint32_t kPartLeast = 512, kPartLong = 8192;
+// Small tiles serve up to kFewMost rows of a sequence and key/value head, on
+// average, and more where all their tiles run at about once and the tokens are
+// not many (us, 32 heads over 8, small tiles against large ones): 512 queries
+// at 512 tokens 13 / 18, 4 times 128 at 2000 37 / 41, 8 times 64 at 1000 23 /
+// 28; past that 8 times 128 at 1000 39 / 30, 32 at 30000 42 / 37.  64 times 16
+// at 4000 tokens: 157 / 164, 64 times 24 206 / 167.
+constexpr uint32_t kFewMost = 64, kFewTilesOfUnit = 4, kFewTokens = 4096;
 
 KvAttendPlan plan_kv_attend(const KvAttendArgs &a, uint32_t dim) {
   KvAttendPlan p;
   if (a.seqs.rows == 0 || a.seqs.batch == 0) {
     return p;
   }
+  const uint32_t cus = device_cu_count();
   const uint64_t rows_of_head = uint64_t(a.seqs.rows) * a.group;
-  const bool many = rows_of_head > uint64_t(kFewMost) * a.seqs.batch;
+  const auto tiles_of = [&](uint32_t rows) {
+    return kv_slots(a.seqs, a.group, rows, 1, each_tiles(a, rows)) * a.pool.heads;
+  };
+  // The most tokens that a tile's rows see, from the start of a 32-token group.
+  const auto span_of = [&](uint32_t rows) {
+    const uint64_t all = uint64_t(a.seqs.max_blocks) << a.pool.shift;
+    return a.window == 0 ? all
+                         : std::min<uint64_t>(all, uint64_t(a.window) + rows / a.group + 32);
+  };
+  const bool many = rows_of_head > uint64_t(kFewMost) * a.seqs.batch &&
+                    (tiles_of(kRows) > uint64_t(kFewTilesOfUnit) * cus ||
+                     span_of(kRows) > kFewTokens);
   p.kernel = many ? ULLM_KV_KERNEL_MANY_ROWS : ULLM_KV_KERNEL_FEW_ROWS;
   p.row_tile = many ? kManyRows : kRows;
-  const uint64_t tiles =
-      kv_slots(a.seqs, a.group, p.row_tile, 1, each_tiles(a, p.row_tile)) * a.pool.heads;
-  // The most tokens that a tile's rows see, from the start of a 32-token group.
-  uint64_t span = uint64_t(a.seqs.max_blocks) << a.pool.shift;
-  if (a.window != 0) {
-    span = std::min<uint64_t>(span, uint64_t(a.window) + p.row_tile / a.group + 32);
-  }
-  const uint32_t cus = device_cu_count();
-  const uint64_t split = std::max<uint64_t>((many ? 3 : 1) * cus / tiles, 1);
+  const uint64_t tiles = tiles_of(p.row_tile), span = span_of(p.row_tile);
+  const uint64_t split = tiles < cus ? (!many ? 1 : dim == 64 ? 3 : 2) * cus / tiles
+                         : many && span > kPartLong && tiles < 2 * cus ? 2
+                                                                       : 1;
   const uint64_t part = std::max<uint64_t>((span + split - 1) / split, kPartLeast);
   const uint64_t most = many ? uint64_t(1) << 31 : uint64_t(64) << a.pool.shift;
   p.part_tokens = uint32_t(std::min<uint64_t>((part + kStep - 1) / kStep * kStep, most));
