@@ -1564,7 +1564,7 @@ static hipError_t launch_attend(const KvAttendArgs &a, const KvAttendPlan &p, vo
       }
       return e;
     };
-    const bool longer = p.part_tokens > uint64_t(kManyBlocks) << a.pool.shift;
+    const bool longer = p.part_tokens > kv_part_limit(kManyBlocks, a.pool.shift, a.window);
     const hipError_t e = longer ? many(many_rows_kernel<D, true>) : many(many_rows_kernel<D, false>);
     if (e != hipSuccess) {
       return e;

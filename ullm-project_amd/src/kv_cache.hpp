@@ -194,6 +194,15 @@ __device__ __forceinline__ KvSlot kv_find_slot(const KvSeqs &s, uint32_t id, uin
   }
   return r;
 }
+// The most tokens of a part that touches at most `blocks` blocks of 2^shift
+// tokens, wherever it starts: with a window the first part of a tile starts at
+// any 32-token group, so that up to a block less 32 tokens precede it in its
+// first block; without one parts start at multiples of their size, which is
+// one of 64.
+constexpr uint64_t kv_part_limit(uint32_t blocks, uint32_t shift, uint32_t window) {
+  return (uint64_t(blocks) << shift) - (window != 0 ? (1u << shift) - 32u : 0u);
+}
+
 inline uint64_t kv_slots(const KvSeqs &s, uint64_t mult, uint64_t tile, uint64_t extra,
                          uint64_t each_slots) {
   return s.starts == nullptr ? uint64_t(s.batch) * each_slots
