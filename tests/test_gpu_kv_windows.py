@@ -50,3 +50,36 @@ def test_window_of_many_rows_over_all_held_blocks(uh, gpu, bt, window, rows):
                                              64 ** -0.5, window)
     within(out[at], ref, tol, "out")
     within(lse[at], rlse, ltol, "lse")
+
+
+@pytest.mark.parametrize("bt,window,dim,batch,rows", [
+    (64, 4096, 128, 40, 1), (64, 8192, 128, 17, 1), (128, 8192, 64, 40, 1),
+    (128, 8100, 64, 40, 1), (32, 4096, 64, 40, 1), (64, 4096, 64, 20, 4)])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_window_of_few_rows_over_all_looked_up_blocks(uh, gpu, bt, window, dim, batch, rows,
+                                                      accumulate):
+    """Parts of 64 blocks' tokens that touch one block more: sequences that
+    share one table and end at every place in a block."""
+    heads, kv_heads = 32, 8
+    s = Sequence(uh, gpu, window + 640, bt, kv_heads, dim, window + bt + rows, last=800)
+    lengths = torch.tensor([s.length - 15 * i for i in range(batch)], dtype=torch.int32,
+                           device=gpu)
+    tables = s.table.expand(batch, -1).contiguous()
+    q = s.queries(batch * rows, heads)
+    plan = s.cache.attend_plan(q, lengths, tables, window=window, accumulate=accumulate)
+    assert plan.kernel == uh.KV_KERNEL_FEW_ROWS
+    lse = torch.empty((batch * rows, heads), device=gpu)
+    out = s.cache.attend(q, lengths, tables, window=window, accumulate=accumulate, lse=lse)
+    added, bound = 0, 0
+    for b, n in enumerate(lengths.tolist()):
+        at = slice(b * rows, (b + 1) * rows)
+        ref, tol, rlse, ltol, p, ptol = attention64(
+            q[at], s.k, s.v, list(range(n - rows, n)), dim ** -0.5, window)
+        within(out[at], ref, tol, "out")
+        within(lse[at], rlse, ltol, "lse")
+        shape = (rows, kv_heads, heads // kv_heads, s.length)
+        added = added + p.view(shape).sum((0, 2)).T
+        bound = bound + ptol.view(shape).sum((0, 2)).T
+    if accumulate:
+        w = s.cache.gather_weights(lengths[:1], s.table, s.length)
+        within(w, added, bound + batch * 2.0 ** -23 * added, "weights")

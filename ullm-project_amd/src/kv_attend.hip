@@ -525,7 +525,7 @@ __global__ __launch_bounds__(W * kWave, 3) void few_rows_kernel(KvAttendArgs a, 
   const uint64_t row = t.first_row + r / a.group;
   // Three loads that wait for none: the query, the block numbers of the part
   // (with a window they depend on the length) and the length.  Lane i: block i
-  // of the part, which spans at most 64.
+  // of the part, which touches at most 64 (kv_part_limit).
   const Query<D> q = load_query<D>(a.q + row * a.q_row + head * a.q_head, a.vec, a.q_sign, g);
   const int32_t *table = a.seqs.tables + t.seq * a.seqs.stride;
   uint32_t block0 = part * x.part_tokens >> a.pool.shift;
@@ -1488,7 +1488,7 @@ static uint64_t each_tiles(const KvAttendArgs &a, uint32_t rows) {
 // whole 343; 4 times 300: 406, whole 488), and not if they are short (16 times
 // 64 at 2000: 51, in three 64; 1024 at 1024: 30, in two 45).  A part has at least kPartLeast
 // tokens (333 tokens of 8 heads: whole 5.7 us, in two parts 7.8), with few rows
-// at most 64 blocks, what a wave looks up with one load.
+// those of at most 64 blocks, what a wave looks up with one load.
 constexpr uint32_t kPartLeast = 512, kPartLong = 8192;
 // Small tiles serve up to kFewMost rows of a sequence and key/value head, on
 // average, and more where all their tiles run at about once and the tokens are
@@ -1524,7 +1524,8 @@ KvAttendPlan plan_kv_attend(const KvAttendArgs &a, uint32_t dim) {
                          : many && span > kPartLong && tiles < 2 * cus ? 2
                                                                        : 1;
   const uint64_t part = std::max<uint64_t>((span + split - 1) / split, kPartLeast);
-  const uint64_t most = many ? uint64_t(1) << 31 : uint64_t(64) << a.pool.shift;
+  const uint64_t most =
+      many ? uint64_t(1) << 31 : kv_part_limit(kWave, a.pool.shift, a.window) / kStep * kStep;
   p.part_tokens = uint32_t(std::min<uint64_t>((part + kStep - 1) / kStep * kStep, most));
   p.parts = uint32_t((span + p.part_tokens - 1) / p.part_tokens);
   // Scores cost 8 bytes for each row and token, a second pass over the keys
