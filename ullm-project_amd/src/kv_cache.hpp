@@ -203,6 +203,22 @@ constexpr uint64_t kv_part_limit(uint32_t blocks, uint32_t shift, uint32_t windo
   return (uint64_t(blocks) << shift) - (window != 0 ? (1u << shift) - 32u : 0u);
 }
 
+// Keys from .. from + width, cut into at most 4096 bins of 2^shift keys, and
+// the keys of one of the bins that has any: its end is the range's where it
+// reaches past that, for past 2^32 keys begin again at 0.
+struct KvKeyRange {
+  uint32_t from, width;
+};
+constexpr uint32_t kKvBinBits = 12;
+__host__ __device__ constexpr uint32_t kv_bin_shift(KvKeyRange r) {
+  const uint32_t bits = 32 - uint32_t(__builtin_clz(r.width | 1));
+  return bits > kKvBinBits ? bits - kKvBinBits : 0;
+}
+__host__ __device__ constexpr KvKeyRange kv_bin_keys(KvKeyRange r, uint32_t shift, uint32_t bin) {
+  const uint32_t skipped = bin << shift, most = (1u << shift) - 1;
+  return {r.from + skipped, r.width - skipped < most ? r.width - skipped : most};
+}
+
 inline uint64_t kv_slots(const KvSeqs &s, uint64_t mult, uint64_t tile, uint64_t extra,
                          uint64_t each_slots) {
   return s.starts == nullptr ? uint64_t(s.batch) * each_slots

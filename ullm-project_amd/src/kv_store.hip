@@ -415,7 +415,7 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 constexpr uint32_t kSelectThreads = 1024, kSelectWaves = kSelectThreads / kWave;
-constexpr uint32_t kSelectBins = 4096;
+constexpr uint32_t kSelectBins = 1u << kKvBinBits;
 
 // Exclusive sums over the workgroup in the order of the threads; `sums`: one
 // per wave.
@@ -559,23 +559,23 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(KvEvictArg
     atomicMax(&range[1], most);
   }
   __syncthreads();
-  uint32_t from = range[0] + 1, width = range[1] - from;  // keys from .. from + width
+  KvKeyRange cut{range[0] + 1, range[1] - (range[0] + 1)};
   uint32_t last;  // tokens of keys above it stay, and of this one `want`
   for (;;) {
-    last = from;
-    if (width == 0) {
+    last = cut.from;
+    if (cut.width == 0) {
       break;
     }
     for (uint32_t i = tid; i < kSelectBins; i += kSelectThreads) {
       hist[i] = 0;
     }
     __syncthreads();
-    const uint32_t bits = 32 - __builtin_clz(width), shift = bits > 12 ? bits - 12 : 0;
+    const uint32_t shift = kv_bin_shift(cut);
     each_span([&](uint32_t) __attribute__((always_inline)) {
 #pragma unroll
       for (uint32_t k = 0; k < K; ++k) {
-        const uint32_t off = keys[k] - from;
-        if (off <= width) {
+        const uint32_t off = keys[k] - cut.from;
+        if (off <= cut.width) {
           atomicAdd(&hist[kSelectBins - 1 - (off >> shift)], 1u);
         }
       }
@@ -600,11 +600,10 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(KvEvictArg
       upto += n[i];
     }
     __syncthreads();
-    from += pick[0] << shift;
+    cut = kv_bin_keys(cut, shift, pick[0]);
     want = pick[1];
-    width = (1u << shift) - 1;
     if (want == pick[2]) {
-      last = from - 1;
+      last = cut.from - 1;
       want = 0;
       break;
     }
