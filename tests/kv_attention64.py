@@ -5,11 +5,11 @@ stay cheap."""
 import torch
 
 
-def attention64(q, k, v, positions, scale, window=0):
+def attention64(q, k, v, positions, scale, window=0, absent=None):
     """q [rows][heads][dim] at `positions` over the tokens k, v
-    [length][kv_heads][dim] (bf16 or wider).  Returns out, its bound, lse, its
-    bound, all float64; with them the weights [rows][heads][length] and their
-    bound.
+    [length][kv_heads][dim] (bf16 or wider), but for the tokens that `absent`
+    [length] marks.  Returns out, its bound, lse, its bound, all float64; with
+    them the weights [rows][heads][length] and their bound.
 
     The bound: products of bf16 are exact and their f32 sums within 2^-20 of
     the sum of magnitudes; a weight enters the product with V in f16, with a
@@ -24,6 +24,8 @@ def attention64(q, k, v, positions, scale, window=0):
     sees = tok <= pos
     if window:
         sees &= tok > pos - window
+    if absent is not None:
+        sees &= ~absent
     got = []
     for h in range(heads):
         kh, vh, x = k[:, h // group], v[:, h // group], q[:, h]

@@ -375,6 +375,8 @@ __device__ __forceinline__ void attend_group(RowState<D> &st, Group<D> &x, const
       *reinterpret_cast<f32x4 *>(scores_to + t0 + 16 * i + 4 * g) = s[i];
     }
   }
+  // A block out of the pool has no say: its codes are those of another one.
+  ev = present ? ev : st.acc_exp;
   if (ev > st.acc_exp + kUp) {
     const float f = exp2_int(max(st.acc_exp - ev, -126));
 #pragma unroll
@@ -966,7 +968,8 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows_kernel(KvAttendAr
       }
       if (now.exp_code[u] != code) {
         code = now.exp_code[u];
-        const int ev = int(code & 0xffffu) - int(kExpCode);
+        // A block out of the pool has no say: its codes are those of another one.
+        const int ev = (code & kAbsent) != 0 ? acc_exp : int(code & 0xffffu) - int(kExpCode);
         if (ev > acc_exp + kUp) {
           const float f = exp2_int(max(acc_exp - ev, -126));
 #pragma unroll
