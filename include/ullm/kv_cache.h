@@ -134,7 +134,9 @@ typedef struct ullm_kv_cache_gather_desc_t {
  * reads key/value head h / (heads / kv_heads).  Scores, sums and accumulators
  * are f32, the softmax weights enter the product with V in f16, 2^11 for the
  * largest of a row: each with a relative error of 2^-11, and those below 2^-25
- * of the largest with an absolute one of 2^-36 of it. */
+ * of the largest with an absolute one of 2^-36 of it.  So it is for values
+ * beside blocks with exponents up to 60 above theirs; next to larger ones they
+ * may be lost. */
 typedef struct ullm_kv_cache_attend_desc_t {
   uint32_t struct_size;
   uint32_t abi_version;

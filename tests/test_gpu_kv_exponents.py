@@ -63,3 +63,40 @@ def test_absent_blocks_leave_no_trace(uh, gpu, rows, few, dim, bt):
     """A table entry that names no block, while the pool's first one holds
     values of 2^120."""
     _case(uh, gpu, [1.0] * 9, rows, few, dim, bt, seed=1, absent=(0, 3, 7))
+
+
+@pytest.mark.parametrize("rows,few", SHAPES)
+@pytest.mark.parametrize("stds", [
+    [1.0, 2.0 ** 60, 1.0, 1.0, 1.0, 1.0], [2.0 ** 60, 1.0, 2.0 ** -20, 1.0, 2.0 ** -14, 1.0],
+    [1.0, 2.0 ** 17, 1.0, 2.0 ** 34, 1.0, 2.0 ** 51], [2.0 ** -60, 2.0 ** -30, 1.0, 2.0 ** 16,
+                                                       2.0 ** 15, 2.0 ** 14],
+    [1.0, 0.0, 1.0, 0.0, 2.0 ** -16, 1.0]])
+def test_large_values_in_some_dimensions(uh, gpu, rows, few, stds):
+    """What one block holds in some dimensions takes nothing from the others'
+    dimensions, which it is zero in."""
+    _case(uh, gpu, stds, rows, few, seed=2)
+    _case(uh, gpu, stds, rows, few, dim=64, bt=128, seed=3)
+
+
+# With a short window the kernel of many rows takes calls of 1024 tiles of 16.
+WINDOWS = [(1, True), (40, True), (2100, False)]
+
+
+@pytest.mark.parametrize("rows,few", WINDOWS)
+@pytest.mark.parametrize("window", [70, 192])
+def test_large_values_out_of_the_window(uh, gpu, rows, few, window):
+    """A block of 2^60 times the others' values that some rows of a tile see
+    and the next ones do not."""
+    if few:
+        _case(uh, gpu, [1.0, 1.0, 1.0, 2.0 ** 60, 1.0, 1.0], rows, few, seed=4, window=window)
+    else:
+        _case(uh, gpu, [1.0, 2.0 ** 60, 1.0, 1.0, 1.0, 1.0], rows, few, seed=4, window=window)
+
+
+@pytest.mark.parametrize("rows,few", WINDOWS)
+def test_large_tokens_of_a_block_that_is_seen_in_part(uh, gpu, rows, few):
+    """The block's exponent is that of a token out of every row's window."""
+    def change(v):
+        v[128] = 2.0 ** 60
+
+    _case(uh, gpu, [1.0] * 6, rows, few, seed=5, window=60 if rows > 1 else 200, change=change)

@@ -22,10 +22,11 @@
 // error 2^-11 each (bf16's 2^-8 would be the largest error of rows that see
 // few tokens), absolute 2^-36 of the largest weight.  Values enter as f16 too,
 // code * 2^d with d = (block's exponent) - (accumulator's exponent) in -15 .. 7,
-// where every E4M3 code is exact.  A block further below shifts its weights
-// down instead (kept exact in the sum, which is f32), one further above raises
-// the accumulator's exponent: blocks of any exponents meet in one product with
-// an error below 2^-60 of the largest value.
+// where every E4M3 code is exact.  A block outside of that moves the
+// accumulator's exponent to its own, which is exact in f32; but no further than
+// kSpread below the highest so far, where the accumulators end.  The exponents
+// are those of whole blocks, of tokens too that a row does not see: its own
+// values keep their precision beside any of up to 2^kSpread times their size.
 #include <algorithm>
 
 #include "kernels.hpp"
@@ -39,6 +40,9 @@ constexpr uint32_t kWaves = 4;
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr int kOff = 11;             // weights are at most 2^kOff in f16
 constexpr int kDown = -15, kUp = 7;  // exponents at which codes are exact in f16
+// Sums of 2^20 codes of 448 * 2^kUp with weights of 2^15 stay below 2^51, and
+// below 2^111 where their exponent is 60 lower.
+constexpr int kSpread = 60;
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
@@ -273,13 +277,30 @@ __device__ __forceinline__ void load_group_values(Group<D> &x, const uint8_t *un
   }
 }
 
+// The exponent of accumulators, sums over 2^now; `top`: the highest so far.
+struct SumExponent {
+  int now = kKvExpMin, top = kKvExpMin;
+
+  __device__ bool holds(int block) const { return block <= now + kUp && block >= now + kDown; }
+  // Towards that of a block; returns what the accumulators are multiplied by.
+  __device__ float move(int block) {
+    top = max(top, block);
+    const int to = max(block, top - kSpread);
+    const float f = exp2_int(max(now - to, -126));
+    now = to;
+    return f;
+  }
+  // Power of two of a block's codes as they enter the product.
+  __device__ float power(int block) const { return exp2_int(max(block - now, -126)); }
+};
+
 // What a row has met so far: the running maximum and the sum of 2^kOff
-// exp2(score - m) (this lane's part of it), and its accumulators, which hold
-// sums over 2^acc_exp.
+// exp2(score - m) (this lane's part of it), and its accumulators with their
+// exponent.
 template <int D>
 struct RowState {
   float m, l;
-  int acc_exp;
+  SumExponent exp;
   f32x4 o[D / 16];
 };
 
@@ -376,18 +397,15 @@ __device__ __forceinline__ void attend_group(RowState<D> &st, Group<D> &x, const
     }
   }
   // A block out of the pool has no say: its codes are those of another one.
-  ev = present ? ev : st.acc_exp;
-  if (ev > st.acc_exp + kUp) {
-    const float f = exp2_int(max(st.acc_exp - ev, -126));
+  ev = present ? ev : st.exp.now;
+  if (!st.exp.holds(ev)) {
+    const float f = st.exp.move(ev);
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {
       st.o[i] *= f;
     }
-    st.acc_exp = ev;
   }
-  const int d = ev - st.acc_exp;
-  const float pv = exp2_int(d < kDown ? kDown : d);
-  const int shift = d < kDown ? max(d - kDown, -100) : 0;
+  const float pv = st.exp.power(ev);
   float top = s[0][0];  // fmaxf passes NaN over: it makes the sum below NaN
 #pragma unroll
   for (int i = 1; i < 8; ++i) {
@@ -408,10 +426,10 @@ __device__ __forceinline__ void attend_group(RowState<D> &st, Group<D> &x, const
   float p[8], sum = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    p[i] = exp2_fast(s[i / 4][i % 4] - (ref - float(kOff + shift)));
+    p[i] = exp2_fast(s[i / 4][i % 4] - (ref - float(kOff)));
     sum += p[i];
   }
-  st.l += sum * exp2_int(-shift);
+  st.l += sum;
   u32x4 pw;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -547,7 +565,6 @@ __global__ __launch_bounds__(W * kWave, 3) void few_rows_kernel(KvAttendArgs a, 
   RowState<D> st;
   st.m = -INFINITY;
   st.l = 0.f;
-  st.acc_exp = kKvExpMin;
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
     st.o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -599,7 +616,7 @@ __global__ __launch_bounds__(W * kWave, 3) void few_rows_kernel(KvAttendArgs a, 
   }
   // Means of the wave's tokens, to be joined by their sums.
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  const float power = exp2_int(st.acc_exp);
+  const float power = exp2_int(st.exp.now);
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
     *reinterpret_cast<f32x4 *>(&part_o[wave][col][16 * i + 4 * g]) = st.o[i] * inv * power;
@@ -914,16 +931,12 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows_kernel(KvAttendAr
   const uint32_t key_at = tok / 16 * (D / 64) * 1024 + tok % 16 * 16 + h * 256;
   // The instructions of a group are what bounds this loop (a SIMD issues one
   // in four cycles, whatever its kind): what changes rarely is kept ready and
-  // changed under a branch.  bias: kOff + shift - m, what a scaled score
-  // becomes a power of two with; limit: the unscaled score past which m grows;
-  // power, unshift: those of the last exponent code.
-  int acc_exp = kKvExpMin;
+  // changed under a branch.  bias: kOff - m, what a scaled score becomes a
+  // power of two with; limit: the unscaled score past which m grows; power:
+  // that of the last exponent code.
+  SumExponent exp;
   uint32_t code = ~0u;
-  float bias = 0.f, limit = -INFINITY, power = 1.f, unshift = 1.f;
-  int shift = 0;
-  const auto new_bias = [&] {
-    bias = float(kOff + shift) - (st.m == -INFINITY ? 0.f : st.m);
-  };
+  float bias = float(kOff), limit = -INFINITY, power = 1.f;
   bool dirty = false;  // a NaN value in a group that some rows do not see
   for (uint32_t step = 0; step < steps; ++step) {
     wait_copies<0>();
@@ -969,20 +982,15 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows_kernel(KvAttendAr
       if (now.exp_code[u] != code) {
         code = now.exp_code[u];
         // A block out of the pool has no say: its codes are those of another one.
-        const int ev = (code & kAbsent) != 0 ? acc_exp : int(code & 0xffffu) - int(kExpCode);
-        if (ev > acc_exp + kUp) {
-          const float f = exp2_int(max(acc_exp - ev, -126));
+        const int ev = (code & kAbsent) != 0 ? exp.now : int(code & 0xffffu) - int(kExpCode);
+        if (!exp.holds(ev)) {
+          const float f = exp.move(ev);
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
             st.o[c] *= f;
           }
-          acc_exp = ev;
         }
-        const int d = ev - acc_exp;
-        power = exp2_int(d < kDown ? kDown : d);
-        shift = d < kDown ? max(d - kDown, -100) : 0;
-        unshift = exp2_int(-shift);
-        new_bias();
+        power = exp.power(ev);
       }
       if (((grp - whole.first) | (code & kAbsent)) >= whole.count) {
         const int32_t t0 = int32_t(grp * 32);
@@ -1019,7 +1027,7 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows_kernel(KvAttendAr
         st.l *= keep;
         st.m = m;
         limit = (m + kSlack) / a.scale_log2;
-        new_bias();
+        bias = float(kOff) - (m == -INFINITY ? 0.f : m);
       }
       float sum = 0.f;
       u32x4 p[2];
@@ -1031,7 +1039,7 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows_kernel(KvAttendAr
         sum += p1;
         p[e / 8][e % 8 / 2] = f32x2_to_f16x2(p0, p1);
       }
-      st.l = __builtin_fmaf(sum, unshift, st.l);
+      st.l += sum;
       add_values<D>(st, units, p, power);
     }
   }
@@ -1051,7 +1059,7 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows_kernel(KvAttendAr
     const auto half =
         __builtin_amdgcn_permlane32_swap(f32_bits(st.l), f32_bits(st.l), false, false);
     const float sum = bits_f32(half[0]) + bits_f32(half[1]);
-    const float join = sum == 0.f ? 0.f : 1.0f / sum, unit = exp2_int(acc_exp);
+    const float join = sum == 0.f ? 0.f : 1.0f / sum, unit = exp2_int(exp.now);
     const RowSink out = sink(32 * wave + i);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
@@ -1090,7 +1098,6 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows_kernel(KvAttendAr
     RowState<D> rs;
     rs.m = -INFINITY;
     rs.l = 0.f;
-    rs.acc_exp = kKvExpMin;
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) {
       rs.o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1109,7 +1116,7 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows_kernel(KvAttendAr
     }
     float l = rs.l + __shfl_xor(rs.l, 16, kWave);
     l += __shfl_xor(l, 32, kWave);
-    const float join = l == 0.f ? 0.f : 1.0f / l, power = exp2_int(rs.acc_exp);
+    const float join = l == 0.f ? 0.f : 1.0f / l, power = exp2_int(rs.exp.now);
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) {
       store4(a, x, out, D, 16 * c + 4 * g, rs.o[c] * join * power);
