@@ -10,7 +10,9 @@ it, so fixed stand-ins keep the chain well-defined and bounded:
     context=N it is attention over an 8-bit key/value cache of up to N tokens
     for each sequence instead: prompt() takes the sequences' first rows,
     step() one more each, and with evict_to=T evict() cuts each sequence to
-    the T tokens per head that received most of the weight.  Queries, keys
+    the T tokens per head that received most of the weight.  A call that a
+    sequence has no room for (N in whole blocks) raises ValueError; steps
+    replayed from a HIP graph are announced by replayed().  Queries, keys
     and values are the strided thirds of the qkv output.  Scores are not
     scaled (scale = 1 instead of 1 / sqrt(128)): those of unit normal rows
     are then far apart, and the output of a row stays near unit RMS however
@@ -138,12 +140,29 @@ class DecodeStack:
         self.tables = ids[:self.m * columns].view(self.m, columns)
         self.spare = ids[self.m * columns:].view(self.m, moved)
         self.lengths = torch.zeros((self.m,), dtype=torch.int32, device=self.dev)
+        self.room = columns * block_tokens
+        self.held = [0] * self.m        # lengths, as far as the host knows
         self.caches = [self.uh.KvCache(ids.numel(), self.kv_heads, dim,
                                        block_tokens=block_tokens,
                                        track_weights=self.evict_to > 0,
                                        device=torch.device(self.dev).index or 0)
                        for _ in range(self.layers)]
         self.attn = torch.empty((self.m, self.hidden), dtype=torch.bfloat16, device=self.dev)
+
+    def _grow(self, counts):
+        """Count new tokens of the sequences: the kernels take a length past
+        the tables as their end and would write over the last token."""
+        held = [n + c for n, c in zip(self.held, counts)]
+        if max(held) > self.room:
+            raise ValueError(f"a sequence would hold {max(held)} tokens, there is room for "
+                             f"{self.room}")
+        self.held = held
+
+    def replayed(self, steps=1):
+        """Announce replays of a graph that captured step(), before they run;
+        the captured call itself has not been counted."""
+        if self.caches:
+            self._grow([steps] * self.m)
 
     def _attention(self, layer, qkv, out, starts, stream):
         """Store the rows' keys and values, attend from their queries."""
@@ -174,6 +193,8 @@ class DecodeStack:
         every sequence grows by the step's token (on torch's current stream,
         which `stream` must then be)."""
         if self.caches:
+            if not self.torch.cuda.is_current_stream_capturing():
+                self._grow([1] * self.m)
             self.lengths.add_(1)
         self._layers(self.h0, self.h, self.qkv_out, self.attn if self.caches else None,
                      self.o_out, self.act, None, stream)
@@ -187,6 +208,7 @@ class DecodeStack:
         torch, rows = self.torch, h.shape[0]
         if not self.caches or len(counts) != self.m or min(counts) < 1 or sum(counts) != rows:
             raise ValueError("prompt needs a cache, and a count of rows for each sequence")
+        self._grow(counts)
         n = torch.tensor(counts, dtype=torch.int32, device=self.dev)
         ends = n.cumsum(0, dtype=torch.int32)
         starts = torch.cat([torch.zeros_like(ends[:1]), ends])
@@ -213,6 +235,7 @@ class DecodeStack:
         self.tables[:, :moved] = self.spare
         self.spare.copy_(left[:, :moved])
         self.lengths.copy_(lengths)
+        self.held = [min(n, self.evict_to) for n in self.held]
 
     def destroy(self):
         for cache in self.caches:
