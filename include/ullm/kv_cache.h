@@ -145,7 +145,9 @@ typedef struct ullm_kv_cache_attend_desc_t {
   const void *q;            /* device bf16 [rows][heads][head_dim] */
   uint64_t q_row_stride;    /* elements, 0 = heads * head_dim */
   uint64_t q_head_stride;   /* elements, 0 = head_dim */
-  void *out;                /* device bf16 [rows][heads][head_dim] */
+  void *out;                /* device bf16 [rows][heads][head_dim]: q itself,
+                               with its strides and without ACCUMULATE, or
+                               memory that does not overlap q */
   uint64_t out_row_stride;  /* elements, 0 = heads * head_dim */
   uint64_t out_head_stride; /* elements, 0 = head_dim */
   float *lse;               /* device f32 [rows][heads], or null */

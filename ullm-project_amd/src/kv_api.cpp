@@ -474,9 +474,19 @@ extern "C" ULLM_HIP_API ullm_status_t ullm_kv_cache_attend(
       return st;
     }
     const ullm_kv_cache_t *c = desc->cache;
+    const ullm::KvAttendArgs a = attend_args(desc);
+    if (desc->out == desc->q) {
+      // A workgroup reads its queries before it writes their results; the
+      // second pass for the weights comes after all results.
+      if (a.accumulate) {
+        return fail(error_sink, "out must not be q with ACCUMULATE");
+      }
+      if ((a.seqs.rows > 1 && a.out_row != a.q_row) || (a.heads > 1 && a.out_head != a.q_head)) {
+        return fail(error_sink, "out in place of q needs the strides of q");
+      }
+    }
     DeviceScope scope(c->device);
     HIP_TRY(error_sink, "hipSetDevice", scope.error());
-    const ullm::KvAttendArgs a = attend_args(desc);
     const ullm::KvAttendPlan p = ullm::plan_kv_attend(a, c->head_dim);
     // A launch counts its threads in 32 bits; the join has a wave for each row.
     if (p.grid > UINT32_MAX / 512 ||

@@ -887,8 +887,9 @@ class KvCache:
         strides honoured) over the cached tokens, bf16 [rows][heads][head_dim].  ``scale``
         defaults to 1 / sqrt(head_dim); with ``window`` a query sees that many
         tokens; ``lse`` (f32 [rows][heads]) receives the log of each row's sum;
-        ``accumulate`` adds to the weights of the tokens.  A query that sees
-        no token gives zeros."""
+        ``accumulate`` adds to the weights of the tokens.  ``out`` may be q
+        itself, but not with ``accumulate``.  A query that sees no token gives
+        zeros."""
         out, fields = self._attend_fields(q, lengths, tables, starts, out, lse, scale, window,
                                           accumulate, stream, workspace)
         _packed(KvAttendDesc).call(lib().ullm_kv_cache_attend, *fields)
