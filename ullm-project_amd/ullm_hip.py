@@ -681,6 +681,10 @@ def release_workspaces(device: int = 0) -> None:
 
 # --------------------------------------------------------- key/value cache
 
+def _misfit(e):
+    return ValueError(f"an argument does not fit its field: {e}")
+
+
 class _Packed:
     """A descriptor filled in one pack of its flattened fields, header first
     and reserved words left out (they stay zero): 0.6 us for the 25 fields of
@@ -704,12 +708,18 @@ class _Packed:
         self.sink_ref = self.sink.ref
 
     def fill(self, *fields):
-        self.pack(*fields)
+        try:
+            self.pack(*fields)
+        except struct.error as e:
+            raise _misfit(e) from None
         return self.ref
 
     def call(self, fn, *fields):
         """fn(descriptor of these fields), its error raised."""
-        self.pack(*fields)
+        try:
+            self.pack(*fields)
+        except struct.error as e:
+            raise _misfit(e) from None
         st = fn(self.ref, self.sink_ref)
         if st:
             raise HipError(st, self.sink.text())
@@ -728,7 +738,7 @@ def _strides3(t, name, heads, dim):
     """(rows, row stride, head stride) of a bf16 [rows][heads][dim] tensor."""
     shape = t.shape
     if len(shape) != 3 or shape[1] != heads or shape[2] != dim \
-            or t.dtype is not _torch().bfloat16:
+            or t.dtype is not (_torch_module or _torch()).bfloat16:
         raise ValueError(f"{name} must be bfloat16 [rows][{heads}][{dim}]")
     if t.is_contiguous():
         return shape[0], heads * dim, dim
@@ -791,8 +801,11 @@ class KvCache:
     # -- calls -------------------------------------------------------------
     def _seqs(self, lengths, tables, rows, starts):
         """The fields of a ullm_kv_sequences_t."""
-        i32 = _torch().int32
-        batch, columns = tables.shape
+        i32 = (_torch_module or _torch()).int32
+        shape = tables.shape
+        if len(shape) != 2:
+            raise ValueError("tables must be int32 [batch][columns] and lengths int32 [batch]")
+        batch, columns = shape
         if tables.dtype is not i32 or lengths.dtype is not i32 or lengths.shape != (batch,) \
                 or not lengths.is_contiguous():
             raise ValueError("tables must be int32 [batch][columns] and lengths int32 [batch]")
@@ -823,7 +836,7 @@ class KvCache:
         if v_rows != rows:
             raise ValueError("k and v must have the same number of rows")
         if weights is not None and (weights.shape != (rows, heads)
-                                    or weights.dtype is not _torch().float32
+                                    or weights.dtype is not (_torch_module or _torch()).float32
                                     or not weights.is_contiguous()):
             raise ValueError("weights must be a contiguous float32 [rows][kv_heads] tensor")
         _packed(KvAppendDesc).call(
@@ -831,6 +844,10 @@ class KvCache:
             self.handle or 0, *self._seqs(lengths, tables, rows, starts), k.data_ptr(), k_row,
             k_head, v.data_ptr(), v_row, v_head, 0 if weights is None else weights.data_ptr(),
             _stream(stream) or 0)
+
+    def _gatherable(self, lengths, tables, rows, starts):
+        if rows < 0:
+            raise ValueError("rows must not be negative")
 
     def _gather(self, lengths, tables, rows, starts, k, v, weights, stream):
         _packed(KvGatherDesc).call(
@@ -842,7 +859,8 @@ class KvCache:
         """Keys and values of each sequence's last rows (``rows`` in all), bf16
         [rows][kv_heads][head_dim] and exact: appending them again stores the
         same values.  Rows that name no token are zero."""
-        kv = tables.new_empty((2, rows, self.kv_heads, self.head_dim), dtype=_torch().bfloat16)
+        self._gatherable(lengths, tables, rows, starts)
+        kv = tables.new_empty((2, rows, self.kv_heads, self.head_dim), dtype=(_torch_module or _torch()).bfloat16)
         at = kv.data_ptr()
         self._gather(lengths, tables, rows, starts, at,
                      at + rows * self.kv_heads * self.head_dim * 2, 0, stream)
@@ -850,17 +868,23 @@ class KvCache:
 
     def gather_weights(self, lengths, tables, rows, starts=None, stream=None):
         """The weights of each sequence's last rows, f32 [rows][kv_heads]."""
-        w = tables.new_empty((rows, self.kv_heads), dtype=_torch().float32)
+        self._gatherable(lengths, tables, rows, starts)
+        w = tables.new_empty((rows, self.kv_heads), dtype=(_torch_module or _torch()).float32)
         self._gather(lengths, tables, rows, starts, 0, 0, w.data_ptr(), stream)
         return w
 
     def _attend_fields(self, q, lengths, tables, starts, out, lse, scale, window, accumulate,
                        stream, workspace):
-        heads, dim = q.shape[1], self.head_dim
+        dim, shape = self.head_dim, q.shape
+        if len(shape) != 3:
+            raise ValueError(f"q must be bfloat16 [rows][heads][{dim}]")
+        if not 0 <= window < 1 << 32:
+            raise ValueError("window must not be negative, and below 2^32")
+        heads = shape[1]
         rows, q_row, q_head = _strides3(q, "q", heads, dim)
         if out is None:
             # empty_like costs 0.6 us, new_empty 1.5.
-            out = _torch().empty_like(q) if q.is_contiguous() else \
+            out = (_torch_module or _torch()).empty_like(q) if q.is_contiguous() else \
                 q.new_empty((rows, heads, dim))
             out_row, out_head = 0, 0
         else:
@@ -870,7 +894,7 @@ class KvCache:
         if lse is None:
             lse_at = 0
         elif lse.shape != (rows, heads) or not lse.is_contiguous() \
-                or lse.dtype is not _torch().float32:
+                or lse.dtype is not (_torch_module or _torch()).float32:
             raise ValueError("lse must be a contiguous float32 [rows][heads] tensor")
         else:
             lse_at = lse.data_ptr()
@@ -912,16 +936,18 @@ class KvCache:
         them its first ``sink`` and last ``recent``, into the blocks of
         ``new_tables``.  Returns (lengths int32 [batch], positions that stay
         int32 [batch][kv_heads][keep], ascending, then -1)."""
+        if keep < 0 or sink < 0 or recent < 0:
+            raise ValueError("keep, sink and recent must not be negative")
+        seqs = self._seqs(lengths, tables, 0, None)
         batch = tables.shape[0]
         columns = -(-keep // self.block_tokens)
-        if new_tables.dtype is not _torch().int32 or new_tables.dim() != 2 \
+        if new_tables.dtype is not (_torch_module or _torch()).int32 or new_tables.dim() != 2 \
                 or new_tables.shape[0] != batch or new_tables.shape[1] < columns \
                 or (columns > 1 and new_tables.stride(1) != 1) \
                 or (batch > 1 and new_tables.stride(0) < columns):
             raise ValueError(f"new_tables must be int32 [batch][{columns} or more]")
-        seqs = self._seqs(lengths, tables, 0, None)
         lens = tables.new_empty((batch,))
-        kept = tables.new_empty((batch, self.kv_heads, max(keep, 0)))
+        kept = tables.new_empty((batch, self.kv_heads, keep))
         _packed(KvEvictDesc).call(
             lib().ullm_kv_cache_evict,
             self.handle or 0, *seqs, new_tables.data_ptr(),
