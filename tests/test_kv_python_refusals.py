@@ -70,3 +70,29 @@ def test_valid_arguments_reach_the_library(uh, cache):
                  lambda: cache.evict(n, t, t, 64)):
         with pytest.raises(uh.HipError, match="handle is null"):
             call()
+
+
+def test_tensors_of_another_device_are_refused(cache):
+    """The kernels would follow their addresses."""
+    q, n, t = _args()
+    kv, w = q[:, :2], torch.zeros(2, 2)
+    s = torch.zeros(3, dtype=torch.int32)
+    lse, ws = torch.zeros(2, 4), torch.zeros(256, dtype=torch.uint8)
+
+    class Other(torch.Tensor):
+        def get_device(self):
+            return 0
+
+    def one_elsewhere(fn, names, **args):
+        for name in names:
+            with pytest.raises(ValueError, match="on GPU"):
+                fn(**{**args, name: args[name].as_subclass(Other)})
+
+    one_elsewhere(cache.append, ["k", "v", "lengths", "tables", "starts", "weights"],
+                  k=kv, v=kv, lengths=n, tables=t, starts=s, weights=w)
+    one_elsewhere(cache.attend, ["q", "lengths", "tables", "starts", "out", "lse", "workspace"],
+                  q=q, lengths=n, tables=t, starts=s, out=q.clone(), lse=lse, workspace=ws)
+    for fn in (cache.gather, cache.gather_weights):
+        one_elsewhere(fn, ["lengths", "tables", "starts"], lengths=n, tables=t, rows=2, starts=s)
+    one_elsewhere(cache.evict, ["lengths", "tables", "new_tables"], lengths=n, tables=t,
+                  new_tables=t, keep=64)

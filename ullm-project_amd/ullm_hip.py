@@ -799,6 +799,11 @@ class KvCache:
         return i
 
     # -- calls -------------------------------------------------------------
+    def _elsewhere(self):
+        """What a call raises where a tensor is not in the memory of the
+        cache's device: the kernels would follow its address."""
+        return ValueError(f"every tensor must be on GPU {self.device}, that of the cache")
+
     def _seqs(self, lengths, tables, rows, starts):
         """The fields of a ullm_kv_sequences_t."""
         i32 = (_torch_module or _torch()).int32
@@ -830,7 +835,12 @@ class KvCache:
         """Quantize and store new tokens: k, v bf16 [rows][kv_heads][head_dim]
         (row and head strides honoured).  ``weights`` (f32 [rows][kv_heads])
         restores weights read by ``gather_weights``; without it they are 0."""
-        heads, dim = self.kv_heads, self.head_dim
+        heads, dim, here = self.kv_heads, self.head_dim, self.device
+        if k.get_device() != here or v.get_device() != here or lengths.get_device() != here \
+                or tables.get_device() != here \
+                or starts is not None and starts.get_device() != here \
+                or weights is not None and weights.get_device() != here:
+            raise self._elsewhere()
         rows, k_row, k_head = _strides3(k, "k", heads, dim)
         v_rows, v_row, v_head = _strides3(v, "v", heads, dim)
         if v_rows != rows:
@@ -846,8 +856,12 @@ class KvCache:
             _stream(stream) or 0)
 
     def _gatherable(self, lengths, tables, rows, starts):
+        here = self.device
         if rows < 0:
             raise ValueError("rows must not be negative")
+        if lengths.get_device() != here or tables.get_device() != here \
+                or starts is not None and starts.get_device() != here:
+            raise self._elsewhere()
 
     def _gather(self, lengths, tables, rows, starts, k, v, weights, stream):
         _packed(KvGatherDesc).call(
@@ -875,11 +889,18 @@ class KvCache:
 
     def _attend_fields(self, q, lengths, tables, starts, out, lse, scale, window, accumulate,
                        stream, workspace):
-        dim, shape = self.head_dim, q.shape
+        here, dim, shape = self.device, self.head_dim, q.shape
         if len(shape) != 3:
             raise ValueError(f"q must be bfloat16 [rows][heads][{dim}]")
         if not 0 <= window < 1 << 32:
             raise ValueError("window must not be negative, and below 2^32")
+        if q.get_device() != here or lengths.get_device() != here \
+                or tables.get_device() != here \
+                or starts is not None and starts.get_device() != here \
+                or out is not None and out.get_device() != here \
+                or lse is not None and lse.get_device() != here \
+                or workspace is not None and workspace.get_device() != here:
+            raise self._elsewhere()
         heads = shape[1]
         rows, q_row, q_head = _strides3(q, "q", heads, dim)
         if out is None:
@@ -936,8 +957,12 @@ class KvCache:
         them its first ``sink`` and last ``recent``, into the blocks of
         ``new_tables``.  Returns (lengths int32 [batch], positions that stay
         int32 [batch][kv_heads][keep], ascending, then -1)."""
+        here = self.device
         if keep < 0 or sink < 0 or recent < 0:
             raise ValueError("keep, sink and recent must not be negative")
+        if tables.get_device() != here or lengths.get_device() != here \
+                or new_tables.get_device() != here:
+            raise self._elsewhere()
         seqs = self._seqs(lengths, tables, 0, None)
         batch = tables.shape[0]
         columns = -(-keep // self.block_tokens)
