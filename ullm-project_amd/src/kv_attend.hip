@@ -1507,6 +1507,13 @@ constexpr uint32_t kPartLeast = 512, kPartLong = 8192;
 // 28; past that 8 times 128 at 1000 39 / 30, 32 at 30000 42 / 37.  64 times 16
 // at 4000 tokens: 157 / 164, 64 times 24 206 / 167.
 constexpr uint32_t kFewMost = 64, kFewTilesOfUnit = 4, kFewTokens = 4096;
+// Stored scores cost 8 bytes for each row and token, a second pass over the keys
+// `dim` bytes for each token.  Scores have a place for each token of the tables,
+// in use or not: past kMostScores bytes, under a hundredth of the memory, the
+// second pass is taken (64 sequences of 2000 tokens, 32 heads, tables of 131072
+// tokens: 1.1 GB of scores and 190 us, second pass 303; tables of 2048 tokens:
+// 61 and 111).
+constexpr uint64_t kMostScores = uint64_t(1) << 31;
 
 KvAttendPlan plan_kv_attend(const KvAttendArgs &a, uint32_t dim) {
   KvAttendPlan p;
@@ -1538,9 +1545,10 @@ KvAttendPlan plan_kv_attend(const KvAttendArgs &a, uint32_t dim) {
       many ? uint64_t(1) << 31 : kv_part_limit(kWave, a.pool.shift, a.window) / kStep * kStep;
   p.part_tokens = uint32_t(std::min<uint64_t>((part + kStep - 1) / kStep * kStep, most));
   p.parts = uint32_t((span + p.part_tokens - 1) / p.part_tokens);
-  // Scores cost 8 bytes for each row and token, a second pass over the keys
-  // `dim` bytes for each token.
-  p.keep_scores = a.accumulate && !many && rows_of_head <= uint64_t(dim) / 8 * a.seqs.batch;
+  const uint64_t scores = uint64_t(a.seqs.rows) * a.heads * sizeof(float) *
+                          (uint64_t(a.seqs.max_blocks) << a.pool.shift);
+  p.keep_scores = a.accumulate && !many && rows_of_head <= uint64_t(dim) / 8 * a.seqs.batch &&
+                  scores <= kMostScores;
   p.one_tile = rows_of_head <= uint64_t(kRows) * a.seqs.batch;
   p.grid = tiles * p.parts;
   // Eight waves shorten the walk of a lone workgroup (333 tokens: 5.7 against
