@@ -33,7 +33,8 @@
  * positions lengths[b] - n .. lengths[b] - 1.  Rows at negative positions
  * name no token.  `tables`, `lengths` and `starts` are device memory, read in
  * stream order; lengths past max_blocks * block_tokens and starts outside
- * 0 .. rows are taken as those bounds.
+ * 0 .. rows are taken as those bounds.  Results of rows that no sequence owns
+ * are left as they are.
  */
 #ifndef ULLM_KV_CACHE_H
 #define ULLM_KV_CACHE_H
@@ -153,7 +154,8 @@ typedef struct ullm_kv_cache_attend_desc_t {
   float *lse;               /* device f32 [rows][heads], or null */
   uint32_t heads;           /* a multiple of kv_heads */
   uint32_t window;          /* tokens a query sees, 0 = all up to its own */
-  float scale;              /* finite */
+  float scale;              /* finite, as is scale * log2(e); 0 and magnitudes
+                               below count as 2^-120 / log2(e) */
   uint32_t flags;           /* ULLM_KV_ATTEND_* */
   void *stream;
   /* Device scratch of ullm_kv_attend_plan_t.workspace_bytes; null =

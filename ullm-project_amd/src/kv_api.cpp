@@ -154,6 +154,9 @@ ullm_status_t validate_append(const ullm_kv_cache_append_desc_t *d, ullm_error_s
   return ULLM_STATUS_OK;
 }
 
+// A scale in units of log2.
+float log2_scale(float scale) { return float(double(scale) * 1.44269504088896340736); }
+
 ullm_status_t validate_attend(const ullm_kv_cache_attend_desc_t *d, ullm_error_sink_t *sink) {
   ullm_status_t st = validate_call(d, sink, "attend descriptor is null");
   if (st != ULLM_STATUS_OK) {
@@ -173,8 +176,8 @@ ullm_status_t validate_attend(const ullm_kv_cache_attend_desc_t *d, ullm_error_s
   if ((d->flags & ULLM_KV_ATTEND_ACCUMULATE) != 0 && c->weights == nullptr) {
     return fail(sink, "ACCUMULATE needs a cache that tracks weights");
   }
-  if (!std::isfinite(d->scale)) {
-    return fail(sink, "scale must be finite");
+  if (!std::isfinite(log2_scale(d->scale))) {
+    return fail(sink, "scale must be finite, and in units of log2 too");
   }
   for (const uint64_t s :
        {d->q_row_stride, d->q_head_stride, d->out_row_stride, d->out_head_stride}) {
@@ -216,7 +219,7 @@ ullm::KvAttendArgs attend_args(const ullm_kv_cache_attend_desc_t *d) {
   a.window = d->window;
   // A scale of 0 becomes one that leaves every score at 0 but a token that is
   // not seen at -infinity.
-  a.scale_log2 = std::max(std::fabs(float(double(d->scale) * 1.44269504088896340736)), 0x1p-120f);
+  a.scale_log2 = std::max(std::fabs(log2_scale(d->scale)), 0x1p-120f);
   a.q_sign = d->scale < 0.f ? 0x80008000u : 0u;
   a.accumulate = (d->flags & ULLM_KV_ATTEND_ACCUMULATE) != 0;
   return a;
