@@ -874,7 +874,8 @@ class KvCache:
         [rows][kv_heads][head_dim] and exact: appending them again stores the
         same values.  Rows that name no token are zero."""
         self._gatherable(lengths, tables, rows, starts)
-        kv = tables.new_empty((2, rows, self.kv_heads, self.head_dim), dtype=(_torch_module or _torch()).bfloat16)
+        kv = tables.new_empty((2, rows, self.kv_heads, self.head_dim),
+                              dtype=(_torch_module or _torch()).bfloat16)
         at = kv.data_ptr()
         self._gather(lengths, tables, rows, starts, at,
                      at + rows * self.kv_heads * self.head_dim * 2, 0, stream)
