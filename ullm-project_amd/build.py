@@ -26,7 +26,7 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["abi_v1.cpp", "linear_api.cpp", "safetensors.cpp", "evidence.hip", "noalloc.hip", "weights.hip",
            "gemv.hip", "gemm_wq.hip", "gemm_fp8.hip", "kv_api.cpp", "kv_store.hip",
-           "kv_attend.hip"]
+           "kv_attend.hip", "kv_store4.hip", "kv_attend4.hip"]
 
 COMMON = [
     "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden",

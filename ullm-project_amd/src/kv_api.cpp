@@ -1,4 +1,4 @@
-// kv_api.cpp -- C entry points of the 8-bit key/value cache.
+// kv_api.cpp -- C entry points of the 8-bit and the 4-bit key/value cache.
 //
 // Validation order per entry, as in linear_api.cpp: sink, descriptor header
 // (size, version), reserved words, handle, sizes and enums, pointers; only
@@ -16,6 +16,7 @@
 #include "abi_common.hpp"
 #include "host_common.hpp"
 #include "kv_cache.hpp"
+#include "kv_cache4.hpp"
 
 namespace {
 
@@ -92,6 +93,8 @@ ullm_status_t validate_seqs(const ullm_kv_cache_t *c, const ullm_kv_sequences_t 
   return ULLM_STATUS_OK;
 }
 
+bool four_bits(const ullm_kv_cache_t *c) { return (c->flags & ULLM_KV_CACHE_4_BITS) != 0; }
+
 bool no_work(const ullm_kv_sequences_t &s) { return s.batch == 0 || s.rows == 0; }
 
 ullm::KvPool pool_of(const ullm_kv_cache_t *c) {
@@ -154,6 +157,72 @@ ullm_status_t validate_append(const ullm_kv_cache_append_desc_t *d, ullm_error_s
   return ULLM_STATUS_OK;
 }
 
+// Rows of a tensor [rows][heads][dim] that is written do not overlap.
+bool rows_apart(const Strides &s, uint64_t rows, uint64_t heads, uint64_t dim) {
+  return s.row >= (heads - 1) * s.head + dim || rows == 0 || s.head >= (rows - 1) * s.row + dim;
+}
+
+ullm_status_t validate_append_rotary(const ullm_kv_cache_append_rotary_desc_t *d,
+                                     ullm_error_sink_t *sink) {
+  ullm_status_t st = validate_call(d, sink, "append_rotary descriptor is null");
+  if (st != ULLM_STATUS_OK) {
+    return st;
+  }
+  const ullm_kv_cache_t *c = d->cache;
+  if (d->heads % c->kv_heads != 0) {
+    return fail(sink, "heads must be a multiple of the cache's kv_heads, or 0");
+  }
+  st = validate_seqs(c, d->seqs, true, std::max(d->heads, c->kv_heads), sink);
+  if (st != ULLM_STATUS_OK) {
+    return st;
+  }
+  if ((d->flags & ~ULLM_KV_ROTARY_INTERLEAVED) != 0) {
+    return fail(sink, "unknown rotary flags");
+  }
+  if (d->rotary_dims == 0 || d->rotary_dims % 2 != 0 || d->rotary_dims > c->head_dim) {
+    return fail(sink, "rotary_dims must be even, from 2 to head_dim");
+  }
+  if (d->axes == 0 || d->axes > 4) {
+    return fail(sink, "axes must be 1 to 4");
+  }
+  if (d->positions == nullptr && d->axes != 1) {
+    return fail(sink, "more than one axis needs positions");
+  }
+  if (d->position_stride != 0 && d->position_stride < d->seqs.rows && d->axes > 1) {
+    return fail(sink, "position_stride is smaller than rows");
+  }
+  for (const uint64_t s : {d->q_row_stride, d->q_head_stride, d->q_out_row_stride,
+                           d->q_out_head_stride, d->k_row_stride, d->k_head_stride,
+                           d->v_row_stride, d->v_head_stride}) {
+    if (s != 0 && s < c->head_dim) {
+      return fail(sink, "a q, q_out, k or v stride is smaller than head_dim");
+    }
+  }
+  const Strides o = strides_of(d->q_out_row_stride, d->q_out_head_stride, d->heads, c->head_dim);
+  if (d->heads != 0 && !rows_apart(o, d->seqs.rows, d->heads, c->head_dim)) {
+    return fail(sink, "q_out strides make rows overlap");
+  }
+  if (d->weights != nullptr && c->weights == nullptr) {
+    return fail(sink, "weights are given but the cache does not track weights");
+  }
+  if (no_work(d->seqs)) {
+    return ULLM_STATUS_OK;
+  }
+  if (d->k == nullptr || d->v == nullptr || d->inv_freq == nullptr) {
+    return fail(sink, "k, v or inv_freq pointer is null");
+  }
+  if (d->heads != 0 && (d->q == nullptr || d->q_out == nullptr)) {
+    return fail(sink, "q or q_out pointer is null");
+  }
+  if (d->heads != 0 && d->q_out == d->q) {
+    const Strides q = strides_of(d->q_row_stride, d->q_head_stride, d->heads, c->head_dim);
+    if ((d->seqs.rows > 1 && o.row != q.row) || (d->heads > 1 && o.head != q.head)) {
+      return fail(sink, "q_out in place of q needs the strides of q");
+    }
+  }
+  return ULLM_STATUS_OK;
+}
+
 // A scale in units of log2.
 float log2_scale(float scale) { return float(double(scale) * 1.44269504088896340736); }
 
@@ -186,16 +255,33 @@ ullm_status_t validate_attend(const ullm_kv_cache_attend_desc_t *d, ullm_error_s
     }
   }
   const Strides o = strides_of(d->out_row_stride, d->out_head_stride, d->heads, c->head_dim);
-  const bool rows_outer = o.row >= (d->heads - 1) * o.head + c->head_dim;
-  const bool heads_outer =
-      d->seqs.rows == 0 || o.head >= (d->seqs.rows - 1) * o.row + c->head_dim;
-  if (!rows_outer && !heads_outer) {
+  if (!rows_apart(o, d->seqs.rows, d->heads, c->head_dim)) {
     return fail(sink, "out strides make rows overlap");
   }
   if (!no_work(d->seqs) && (d->q == nullptr || d->out == nullptr)) {
     return fail(sink, "q or out pointer is null");
   }
   return ULLM_STATUS_OK;
+}
+
+// What append and append_rotary share of a launch.
+template <typename D>
+ullm::KvAppendArgs append_args(const D *d) {
+  const ullm_kv_cache_t *c = d->cache;
+  const Strides k = strides_of(d->k_row_stride, d->k_head_stride, c->kv_heads, c->head_dim);
+  const Strides v = strides_of(d->v_row_stride, d->v_head_stride, c->kv_heads, c->head_dim);
+  ullm::KvAppendArgs a{};
+  a.pool = pool_of(c);
+  a.seqs = seqs_of(d->seqs);
+  a.k = static_cast<const uint16_t *>(d->k);
+  a.v = static_cast<const uint16_t *>(d->v);
+  a.k_row = k.row;
+  a.k_head = k.head;
+  a.v_row = v.row;
+  a.v_head = v.head;
+  a.vec = aligned(d->k, k, 16) && aligned(d->v, v, 16);
+  a.weights = d->weights;
+  return a;
 }
 
 ullm::KvAttendArgs attend_args(const ullm_kv_cache_attend_desc_t *d) {
@@ -223,6 +309,11 @@ ullm::KvAttendArgs attend_args(const ullm_kv_cache_attend_desc_t *d) {
   a.q_sign = d->scale < 0.f ? 0x80008000u : 0u;
   a.accumulate = (d->flags & ULLM_KV_ATTEND_ACCUMULATE) != 0;
   return a;
+}
+
+ullm::KvAttendPlan plan_of(const ullm_kv_cache_t *c, const ullm::KvAttendArgs &a) {
+  return four_bits(c) ? ullm::plan_kv4_attend(a, c->head_dim)
+                      : ullm::plan_kv_attend(a, c->head_dim);
 }
 
 }  // namespace
@@ -253,7 +344,7 @@ extern "C" ULLM_HIP_API ullm_status_t ullm_kv_cache_create(const ullm_kv_cache_d
     if (desc->head_dim != 64 && desc->head_dim != 128) {
       return write_error(error_sink, ULLM_STATUS_UNSUPPORTED, "head_dim must be 64 or 128");
     }
-    if ((desc->flags & ~ULLM_KV_CACHE_TRACK_WEIGHTS) != 0) {
+    if ((desc->flags & ~(ULLM_KV_CACHE_TRACK_WEIGHTS | ULLM_KV_CACHE_4_BITS)) != 0) {
       return fail(error_sink, "unknown cache flags");
     }
     if (cache == nullptr) {
@@ -285,20 +376,26 @@ extern "C" ULLM_HIP_API ullm_status_t ullm_kv_cache_create(const ullm_kv_cache_d
     c->flags = desc->flags;
     c->device = desc->device;
     const uint64_t units = desc->blocks * desc->kv_heads;
-    const uint64_t code_bytes = units * 2 * desc->head_dim * desc->block_tokens;
+    const bool four = four_bits(c);
+    const uint64_t code_bytes =
+        four ? units * (desc->block_tokens / 32) * ullm::kv4_chunk_bytes(desc->head_dim)
+             : units * 2 * desc->head_dim * desc->block_tokens;
+    const uint64_t exp_bytes = four ? 0 : units * 2;  // 4 bits: beside the codes
     const uint64_t weight_bytes = (desc->flags & ULLM_KV_CACHE_TRACK_WEIGHTS) != 0
                                       ? units * desc->block_tokens * sizeof(float)
                                       : 0;
     HIP_TRY(error_sink, "hipMalloc (cache codes)", hipMalloc(&c->codes, code_bytes));
-    HIP_TRY(error_sink, "hipMalloc (cache exponents)", hipMalloc(&c->exps, units * 2));
     HIP_TRY(error_sink, "hipMemset", hipMemset(c->codes, 0, code_bytes));
-    HIP_TRY(error_sink, "hipMemset", hipMemset(c->exps, 0, units * 2));
+    if (exp_bytes != 0) {
+      HIP_TRY(error_sink, "hipMalloc (cache exponents)", hipMalloc(&c->exps, exp_bytes));
+      HIP_TRY(error_sink, "hipMemset", hipMemset(c->exps, 0, exp_bytes));
+    }
     if (weight_bytes != 0) {
       HIP_TRY(error_sink, "hipMalloc (cache weights)", hipMalloc(&c->weights, weight_bytes));
       HIP_TRY(error_sink, "hipMemset", hipMemset(c->weights, 0, weight_bytes));
     }
     HIP_TRY(error_sink, "hipStreamSynchronize", hipStreamSynchronize(nullptr));
-    c->device_bytes = code_bytes + units * 2 + weight_bytes;
+    c->device_bytes = code_bytes + exp_bytes + weight_bytes;
     {
       std::lock_guard<std::mutex> lock(g_caches_mutex);
       g_caches.insert(c);
@@ -378,23 +475,55 @@ extern "C" ULLM_HIP_API ullm_status_t ullm_kv_cache_append(
     const ullm_kv_cache_t *c = desc->cache;
     DeviceScope scope(c->device);
     HIP_TRY(error_sink, "hipSetDevice", scope.error());
-    const Strides k = strides_of(desc->k_row_stride, desc->k_head_stride, c->kv_heads,
+    const hipStream_t stream = static_cast<hipStream_t>(desc->stream);
+    const ullm::KvAppendArgs a = append_args(desc);
+    if (four_bits(c)) {
+      ullm::KvRotateArgs r{};
+      r.append = a;
+      HIP_TRY(error_sink, "cache append kernel", ullm::launch_kv4_append(r, c->head_dim, stream));
+    } else {
+      HIP_TRY(error_sink, "cache append kernel", ullm::launch_kv_append(a, c->head_dim, stream));
+    }
+    return ULLM_STATUS_OK;
+  });
+}
+
+extern "C" ULLM_HIP_API ullm_status_t ullm_kv_cache_append_rotary(
+    const ullm_kv_cache_append_rotary_desc_t *desc, ullm_error_sink_t *error_sink) {
+  ULLM_ENTRY(error_sink, "cache append_rotary", {
+    const ullm_status_t st = validate_append_rotary(desc, error_sink);
+    if (st != ULLM_STATUS_OK || no_work(desc->seqs)) {
+      return st;
+    }
+    const ullm_kv_cache_t *c = desc->cache;
+    DeviceScope scope(c->device);
+    HIP_TRY(error_sink, "hipSetDevice", scope.error());
+    const Strides q = strides_of(desc->q_row_stride, desc->q_head_stride, desc->heads,
                                  c->head_dim);
-    const Strides v = strides_of(desc->v_row_stride, desc->v_head_stride, c->kv_heads,
+    const Strides o = strides_of(desc->q_out_row_stride, desc->q_out_head_stride, desc->heads,
                                  c->head_dim);
-    ullm::KvAppendArgs a{};
-    a.pool = pool_of(c);
-    a.seqs = seqs_of(desc->seqs);
-    a.k = static_cast<const uint16_t *>(desc->k);
-    a.v = static_cast<const uint16_t *>(desc->v);
-    a.k_row = k.row;
-    a.k_head = k.head;
-    a.v_row = v.row;
-    a.v_head = v.head;
-    a.vec = aligned(desc->k, k, 16) && aligned(desc->v, v, 16);
-    a.weights = desc->weights;
-    HIP_TRY(error_sink, "cache append kernel",
-            ullm::launch_kv_append(a, c->head_dim, static_cast<hipStream_t>(desc->stream)));
+    ullm::KvRotateArgs a{};
+    a.append = append_args(desc);
+    a.rotary.inv_freq = desc->inv_freq;
+    a.rotary.positions = desc->positions;
+    a.rotary.position_stride =
+        desc->position_stride != 0 ? desc->position_stride : desc->seqs.rows;
+    a.rotary.pair_axes = desc->pair_axes;
+    a.rotary.dims = desc->rotary_dims;
+    a.rotary.axes = desc->axes;
+    a.rotary.interleaved = (desc->flags & ULLM_KV_ROTARY_INTERLEAVED) != 0;
+    a.q = static_cast<const uint16_t *>(desc->q);
+    a.q_out = static_cast<uint16_t *>(desc->q_out);
+    a.q_row = q.row;
+    a.q_head = q.head;
+    a.out_row = o.row;
+    a.out_head = o.head;
+    a.q_vec = aligned(desc->q, q, 16) && aligned(desc->q_out, o, 16);
+    a.group = desc->heads / c->kv_heads;
+    const auto launch =
+        four_bits(c) ? ullm::launch_kv4_append : ullm::launch_kv8_append_rotary;
+    HIP_TRY(error_sink, "cache append_rotary kernel",
+            launch(a, c->head_dim, static_cast<hipStream_t>(desc->stream)));
     return ULLM_STATUS_OK;
   });
 }
@@ -431,8 +560,9 @@ extern "C" ULLM_HIP_API ullm_status_t ullm_kv_cache_gather(
     a.k = static_cast<uint16_t *>(desc->k);
     a.v = static_cast<uint16_t *>(desc->v);
     a.weights = desc->weights;
+    const auto launch = four_bits(c) ? ullm::launch_kv4_gather : ullm::launch_kv_gather;
     HIP_TRY(error_sink, "cache gather kernel",
-            ullm::launch_kv_gather(a, c->head_dim, static_cast<hipStream_t>(desc->stream)));
+            launch(a, c->head_dim, static_cast<hipStream_t>(desc->stream)));
     return ULLM_STATUS_OK;
   });
 }
@@ -457,7 +587,7 @@ extern "C" ULLM_HIP_API ullm_status_t ullm_kv_cache_attend_plan(
     if (!no_work(desc->seqs)) {
       DeviceScope scope(desc->cache->device);
       HIP_TRY(error_sink, "hipSetDevice", scope.error());
-      p = ullm::plan_kv_attend(attend_args(desc), desc->cache->head_dim);
+      p = plan_of(desc->cache, attend_args(desc));
     }
     plan->kernel = p.kernel;
     plan->row_tile = p.row_tile;
@@ -490,7 +620,7 @@ extern "C" ULLM_HIP_API ullm_status_t ullm_kv_cache_attend(
     }
     DeviceScope scope(c->device);
     HIP_TRY(error_sink, "hipSetDevice", scope.error());
-    const ullm::KvAttendPlan p = ullm::plan_kv_attend(a, c->head_dim);
+    const ullm::KvAttendPlan p = plan_of(c, a);
     // A launch counts its threads in 32 bits; the join has a wave for each row.
     if (p.grid > UINT32_MAX / 512 ||
         (p.parts > 1 && p.grid / p.parts > UINT32_MAX / 512 / p.row_tile)) {
@@ -518,9 +648,9 @@ extern "C" ULLM_HIP_API ullm_status_t ullm_kv_cache_attend(
         return st;
       }
     }
+    const auto launch = four_bits(c) ? ullm::launch_kv4_attend : ullm::launch_kv_attend;
     HIP_TRY(error_sink, "cache attend kernel",
-            ullm::launch_kv_attend(a, c->head_dim, p, ws,
-                                   static_cast<hipStream_t>(desc->stream)));
+            launch(a, c->head_dim, p, ws, static_cast<hipStream_t>(desc->stream)));
     return ULLM_STATUS_OK;
   });
 }
@@ -574,8 +704,9 @@ extern "C" ULLM_HIP_API ullm_status_t ullm_kv_cache_evict(
     a.keep = uint32_t(desc->keep);
     a.sink = uint32_t(desc->sink);
     a.recent = uint32_t(desc->recent);
+    const auto launch = four_bits(c) ? ullm::launch_kv4_evict : ullm::launch_kv_evict;
     HIP_TRY(error_sink, "cache evict kernels",
-            ullm::launch_kv_evict(a, c->head_dim, static_cast<hipStream_t>(desc->stream)));
+            launch(a, c->head_dim, static_cast<hipStream_t>(desc->stream)));
     return ULLM_STATUS_OK;
   });
 }

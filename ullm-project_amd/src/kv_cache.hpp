@@ -105,6 +105,9 @@ struct KvAttendPlan {
 hipError_t launch_kv_append(const KvAppendArgs &a, uint32_t dim, hipStream_t s);
 hipError_t launch_kv_gather(const KvGatherArgs &a, uint32_t dim, hipStream_t s);
 hipError_t launch_kv_evict(const KvEvictArgs &a, uint32_t dim, hipStream_t s);
+// The selection of an eviction, and weights alone: they know no codes.
+void launch_kv_evict_select(const KvEvictArgs &a, hipStream_t s);
+void launch_kv_gather_weights(const KvGatherArgs &a, hipStream_t s);
 KvAttendPlan plan_kv_attend(const KvAttendArgs &a, uint32_t dim);
 hipError_t launch_kv_attend(const KvAttendArgs &a, uint32_t dim, const KvAttendPlan &p,
                             void *workspace, hipStream_t s);

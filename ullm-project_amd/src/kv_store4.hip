@@ -1,0 +1,693 @@
+// kv_store4.hip -- what writes and moves the tokens of the 4-bit key/value
+// cache, and the appends that rotate: append, gather and evict.  All are bound
+// by HBM and launches.
+#include "kv_cache4.hpp"
+#include "kv_rotary.hpp"
+#include "kv_store.hpp"
+
+namespace ullm {
+namespace {
+
+// ------------------------------------------------------------- 4-bit codes
+
+// Smallest exponent e with a <= 6 * 2^e = 1.5 * 2^(e + 2), clamped, plus 127, of
+// the largest magnitude's f32 bits; of infinities and NaN kKv4ExpNan.
+__device__ __forceinline__ uint32_t key_exp4(uint32_t a) {
+  const int e = int(a >> 23) - 127 - 2 + ((a & 0x7fffffu) > 0x400000u ? 1 : 0);
+  const int c = e < kKvExpMin ? kKvExpMin : e > kKvExpMax ? kKvExpMax : e;
+  return a >= 0x7f800000u ? kKv4ExpNan : uint32_t(c + 127);
+}
+__device__ __forceinline__ float exp4_power(uint32_t e) { return bits_f32(e << 23); }
+
+// Smallest number of 6 significant bits, within the f16 ones that are allowed,
+// whose 6-fold reaches a magnitude.  Products by 6 of such numbers are exact, so
+// the comparisons decide; the quotient before them only has to be near.
+__device__ __forceinline__ float value_scale4(float a) {
+  constexpr uint32_t kStep = 1u << 18;
+  float s = bits_f32(f32_bits(a * (0.999999f / 6.f)) & ~(kStep - 1));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    s = 6.f * s < a ? bits_f32(f32_bits(s) + kStep) : s;
+  }
+  return fminf(fmaxf(s, kScaleLeast), kScaleMost);
+}
+
+// Sixteen codes, low nibble first, of sixteen numbers over a power of two.
+__device__ __forceinline__ u32x2 encode4(const float (&x)[16], float power) {
+  u32x2 r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[8 * i], x[8 * i + 1], power, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[8 * i + 2], x[8 * i + 3], power, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[8 * i + 4], x[8 * i + 5], power, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[8 * i + 6], x[8 * i + 7], power, 3);
+    r[i] = w;
+  }
+  return r;
+}
+// Of sixteen bf16 over any scale s.  The quotient is exact where it is a border
+// of two codes (a number of at most 4 significant bits): x / s rounded, and once
+// more by its remainder.
+__device__ __forceinline__ u32x2 encode4_scaled(const float (&x)[16], float s) {
+  const float inv = 1.f / s;
+  float y[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    y[i] = x[i] * inv;
+    y[i] = __builtin_fmaf(__builtin_fmaf(-y[i], s, x[i]), inv, y[i]);
+  }
+  return encode4(y, 1.f);
+}
+// Four codes, a byte each in w, as bf16 times a scale.
+__device__ __forceinline__ u32x2 decode4_bytes(uint32_t w, float s) {
+  const uint32_t t = w | w >> 4;  // bytes 0 and 2: two codes each
+  const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(t, 1.f, 0);
+  const auto hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(t, 1.f, 2);
+  return {f32x2_to_bf16x2(lo[0] * s, lo[1] * s), f32x2_to_bf16x2(hi[0] * s, hi[1] * s)};
+}
+
+__device__ __forceinline__ void unpack16(const Bf16x16 &x, float (&f)[16]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t w = x.w[i / 4][i % 4];
+    f[2 * i] = bits_f32(w << 16);
+    f[2 * i + 1] = bits_f32(w & 0xffff0000u);
+  }
+}
+// Bits of the largest magnitude of sixteen numbers (NaN above all) over the
+// lanes that differ in the bits of `lanes`.
+template <uint32_t LANES>
+__device__ __forceinline__ uint32_t largest16(const float (&f)[16]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    top = max(top, f32_bits(f[i]) & 0x7fffffffu);
+  }
+#pragma unroll
+  for (uint32_t off = 1; off < LANES; off <<= 1) {
+    top = max(top, uint32_t(__shfl_xor(int(top), off, kWave)));
+  }
+  return top;
+}
+
+// ----------------------------------------------------------------- rotation
+
+// 32 tokens of a sequence, of which lo .. hi - 1 are rows of the call: row
+// `row0` + t is token t, at place `base` + t.
+struct Span {
+  int64_t row0, base;
+  uint32_t lo, hi;
+};
+
+// Cosines and sines of the span's rows and of all pairs.
+template <int D>
+__device__ __forceinline__ void span_turns(const KvRotary &r, const Span &s, Turn (*turns)[D / 2]) {
+  const uint32_t j = threadIdx.x % (D / 2);
+  if (j >= r.dims / 2) {
+    return;
+  }
+  const float f = r.inv_freq[j];
+  const uint32_t axis = r.pair_axes == nullptr ? 0u : min(uint32_t(r.pair_axes[j]), r.axes - 1);
+  const int32_t *at = r.positions + axis * r.position_stride;
+  for (uint32_t t = s.lo + threadIdx.x / (D / 2); t < s.hi; t += kThreads / (D / 2)) {
+    turns[t][j] = turn_of(r.positions == nullptr ? int32_t(s.base + t) : at[s.row0 + t], f);
+  }
+}
+
+// Eight pairs (8u ..) of a row, rotated; where[] are their dims.
+template <int D>
+struct Pairs {
+  float first[8], second[8];
+};
+// Whether eight pairs are two runs of eight dims, or one of sixteen, that start
+// at multiples of eight.
+__device__ __forceinline__ bool pairs_in_runs(const KvRotary &r) {
+  return r.interleaved || r.dims % 16 == 0;
+}
+__device__ __forceinline__ bool neighbours(const KvRotary &r, uint32_t u) {
+  return r.interleaved || 8 * u >= r.dims / 2;
+}
+template <int D>
+__device__ __forceinline__ Pairs<D> load_pairs(const uint16_t *row, const KvRotary &r, uint32_t u,
+                                               bool vec) {
+  Pairs<D> p;
+  if (vec && pairs_in_runs(r)) {
+    const PairDims d = pair_dims(8 * u, r.dims, r.interleaved);
+    const bool side = neighbours(r, u);
+    const u32x4 a = *reinterpret_cast<const u32x4 *>(row + d.first);
+    const u32x4 b = *reinterpret_cast<const u32x4 *>(row + (side ? d.first + 8 : d.second));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t near = i < 4 ? a[i % 4] : b[i % 4];
+      const uint32_t x = side ? near << 16 : i % 2 == 0 ? a[i / 2] << 16 : a[i / 2] & 0xffff0000u;
+      const uint32_t y = side           ? near & 0xffff0000u
+                         : i % 2 == 0 ? b[i / 2] << 16
+                                      : b[i / 2] & 0xffff0000u;
+      p.first[i] = bits_f32(x);
+      p.second[i] = bits_f32(y);
+    }
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      const PairDims d = pair_dims(8 * u + i, r.dims, r.interleaved);
+      p.first[i] = bf16_to_f32(row[d.first]);
+      p.second[i] = bf16_to_f32(row[d.second]);
+    }
+  }
+  return p;
+}
+template <int D>
+__device__ __forceinline__ void rotate_pairs(Pairs<D> &p, const KvRotary &r, uint32_t u,
+                                             const Turn *turns) {
+#pragma unroll
+  for (uint32_t i = 0; i < 8; ++i) {
+    const uint32_t j = 8 * u + i;
+    if (j < r.dims / 2) {
+      const Turn w = turns[j];
+      const double x = p.first[i], y = p.second[i];
+      p.first[i] = to_odd(fma(x, w.c, -(y * w.s)));
+      p.second[i] = to_odd(fma(y, w.c, x * w.s));
+    }
+  }
+}
+template <int D>
+__device__ __forceinline__ void store_pairs(uint16_t *row, const Pairs<D> &p, const KvRotary &r,
+                                            uint32_t u, bool vec) {
+  if (vec && pairs_in_runs(r)) {
+    const PairDims d = pair_dims(8 * u, r.dims, r.interleaved);
+    const bool side = neighbours(r, u);
+    u32x4 a, b;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const auto pair = [](float x, float y) { return f32x2_to_bf16x2(x, y); };
+      a[i] = side ? pair(p.first[i], p.second[i]) : pair(p.first[2 * i], p.first[2 * i + 1]);
+      b[i] = side ? pair(p.first[4 + i], p.second[4 + i])
+                  : pair(p.second[2 * i], p.second[2 * i + 1]);
+    }
+    *reinterpret_cast<u32x4 *>(row + d.first) = a;
+    *reinterpret_cast<u32x4 *>(row + (side ? d.first + 8 : d.second)) = b;
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      const PairDims d = pair_dims(8 * u + i, r.dims, r.interleaved);
+      row[d.first] = f32_to_bf16(p.first[i]);
+      row[d.second] = f32_to_bf16(p.second[i]);
+    }
+  }
+}
+
+// Rows of rotated keys in LDS.
+template <int D>
+struct KeyImage {
+  alignas(16) float x[32][D + 4];
+};
+
+// The span's queries of a key/value head's group, rotated to their place, and
+// its keys, rotated into LDS (where the span has tokens in the cache).
+template <int D>
+__device__ __forceinline__ void rotate_span(const KvRotateArgs &a, const Span &s, uint32_t head,
+                                            const Turn (*turns)[D / 2], KeyImage<D> *keys) {
+  constexpr uint32_t kUnits = D / 16;
+  const uint32_t n = s.hi - s.lo, heads = a.group + (keys != nullptr ? 1u : 0u);
+  for (uint32_t i = threadIdx.x; i < heads * n * kUnits; i += kThreads) {
+    const uint32_t u = i % kUnits, h = i / kUnits / n, t = s.lo + i / kUnits % n;
+    const uint64_t row = uint64_t(s.row0 + t);
+    if (h < a.group) {
+      const uint32_t qh = head * a.group + h;
+      Pairs<D> p = load_pairs<D>(a.q + row * a.q_row + qh * a.q_head, a.rotary, u, a.q_vec);
+      rotate_pairs<D>(p, a.rotary, u, turns[t]);
+      store_pairs<D>(a.q_out + row * a.out_row + qh * a.out_head, p, a.rotary, u, a.q_vec);
+    } else {
+      Pairs<D> p = load_pairs<D>(a.append.k + row * a.append.k_row + head * a.append.k_head,
+                                 a.rotary, u, a.append.vec);
+      rotate_pairs<D>(p, a.rotary, u, turns[t]);
+#pragma unroll
+      for (uint32_t e = 0; e < 8; ++e) {
+        const PairDims d = pair_dims(8 * u + e, a.rotary.dims, a.rotary.interleaved);
+        keys->x[t][d.first] = p.first[e];
+        keys->x[t][d.second] = p.second[e];
+      }
+    }
+  }
+}
+
+// --------------------------------------------------------------- append, 4 bits
+
+// One workgroup stores the new tokens among 32 of one head.  Keys go from
+// memory, or rotated from LDS, to their codes and memory; values' codes are
+// brought into dwords of eight tokens in LDS.  A dword that new tokens share
+// with earlier ones is read and written by this workgroup alone.
+template <int D, bool ROTATE>
+__global__ __launch_bounds__(kThreads) void append4_kernel(KvRotateArgs ra, uint32_t each_slots) {
+  using Chunk = Kv4Chunk<D>;
+  constexpr uint32_t kUnits = D / 16, kPitch = D + 16;
+  __shared__ Turn turns[ROTATE ? 32 : 1][D / 2];
+  __shared__ KeyImage<ROTATE ? D : 4> rotated;
+  __shared__ __align__(16) uint8_t values[32 * kPitch];  // a code to a byte
+  const KvAppendArgs &a = ra.append;
+  const uint32_t head = blockIdx.y, tid = threadIdx.x;
+  const KvSlot slot = kv_find_slot(a.seqs, blockIdx.x, 1, 32, 2, each_slots);
+  if (slot.seq >= a.seqs.batch) {
+    return;
+  }
+  const uint32_t length = kv_length(a.seqs, a.pool.shift, slot.seq);
+  const int64_t origin = int64_t(length) - slot.rows.count;  // place of the first row
+  Span s;
+  s.base = (origin >> 5) * 32 + int64_t(slot.local) * 32;
+  s.lo = origin > s.base ? uint32_t(origin - s.base) : 0u;
+  s.hi = uint32_t(min(max(int64_t(length) - s.base, int64_t(0)), int64_t(32)));
+  s.row0 = int64_t(slot.rows.first) + (s.base - origin);
+  if (s.lo >= s.hi) {
+    return;
+  }
+  // Places before the first token have no block, but queries.
+  const int32_t id = s.base < 0 ? -1
+                                : kv_block(a.seqs.tables + slot.seq * a.seqs.stride, a.seqs,
+                                           a.pool.blocks, uint32_t(s.base) >> a.pool.shift);
+  if constexpr (ROTATE) {
+    span_turns<D>(ra.rotary, s, turns);
+    __syncthreads();
+    rotate_span<D>(ra, s, head, turns, id < 0 ? nullptr : &rotated);
+    __syncthreads();
+  }
+  if (id < 0) {
+    return;
+  }
+  const uint32_t in_block = uint32_t(s.base) & ((1u << a.pool.shift) - 1);
+  const uint64_t unit = uint64_t(id) * a.pool.heads + head;
+  uint8_t *chunk = kv4_chunk<D>(a.pool, unit, in_block);
+  for (uint32_t i = tid; i < (s.hi - s.lo) * kUnits; i += kThreads) {
+    const uint32_t t = s.lo + i / kUnits, c = i % kUnits;
+    const uint64_t row = uint64_t(s.row0 + t);
+    float k[16], v[16];
+    if constexpr (ROTATE) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 w = *reinterpret_cast<const f32x4 *>(&rotated.x[t][c * 16 + 4 * j]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          k[4 * j + e] = w[e];
+        }
+      }
+    } else {
+      unpack16(load16(a.k + head * a.k_head + row * a.k_row + c * 16, a.vec), k);
+    }
+    unpack16(load16(a.v + head * a.v_head + row * a.v_row + c * 16, a.vec), v);
+    const uint32_t e = key_exp4(largest16<2>(k));
+    *reinterpret_cast<u32x2 *>(chunk + kv4_key_byte<D>(t, c * 16)) = encode4(k, exp4_power(e));
+    if (c % 2 == 0) {
+      chunk[Chunk::kExps + kv4_exp_byte(t, c * 16)] = uint8_t(e);
+    }
+    const uint32_t top = largest16<kUnits>(v);
+    const float scale = value_scale4(bits_f32(top));
+    const u32x2 w = encode4_scaled(v, scale);
+    uint8_t *to = values + t * kPitch + c * 16;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // four codes of w to four bytes
+      const uint32_t h = w[j / 2] >> (16 * (j % 2)) & 0xffffu;
+      const uint32_t b = (h | h << 8) & 0x00ff00ffu;
+      reinterpret_cast<uint32_t *>(to)[j] = (b | b << 4) & 0x0f0f0f0fu;
+    }
+    if (c == 0) {
+      *reinterpret_cast<uint16_t *>(chunk + Chunk::kScales + kv4_scale_byte(t)) =
+          top >= 0x7f800000u ? uint16_t(0x7e00) : f32_to_f16(scale);
+    }
+  }
+  __syncthreads();
+  for (uint32_t i = tid; i < 4 * D; i += kThreads) {
+    const uint32_t g = i / D, d = i % D;
+    uint32_t w = 0, fresh = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+      const uint32_t t = 4 * g + j % 4 + 16 * (j / 4);
+      const bool is_new = t >= s.lo && t < s.hi;
+      const uint32_t code = is_new ? values[t * kPitch + d] : 0u;
+      w |= code << (4 * j);
+      fresh |= is_new ? 15u << (4 * j) : 0u;
+    }
+    if (fresh != 0) {
+      uint32_t *at = reinterpret_cast<uint32_t *>(chunk + Chunk::kSide + kv4_value_dword(g, d));
+      *at = fresh == ~0u ? w : w | (*at & ~fresh);
+    }
+  }
+  if (a.pool.weights != nullptr) {
+    for (uint32_t t = s.lo + tid; t < s.hi; t += kThreads) {
+      a.pool.weights[(unit << a.pool.shift) + in_block + t] =
+          a.weights != nullptr ? a.weights[uint64_t(s.row0 + t) * a.pool.heads + head] : 0.f;
+    }
+  }
+}
+
+// ------------------------------------------------------- append, 8 bits, rotated
+
+// One workgroup stores the new tokens of one block and head, as append_kernel
+// does; keys come rotated from LDS, 32 tokens at a time.
+template <int D, uint32_t bt>
+__global__ __launch_bounds__(kThreads) void append8_rotary_kernel(KvRotateArgs ra,
+                                                                  uint32_t each_slots) {
+  constexpr uint32_t kUnits = D / 16, kSpans = bt / 32;
+  constexpr uint32_t kEach = (32 * kUnits + kThreads - 1) / kThreads;  // of a thread and span
+  __shared__ Turn turns[32][D / 2];
+  __shared__ KeyImage<D> rotated;
+  __shared__ __align__(16) uint8_t image[bt * D];
+  const KvAppendArgs &a = ra.append;
+  const uint32_t head = blockIdx.y, tid = threadIdx.x;
+  const KvSlot slot = kv_find_slot(a.seqs, blockIdx.x, 1, bt, 2, each_slots);
+  if (slot.seq >= a.seqs.batch) {
+    return;
+  }
+  const uint32_t length = kv_length(a.seqs, a.pool.shift, slot.seq);
+  const int64_t origin = int64_t(length) - slot.rows.count;
+  const int64_t base = (origin >> a.pool.shift) * bt + int64_t(slot.local) * bt;
+  const uint32_t lo = origin > base ? uint32_t(origin - base) : 0u;
+  const uint32_t hi = uint32_t(min(max(int64_t(length) - base, int64_t(0)), int64_t(bt)));
+  if (lo >= hi) {
+    return;
+  }
+  const int64_t row0 = int64_t(slot.rows.first) + (base - origin);
+  const int32_t id = base < 0 ? -1
+                              : kv_block(a.seqs.tables + slot.seq * a.seqs.stride, a.seqs,
+                                         a.pool.blocks, uint32_t(base) >> a.pool.shift);
+  const uint64_t unit = uint64_t(id < 0 ? 0 : id) * a.pool.heads + head;
+  const int ek0 = a.pool.exps[unit * 2], ev0 = a.pool.exps[unit * 2 + 1];
+  // Unit r of this thread in a span: token t of the span, dims 16c .. 16c + 15.
+  const auto token = [&](uint32_t r) { return (tid + r * kThreads) / kUnits; };
+  const uint32_t c = tid % kUnits;
+  float x[kSpans * kEach][16];
+  Bf16x16 y[kSpans * kEach];
+  uint32_t ak = 0, av = 0;
+#pragma unroll
+  for (uint32_t p = 0; p < kSpans; ++p) {
+    Span s;
+    s.base = base + 32 * p;
+    s.row0 = row0 + 32 * p;
+    s.lo = lo > 32 * p ? min(lo - 32 * p, 32u) : 0u;
+    s.hi = hi > 32 * p ? min(hi - 32 * p, 32u) : 0u;
+    s.lo = min(s.lo, s.hi);
+    span_turns<D>(ra.rotary, s, turns);
+    __syncthreads();
+    rotate_span<D>(ra, s, head, turns, id < 0 ? nullptr : &rotated);
+    __syncthreads();
+#pragma unroll
+    for (uint32_t r = 0; r < kEach; ++r) {
+      const uint32_t t = token(r), i = p * kEach + r;
+      y[i] = Bf16x16{};
+      const bool live = id >= 0 && t >= s.lo && t < s.hi;
+      if (live) {
+        y[i] = load16(a.v + head * a.v_head + uint64_t(s.row0 + t) * a.v_row + c * 16, a.vec);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 w =
+            *reinterpret_cast<const f32x4 *>(&rotated.x[live ? t : 0][c * 16 + 4 * j]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[i][4 * j + e] = live ? w[e] : 0.f;
+          const uint32_t m = f32_bits(x[i][4 * j + e]) & 0x7fffffffu;
+          ak = max(ak, m < 0x7f800000u ? m : 0u);  // infinities and NaN do not count
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (id < 0) {
+    return;
+  }
+  av = largest_magnitude(y);
+  block_umax2(ak, av);
+  int ek = exponent_for_f32(ak), ev = exponent_for(av);
+  float fk = 1.f, fv = 1.f;  // factor of the codes that were there
+  if (lo > 0) {
+    ek = max(ek, ek0);
+    ev = max(ev, ev0);
+    fk = exp2_int(max(ek0 - ek, -126));
+    fv = exp2_int(max(ev0 - ev, -126));
+  }
+  if (tid == 0) {  // all have read the old ones
+    a.pool.exps[unit * 2] = int8_t(ek);
+    a.pool.exps[unit * 2 + 1] = int8_t(ev);
+  }
+  uint8_t *kc = a.pool.codes + unit * (uint64_t(2 * D) << a.pool.shift);
+  uint8_t *vc = kc + (uint64_t(D) << a.pool.shift);
+  rescale_keys<D>(kc, lo, fk);
+#pragma unroll
+  for (uint32_t i = 0; i < kSpans * kEach; ++i) {
+    const uint32_t t = 32 * (i / kEach) + token(i % kEach);
+    if (token(i % kEach) < 32 && t >= lo && t < hi) {
+      *reinterpret_cast<u32x4 *>(kc + kv_key_unit<D>(t, c)) = encode16(x[i], ek);
+      place_value<D>(image, t, c, encode16(y[i], ev));
+    }
+  }
+  __syncthreads();
+  store_values<D>(image, vc, lo, hi, fv);
+  if (a.pool.weights != nullptr) {
+    for (uint32_t t = lo + tid; t < hi; t += kThreads) {
+      a.pool.weights[(unit << a.pool.shift) + t] =
+          a.weights != nullptr ? a.weights[uint64_t(row0 + t) * a.pool.heads + head] : 0.f;
+    }
+  }
+}
+
+// ------------------------------------------------------------------- gather
+
+// One workgroup reads 32 tokens of one head; values are brought into rows in
+// LDS, a code to a byte.
+template <int D>
+__global__ __launch_bounds__(kThreads) void gather4_kernel(KvGatherArgs a, uint32_t each_slots) {
+  using Chunk = Kv4Chunk<D>;
+  constexpr uint32_t kUnits = D / 16, kPitch = D + 16;
+  __shared__ __align__(16) uint8_t values[32 * kPitch];
+  const uint32_t head = blockIdx.y, tid = threadIdx.x;
+  const KvSlot slot = kv_find_slot(a.seqs, blockIdx.x, 1, 32, 2, each_slots);
+  if (slot.seq >= a.seqs.batch) {
+    return;
+  }
+  const KvRows rows = slot.rows;
+  const uint32_t length = kv_length(a.seqs, a.pool.shift, slot.seq);
+  const int64_t origin = int64_t(length) - rows.count;  // place of the first row
+  const int64_t base = (origin >> 5) * 32 + int64_t(slot.local) * 32;
+  const uint32_t lo = origin > base ? uint32_t(origin - base) : 0u;  // tokens lo .. hi - 1
+  const uint32_t hi = uint32_t(min(max(length - base, int64_t(0)), int64_t(32)));
+  if (lo >= hi) {
+    return;
+  }
+  // Rows before the first token, and those of no block, are zeros.
+  const int32_t id = base < 0 ? -1
+                              : kv_block(a.seqs.tables + slot.seq * a.seqs.stride, a.seqs,
+                                         a.pool.blocks, uint32_t(base) >> a.pool.shift);
+  const uint32_t in_block = uint32_t(base) & ((1u << a.pool.shift) - 1);
+  const uint64_t unit = uint64_t(id < 0 ? 0 : id) * a.pool.heads + head;
+  const uint8_t *chunk = kv4_chunk<D>(a.pool, unit, in_block);
+  const int64_t row0 = int64_t(rows.first) + (base - origin);
+  if (a.v != nullptr) {
+    // Unit i: a lane's 16 bytes, dims d + 16 * 0 .. 3 of eight tokens.
+    for (uint32_t i = tid; i < D; i += kThreads) {
+      const uint32_t g = i % 64 / 16, d = i / 64 * 64 + i % 16;
+      const u32x4 w = *reinterpret_cast<const u32x4 *>(chunk + Chunk::kSide + i * 16);
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) {
+        uint8_t *to = values + (4 * g + j % 4 + 16 * (j / 4)) * kPitch + d;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          to[16 * n] = uint8_t(w[n] >> (4 * j) & 15u);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  for (uint32_t i = tid; i < (hi - lo) * kUnits; i += kThreads) {
+    const uint32_t t = lo + i / kUnits, c = i % kUnits;
+    const uint64_t to = (uint64_t(row0 + t) * a.pool.heads + head) * D + c * 16;
+    u32x4 o[2] = {};
+    if (a.k != nullptr) {
+      if (id >= 0) {
+        const u32x2 w = *reinterpret_cast<const u32x2 *>(chunk + kv4_key_byte<D>(t, c * 16));
+        const float power = exp4_power(chunk[Chunk::kExps + kv4_exp_byte(t, c * 16)]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          o[j] = __builtin_bit_cast(u32x4, codes4_to_bf16(w[j], power));
+        }
+      }
+      reinterpret_cast<u32x4 *>(a.k + to)[0] = o[0];
+      reinterpret_cast<u32x4 *>(a.k + to)[1] = o[1];
+    }
+    if (a.v != nullptr) {
+      o[0] = o[1] = u32x4{};
+      if (id >= 0) {
+        const float s = f16_to_f32(
+            *reinterpret_cast<const uint16_t *>(chunk + Chunk::kScales + kv4_scale_byte(t)));
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(values + t * kPitch + c * 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const u32x2 b = decode4_bytes(w[j], s);
+          o[j / 2][j % 2 * 2] = b.x;
+          o[j / 2][j % 2 * 2 + 1] = b.y;
+        }
+      }
+      reinterpret_cast<u32x4 *>(a.v + to)[0] = o[0];
+      reinterpret_cast<u32x4 *>(a.v + to)[1] = o[1];
+    }
+  }
+  if (a.weights != nullptr && tid >= lo && tid < hi) {
+    a.weights[uint64_t(row0 + tid) * a.pool.heads + head] =
+        id < 0 ? 0.f : a.pool.weights[(unit << a.pool.shift) + in_block + tid];
+  }
+}
+
+// -------------------------------------------------------------------- evict
+
+// One workgroup fills 32 tokens of one head of the new tables with those that
+// stay.  Tokens have their own scales, so codes move as they are: keys whole,
+// of values' dwords a token's nibble to its new place among eight.
+template <int D>
+__global__ __launch_bounds__(kThreads) void evict4_move_kernel(KvEvictArgs a) {
+  using Chunk = Kv4Chunk<D>;
+  constexpr uint32_t kKeyBytes = D / 8;  // of a lane's run: 16, or 8 with 64 dims
+  constexpr uint64_t kNone = ~uint64_t(0);
+  __shared__ uint64_t from[32];   // offset of the token's chunk, kNone: it has no block
+  __shared__ uint32_t place[32];  // its number there
+  const uint32_t head = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const uint32_t base = blockIdx.x * 32;
+  const uint32_t length = kv_length(a.seqs, a.pool.shift, b);
+  const uint32_t stay = length < a.keep ? length : a.keep;
+  const int32_t raw =
+      base < stay ? a.new_tables[b * a.new_stride + (base >> a.pool.shift)] : -1;
+  if (raw < 0 || uint32_t(raw) >= a.pool.blocks) {
+    return;
+  }
+  const uint32_t n = min(stay - base, 32u), mask = (1u << a.pool.shift) - 1;
+  const uint64_t dst = uint64_t(raw) * a.pool.heads + head;
+  uint8_t *to = kv4_chunk<D>(a.pool, dst, base & mask);
+  if (tid < 32) {
+    uint64_t at = kNone;
+    uint32_t t = 0;
+    if (tid < n) {
+      t = uint32_t(a.kept[(uint64_t(b) * a.pool.heads + head) * a.keep + base + tid]);
+      const int32_t id = kv_block(a.seqs.tables + b * a.seqs.stride, a.seqs, a.pool.blocks,
+                                  t >> a.pool.shift);
+      float weight = 0.f;
+      if (id >= 0) {
+        const uint64_t src = uint64_t(id) * a.pool.heads + head;
+        at = uint64_t(kv4_chunk<D>(a.pool, src, t & mask) - a.pool.codes);
+        weight = a.pool.weights[(src << a.pool.shift) + (t & mask)];
+      }
+      a.pool.weights[(dst << a.pool.shift) + (base & mask) + tid] = weight;
+    }
+    from[tid] = at;
+    place[tid] = t % 32;
+    // A token of no block is zeros, as if appended.
+    *reinterpret_cast<uint16_t *>(to + Chunk::kScales + kv4_scale_byte(tid)) =
+        at != kNone ? *reinterpret_cast<const uint16_t *>(a.pool.codes + at + Chunk::kScales +
+                                                          kv4_scale_byte(t % 32))
+                    : f32_to_f16(kScaleLeast);
+  }
+  __syncthreads();
+  if (tid < 128) {  // keys: token tid / 4, run g of four
+    const uint32_t i = tid / 4, g = tid % 4;
+    const uint64_t at = from[i];
+    const uint32_t d = D / 4 * g;
+    const uint8_t *src = a.pool.codes + (at != kNone ? at : 0);
+    u32x4 w = {};
+    uint8_t e = uint8_t(kKvExpMin + 127);
+    if (at != kNone) {
+      if constexpr (kKeyBytes == 16) {
+        w = *reinterpret_cast<const u32x4 *>(src + kv4_key_byte<D>(place[i], d));
+      } else {
+        const u32x2 half = *reinterpret_cast<const u32x2 *>(src + kv4_key_byte<D>(place[i], d));
+        w.x = half.x;
+        w.y = half.y;
+      }
+      e = src[Chunk::kExps + kv4_exp_byte(place[i], d)];
+    }
+    if constexpr (kKeyBytes == 16) {
+      *reinterpret_cast<u32x4 *>(to + kv4_key_byte<D>(i, d)) = w;
+    } else {
+      *reinterpret_cast<u32x2 *>(to + kv4_key_byte<D>(i, d)) = u32x2{w.x, w.y};
+    }
+    if (d % 32 == 0) {
+      to[Chunk::kExps + kv4_exp_byte(i, d)] = e;
+    }
+  } else if (tid - 128 < D) {  // values: the 16 bytes of a lane for eight new tokens
+    const uint32_t l = tid - 128, g = l % 64 / 16;
+    u32x4 w = {};
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+      const uint32_t i = 4 * g + j % 4 + 16 * (j / 4), p = place[i];
+      const uint64_t at = from[i];
+      if (at != kNone) {
+        const u32x4 x = *reinterpret_cast<const u32x4 *>(
+            a.pool.codes + at + Chunk::kSide + l / 64 * 1024 +
+            (l % 16 + 16 * kv4_value_group(p)) * 16);
+        const uint32_t shift = 4 * kv4_value_slot(p);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          w[k] |= (x[k] >> shift & 15u) << (4 * j);
+        }
+      }
+    }
+    reinterpret_cast<u32x4 *>(to + Chunk::kSide)[l] = w;
+  }
+}
+
+}  // namespace
+
+hipError_t launch_kv4_append(const KvRotateArgs &a, uint32_t dim, hipStream_t s) {
+  const KvSeqs &q = a.append.seqs;
+  // n rows touch at most (n + 30) / 32 + 1 chunks.
+  const uint32_t each = q.each == 0 ? 1 : (q.each + 30) / 32 + 1;
+  const dim3 grid(uint32_t(kv_slots(q, 1, 32, 2, each)), a.append.pool.heads);
+  const auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(a, each); };
+  if (a.rotary.dims != 0) {
+    launch(dim == 64 ? append4_kernel<64, true> : append4_kernel<128, true>);
+  } else {
+    launch(dim == 64 ? append4_kernel<64, false> : append4_kernel<128, false>);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_kv8_append_rotary(const KvRotateArgs &a, uint32_t dim, hipStream_t s) {
+  const KvSeqs &q = a.append.seqs;
+  const uint32_t bt = 1u << a.append.pool.shift;
+  const uint32_t each = q.each == 0 ? 1 : (q.each + bt - 2) / bt + 1;
+  const dim3 grid(uint32_t(kv_slots(q, 1, bt, 2, each)), a.append.pool.heads);
+  const auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(a, each); };
+  if (dim == 64) {
+    launch(bt == 32   ? append8_rotary_kernel<64, 32>
+           : bt == 64 ? append8_rotary_kernel<64, 64>
+                      : append8_rotary_kernel<64, 128>);
+  } else {
+    launch(bt == 32   ? append8_rotary_kernel<128, 32>
+           : bt == 64 ? append8_rotary_kernel<128, 64>
+                      : append8_rotary_kernel<128, 128>);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_kv4_gather(const KvGatherArgs &a, uint32_t dim, hipStream_t s) {
+  if (a.k == nullptr && a.v == nullptr) {
+    launch_kv_gather_weights(a, s);
+    return hipGetLastError();
+  }
+  const uint32_t each = a.seqs.each == 0 ? 1 : (a.seqs.each + 30) / 32 + 1;
+  const dim3 grid(uint32_t(kv_slots(a.seqs, 1, 32, 2, each)), a.pool.heads);
+  if (dim == 64) {
+    gather4_kernel<64><<<grid, kThreads, 0, s>>>(a, each);
+  } else {
+    gather4_kernel<128><<<grid, kThreads, 0, s>>>(a, each);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_kv4_evict(const KvEvictArgs &a, uint32_t dim, hipStream_t s) {
+  launch_kv_evict_select(a, s);
+  const dim3 grid((a.keep + 31) / 32, a.pool.heads, a.seqs.batch);
+  if (dim == 64) {
+    evict4_move_kernel<64><<<grid, kThreads, 0, s>>>(a);
+  } else {
+    evict4_move_kernel<128><<<grid, kThreads, 0, s>>>(a);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace ullm

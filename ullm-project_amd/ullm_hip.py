@@ -87,6 +87,8 @@ GEMV_REGISTER_STAGED = 4
 GEMV_SPLIT_K = 5
 BACKEND_HIP = 1
 KV_CACHE_TRACK_WEIGHTS = 1
+KV_CACHE_4_BITS = 4
+KV_ROTARY_INTERLEAVED = 1
 KV_ATTEND_ACCUMULATE = 1
 KV_KERNEL_FEW_ROWS = 1
 KV_KERNEL_MANY_ROWS = 2
@@ -245,6 +247,18 @@ class KvAppendDesc(ctypes.Structure):
                 ("reserved", _u64 * 4)]
 
 
+class KvAppendRotaryDesc(ctypes.Structure):
+    _fields_ = [("struct_size", _u32), ("abi_version", _u32), ("cache", _vp),
+                ("seqs", KvSequences), ("q", _vp), ("q_row_stride", _u64),
+                ("q_head_stride", _u64), ("q_out", _vp), ("q_out_row_stride", _u64),
+                ("q_out_head_stride", _u64), ("k", _vp), ("k_row_stride", _u64),
+                ("k_head_stride", _u64), ("v", _vp), ("v_row_stride", _u64),
+                ("v_head_stride", _u64), ("weights", _vp), ("inv_freq", _vp),
+                ("positions", _vp), ("position_stride", _u64), ("pair_axes", _vp),
+                ("heads", _u32), ("rotary_dims", _u32), ("axes", _u32), ("flags", _u32),
+                ("stream", _vp), ("reserved", _u64 * 4)]
+
+
 class KvGatherDesc(ctypes.Structure):
     _fields_ = [("struct_size", _u32), ("abi_version", _u32), ("cache", _vp),
                 ("seqs", KvSequences), ("k", _vp), ("v", _vp), ("weights", _vp),
@@ -344,6 +358,8 @@ _SIGNATURES = {
     "ullm_kv_cache_destroy": [ctypes.POINTER(_vp), ctypes.POINTER(ErrorSink)],
     "ullm_kv_cache_query": [_vp, ctypes.POINTER(KvCacheInfo), ctypes.POINTER(ErrorSink)],
     "ullm_kv_cache_append": [ctypes.POINTER(KvAppendDesc), ctypes.POINTER(ErrorSink)],
+    "ullm_kv_cache_append_rotary": [ctypes.POINTER(KvAppendRotaryDesc),
+                                    ctypes.POINTER(ErrorSink)],
     "ullm_kv_cache_gather": [ctypes.POINTER(KvGatherDesc), ctypes.POINTER(ErrorSink)],
     "ullm_kv_cache_attend": [ctypes.POINTER(KvAttendDesc), ctypes.POINTER(ErrorSink)],
     "ullm_kv_cache_attend_plan": [ctypes.POINTER(KvAttendDesc), ctypes.POINTER(KvAttendPlan),
@@ -755,7 +771,8 @@ def _strides3(t, name, heads, dim):
 
 class KvCache:
     """Keys and values in 8 bits (E4M3) with a power-of-two scale for each
-    block of tokens and head (opaque native handle; ullm/kv_cache.h).
+    block of tokens and head, or with ``bits=4`` as E2M1 with scales of each
+    token (opaque native handle; ullm/kv_cache.h, ullm/kv_cache4.h).
 
     A call takes the rows of all its sequences in one tensor: sequence b owns
     rows ``starts[b]`` to ``starts[b + 1] - 1`` (``starts`` int32 [batch + 1]
@@ -765,18 +782,21 @@ class KvCache:
     token has received, for ``attend(accumulate=True)`` and ``evict``."""
 
     def __init__(self, blocks, kv_heads, head_dim, block_tokens=64, track_weights=False,
-                 device=0):
+                 device=0, bits=8):
         self.handle = None
+        if bits not in (4, 8):
+            raise ValueError("bits must be 4 or 8")
         s = _Sink()
         d = new(KvCacheDesc, blocks=blocks, block_tokens=block_tokens, kv_heads=kv_heads,
-                head_dim=head_dim, flags=KV_CACHE_TRACK_WEIGHTS if track_weights else 0,
-                device=device)
+                head_dim=head_dim, device=device,
+                flags=(KV_CACHE_TRACK_WEIGHTS if track_weights else 0) |
+                      (KV_CACHE_4_BITS if bits == 4 else 0))
         h = _vp()
         _check(lib().ullm_kv_cache_create(ctypes.byref(d), ctypes.byref(h), s.ref), s)
         self.handle = h.value
         self.blocks, self.block_tokens = blocks, block_tokens
         self.kv_heads, self.head_dim = kv_heads, head_dim
-        self.track_weights, self.device = track_weights, device
+        self.track_weights, self.device, self.bits = track_weights, device, bits
 
     # -- lifetime ----------------------------------------------------------
     def destroy(self):
@@ -854,6 +874,82 @@ class KvCache:
             self.handle or 0, *self._seqs(lengths, tables, rows, starts), k.data_ptr(), k_row,
             k_head, v.data_ptr(), v_row, v_head, 0 if weights is None else weights.data_ptr(),
             _stream(stream) or 0)
+
+    def append_rotary(self, q, k, v, lengths, tables, inv_freq, starts=None, positions=None,
+                      pair_axes=None, interleaved=False, out=None, weights=None, stream=None):
+        """append() of keys that their positions still have to rotate, and the
+        rotated queries of the same rows: q bf16 [rows][heads][head_dim] (row
+        and head strides honoured; None: keys alone), the result in ``out``
+        (may be q itself) or a new tensor.
+
+        ``inv_freq`` (f32 [pairs]) is each pair's angle of one position; pair j
+        has dims j and j + pairs, or 2j and 2j + 1 if ``interleaved``, and dims
+        past 2 * pairs stay as they are.  Positions are the rows' places in
+        their sequences, or ``positions`` (int32 [rows] or [axes][rows]), with
+        ``pair_axes`` (uint8 [pairs]) for the axis of each pair."""
+        heads, dim, here = self.kv_heads, self.head_dim, self.device
+        torch = _torch_module or _torch()
+        for t in (q, k, v, lengths, tables, inv_freq, starts, positions, pair_axes, out, weights):
+            if t is not None and t.get_device() != here:
+                raise self._elsewhere()
+        rows, k_row, k_head = _strides3(k, "k", heads, dim)
+        v_rows, v_row, v_head = _strides3(v, "v", heads, dim)
+        if v_rows != rows:
+            raise ValueError("k and v must have the same number of rows")
+        if weights is not None and (weights.shape != (rows, heads)
+                                    or weights.dtype is not torch.float32
+                                    or not weights.is_contiguous()):
+            raise ValueError("weights must be a contiguous float32 [rows][kv_heads] tensor")
+        if len(inv_freq.shape) != 1 or inv_freq.dtype is not torch.float32 \
+                or not inv_freq.is_contiguous():
+            raise ValueError("inv_freq must be a contiguous float32 [pairs] tensor")
+        pairs, axes, at_axes = inv_freq.shape[0], 1, 0
+        if pair_axes is not None:
+            if pair_axes.shape != (pairs,) or pair_axes.dtype is not torch.uint8 \
+                    or not pair_axes.is_contiguous():
+                raise ValueError("pair_axes must be a contiguous uint8 [pairs] tensor")
+            at_axes = pair_axes.data_ptr()
+        at_positions, position_stride = 0, 0
+        if positions is not None:
+            shape = positions.shape
+            if positions.dtype is not torch.int32 or len(shape) not in (1, 2) \
+                    or shape[-1] != rows or (rows > 1 and positions.stride(-1) != 1):
+                raise ValueError("positions must be int32 [rows] or [axes][rows]")
+            at_positions = positions.data_ptr()
+            if len(shape) == 2:
+                axes = shape[0]
+                position_stride = positions.stride(0) if axes > 1 else 0
+                if axes > 1 and position_stride < rows:
+                    raise ValueError("rows of positions must not overlap")
+        if q is None:
+            if out is not None:
+                raise ValueError("out needs q")
+            q_fields = (0,) * 6
+            q_heads = 0
+        else:
+            if len(q.shape) != 3:
+                raise ValueError(f"q must be bfloat16 [rows][heads][{dim}]")
+            q_heads = q.shape[1]
+            q_rows, q_row, q_head = _strides3(q, "q", q_heads, dim)
+            if out is None:
+                out = torch.empty_like(q) if q.is_contiguous() else \
+                    q.new_empty((rows, q_heads, dim))
+                out_rows, out_row, out_head = rows, 0, 0
+            else:
+                out_rows, out_row, out_head = _strides3(out, "out", q_heads, dim)
+            if q_rows != rows or out_rows != rows:
+                raise ValueError("q, k, v and out must have the same number of rows")
+            if q_heads == 0:
+                raise ValueError("q must have heads")
+            q_fields = (q.data_ptr(), q_row, q_head, out.data_ptr(), out_row, out_head)
+        _packed(KvAppendRotaryDesc).call(
+            lib().ullm_kv_cache_append_rotary,
+            self.handle or 0, *self._seqs(lengths, tables, rows, starts), *q_fields,
+            k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head,
+            0 if weights is None else weights.data_ptr(), inv_freq.data_ptr(), at_positions,
+            position_stride, at_axes, q_heads, 2 * pairs, axes,
+            KV_ROTARY_INTERLEAVED if interleaved else 0, _stream(stream) or 0)
+        return out
 
     def _gatherable(self, lengths, tables, rows, starts):
         here = self.device
