@@ -908,199 +908,34 @@ __global__ __launch_bounds__(256) void add_scores_kernel(KvAttendArgs a, Scratch
   unsafeAtomicAdd(&a.pool.weights[(unit << a.pool.shift) + (t & ((1u << a.pool.shift) - 1))], sum);
 }
 
-// Adds the weights that tokens receive from all rows of their sequence, by a
-// second product of keys and queries: a wave owns 32 tokens, whose keys it
-// holds as operands, and the rows pass by in tiles of 64 that the workgroup
-// stages in LDS, the next tile on its way meanwhile.  Each token's sum has a
-// fixed order; the addition is atomic for blocks that several sequences of a
-// call share.  Bound as the products above are: 8 products and 48 other vector
-// instructions for 32 rows and 32 tokens.  (509 queries of 32 heads at 16384
-// tokens: 86 us; with four offsets a lane to move on and rows on their way in
-// registers, 125.)
-//
-// LDS holds a tile as D / 32 planes of 64 bytes of each row; 16-byte chunk k of
-// row r is at place k ^ r / 4 % 4 of the 64, so that 16 neighbours read 16
-// groups of banks and a wave copies 16 rows at once, a lane always the same.
-constexpr uint32_t kWeightTokens = 32 * kWaves, kWeightRows = 64;
-
+// The keys of add_weights_kernel: lane l's part of the A operands of 32 tokens,
+// dims 16 * (2 * (c / 2) + l / 32) + 8 * (c % 2) .. + 7 in operand c.
 template <int D>
-__global__ __launch_bounds__(kWaves * kWave, 4) void add_weights_kernel(KvAttendArgs a,
-                                                                        const RowStats *stats) {
-  constexpr uint32_t kPlane = kWeightRows * 64;
-  static_assert(kWeightRows == 16 * kWaves, "a wave copies 16 rows of each plane");
-  extern __shared__ __align__(1024) uint8_t weight_rows[];
-  const auto rows_lds = [](uint32_t stage) { return weight_rows + stage * (D / 32 * kPlane); };
-  const uint32_t kvh = blockIdx.y, b = blockIdx.z;
-  const uint32_t lane = threadIdx.x % kWave;
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const uint32_t h = lane / 32, i = lane % 32;
-  const uint32_t first = blockIdx.x * kWeightTokens;
-  const uint32_t length = kv_length(a.seqs, a.pool.shift, b);
-  if (first >= length) {
-    return;
-  }
-  const KvRows rows = kv_rows(a.seqs, b);
-  const int64_t origin = int64_t(length) - rows.count;
-  const uint32_t all = rows.count * a.group;
-  // Queries before the first token, or past the last one's window, see none.
-  const int64_t from = int64_t(first) - origin;
-  const uint32_t begin = from <= 0 ? 0u
-                         : from < int64_t(rows.count) ? uint32_t(from) * a.group / kWeightRows * kWeightRows
-                                                      : all;
-  const int64_t past = a.window != 0 ? int64_t(first) + kWeightTokens - 1 + a.window - origin
-                                     : int64_t(rows.count);
-  const uint32_t end = past <= 0 ? 0u
-                       : past < int64_t(rows.count) ? uint32_t(past) * a.group
-                                                    : all;
-
-  const uint32_t t0 = first + 32 * wave;
-  const int32_t id = t0 < length ? kv_block(a.seqs.tables + b * a.seqs.stride, a.seqs,
-                                            a.pool.blocks, t0 >> a.pool.shift)
-                                 : -1;
-  const uint64_t unit = uint64_t(id < 0 ? 0 : id) * a.pool.heads + kvh;
-  const uint32_t in_block = t0 & ((1u << a.pool.shift) - 1);
-  const uint8_t *keys =
-      a.pool.codes + unit * (uint64_t(2 * D) << a.pool.shift) + uint64_t(in_block) * D;
-  const float power = exp2_int(a.pool.exps[unit * 2]);
-  bf16x8 k[D / 16];
+struct WeightKeys8 {
+  static constexpr int kDim = D;
+  static __device__ __forceinline__ void load(const KvPool &pool, uint64_t unit, uint32_t in_block,
+                                              uint32_t lane, bf16x8 (&k)[D / 16]) {
+    const uint32_t h = lane / 32, i = lane % 32;
+    const uint8_t *keys = pool.codes + unit * (uint64_t(2 * D) << pool.shift) +
+                          uint64_t(in_block) * D;
+    const float power = exp2_int(pool.exps[unit * 2]);
 #pragma unroll
-  for (int c = 0; c < D / 32; ++c) {
-    const u32x4 w = *reinterpret_cast<const u32x4 *>(
-        keys + (i / 16 * (D / 64) + c / 2) * 1024 + (i % 16 + 16 * (c % 2 * 2 + h)) * 16);
-    k[2 * c] = flip(codes_to_bf16(w.x, w.y, power), a.q_sign);
-    k[2 * c + 1] = flip(codes_to_bf16(w.z, w.w, power), a.q_sign);
-  }
-
-  // A row's query, head of the group and offset, moved on by whole tiles
-  // without a division or product; rows past the end are the last one's.
-  const uint32_t tile_queries = kWeightRows / a.group, tile_heads = kWeightRows % a.group;
-  const uint64_t tile_step = tile_queries * a.q_row + tile_heads * a.q_head;
-  const uint64_t wrap_step = a.q_row - a.group * a.q_head;
-  const uint64_t last_row = (rows.count - 1) * a.q_row + (a.group - 1) * a.q_head;
-  struct RowAt {
-    uint32_t query, head;
-    uint64_t offset;
-  };
-  const auto row_at = [&](uint32_t r) {
-    return RowAt{r / a.group, r % a.group, r / a.group * a.q_row + r % a.group * a.q_head};
-  };
-  const auto next_tile = [&](RowAt &r) {
-    r.head += tile_heads;
-    const bool carry = r.head >= a.group;
-    r.head -= carry ? a.group : 0u;
-    r.query += tile_queries + (carry ? 1u : 0u);
-    r.offset += tile_step + (carry ? wrap_step : 0u);
-  };
-  RowAt mine = row_at(begin + 16 * wave + lane / 4);
-  const uint16_t *q_rows = a.q + rows.first * a.q_row + uint64_t(kvh) * a.group * a.q_head +
-                           (lane % 4 ^ lane / 16) * 8;
-  const auto start_tile = [&](uint8_t *to) {
-    const uint16_t *from = q_rows + (mine.query < rows.count ? mine.offset : last_row);
-    to += wave * 1024;
-    next_tile(mine);
-    if (a.vec) {
-#pragma unroll
-      for (uint32_t c = 0; c < D / 32; ++c) {
-        copy_to_lds(reinterpret_cast<const uint8_t *>(from + c * 32), to + c * kPlane);
-      }
-    } else {
-#pragma unroll
-      for (uint32_t c = 0; c < D / 32; ++c) {
-        *reinterpret_cast<bf16x8 *>(to + c * kPlane + lane * 16) =
-            load_query8(from + c * 32, false, 0);
-      }
-    }
-  };
-  const RowStats *row_stats = stats + stats_at(a, kvh, rows.first);
-  RowStats next[2];
-  const auto load_stats = [&](uint32_t r0) {
-#pragma unroll
-    for (uint32_t u = 0; u < 2; ++u) {
-      next[u] = row_stats[min(r0 + 32 * u + i, all - 1)];
-    }
-  };
-  // Rows that see some of the wave's tokens, and all of them.
-  struct Range {
-    uint32_t first, end;
-  };
-  const auto range = [&](int64_t from, int64_t past) {
-    const auto row = [&](int64_t query) {
-      return uint32_t(min(max(query - origin, int64_t(0)), int64_t(rows.count))) * a.group;
-    };
-    return Range{uniform(row(from)), a.window != 0 ? uniform(row(past + a.window)) : all};
-  };
-  const Range seen = range(t0, int64_t(t0) + 31), whole = range(int64_t(t0) + 31, t0);
-  float sum[16] = {};
-  uint32_t stage = 0;
-  if (begin < end) {
-    load_stats(begin);
-    start_tile(rows_lds(0));
-  }
-  for (uint32_t r0 = begin; r0 < end; r0 += kWeightRows, stage ^= 1) {
-    wait_copies<0>();
-    step_barrier();
-    const RowStats now[2] = {next[0], next[1]};
-    if (r0 + kWeightRows < end) {
-      load_stats(r0 + kWeightRows);
-      start_tile(rows_lds(stage ^ 1));
-    }
-    if (id < 0 || r0 + kWeightRows <= seen.first || r0 >= seen.end) {
-      continue;
-    }
-    const bool edge = r0 < whole.first || r0 + kWeightRows > whole.end;
-    const uint8_t *tile = rows_lds(stage) + i * 64;
-#pragma unroll
-    for (uint32_t u = 0; u < 2; ++u) {
-      bf16x8 q[D / 16];
-#pragma unroll
-      for (uint32_t c = 0; c < D / 16; ++c) {
-        const uint32_t place = (2 * h + c % 2) ^ i / 4 % 4;
-        q[c] = *reinterpret_cast<const bf16x8 *>(tile + c / 2 * kPlane + 32 * u * 64 + place * 16);
-      }
-      f32x16 s = f32x16{};
-#pragma unroll
-      for (uint32_t c = 0; c < D / 16; ++c) {
-        s = mfma32_bf16(k[c], q[c], s);
-      }
-      float inv_sum = now[u].inv_sum;
-      if (edge) {
-        // A row of NaN gives it to what it sees, and nothing to the rest.
-        const bool bad = inv_sum != inv_sum;
-        const float add = bad ? inv_sum : 0.f;
-        inv_sum = bad ? 1.f : inv_sum;
-        const uint32_t r = r0 + 32 * u + i;
-        const int32_t pos = int32_t(origin + r / a.group);
-        const int32_t oldest = oldest_hidden(pos, a.window);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int32_t tok = int32_t(t0) + e / 4 * 8 + 4 * int32_t(h) + e % 4;
-          s[e] = r < all && tok <= pos && tok > oldest ? s[e] + add : -INFINITY;
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        sum[e] = __builtin_fmaf(exp2_fast(__builtin_fmaf(s[e], a.scale_log2, -now[u].top)),
-                                inv_sum, sum[e]);
-      }
+    for (int c = 0; c < D / 32; ++c) {
+      const u32x4 w = *reinterpret_cast<const u32x4 *>(
+          keys + (i / 16 * (D / 64) + c / 2) * 1024 + (i % 16 + 16 * (c % 2 * 2 + h)) * 16);
+      k[2 * c] = codes_to_bf16(w.x, w.y, power);
+      k[2 * c + 1] = codes_to_bf16(w.z, w.w, power);
     }
   }
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      sum[e] += __shfl_xor(sum[e], off, kWave);
-    }
-    const uint32_t t = e / 4 * 8 + 4 * h + e % 4;
-    if (i == uint32_t(e) && id >= 0 && t0 + t < length) {
-      unsafeAtomicAdd(&a.pool.weights[(unit << a.pool.shift) + in_block + t], sum[e]);
-    }
-  }
-}
+  // The 32 dims and the eight of them that operand c has in half h.
+  static __device__ __forceinline__ uint32_t plane(uint32_t, uint32_t c) { return c / 2; }
+  static __device__ __forceinline__ uint32_t chunk(uint32_t h, uint32_t c) { return 2 * h + c % 2; }
+};
 
 }  // namespace
 
 Scratch scratch_of(const KvAttendArgs &a, uint32_t dim, const KvAttendPlan &p, void *ws,
-                          uint64_t *bytes) {
+                   uint64_t *bytes) {
   Scratch x{};
   x.parts = p.parts;
   x.part_tokens = p.part_tokens;
@@ -1259,16 +1094,10 @@ static hipError_t launch_attend(const KvAttendArgs &a, const KvAttendPlan &p, vo
     few(few_rows_kernel<D, 8, false, false>, few_rows_kernel<D, 4, false, false>);
   }
   launch_join_parts(a, D, p, x, s);
-  if (a.accumulate) {
-    const uint64_t tokens = uint64_t(a.seqs.max_blocks) << a.pool.shift;
-    if (x.scores != nullptr) {
-      launch_add_scores(a, x, s);
-    } else {
-      const dim3 grid(uint32_t((tokens + kWeightTokens - 1) / kWeightTokens), a.pool.heads,
-                      a.seqs.batch);
-      add_weights_kernel<D>
-          <<<grid, kWaves * kWave, 2 * kWeightRows * D * 2, s>>>(a, x.stats);
-    }
+  if (a.accumulate && x.scores != nullptr) {
+    launch_add_scores(a, x, s);
+  } else if (a.accumulate) {
+    launch_add_weights(add_weights_kernel<WeightKeys8<D>>, a, D, x.stats, s);
   }
   return hipGetLastError();
 }

@@ -11,11 +11,11 @@
 // beside the bare codes, while the row's sum takes p in f32.  Powers are taken
 // over a reference M that follows the largest of score + log2(s) (not of the
 // score alone), so that the largest p' is near 2^kOff: what a token adds to the
-// result decides how exactly it enters, whatever the scales of the others.  M
-// moves when some p' passes 2^15: the weights of a group are computed first and
-// looked at after.  With scales from 2^-19 to 2^16 the p of a row's sum stay
-// within 2^-28 and 2^52 of what they would be over the largest score, far inside
-// f32.
+// result decides how exactly it enters, whatever the scales of the others.  M is
+// left alone while (largest score) + log2(largest s) of a lane's tokens, which no
+// sum passes, stays within kSlack of it; else it moves to the largest sum.  With
+// scales from 2^-19 to 2^16 the p of a row's sum stay within 2^-28 and 2^34 of
+// what they would be over the largest score, far inside f32.
 //
 // NaN.  Codes are finite, NaN is in a key's exponent or a value's scale, so that
 // it can reach a row only through its score or its weight: tokens that a row
@@ -27,6 +27,10 @@
 
 namespace ullm {
 namespace {
+
+// A reference may lag by this much: weights then reach 2^(kOff + kSlack) = 2^15
+// in f16.
+constexpr float kSlack = 4.f;
 
 // A row's query as B operands: lane group g holds dims D / 4 * g + 8c .. + 7 in
 // q[c], the order of the keys' codes.
@@ -98,10 +102,19 @@ __device__ __forceinline__ uint32_t max_f16(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(h2, a),
                                                                 __builtin_bit_cast(h2, b)));
 }
-// Whether one of two weights (not negative, or NaN) has passed 2^15; infinity has.
-__device__ __forceinline__ bool past_limit(uint32_t w) {
-  const auto past = [](uint32_t h) { return h > 0x7800u && h <= 0x7c00u; };
-  return past(w & 0xffffu) || past(w >> 16);
+// log2 of the larger of two scales, or of the smallest there is.
+__device__ __forceinline__ float largest_log2(uint32_t scales) {
+  const float s = fmaxf(f16_to_f32(uint16_t(scales)), f16_to_f32(uint16_t(scales >> 16)));
+  return __builtin_amdgcn_logf(fmaxf(s, kScaleLeast));
+}
+// Whether one of eight scales is NaN.
+__device__ __forceinline__ bool any_nan(u32x4 scales) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w |= (scales[i] & 0x7fff7fffu) + 0x03ff03ffu;  // past infinity: a carry into the sign
+  }
+  return (w & 0x80008000u) != 0;
 }
 // log2 of a scale in a word's lower or upper half.  Also of what has none: the
 // zero of a token that was never written, NaN; their tokens have a score and a
@@ -152,49 +165,41 @@ __device__ __forceinline__ void attend_group4(RowState4<D> &st, Group4<D> &x, co
       *reinterpret_cast<f32x4 *>(scores_to + t0 + 16 * i + 4 * g) = s[i];
     }
   }
-  float p[8];
-  u32x4 pw;
-  const auto weigh = [&] {
-    const float bias = float(kOff) - (st.m == -INFINITY ? 0.f : st.m);
-    uint32_t top = 0;
+  float top = s[0][0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    top = fmaxf(top, s[i / 4][i % 4]);
+  }
+  const uint32_t most =
+      max_f16(max_f16(x.scales.x, x.scales.y), max_f16(x.scales.z, x.scales.w));
+  if (__any(top + largest_log2(most) > st.m + kSlack)) {
+    float now = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      p[i] = exp2_fast(s[i / 4][i % 4] + bias);
+      now = fmaxf(now, s[i / 4][i % 4] + scale_log2_of(x.scales[i / 2], i % 2));
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      pw[i] = scaled_weights(p[2 * i], p[2 * i + 1], x.scales[i]);
-      top = max_f16(top, pw[i]);
-    }
-    return past_limit(top);
-  };
-  // The first tokens that a row sees always set its reference.
-  bool grow = st.m == -INFINITY;
-  grow = weigh() || grow;
-  if (__any(grow)) {
-    float top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float y = s[i / 4][i % 4] + scale_log2_of(x.scales[i / 2], i % 2);
-      top = fmaxf(top, y);  // passes NaN over: it makes the sum below NaN
-    }
-    top = max_groups(top);
-    const float now = fmaxf(st.m, top);
-    const float keep = st.m == -INFINITY ? 1.f : exp2_fast(st.m - now);
+    now = fmaxf(st.m, max_groups(now));
+    const float keep = now == -INFINITY ? 1.f : exp2_fast(st.m - now);
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {
       st.o[i] *= keep;
     }
     st.l *= keep;
     st.m = now;
-    weigh();
   }
-  float sum = 0.f;
+  const float bias = float(kOff) - (st.m == -INFINITY ? 0.f : st.m);
+  float p[8], sum = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
+    p[i] = exp2_fast(s[i / 4][i % 4] + bias);
     sum += p[i];
   }
   st.l += sum;
+  u32x4 pw;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    pw[i] = scaled_weights(p[2 * i], p[2 * i + 1], x.scales[i]);
+  }
   const f16x8 pb = __builtin_bit_cast(f16x8, pw);
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
@@ -290,95 +295,339 @@ __global__ __launch_bounds__(W * kWave, 3) void few_rows4_kernel(KvAttendArgs a,
   join_waves<D, W>(join, a, x, t, kvh, part, parts, st.m, st.l, st.o, 1.f);
 }
 
-// Adds the weights that tokens receive from all rows of their sequence, by a
-// second product of keys and queries: a wave owns 32 tokens and walks the rows,
-// 16 at a time.
+// ------------------------------------------------------------- many rows
+//
+// 128 rows to a workgroup, 32 to a wave, with 32 x 32 x 16 products, as
+// many_rows_kernel does: steps of 64 tokens go through a ring of two stages in
+// LDS, filled by copies that no register waits for; every wave converts what it
+// reads.
+//
+// Order of the operands (lane l, half h = l / 32, i = l % 32):
+//   keys: row i of the product is token i with bits 3 and 4 exchanged, so that
+//     element e of a result is token {0, 16, 8, 24}[e / 4] + 4h + e % 4 and
+//     elements 8c .. 8c + 7 are the 8 tokens of group 2c + h of the values; half
+//     h has dims D / 2 * h .. of the contraction, so two exponents at most;
+//   values: accumulator m, row i is dim D / 2 * (i / 16) + 16 m + i % 16: a lane's
+//     run of dims, read at once, serves all accumulators.
+constexpr uint32_t kManyRows = 128, kStages = 2, kManyBlocks = 512;
+
 template <int D>
-__global__ __launch_bounds__(kWaves * kWave) void add_weights4_kernel(KvAttendArgs a,
-                                                                      const RowStats *stats) {
-  const uint32_t kvh = blockIdx.y, b = blockIdx.z;
-  const uint32_t lane = threadIdx.x % kWave, g = lane / 16, col = lane % 16;
+struct Many4 {
+  // A chunk's place in LDS: codes, then exponents and scales, copied by 64 lanes.
+  static constexpr uint32_t kCodes = 2 * Kv4Chunk<D>::kSide, kTail = Kv4Chunk<D>::kBytes - kCodes;
+  static constexpr uint32_t kSlot = kCodes + 1024, kLds = kStages * 2 * kSlot;
+};
+
+// LONG: a part may have more blocks than LDS holds entries of, which are then
+// replaced on the way.
+template <int D, bool LONG>
+__global__ __launch_bounds__(kWaves * kWave, 3) void many_rows4_kernel(KvAttendArgs a, Scratch x,
+                                                                       uint32_t each_slots) {
+  using Chunk = Kv4Chunk<D>;
+  constexpr uint32_t kSlot = Many4<D>::kSlot;
+  extern __shared__ __align__(1024) uint8_t many_ring4[];
+  const auto ring = [](uint32_t stage) { return many_ring4 + stage * 2 * kSlot; };
+  // Where a block's chunks start; one out of the pool has the first one's, plus 1.
+  __shared__ uint64_t entries[kManyBlocks];
+  const uint32_t kvh = blockIdx.x % a.pool.heads;
+  const uint32_t rest = blockIdx.x / a.pool.heads, slots = gridDim.x / a.pool.heads / x.parts;
+  const uint32_t part = rest % x.parts;
+  Tile t;
+  if (!tile_rows_last_first(a, rest / x.parts, slots, kManyRows, each_slots, &t)) {
+    return;
+  }
+  tile_tokens(a, kv_length(a.seqs, a.pool.shift, t.seq), &t);
+  const uint32_t parts = part_count(t, x.part_tokens);
+  if (part != 0 && part >= parts) {
+    return;
+  }
+  const uint32_t lane = threadIdx.x % kWave;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const uint32_t length = kv_length(a.seqs, a.pool.shift, b);
-  const uint32_t t0 = (blockIdx.x * kWaves + wave) * 32;
-  if (t0 >= length) {
-    return;
-  }
-  const int32_t id = kv_block(a.seqs.tables + b * a.seqs.stride, a.seqs, a.pool.blocks,
-                              t0 >> a.pool.shift);
-  const KvRows rows = kv_rows(a.seqs, b);
-  const uint32_t all = rows.count * a.group;
-  if (id < 0 || all == 0) {
-    return;
-  }
-  const int64_t origin = int64_t(length) - rows.count;
-  const uint64_t unit = uint64_t(id) * a.pool.heads + kvh;
-  const uint32_t in_block = t0 & ((1u << a.pool.shift) - 1);
-  Group4<D> x;
-  load_keys4<D, false>(x, kv4_chunk<D>(a.pool, unit, in_block), lane);
-  float sum[8] = {};
-  for (uint32_t r0 = 0; r0 < all; r0 += kRows) {
-    const uint32_t r = r0 + col < all ? r0 + col : all - 1, head = kvh * a.group + r % a.group;
-    const uint64_t row = rows.first + r / a.group;
-    const Query4<D> q = load_query4<D>(a.q + row * a.q_row + head * a.q_head, a.vec, a.q_sign, g);
-    const RowStats st = stats[stats_at(a, kvh, rows.first) + r];
-    const int32_t pos = int32_t(origin + r / a.group), oldest = oldest_hidden(pos, a.window);
+  const uint32_t h = lane / 32, i = lane % 32;
+  // The wave's rows; rows past the end see what the last one does.
+  const uint32_t last = t.live - 1;
+  const uint32_t w0 = min(32 * wave, last), w1 = min(32 * wave + 31, last);
+  const uint32_t r = t.r0 + min(32 * wave + i, last);
+  const uint32_t head = kvh * a.group + r % a.group;
+  const uint64_t row = t.first_row + r / a.group;
+  const int32_t pos = int32_t(t.origin + r / a.group), oldest = oldest_hidden(pos, a.window);
+  const int32_t low = int32_t(t.origin + (t.r0 + w0) / a.group);
+  const int32_t high = int32_t(t.origin + (t.r0 + w1) / a.group);
+  bf16x8 q[D / 16];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const f32x4 s = products4<D>(x, i, q);
+  for (int c = 0; c < D / 16; ++c) {
+    q[c] = load_query8(a.q + row * a.q_row + head * a.q_head + D / 2 * h + 8 * c, a.vec, a.q_sign);
+  }
+  const uint32_t from = t.begin / 32 + part * (x.part_tokens / 32);
+  const uint32_t all = (t.end + 31) / 32;
+  const uint32_t to = min(all, from + x.part_tokens / 32);
+  const int32_t *table = a.seqs.tables + t.seq * a.seqs.stride;
+  // LDS holds the blocks `held` .. held + kManyBlocks - 1 of the sequence, as
+  // far as the part goes.
+  uint32_t held = from * 32 >> a.pool.shift;
+  const auto hold_blocks = [&] {
+    const uint32_t end = to > from ? ((to * 32 - 1) >> a.pool.shift) + 1 : held;
+    for (uint32_t b = threadIdx.x; b < kManyBlocks && held + b < end; b += kWaves * kWave) {
+      const int32_t id = kv_block(table, a.seqs, a.pool.blocks, held + b);
+      const uint8_t *first =
+          kv4_chunk<D>(a.pool, uint64_t(id < 0 ? 0 : id) * a.pool.heads + kvh, 0);
+      entries[b] = reinterpret_cast<uint64_t>(first) | (id < 0 ? 1u : 0u);
+    }
+  };
+  hold_blocks();
+  // bias: what a scaled score becomes a power of two with.
+  float m = -INFINITY, l = 0.f, limit = -INFINITY, bias = float(kOff);
+  f32x16 o[D / 32];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int32_t tok = int32_t(t0 + 16 * i + 4 * g + j);
-        const bool see = r0 + col < all && tok <= pos && tok > oldest;
-        // A row of NaN gives it to what it sees, and nothing to the rest.
-        const float p = exp2_fast(s[j] * a.scale_log2 - st.top) * st.inv_sum;
-        sum[4 * i + j] += see ? p : 0.f;
+  for (int c = 0; c < D / 32; ++c) {
+    o[c] = f32x16{};
+  }
+  __syncthreads();
+
+  const uint32_t in_mask = (1u << a.pool.shift) - 1;
+  // Copies a step's two chunks (one past the end is the last one again); returns
+  // which of them are of no block.
+  const auto start_step = [&](uint32_t grp0, uint8_t *stage) {
+    uint32_t absent = 0;
+#pragma unroll
+    for (uint32_t u = 0; u < 2; ++u) {
+      const uint32_t tok = min(grp0 + u, to - 1) * 32;
+      const u32x2 e =
+          *reinterpret_cast<const u32x2 *>(&entries[(tok >> a.pool.shift) - held]);
+      const uint32_t low_bits = uniform(e.x);
+      absent |= (low_bits & 1u) << u;
+      const uint8_t *chunk =
+          reinterpret_cast<const uint8_t *>(uint64_t(uniform(e.y)) << 32 | (low_bits & ~1u)) +
+          (tok & in_mask) / 32 * Chunk::kBytes;
+      uint8_t *slot = stage + u * kSlot;
+      if (D == 128) {
+        copy_to_lds(chunk + wave * 1024 + lane * 16, slot + wave * 1024);
+      } else if (wave / 2 == u) {
+        copy_to_lds(chunk + wave % 2 * 1024 + lane * 16, slot + wave % 2 * 1024);
+      }
+      if (wave == 2 + u) {
+        constexpr uint32_t kLanes = Many4<D>::kTail / 16;
+        copy_to_lds(chunk + Many4<D>::kCodes + lane % kLanes * 16, slot + Many4<D>::kCodes);
+      }
+    }
+    return absent;
+  };
+  // Chunks that some of the wave's rows see, and of those the ones that every
+  // row sees whole: [first, first + count) each.
+  struct Range {
+    uint32_t first, count;
+  };
+  const auto range = [](int64_t first, int64_t end) {
+    return Range{uniform(uint32_t(first)), uniform(uint32_t(end > first ? end - first : 0))};
+  };
+  const Range some = range((int64_t(oldest_hidden(low, a.window)) + 1) / 32,
+                           high < 0 ? 0 : min(int64_t(high / 32 + 1), int64_t(to)));
+  const Range whole = range((int64_t(oldest_hidden(high, a.window)) + 1 + 31) / 32,
+                            low < 0 ? 0 : (int64_t(low) + 1) / 32);
+  const uint32_t steps = to > from ? (to - from + 1) / 2 : 0;
+  uint32_t next = 0;
+  if (steps != 0) {
+    next = start_step(from, ring(0));
+  }
+  // Lane's token in a chunk of keys: i with bits 3 and 4 exchanged.
+  const uint32_t tok = (i & 7) | (i & 8) << 1 | (i & 16) >> 1;
+  // (A register each: taken apart again in the loop they would not fit.)
+  const uint32_t key_at = opaque_u32(kv4_key_byte<D>(tok, D / 2 * h));
+  const uint32_t exp_at = opaque_u32(Chunk::kExps + kv4_exp_byte(tok, D / 2 * h));
+  const uint32_t value_at =
+      opaque_u32(Chunk::kSide + kv4_value_dword(h, D / 2 * (i / 16) + i % 16));
+  const uint32_t scale_at = opaque_u32(Chunk::kScales + 16 * h);
+  for (uint32_t step = 0; step < steps; ++step) {
+    wait_copies<0>();
+    step_barrier();
+    const uint32_t absent = next;
+    const uint8_t *stage = ring(step % kStages);
+    if (step + 1 < steps) {
+      const uint32_t grp0 = from + 2 * step + 2;
+      if (LONG && (min(grp0 + 1, to - 1) * 32 >> a.pool.shift) - held >= kManyBlocks) {
+        // No wave is past this step's barrier without the entries it read.
+        held = grp0 * 32 >> a.pool.shift;
+        hold_blocks();
+        __syncthreads();
+      }
+      next = start_step(grp0, ring((step + 1) % kStages));
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < 2; ++u) {
+      const uint32_t grp = from + 2 * step + u;
+      if (grp - some.first >= some.count) {
+        continue;
+      }
+      const uint8_t *chunk = stage + u * kSlot;
+      // Keys: with 128 dims two runs of 32 dims, with 64 of 16.
+      u32x4 keys[D / 64];
+      float power[D / 64];
+      if constexpr (D == 128) {
+#pragma unroll
+        for (uint32_t c = 0; c < 2; ++c) {
+          keys[c] = *reinterpret_cast<const u32x4 *>(chunk + key_at + c * 256);
+          power[c] = bits_f32(uint32_t(chunk[exp_at + c * 32]) << 23);
+        }
+      } else {
+        const u32x2 w0 = *reinterpret_cast<const u32x2 *>(chunk + key_at);
+        const u32x2 w1 = *reinterpret_cast<const u32x2 *>(chunk + key_at + 256);
+        keys[0] = u32x4{w0.x, w0.y, w1.x, w1.y};
+        power[0] = bits_f32(uint32_t(chunk[exp_at]) << 23);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      f32x16 s = f32x16{};
+#pragma unroll
+      for (uint32_t c = 0; c < D / 16; ++c) {
+        s = mfma32_bf16(codes4_to_bf16(keys[c / 4][c % 4], power[c / 4]), q[c], s);
+        if (c % 2 == 1) {
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      u32x4 scales[2], values[2];
+#pragma unroll
+      for (uint32_t c = 0; c < 2; ++c) {
+        scales[c] = *reinterpret_cast<const u32x4 *>(chunk + scale_at + c * 32);
+        if constexpr (D == 128) {
+          values[c] = *reinterpret_cast<const u32x4 *>(chunk + value_at + c * 512);
+        } else {
+          const u32x2 w = *reinterpret_cast<const u32x2 *>(chunk + value_at + c * 512);
+          values[c] = u32x4{w.x, w.y, 0u, 0u};
+        }
+      }
+      const uint32_t gone = absent >> u << 31;
+      const bool edge = ((grp - whole.first) | gone) >= whole.count;
+      const auto seen = [&](int e) {
+        const int32_t at =
+            int32_t(grp * 32) + int32_t((e / 4 % 2) * 16 + e / 8 * 8 + 4 * h + e % 4);
+        return gone == 0 && at <= pos && at > oldest;
+      };
+      if (edge) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          s[e] = seen(e) ? s[e] : -INFINITY;
+        }
+      }
+      float top = s[0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) {
+        top = fmaxf(top, s[e]);
+      }
+      const uint32_t most = max_f16(max_f16(max_f16(scales[0].x, scales[0].y),
+                                            max_f16(scales[0].z, scales[0].w)),
+                                    max_f16(max_f16(scales[1].x, scales[1].y),
+                                            max_f16(scales[1].z, scales[1].w)));
+      if (__any(__builtin_fmaf(top, a.scale_log2, largest_log2(most)) > limit)) {
+        float now = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          now = fmaxf(now, __builtin_fmaf(s[e], a.scale_log2,
+                                          scale_log2_of(scales[e / 8][e % 8 / 2], e % 2)));
+        }
+        const auto both =
+            __builtin_amdgcn_permlane32_swap(f32_bits(now), f32_bits(now), false, false);
+        now = fmaxf(m, fmaxf(bits_f32(both[0]), bits_f32(both[1])));
+        const float keep = now == -INFINITY ? 1.f : exp2_fast(m - now);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          o[c] *= keep;
+        }
+        l *= keep;
+        m = now;
+        limit = m + kSlack;
+        bias = float(kOff) - (m == -INFINITY ? 0.f : m);
+      }
+      u32x4 p[2];
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float p0 = exp2_fast(__builtin_fmaf(s[e], a.scale_log2, bias));
+        const float p1 = exp2_fast(__builtin_fmaf(s[e + 1], a.scale_log2, bias));
+        sum += p0;
+        sum += p1;
+        p[e / 8][e % 8 / 2] = scaled_weights(p0, p1, scales[e / 8][e % 8 / 2]);
+      }
+      l += sum;
+      if (edge && __any(any_nan(scales[0]) || any_nan(scales[1]))) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const uint32_t w = p[e / 8][e % 8 / 2];
+          p[e / 8][e % 8 / 2] = seen(e) ? w : w & (e % 2 == 0 ? 0xffff0000u : 0x0000ffffu);
+        }
+      }
+#pragma unroll
+      for (uint32_t c = 0; c < 2; ++c) {
+        const f16x8 b = __builtin_bit_cast(f16x8, p[c]);
+#pragma unroll
+        for (uint32_t n = 0; n < D / 32; ++n) {
+          o[n] = mfma32_f16(codes4_to_f16(values[c][n]), b, o[n]);
+          if (n % 2 == 1) {
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
       }
     }
   }
+  wait_copies<0>();  // none may land after the workgroup has gone
+
+  const uint32_t mine = 32 * wave + i, rr = t.r0 + min(mine, last);
+  RowSink out;
+  out.row = t.first_row + rr / a.group;
+  out.head = kvh * a.group + rr % a.group;
+  out.live = mine <= last;
+  out.whole = parts <= 1;
+  out.slot = (out.row * a.heads + out.head) * x.parts + part;
+  const auto half = __builtin_amdgcn_permlane32_swap(f32_bits(l), f32_bits(l), false, false);
+  const float total = bits_f32(half[0]) + bits_f32(half[1]);
+  const float join = total == 0.f ? 0.f : 1.0f / total;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+  for (int n = 0; n < D / 32; ++n) {
 #pragma unroll
-    for (int off = 1; off < 16; off <<= 1) {
-      sum[e] += __shfl_xor(sum[e], off, kWave);
+    for (int e = 0; e < 4; ++e) {
+      f32x4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[j] = o[n][4 * e + j] * join;
+      }
+      store4(a, x, out, D, D / 2 * (e / 2) + 16 * n + 8 * (e % 2) + 4 * h, v);
     }
-    const uint32_t t = 16 * (e / 4) + 4 * g + e % 4;
-    if (col == uint32_t(e) && t0 + t < length) {
-      unsafeAtomicAdd(&a.pool.weights[(unit << a.pool.shift) + in_block + t], sum[e]);
-    }
+  }
+  if (h == 0) {
+    store_sums(a, x, out, m, total);
   }
 }
 
-// Workgroups for each compute unit: tokens are split into that many parts.
-constexpr uint32_t kPartLeast4 = 512;
+// The keys of add_weights_kernel: lane l's part of the A operands of 32 tokens,
+// dims D / 2 * (l / 32) + 8 c .. + 7 in operand c.
+template <int D>
+struct WeightKeys4 {
+  static constexpr int kDim = D;
+  static __device__ __forceinline__ void load(const KvPool &pool, uint64_t unit, uint32_t in_block,
+                                              uint32_t lane, bf16x8 (&k)[D / 16]) {
+    const uint32_t h = lane / 32, i = lane % 32;
+    const uint8_t *chunk = kv4_chunk<D>(pool, unit, in_block);
+#pragma unroll
+    for (uint32_t c = 0; c < D / 16; ++c) {
+      const uint32_t d = D / 2 * h + 8 * c;
+      const uint32_t w = *reinterpret_cast<const uint32_t *>(chunk + kv4_key_byte<D>(i, d));
+      const uint32_t e = chunk[Kv4Chunk<D>::kExps + kv4_exp_byte(i, d)];
+      k[c] = codes4_to_bf16(w, bits_f32(e << 23));
+    }
+  }
+  static __device__ __forceinline__ uint32_t plane(uint32_t h, uint32_t c) {
+    return (D / 2 * h + 8 * c) / 32;
+  }
+  static __device__ __forceinline__ uint32_t chunk(uint32_t, uint32_t c) { return c % 4; }
+};
 
 }  // namespace
 
 KvAttendPlan plan_kv4_attend(const KvAttendArgs &a, uint32_t dim) {
-  KvAttendPlan p;
-  if (a.seqs.rows == 0 || a.seqs.batch == 0) {
-    return p;
-  }
-  const uint32_t cus = device_cu_count();
-  const uint64_t rows_of_head = uint64_t(a.seqs.rows) * a.group;
-  p.kernel = ULLM_KV_KERNEL_FEW_ROWS;
-  p.row_tile = kRows;
-  const uint64_t tiles =
-      kv_slots(a.seqs, a.group, kRows, 1, each_tiles(a, kRows)) * a.pool.heads;
-  const uint64_t tokens = uint64_t(a.seqs.max_blocks) << a.pool.shift;
-  const uint64_t span =
-      a.window == 0 ? tokens : std::min<uint64_t>(tokens, uint64_t(a.window) + kRows / a.group + 32);
-  const uint64_t split = tiles < cus ? cus / tiles : 1;
-  const uint64_t part = std::max<uint64_t>((span + split - 1) / split, kPartLeast4);
-  const uint64_t most = kv_part_limit(kWave, a.pool.shift, a.window) / 64 * 64;
-  p.part_tokens = uint32_t(std::min<uint64_t>((part + 63) / 64 * 64, most));
-  p.parts = uint32_t((span + p.part_tokens - 1) / p.part_tokens);
-  p.one_tile = rows_of_head <= uint64_t(kRows) * a.seqs.batch;
-  p.grid = tiles * p.parts;
-  p.waves = p.grid <= uint64_t(cus) * 64 / dim ? 8 : 4;
-  uint64_t bytes = 0;
-  scratch_of(a, dim, p, nullptr, &bytes);
-  p.workspace = bytes;
+  KvAttendPlan p = plan_kv_attend(a, dim);
+  // A wave has half the bytes on their way that it has with 8 bits: eight waves
+  // where a workgroup has a compute unit to itself, for 128 dims too (131072
+  // tokens of 8 heads: 25.5 us, four waves 31.9; 16 sequences of up to 8192
+  // 22.6, 30.6).
+  p.waves = p.grid <= device_cu_count() ? 8 : 4;
   return p;
 }
 
@@ -395,17 +644,22 @@ static hipError_t launch_attend4(const KvAttendArgs &a, const KvAttendPlan &p, v
       kernel4<<<uint32_t(p.grid), 4 * kWave, 0, s>>>(a, x, each);
     }
   };
-  if (p.one_tile) {
+  if (p.kernel == ULLM_KV_KERNEL_MANY_ROWS) {
+    const bool longer = p.part_tokens > kv_part_limit(kManyBlocks, a.pool.shift, a.window);
+    const auto kernel = longer ? many_rows4_kernel<D, true> : many_rows4_kernel<D, false>;
+    kernel<<<uint32_t(p.grid), kWaves * kWave, Many4<D>::kLds, s>>>(a, x, each);
+  } else if (x.scores != nullptr) {
+    few(few_rows4_kernel<D, 8, true, true>, few_rows4_kernel<D, 4, true, true>);
+  } else if (p.one_tile) {
     few(few_rows4_kernel<D, 8, true, false>, few_rows4_kernel<D, 4, true, false>);
   } else {
     few(few_rows4_kernel<D, 8, false, false>, few_rows4_kernel<D, 4, false, false>);
   }
   launch_join_parts(a, D, p, x, s);
-  if (a.accumulate) {
-    const uint64_t tokens = uint64_t(a.seqs.max_blocks) << a.pool.shift;
-    const dim3 grid(uint32_t((tokens + 32 * kWaves - 1) / (32 * kWaves)), a.pool.heads,
-                    a.seqs.batch);
-    add_weights4_kernel<D><<<grid, kWaves * kWave, 0, s>>>(a, x.stats);
+  if (a.accumulate && x.scores != nullptr) {
+    launch_add_scores(a, x, s);
+  } else if (a.accumulate) {
+    launch_add_weights(add_weights_kernel<WeightKeys4<D>>, a, D, x.stats, s);
   }
   return hipGetLastError();
 }
