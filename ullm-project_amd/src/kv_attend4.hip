@@ -96,16 +96,16 @@ __device__ __forceinline__ uint32_t scaled_weights(float p0, float p1, uint32_t 
   return __builtin_bit_cast(uint32_t, h2{_Float16(__builtin_fmaf(p0, float(s[0]), 0.f)),
                                          _Float16(__builtin_fmaf(p1, float(s[1]), 0.f))});
 }
-// The larger of two pairs of f16, NaN passed over.
-__device__ __forceinline__ uint32_t max_f16(uint32_t a, uint32_t b) {
-  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(h2, a),
-                                                                __builtin_bit_cast(h2, b)));
+// The larger of two pairs of scales, of which NaN is the largest.
+__device__ __forceinline__ uint32_t max_scales(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a),
+                                                                __builtin_bit_cast(u16x2, b)));
 }
-// log2 of the larger of two scales, or of the smallest there is.
+// log2 of the larger of two scales, at least of the smallest there is; of NaN
+// that of the largest.
 __device__ __forceinline__ float largest_log2(uint32_t scales) {
-  const float s = fmaxf(f16_to_f32(uint16_t(scales)), f16_to_f32(uint16_t(scales >> 16)));
-  return __builtin_amdgcn_logf(fmaxf(s, kScaleLeast));
+  const uint32_t most = min(max(scales & 0xffffu, scales >> 16), uint32_t(kScaleMostBits));
+  return __builtin_amdgcn_logf(fmaxf(f16_to_f32(uint16_t(most)), kScaleLeast));
 }
 // Whether one of eight scales is NaN.
 __device__ __forceinline__ bool any_nan(u32x4 scales) {
@@ -171,7 +171,7 @@ __device__ __forceinline__ void attend_group4(RowState4<D> &st, Group4<D> &x, co
     top = fmaxf(top, s[i / 4][i % 4]);
   }
   const uint32_t most =
-      max_f16(max_f16(x.scales.x, x.scales.y), max_f16(x.scales.z, x.scales.w));
+      max_scales(max_scales(x.scales.x, x.scales.y), max_scales(x.scales.z, x.scales.w));
   if (__any(top + largest_log2(most) > st.m + kSlack)) {
     float now = -INFINITY;
 #pragma unroll
@@ -479,9 +479,6 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows4_kernel(KvAttendA
 #pragma unroll
       for (uint32_t c = 0; c < D / 16; ++c) {
         s = mfma32_bf16(codes4_to_bf16(keys[c / 4][c % 4], power[c / 4]), q[c], s);
-        if (c % 2 == 1) {
-          __builtin_amdgcn_sched_barrier(0);
-        }
       }
       u32x4 scales[2], values[2];
 #pragma unroll
@@ -495,16 +492,22 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows4_kernel(KvAttendA
         }
       }
       const uint32_t gone = absent >> u << 31;
-      const bool edge = ((grp - whole.first) | gone) >= whole.count;
-      const auto seen = [&](int e) {
-        const int32_t at =
-            int32_t(grp * 32) + int32_t((e / 4 % 2) * 16 + e / 8 * 8 + 4 * h + e % 4);
-        return gone == 0 && at <= pos && at > oldest;
-      };
-      if (edge) {
+      if (((grp - whole.first) | gone) >= whole.count) {
+        const auto seen = [&](int e) {
+          const int32_t at =
+              int32_t(grp * 32) + int32_t((e / 4 % 2) * 16 + e / 8 * 8 + 4 * h + e % 4);
+          return gone == 0 && at <= pos && at > oldest;
+        };
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           s[e] = seen(e) ? s[e] : -INFINITY;
+        }
+        if (__any(any_nan(scales[0]) || any_nan(scales[1]))) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const uint32_t w = scales[e / 8][e % 8 / 2];
+            scales[e / 8][e % 8 / 2] = seen(e) ? w : w & (e % 2 == 0 ? 0xffff0000u : 0x0000ffffu);
+          }
         }
       }
       float top = s[0];
@@ -512,10 +515,10 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows4_kernel(KvAttendA
       for (int e = 1; e < 16; ++e) {
         top = fmaxf(top, s[e]);
       }
-      const uint32_t most = max_f16(max_f16(max_f16(scales[0].x, scales[0].y),
-                                            max_f16(scales[0].z, scales[0].w)),
-                                    max_f16(max_f16(scales[1].x, scales[1].y),
-                                            max_f16(scales[1].z, scales[1].w)));
+      const uint32_t most = max_scales(max_scales(max_scales(scales[0].x, scales[0].y),
+                                            max_scales(scales[0].z, scales[0].w)),
+                                    max_scales(max_scales(scales[1].x, scales[1].y),
+                                            max_scales(scales[1].z, scales[1].w)));
       if (__any(__builtin_fmaf(top, a.scale_log2, largest_log2(most)) > limit)) {
         float now = -INFINITY;
 #pragma unroll
@@ -547,13 +550,6 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows4_kernel(KvAttendA
         p[e / 8][e % 8 / 2] = scaled_weights(p0, p1, scales[e / 8][e % 8 / 2]);
       }
       l += sum;
-      if (edge && __any(any_nan(scales[0]) || any_nan(scales[1]))) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const uint32_t w = p[e / 8][e % 8 / 2];
-          p[e / 8][e % 8 / 2] = seen(e) ? w : w & (e % 2 == 0 ? 0xffff0000u : 0x0000ffffu);
-        }
-      }
 #pragma unroll
       for (uint32_t c = 0; c < 2; ++c) {
         const f16x8 b = __builtin_bit_cast(f16x8, p[c]);

@@ -59,6 +59,7 @@ __host__ __device__ constexpr uint32_t kv4_scale_byte(uint32_t t) {
 
 constexpr uint32_t kKv4ExpNan = 255;
 constexpr float kScaleLeast = 0x1p-19f, kScaleMost = 64512.f;  // of values
+constexpr uint16_t kScaleMostBits = 0x7be0;                    // in f16
 
 // Eight codes as bf16 operands, times a power of two (NaN where its exponent is
 // that of infinity); as f16 operands.
