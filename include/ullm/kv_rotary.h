@@ -17,9 +17,9 @@
  * each pair's axis.
  *
  * Angles are reduced to a turn, and pairs rotated, in 64 bits: position
- * 2^31 - 1 is as exact as position 1.  Queries are rounded to bf16 once (below
- * 2^-126 by way of f32); keys go from the product in 64 bits to their codes, in
- * caches of 8 and of 4 bits.
+ * 2^31 - 1 is as exact as position 1.  Queries are rounded to f32 and then to
+ * bf16; keys go from the product in 64 bits to their codes, in caches of 8 and of
+ * 4 bits.
  *
  * Every row that a sequence owns has its queries rotated, rows that name no
  * token among them (their place is negative); rows that no sequence owns are

@@ -2,18 +2,24 @@
 rotation with exactly reduced angles (kv_reference4.py).
 
 Rotated queries and stored keys are compared bit for bit: both are rounded
-once from the rotation in 64 bits, whose error of some 2^-52 meets a border of
-two bf16 or two codes with a probability of some 2^-40 for an element."""
+from the rotation in 64 bits, queries to f32 and to bf16, keys to codes.  Its
+error of some 2^-52 meets a border of two floats or two codes with a
+probability of some 2^-28 or 2^-40 for an element."""
 import numpy as np
 import pytest
 import torch
 
 import test_gpu_kv4_cache as T4
 import test_gpu_kv_cache as T8
-from kv_reference4 import rotate, to_bf16
+from kv_reference4 import rotate, to_bf16 as round_bf16
 from test_gpu_kv_cache import f64, same
 
 pytestmark = pytest.mark.gpu
+
+
+def to_bf16(x):
+    with np.errstate(over="ignore"):
+        return round_bf16(x.astype(np.float32).astype(np.float64))
 
 
 def pair(bits, *a, **kw):
@@ -163,7 +169,7 @@ def test_extremes(uh, gpu, bits):
         x[3, 0, 5], x[4, 1, 40], x[5, 0, 127] = float("inf"), float("-inf"), float("nan")
         x[6, 0, 100] = float("inf")                   # a dim that is not rotated
         x[10:20] = (3.38e38 * torch.sign(x[10:20].float())).bfloat16()
-        x[20:30] = (x[20:30].float() * 1e-35).bfloat16()
+        x[20:30] = (x[20:30].float() * 1e-38).bfloat16()
         x[30:40] = 0
         x[64, 0, 0], x[64, 0, 32] = float("inf"), 1.0  # position 0: cosine 1, sine 0
     with np.errstate(invalid="ignore", over="ignore"):

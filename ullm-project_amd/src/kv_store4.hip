@@ -100,9 +100,28 @@ struct Span {
   uint32_t lo, hi;
 };
 
-// Cosines and sines of the span's rows and of all pairs.
+// A thread's part of a span's rows: token t, pairs 8u .. 8u + 7, of heads `head`,
+// `head` + step and so on; none where `head` is none.
+constexpr uint32_t kNoHead = ~0u;
+struct Lot {
+  uint32_t t, u, head, step;
+};
 template <int D>
-__device__ __forceinline__ void span_turns(const KvRotary &r, const Span &s, Turn (*turns)[D / 2]) {
+__device__ __forceinline__ Lot lot_of(const Span &s) {
+  constexpr uint32_t kUnits = D / 16;
+  const uint32_t n = (s.hi - s.lo) * kUnits, step = kThreads / n;
+  const uint32_t head = threadIdx.x / n, i = threadIdx.x % n;
+  return {s.lo + i / kUnits, i % kUnits, head < step ? head : kNoHead, step};
+}
+
+// Cosines and sines of a span: pair j of token t is at [t][j % 8][j / 8], where
+// the threads that read a pair each lie side by side.
+template <int D>
+struct SpanTurns {
+  Turn at[32][8][D / 16];
+};
+template <int D>
+__device__ __forceinline__ void span_turns(const KvRotary &r, const Span &s, SpanTurns<D> *turns) {
   const uint32_t j = threadIdx.x % (D / 2);
   if (j >= r.dims / 2) {
     return;
@@ -111,79 +130,92 @@ __device__ __forceinline__ void span_turns(const KvRotary &r, const Span &s, Tur
   const uint32_t axis = r.pair_axes == nullptr ? 0u : min(uint32_t(r.pair_axes[j]), r.axes - 1);
   const int32_t *at = r.positions + axis * r.position_stride;
   for (uint32_t t = s.lo + threadIdx.x / (D / 2); t < s.hi; t += kThreads / (D / 2)) {
-    turns[t][j] = turn_of(r.positions == nullptr ? int32_t(s.base + t) : at[s.row0 + t], f);
+    turns->at[t][j % 8][j / 8] =
+        turn_of(r.positions == nullptr ? int32_t(s.base + t) : at[s.row0 + t], f);
   }
 }
 
-// Eight pairs (8u ..) of a row, rotated; where[] are their dims.
-template <int D>
-struct Pairs {
-  float first[8], second[8];
+// Eight pairs of a row as they lie in memory: two runs of eight dims, or one of
+// sixteen (`side`: a pair's elements side by side).
+struct RawPairs {
+  u32x4 a, b;
 };
-// Whether eight pairs are two runs of eight dims, or one of sixteen, that start
-// at multiples of eight.
-__device__ __forceinline__ bool pairs_in_runs(const KvRotary &r) {
-  return r.interleaved || r.dims % 16 == 0;
+// Where that is so: pairs of neighbours, dims past the rotated ones among them.
+__device__ __forceinline__ bool side_by_side(const KvRotary &r, uint32_t u, bool runs) {
+  return runs && (r.interleaved || 8 * u >= r.dims / 2);
 }
-__device__ __forceinline__ bool neighbours(const KvRotary &r, uint32_t u) {
-  return r.interleaved || 8 * u >= r.dims / 2;
-}
-template <int D>
-__device__ __forceinline__ Pairs<D> load_pairs(const uint16_t *row, const KvRotary &r, uint32_t u,
-                                               bool vec) {
-  Pairs<D> p;
-  if (vec && pairs_in_runs(r)) {
+__device__ __forceinline__ RawPairs load_pairs(const uint16_t *row, const KvRotary &r, uint32_t u,
+                                               bool runs) {
+  RawPairs p;
+  if (runs) {
     const PairDims d = pair_dims(8 * u, r.dims, r.interleaved);
-    const bool side = neighbours(r, u);
-    const u32x4 a = *reinterpret_cast<const u32x4 *>(row + d.first);
-    const u32x4 b = *reinterpret_cast<const u32x4 *>(row + (side ? d.first + 8 : d.second));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t near = i < 4 ? a[i % 4] : b[i % 4];
-      const uint32_t x = side ? near << 16 : i % 2 == 0 ? a[i / 2] << 16 : a[i / 2] & 0xffff0000u;
-      const uint32_t y = side           ? near & 0xffff0000u
-                         : i % 2 == 0 ? b[i / 2] << 16
-                                      : b[i / 2] & 0xffff0000u;
-      p.first[i] = bits_f32(x);
-      p.second[i] = bits_f32(y);
-    }
+    p.a = *reinterpret_cast<const u32x4 *>(row + d.first);
+    p.b = *reinterpret_cast<const u32x4 *>(
+        row + (side_by_side(r, u, runs) ? d.first + 8 : d.second));
   } else {
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
+    for (uint32_t i = 0; i < 8; i += 2) {
       const PairDims d = pair_dims(8 * u + i, r.dims, r.interleaved);
-      p.first[i] = bf16_to_f32(row[d.first]);
-      p.second[i] = bf16_to_f32(row[d.second]);
+      const PairDims e = pair_dims(8 * u + i + 1, r.dims, r.interleaved);
+      p.a[i / 2] = row[d.first] | uint32_t(row[e.first]) << 16;
+      p.b[i / 2] = row[d.second] | uint32_t(row[e.second]) << 16;
     }
   }
   return p;
 }
+
+// A thread's eight turns, and which of its pairs they are for.
+struct Turns8 {
+  Turn w[8];
+  uint32_t live;
+};
 template <int D>
-__device__ __forceinline__ void rotate_pairs(Pairs<D> &p, const KvRotary &r, uint32_t u,
-                                             const Turn *turns) {
+__device__ __forceinline__ Turns8 load_turns(const SpanTurns<D> &turns, const KvRotary &r,
+                                             const Lot &lot) {
+  Turns8 v;
+  const uint32_t pairs = r.dims / 2, first = 8 * lot.u;
+  v.live = first >= pairs ? 0u : pairs - first >= 8 ? 0xffu : (1u << (pairs - first)) - 1;
 #pragma unroll
   for (uint32_t i = 0; i < 8; ++i) {
-    const uint32_t j = 8 * u + i;
-    if (j < r.dims / 2) {
-      const Turn w = turns[j];
-      const double x = p.first[i], y = p.second[i];
-      p.first[i] = to_odd(fma(x, w.c, -(y * w.s)));
-      p.second[i] = to_odd(fma(y, w.c, x * w.s));
-    }
+    v.w[i] = turns.at[lot.t][i][lot.u];
   }
+  return v;
 }
-template <int D>
-__device__ __forceinline__ void store_pairs(uint16_t *row, const Pairs<D> &p, const KvRotary &r,
-                                            uint32_t u, bool vec) {
-  if (vec && pairs_in_runs(r)) {
+
+// Pair i, rotated: both its elements as ROUND makes a float of a double.
+template <typename ROUND>
+__device__ __forceinline__ void rotate_pair(const RawPairs &p, bool side, const Turns8 &v, int i,
+                                            float &first, float &second, ROUND round) {
+  const uint32_t near = i < 4 ? p.a[i % 4] : p.b[i % 4];
+  const uint32_t far0 = p.a[i / 2], far1 = p.b[i / 2];
+  const uint32_t x = side ? near << 16 : i % 2 == 0 ? far0 << 16 : far0 & 0xffff0000u;
+  const uint32_t y = side           ? near & 0xffff0000u
+                     : i % 2 == 0 ? far1 << 16
+                                  : far1 & 0xffff0000u;
+  const double dx = bits_f32(x), dy = bits_f32(y);
+  const bool live = (v.live >> i & 1u) != 0;
+  const float rx = round(fma(dx, v.w[i].c, -(dy * v.w[i].s)));
+  const float ry = round(fma(dy, v.w[i].c, dx * v.w[i].s));
+  first = live ? rx : bits_f32(x);
+  second = live ? ry : bits_f32(y);
+}
+
+// A query's eight pairs, rotated, to their place.
+__device__ __forceinline__ void rotate_query(uint16_t *row, const RawPairs &p, const KvRotary &r,
+                                             const Turns8 &v, uint32_t u, bool runs) {
+  const bool side = side_by_side(r, u, runs);
+  float x[8], y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    rotate_pair(p, side, v, i, x[i], y[i], [](double d) { return float(d); });
+  }
+  if (runs) {
     const PairDims d = pair_dims(8 * u, r.dims, r.interleaved);
-    const bool side = neighbours(r, u);
     u32x4 a, b;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const auto pair = [](float x, float y) { return f32x2_to_bf16x2(x, y); };
-      a[i] = side ? pair(p.first[i], p.second[i]) : pair(p.first[2 * i], p.first[2 * i + 1]);
-      b[i] = side ? pair(p.first[4 + i], p.second[4 + i])
-                  : pair(p.second[2 * i], p.second[2 * i + 1]);
+      a[i] = side ? f32x2_to_bf16x2(x[i], y[i]) : f32x2_to_bf16x2(x[2 * i], x[2 * i + 1]);
+      b[i] = side ? f32x2_to_bf16x2(x[4 + i], y[4 + i]) : f32x2_to_bf16x2(y[2 * i], y[2 * i + 1]);
     }
     *reinterpret_cast<u32x4 *>(row + d.first) = a;
     *reinterpret_cast<u32x4 *>(row + (side ? d.first + 8 : d.second)) = b;
@@ -191,8 +223,8 @@ __device__ __forceinline__ void store_pairs(uint16_t *row, const Pairs<D> &p, co
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
       const PairDims d = pair_dims(8 * u + i, r.dims, r.interleaved);
-      row[d.first] = f32_to_bf16(p.first[i]);
-      row[d.second] = f32_to_bf16(p.second[i]);
+      row[d.first] = f32_to_bf16(x[i]);
+      row[d.second] = f32_to_bf16(y[i]);
     }
   }
 }
@@ -202,49 +234,86 @@ template <int D>
 struct KeyImage {
   alignas(16) float x[32][D + 4];
 };
-
-// The span's queries of a key/value head's group, rotated to their place, and
-// its keys, rotated into LDS (where the span has tokens in the cache).
 template <int D>
-__device__ __forceinline__ void rotate_span(const KvRotateArgs &a, const Span &s, uint32_t head,
-                                            const Turn (*turns)[D / 2], KeyImage<D> *keys) {
-  constexpr uint32_t kUnits = D / 16;
-  const uint32_t n = s.hi - s.lo, heads = a.group + (keys != nullptr ? 1u : 0u);
-  for (uint32_t i = threadIdx.x; i < heads * n * kUnits; i += kThreads) {
-    const uint32_t u = i % kUnits, h = i / kUnits / n, t = s.lo + i / kUnits % n;
-    const uint64_t row = uint64_t(s.row0 + t);
-    if (h < a.group) {
-      const uint32_t qh = head * a.group + h;
-      Pairs<D> p = load_pairs<D>(a.q + row * a.q_row + qh * a.q_head, a.rotary, u, a.q_vec);
-      rotate_pairs<D>(p, a.rotary, u, turns[t]);
-      store_pairs<D>(a.q_out + row * a.out_row + qh * a.out_head, p, a.rotary, u, a.q_vec);
-    } else {
-      Pairs<D> p = load_pairs<D>(a.append.k + row * a.append.k_row + head * a.append.k_head,
-                                 a.rotary, u, a.append.vec);
-      rotate_pairs<D>(p, a.rotary, u, turns[t]);
+__device__ __forceinline__ void rotate_key(KeyImage<D> *to, const RawPairs &p, const KvRotary &r,
+                                           const Turns8 &v, const Lot &lot, bool runs) {
+  const bool side = side_by_side(r, lot.u, runs);
 #pragma unroll
-      for (uint32_t e = 0; e < 8; ++e) {
-        const PairDims d = pair_dims(8 * u + e, a.rotary.dims, a.rotary.interleaved);
-        keys->x[t][d.first] = p.first[e];
-        keys->x[t][d.second] = p.second[e];
-      }
-    }
+  for (int i = 0; i < 8; ++i) {
+    const PairDims d = pair_dims(8 * lot.u + uint32_t(i), r.dims, r.interleaved);
+    rotate_pair(p, side, v, i, to->x[lot.t][d.first], to->x[lot.t][d.second],
+                [](double x) { return to_odd(x); });
   }
 }
 
+// A span on its way: the first loads of keys and queries, issued before their
+// turns are known.
+constexpr uint32_t kAheadHeads = 4;
+template <int D>
+struct Rotation {
+  const KvRotateArgs &a;
+  const Span &s;
+  uint32_t head;  // key/value head
+  Lot lot;
+  bool k_runs, q_runs;
+  RawPairs key, query[kAheadHeads];
+
+  __device__ __forceinline__ Rotation(const KvRotateArgs &args, const Span &span, uint32_t kvh,
+                                      bool keys)
+      : a(args), s(span), head(kvh), lot(lot_of<D>(span)) {
+    const bool runs = a.rotary.interleaved || a.rotary.dims % 16 == 0;
+    k_runs = runs && a.append.vec;
+    q_runs = runs && a.q_vec;
+    if (keys && lot.head == 0) {
+      key = load_pairs(a.append.k + row() * a.append.k_row + head * a.append.k_head, a.rotary,
+                       lot.u, k_runs);
+    }
+    load_queries(lot.head);
+  }
+  __device__ __forceinline__ uint64_t row() const { return uint64_t(s.row0 + lot.t); }
+  __device__ __forceinline__ uint64_t query_head(uint32_t h) const { return head * a.group + h; }
+  __device__ __forceinline__ void load_queries(uint32_t h) {
+#pragma unroll
+    for (uint32_t i = 0; i < kAheadHeads; ++i, h += lot.step) {
+      if (lot.head != kNoHead && h < a.group) {
+        query[i] = load_pairs(a.q + row() * a.q_row + query_head(h) * a.q_head, a.rotary, lot.u,
+                              q_runs);
+      }
+    }
+  }
+  __device__ __forceinline__ void queries(const Turns8 &v) {
+    for (uint32_t h = lot.head; lot.head != kNoHead && h < a.group;) {
+#pragma unroll
+      for (uint32_t i = 0; i < kAheadHeads; ++i, h += lot.step) {
+        if (h < a.group) {
+          rotate_query(a.q_out + row() * a.out_row + query_head(h) * a.out_head, query[i],
+                       a.rotary, v, lot.u, q_runs);
+        }
+      }
+      load_queries(h);
+    }
+  }
+};
+
 // --------------------------------------------------------------- append, 4 bits
 
-// One workgroup stores the new tokens among 32 of one head.  Keys go from
-// memory, or rotated from LDS, to their codes and memory; values' codes are
-// brought into dwords of eight tokens in LDS.  A dword that new tokens share
-// with earlier ones is read and written by this workgroup alone.
+// One workgroup stores the new tokens among 32 of one head, and rotates the
+// queries of its group.  A thread has the same eight pairs of the same token in
+// all heads, so that it reads their turns once.  Keys go from memory, or rotated
+// from LDS, to their codes and memory; values' codes are brought into dwords of
+// eight tokens in LDS.  A dword that new tokens share with earlier ones is read
+// and written by this workgroup alone.
 template <int D, bool ROTATE>
 __global__ __launch_bounds__(kThreads) void append4_kernel(KvRotateArgs ra, uint32_t each_slots) {
   using Chunk = Kv4Chunk<D>;
   constexpr uint32_t kUnits = D / 16, kPitch = D + 16;
-  __shared__ Turn turns[ROTATE ? 32 : 1][D / 2];
-  __shared__ KeyImage<ROTATE ? D : 4> rotated;
-  __shared__ __align__(16) uint8_t values[32 * kPitch];  // a code to a byte
+  // Turns, and when all threads have theirs, keys and values.
+  constexpr uint32_t kImage = ROTATE ? sizeof(KeyImage<D>) : 0;
+  constexpr uint32_t kLds = kImage + 32 * kPitch;
+  __shared__ __align__(16) uint8_t lds[ROTATE && sizeof(SpanTurns<D>) > kLds ? sizeof(SpanTurns<D>)
+                                                                             : kLds];
+  KeyImage<D> *const rotated = reinterpret_cast<KeyImage<D> *>(lds);
+  uint8_t *const values = lds + kImage;  // a code to a byte
   const KvAppendArgs &a = ra.append;
   const uint32_t head = blockIdx.y, tid = threadIdx.x;
   const KvSlot slot = kv_find_slot(a.seqs, blockIdx.x, 1, 32, 2, each_slots);
@@ -265,35 +334,48 @@ __global__ __launch_bounds__(kThreads) void append4_kernel(KvRotateArgs ra, uint
   const int32_t id = s.base < 0 ? -1
                                 : kv_block(a.seqs.tables + slot.seq * a.seqs.stride, a.seqs,
                                            a.pool.blocks, uint32_t(s.base) >> a.pool.shift);
+  // This thread's unit, of at most 256: token t, dims 16c .. 16c + 15.
+  const uint32_t t = s.lo + tid / kUnits, c = tid % kUnits;
+  const bool live = t < s.hi && id >= 0;
+  const uint64_t row = uint64_t(s.row0 + (live ? t : s.lo));
+  const Bf16x16 raw_value = load16(a.v + head * a.v_head + row * a.v_row + c * 16, a.vec);
+  float k[16], v[16];
   if constexpr (ROTATE) {
+    Rotation<D> rotation(ra, s, head, id >= 0);
+    SpanTurns<D> *const turns = reinterpret_cast<SpanTurns<D> *>(lds);
     span_turns<D>(ra.rotary, s, turns);
     __syncthreads();
-    rotate_span<D>(ra, s, head, turns, id < 0 ? nullptr : &rotated);
+    const Turns8 mine = load_turns<D>(*turns, ra.rotary, rotation.lot);
     __syncthreads();
-  }
-  if (id < 0) {
-    return;
-  }
-  const uint32_t in_block = uint32_t(s.base) & ((1u << a.pool.shift) - 1);
-  const uint64_t unit = uint64_t(id) * a.pool.heads + head;
-  uint8_t *chunk = kv4_chunk<D>(a.pool, unit, in_block);
-  for (uint32_t i = tid; i < (s.hi - s.lo) * kUnits; i += kThreads) {
-    const uint32_t t = s.lo + i / kUnits, c = i % kUnits;
-    const uint64_t row = uint64_t(s.row0 + t);
-    float k[16], v[16];
-    if constexpr (ROTATE) {
+    if (id >= 0 && rotation.lot.head == 0) {
+      rotate_key<D>(rotated, rotation.key, ra.rotary, mine, rotation.lot, rotation.k_runs);
+    }
+    rotation.queries(mine);
+    if (id < 0) {
+      return;
+    }
+    __syncthreads();
+    if (live) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const f32x4 w = *reinterpret_cast<const f32x4 *>(&rotated.x[t][c * 16 + 4 * j]);
+        const f32x4 w = *reinterpret_cast<const f32x4 *>(&rotated->x[t][c * 16 + 4 * j]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           k[4 * j + e] = w[e];
         }
       }
-    } else {
-      unpack16(load16(a.k + head * a.k_head + row * a.k_row + c * 16, a.vec), k);
     }
-    unpack16(load16(a.v + head * a.v_head + row * a.v_row + c * 16, a.vec), v);
+  } else {
+    if (id < 0) {
+      return;
+    }
+    unpack16(load16(a.k + head * a.k_head + row * a.k_row + c * 16, a.vec), k);
+  }
+  const uint32_t in_block = uint32_t(s.base) & ((1u << a.pool.shift) - 1);
+  const uint64_t unit = uint64_t(id) * a.pool.heads + head;
+  uint8_t *chunk = kv4_chunk<D>(a.pool, unit, in_block);
+  if (live) {
+    unpack16(raw_value, v);
     const uint32_t e = key_exp4(largest16<2>(k));
     *reinterpret_cast<u32x2 *>(chunk + kv4_key_byte<D>(t, c * 16)) = encode4(k, exp4_power(e));
     if (c % 2 == 0) {
@@ -315,26 +397,33 @@ __global__ __launch_bounds__(kThreads) void append4_kernel(KvRotateArgs ra, uint
     }
   }
   __syncthreads();
-  for (uint32_t i = tid; i < 4 * D; i += kThreads) {
-    const uint32_t g = i / D, d = i % D;
-    uint32_t w = 0, fresh = 0;
+  // Two dwords of a lane's four to a thread: dims d and d + 16 of eight tokens.
+  for (uint32_t i = tid; i < 2 * D; i += kThreads) {
+    const uint32_t g = i / (D / 2), d = i % (D / 2) / 16 * 32 + i % 16;
+    uint32_t fresh = 0;
+    u32x2 w = {0u, 0u};
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j) {
-      const uint32_t t = 4 * g + j % 4 + 16 * (j / 4);
-      const bool is_new = t >= s.lo && t < s.hi;
-      const uint32_t code = is_new ? values[t * kPitch + d] : 0u;
-      w |= code << (4 * j);
+      const uint32_t of = 4 * g + j % 4 + 16 * (j / 4);
+      const bool is_new = of >= s.lo && of < s.hi;
+      const uint8_t *from = values + of * kPitch + d;
+      w.x |= (is_new ? from[0] : 0u) << (4 * j);
+      w.y |= (is_new ? from[16] : 0u) << (4 * j);
       fresh |= is_new ? 15u << (4 * j) : 0u;
     }
     if (fresh != 0) {
-      uint32_t *at = reinterpret_cast<uint32_t *>(chunk + Chunk::kSide + kv4_value_dword(g, d));
-      *at = fresh == ~0u ? w : w | (*at & ~fresh);
+      u32x2 *at = reinterpret_cast<u32x2 *>(chunk + Chunk::kSide + kv4_value_dword(g, d));
+      if (fresh != ~0u) {
+        const u32x2 old = *at;
+        w = u32x2{w.x | (old.x & ~fresh), w.y | (old.y & ~fresh)};
+      }
+      *at = w;
     }
   }
   if (a.pool.weights != nullptr) {
-    for (uint32_t t = s.lo + tid; t < s.hi; t += kThreads) {
-      a.pool.weights[(unit << a.pool.shift) + in_block + t] =
-          a.weights != nullptr ? a.weights[uint64_t(s.row0 + t) * a.pool.heads + head] : 0.f;
+    for (uint32_t i = s.lo + tid; i < s.hi; i += kThreads) {
+      a.pool.weights[(unit << a.pool.shift) + in_block + i] =
+          a.weights != nullptr ? a.weights[uint64_t(s.row0 + i) * a.pool.heads + head] : 0.f;
     }
   }
 }
@@ -348,9 +437,13 @@ __global__ __launch_bounds__(kThreads) void append8_rotary_kernel(KvRotateArgs r
                                                                   uint32_t each_slots) {
   constexpr uint32_t kUnits = D / 16, kSpans = bt / 32;
   constexpr uint32_t kEach = (32 * kUnits + kThreads - 1) / kThreads;  // of a thread and span
-  __shared__ Turn turns[32][D / 2];
-  __shared__ KeyImage<D> rotated;
-  __shared__ __align__(16) uint8_t image[bt * D];
+  // Turns, and when all threads have theirs, rotated keys; at the end values.
+  constexpr uint32_t kFirst = sizeof(SpanTurns<D>) > sizeof(KeyImage<D>) ? sizeof(SpanTurns<D>)
+                                                                         : sizeof(KeyImage<D>);
+  __shared__ __align__(16) uint8_t lds[kFirst > bt * D ? kFirst : bt * D];
+  SpanTurns<D> *const turns = reinterpret_cast<SpanTurns<D> *>(lds);
+  KeyImage<D> *const rotated = reinterpret_cast<KeyImage<D> *>(lds);
+  uint8_t *const image = lds;
   const KvAppendArgs &a = ra.append;
   const uint32_t head = blockIdx.y, tid = threadIdx.x;
   const KvSlot slot = kv_find_slot(a.seqs, blockIdx.x, 1, bt, 2, each_slots);
@@ -385,10 +478,18 @@ __global__ __launch_bounds__(kThreads) void append8_rotary_kernel(KvRotateArgs r
     s.lo = lo > 32 * p ? min(lo - 32 * p, 32u) : 0u;
     s.hi = hi > 32 * p ? min(hi - 32 * p, 32u) : 0u;
     s.lo = min(s.lo, s.hi);
-    span_turns<D>(ra.rotary, s, turns);
-    __syncthreads();
-    rotate_span<D>(ra, s, head, turns, id < 0 ? nullptr : &rotated);
-    __syncthreads();
+    if (s.lo < s.hi) {  // the same for all threads
+      Rotation<D> rotation(ra, s, head, id >= 0);
+      span_turns<D>(ra.rotary, s, turns);
+      __syncthreads();
+      const Turns8 mine = load_turns<D>(*turns, ra.rotary, rotation.lot);
+      __syncthreads();
+      if (id >= 0 && rotation.lot.head == 0) {
+        rotate_key<D>(rotated, rotation.key, ra.rotary, mine, rotation.lot, rotation.k_runs);
+      }
+      rotation.queries(mine);
+      __syncthreads();
+    }
 #pragma unroll
     for (uint32_t r = 0; r < kEach; ++r) {
       const uint32_t t = token(r), i = p * kEach + r;
@@ -400,7 +501,7 @@ __global__ __launch_bounds__(kThreads) void append8_rotary_kernel(KvRotateArgs r
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const f32x4 w =
-            *reinterpret_cast<const f32x4 *>(&rotated.x[live ? t : 0][c * 16 + 4 * j]);
+            *reinterpret_cast<const f32x4 *>(&rotated->x[live ? t : 0][c * 16 + 4 * j]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           x[i][4 * j + e] = live ? w[e] : 0.f;
