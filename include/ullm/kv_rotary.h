@@ -16,10 +16,11 @@
  * example the time, height and width of an image's patch.  `pair_axes` names
  * each pair's axis.
  *
- * Angles are reduced to a turn, and pairs rotated, in 64 bits: position
- * 2^31 - 1 is as exact as position 1.  Queries are rounded to f32 and then to
- * bf16; keys go from the product in 64 bits to their codes, in caches of 8 and of
- * 4 bits.
+ * Angles are reduced to a turn, and their cosines and sines taken, in 64 bits:
+ * position 2^31 - 1 is as exact as position 1.  Queries are then rotated in f32
+ * and rounded to bf16.  Keys are rotated in 64 bits and rounded once, to their
+ * codes (in caches of 8 and of 4 bits), so that a key between two codes does not
+ * depend on the last bits of an f32.
  *
  * Every row that a sequence owns has its queries rotated, rows that name no
  * token among them (their place is negative); rows that no sequence owns are

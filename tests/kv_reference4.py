@@ -146,11 +146,3 @@ def rotate(x, positions, inv_freq, pair_axes=None, interleaved=False):
         y[..., second] = w * np.cos(a) + u * np.sin(a)
     return y
 
-
-def to_bf16(x):
-    """Float64 rounded once to bf16 (ties to even), as float64."""
-    m, e = np.frexp(x)
-    q = np.ldexp(1.0, np.maximum(e, -125) - 8)
-    with np.errstate(invalid="ignore", over="ignore"):
-        r = np.round(x / q) * q
-    return np.where(np.isfinite(x), np.where(np.abs(r) >= 2.0 ** 128, np.copysign(np.inf, x), r), x)

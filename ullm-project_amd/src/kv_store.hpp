@@ -154,8 +154,9 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
   return v;
 }
 // Maxima of two values over the workgroup.
+template <uint32_t THREADS = kThreads>
 __device__ __forceinline__ void block_umax2(uint32_t &a, uint32_t &b) {
-  __shared__ uint32_t red[2][kThreads / kWave];
+  __shared__ uint32_t red[2][THREADS / kWave];
   a = wave_umax(a);
   b = wave_umax(b);
   if (threadIdx.x % kWave == 0) {
@@ -163,7 +164,7 @@ __device__ __forceinline__ void block_umax2(uint32_t &a, uint32_t &b) {
     red[1][threadIdx.x / kWave] = b;
   }
   __syncthreads();
-  for (uint32_t i = 0; i < kThreads / kWave; ++i) {
+  for (uint32_t i = 0; i < THREADS / kWave; ++i) {
     a = red[0][i] > a ? red[0][i] : a;
     b = red[1][i] > b ? red[1][i] : b;
   }
@@ -177,11 +178,12 @@ __device__ __forceinline__ uint32_t value_token(uint32_t g, uint32_t j) {
 
 // The append of a block in 8 bits: the keys of its first `lo` tokens times a
 // factor.
-template <int D>
+template <int D, uint32_t THREADS = kThreads>
 __device__ __forceinline__ void rescale_keys(uint8_t *kc, uint32_t lo, float f) {
   if (f != 1.f) {
-    for (uint32_t u = threadIdx.x; u < lo * (D / 16); u += kThreads) {
-      u32x4 *at = reinterpret_cast<u32x4 *>(kc + kv_key_unit<D>(u / (D / 16), threadIdx.x % (D / 16)));
+    for (uint32_t u = threadIdx.x; u < lo * (D / 16); u += THREADS) {
+      u32x4 *at =
+          reinterpret_cast<u32x4 *>(kc + kv_key_unit<D>(u / (D / 16), threadIdx.x % (D / 16)));
       *at = rescale16(*at, f);
     }
   }
@@ -197,14 +199,14 @@ __device__ __forceinline__ void place_value(uint8_t *image, uint32_t t, uint32_t
 }
 // New values lo .. hi - 1 of the image to memory, beside those before them times
 // a factor.
-template <int D>
+template <int D, uint32_t THREADS = kThreads>
 __device__ __forceinline__ void store_values(const uint8_t *image, uint8_t *vc, uint32_t lo,
                                              uint32_t hi, float fv) {
   const uint32_t tid = threadIdx.x;
   // Units of 8 tokens x 2 dims: unit u of the block's has tokens t .. t + 3 and
   // t + 16 .. t + 19.
   const uint32_t vfrom = fv != 1.f ? 0u : lo / 32 * 32;
-  for (uint32_t u = vfrom * (D / 16) + tid; u < (hi + 31) / 32 * (2 * D); u += kThreads) {
+  for (uint32_t u = vfrom * (D / 16) + tid; u < (hi + 31) / 32 * (2 * D); u += THREADS) {
     const uint32_t t = u / (2 * D) * 32 + u % 64 / 16 * 4;
     // Bytes of the new ones among four tokens from t0 on.  (Signed differences:
     // of an unsigned one that a condition guards the compiler has concluded

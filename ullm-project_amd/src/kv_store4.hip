@@ -1,6 +1,7 @@
 // kv_store4.hip -- what writes and moves the tokens of the 4-bit key/value
 // cache, and the appends that rotate: append, gather and evict.  All are bound
 // by HBM and launches.
+#include "kernels.hpp"
 #include "kv_cache4.hpp"
 #include "kv_rotary.hpp"
 #include "kv_store.hpp"
@@ -93,35 +94,52 @@ __device__ __forceinline__ uint32_t largest16(const float (&f)[16]) {
 
 // ----------------------------------------------------------------- rotation
 
-// 32 tokens of a sequence, of which lo .. hi - 1 are rows of the call: row
+// Up to T tokens of a sequence, of which lo .. hi - 1 are rows of the call: row
 // `row0` + t is token t, at place `base` + t.
 struct Span {
   int64_t row0, base;
   uint32_t lo, hi;
 };
+// That of a sequence's slot; false if it has no rows.
+template <uint32_t T>
+__device__ __forceinline__ bool span_of(const KvSlot &slot, uint32_t length, Span *s) {
+  const int64_t origin = int64_t(length) - slot.rows.count;  // place of the first row
+  // Rounded down, places before the first token too.
+  s->base = (origin >= 0 ? origin / T : -((T - 1 - origin) / int64_t(T))) * T +
+            int64_t(slot.local) * T;
+  s->lo = origin > s->base ? uint32_t(origin - s->base) : 0u;
+  s->hi = uint32_t(min(max(int64_t(length) - s->base, int64_t(0)), int64_t(T)));
+  s->row0 = int64_t(slot.rows.first) + (s->base - origin);
+  return s->lo < s->hi;
+}
+
+// Threads of a workgroup for T tokens: one for each unit of 16 dims at least.
+template <int D, uint32_t T>
+constexpr uint32_t kSpanThreads = T * (D / 16) > kThreads ? T * (D / 16) : kThreads;
 
 // A thread's part of a span's rows: token t, pairs 8u .. 8u + 7, of heads `head`,
-// `head` + step and so on; none where `head` is none.
+// `head` + step and so on; none where `head` is kNoHead.
 constexpr uint32_t kNoHead = ~0u;
 struct Lot {
   uint32_t t, u, head, step;
 };
-template <int D>
+template <int D, uint32_t T>
 __device__ __forceinline__ Lot lot_of(const Span &s) {
   constexpr uint32_t kUnits = D / 16;
-  const uint32_t n = (s.hi - s.lo) * kUnits, step = kThreads / n;
+  const uint32_t n = (s.hi - s.lo) * kUnits, step = kSpanThreads<D, T> / n;
   const uint32_t head = threadIdx.x / n, i = threadIdx.x % n;
   return {s.lo + i / kUnits, i % kUnits, head < step ? head : kNoHead, step};
 }
 
 // Cosines and sines of a span: pair j of token t is at [t][j % 8][j / 8], where
 // the threads that read a pair each lie side by side.
-template <int D>
+template <int D, uint32_t T>
 struct SpanTurns {
-  Turn at[32][8][D / 16];
+  Turn at[T][8][D / 16];
 };
-template <int D>
-__device__ __forceinline__ void span_turns(const KvRotary &r, const Span &s, SpanTurns<D> *turns) {
+template <int D, uint32_t T>
+__device__ __forceinline__ void span_turns(const KvRotary &r, const Span &s,
+                                           SpanTurns<D, T> *turns) {
   const uint32_t j = threadIdx.x % (D / 2);
   if (j >= r.dims / 2) {
     return;
@@ -129,7 +147,7 @@ __device__ __forceinline__ void span_turns(const KvRotary &r, const Span &s, Spa
   const float f = r.inv_freq[j];
   const uint32_t axis = r.pair_axes == nullptr ? 0u : min(uint32_t(r.pair_axes[j]), r.axes - 1);
   const int32_t *at = r.positions + axis * r.position_stride;
-  for (uint32_t t = s.lo + threadIdx.x / (D / 2); t < s.hi; t += kThreads / (D / 2)) {
+  for (uint32_t t = s.lo + threadIdx.x / (D / 2); t < s.hi; t += kSpanThreads<D, T> / (D / 2)) {
     turns->at[t][j % 8][j / 8] =
         turn_of(r.positions == nullptr ? int32_t(s.base + t) : at[s.row0 + t], f);
   }
@@ -163,14 +181,24 @@ __device__ __forceinline__ RawPairs load_pairs(const uint16_t *row, const KvRota
   }
   return p;
 }
+// The elements of pair i.
+struct PairXY {
+  float x, y;
+};
+__device__ __forceinline__ PairXY raw_pair(const RawPairs &p, bool side, int i) {
+  const uint32_t near = i < 4 ? p.a[i % 4] : p.b[i % 4];
+  const uint32_t fx = p.a[i / 2], fy = p.b[i / 2];
+  return {bits_f32(side ? near << 16 : i % 2 == 0 ? fx << 16 : fx & 0xffff0000u),
+          bits_f32(side ? near & 0xffff0000u : i % 2 == 0 ? fy << 16 : fy & 0xffff0000u)};
+}
 
 // A thread's eight turns, and which of its pairs they are for.
 struct Turns8 {
   Turn w[8];
   uint32_t live;
 };
-template <int D>
-__device__ __forceinline__ Turns8 load_turns(const SpanTurns<D> &turns, const KvRotary &r,
+template <int D, uint32_t T>
+__device__ __forceinline__ Turns8 load_turns(const SpanTurns<D, T> &turns, const KvRotary &r,
                                              const Lot &lot) {
   Turns8 v;
   const uint32_t pairs = r.dims / 2, first = 8 * lot.u;
@@ -182,32 +210,18 @@ __device__ __forceinline__ Turns8 load_turns(const SpanTurns<D> &turns, const Kv
   return v;
 }
 
-// Pair i, rotated: both its elements as ROUND makes a float of a double.
-template <typename ROUND>
-__device__ __forceinline__ void rotate_pair(const RawPairs &p, bool side, const Turns8 &v, int i,
-                                            float &first, float &second, ROUND round) {
-  const uint32_t near = i < 4 ? p.a[i % 4] : p.b[i % 4];
-  const uint32_t far0 = p.a[i / 2], far1 = p.b[i / 2];
-  const uint32_t x = side ? near << 16 : i % 2 == 0 ? far0 << 16 : far0 & 0xffff0000u;
-  const uint32_t y = side           ? near & 0xffff0000u
-                     : i % 2 == 0 ? far1 << 16
-                                  : far1 & 0xffff0000u;
-  const double dx = bits_f32(x), dy = bits_f32(y);
-  const bool live = (v.live >> i & 1u) != 0;
-  const float rx = round(fma(dx, v.w[i].c, -(dy * v.w[i].s)));
-  const float ry = round(fma(dy, v.w[i].c, dx * v.w[i].s));
-  first = live ? rx : bits_f32(x);
-  second = live ? ry : bits_f32(y);
-}
-
-// A query's eight pairs, rotated, to their place.
+// A query's eight pairs, rotated in f32, to their place.
 __device__ __forceinline__ void rotate_query(uint16_t *row, const RawPairs &p, const KvRotary &r,
                                              const Turns8 &v, uint32_t u, bool runs) {
   const bool side = side_by_side(r, u, runs);
   float x[8], y[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    rotate_pair(p, side, v, i, x[i], y[i], [](double d) { return float(d); });
+    const PairXY e = raw_pair(p, side, i);
+    const float c = float(v.w[i].c), s = float(v.w[i].s);
+    const bool live = (v.live >> i & 1u) != 0;
+    x[i] = live ? __builtin_fmaf(e.x, c, -(e.y * s)) : e.x;
+    y[i] = live ? __builtin_fmaf(e.y, c, e.x * s) : e.y;
   }
   if (runs) {
     const PairDims d = pair_dims(8 * u, r.dims, r.interleaved);
@@ -230,26 +244,33 @@ __device__ __forceinline__ void rotate_query(uint16_t *row, const RawPairs &p, c
 }
 
 // Rows of rotated keys in LDS.
-template <int D>
+template <int D, uint32_t T>
 struct KeyImage {
-  alignas(16) float x[32][D + 4];
+  alignas(16) float x[T][D + 4];
 };
-template <int D>
-__device__ __forceinline__ void rotate_key(KeyImage<D> *to, const RawPairs &p, const KvRotary &r,
-                                           const Turns8 &v, const Lot &lot, bool runs) {
+// A key's eight pairs, rotated in 64 bits.
+template <int D, uint32_t T>
+__device__ __forceinline__ void rotate_key(KeyImage<D, T> *to, const RawPairs &p,
+                                           const KvRotary &r, const Turns8 &v, const Lot &lot,
+                                           bool runs) {
   const bool side = side_by_side(r, lot.u, runs);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const PairDims d = pair_dims(8 * lot.u + uint32_t(i), r.dims, r.interleaved);
-    rotate_pair(p, side, v, i, to->x[lot.t][d.first], to->x[lot.t][d.second],
-                [](double x) { return to_odd(x); });
+    const PairXY e = raw_pair(p, side, i);
+    const double x = e.x, y = e.y, c = v.w[i].c, s = v.w[i].s;
+    const bool live = (v.live >> i & 1u) != 0;
+    to->x[lot.t][d.first] = live ? to_odd(fma(x, c, -(y * s))) : e.x;
+    to->x[lot.t][d.second] = live ? to_odd(fma(y, c, x * s)) : e.y;
   }
 }
 
-// A span on its way: the first loads of keys and queries, issued before their
-// turns are known.
-constexpr uint32_t kAheadHeads = 4;
-template <int D>
+// The rotation of a span: the first loads of keys and queries are on their way
+// before their turns are known.  More than two heads ahead cost the registers of
+// a fourth wave (14006 tokens of 32 and 8 heads: four ahead 82 us, two 78; with
+// queries in 64 bits 78, in 32 76; heads of a span side by side in the grid 72).
+constexpr uint32_t kAheadHeads = 2;
+template <int D, uint32_t T>
 struct Rotation {
   const KvRotateArgs &a;
   const Span &s;
@@ -260,7 +281,7 @@ struct Rotation {
 
   __device__ __forceinline__ Rotation(const KvRotateArgs &args, const Span &span, uint32_t kvh,
                                       bool keys)
-      : a(args), s(span), head(kvh), lot(lot_of<D>(span)) {
+      : a(args), s(span), head(kvh), lot(lot_of<D, T>(span)) {
     const bool runs = a.rotary.interleaved || a.rotary.dims % 16 == 0;
     k_runs = runs && a.append.vec;
     q_runs = runs && a.q_vec;
@@ -281,7 +302,16 @@ struct Rotation {
       }
     }
   }
-  __device__ __forceinline__ void queries(const Turns8 &v) {
+  // Turns by way of `turns` in LDS; keys (if the span has any) to `keys`, which may
+  // lie in the same place, queries to memory.
+  __device__ __forceinline__ void run(SpanTurns<D, T> *turns, KeyImage<D, T> *keys) {
+    span_turns<D, T>(a.rotary, s, turns);
+    __syncthreads();
+    const Turns8 v = load_turns<D, T>(*turns, a.rotary, lot);
+    __syncthreads();
+    if (keys != nullptr && lot.head == 0) {
+      rotate_key<D, T>(keys, key, a.rotary, v, lot, k_runs);
+    }
     for (uint32_t h = lot.head; lot.head != kNoHead && h < a.group;) {
 #pragma unroll
       for (uint32_t i = 0; i < kAheadHeads; ++i, h += lot.step) {
@@ -292,8 +322,23 @@ struct Rotation {
       }
       load_queries(h);
     }
+    __syncthreads();
   }
 };
+// Sixteen elements of a rotated row.
+template <int D, uint32_t T>
+__device__ __forceinline__ void read_row(const KeyImage<D, T> &keys, uint32_t t, uint32_t c,
+                                         float (&k)[16]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const f32x4 w = *reinterpret_cast<const f32x4 *>(&keys.x[t][c * 16 + 4 * j]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      k[4 * j + e] = w[e];
+    }
+  }
+}
+constexpr size_t larger(size_t a, size_t b) { return a > b ? a : b; }
 
 // --------------------------------------------------------------- append, 4 bits
 
@@ -307,27 +352,18 @@ template <int D, bool ROTATE>
 __global__ __launch_bounds__(kThreads) void append4_kernel(KvRotateArgs ra, uint32_t each_slots) {
   using Chunk = Kv4Chunk<D>;
   constexpr uint32_t kUnits = D / 16, kPitch = D + 16;
+  static_assert(kSpanThreads<D, 32> == kThreads, "a thread for each unit");
   // Turns, and when all threads have theirs, keys and values.
-  constexpr uint32_t kImage = ROTATE ? sizeof(KeyImage<D>) : 0;
-  constexpr uint32_t kLds = kImage + 32 * kPitch;
-  __shared__ __align__(16) uint8_t lds[ROTATE && sizeof(SpanTurns<D>) > kLds ? sizeof(SpanTurns<D>)
-                                                                             : kLds];
-  KeyImage<D> *const rotated = reinterpret_cast<KeyImage<D> *>(lds);
+  constexpr uint32_t kImage = ROTATE ? sizeof(KeyImage<D, 32>) : 0;
+  __shared__ __align__(16) uint8_t
+      lds[larger(ROTATE ? sizeof(SpanTurns<D, 32>) : 0, kImage + 32 * kPitch)];
   uint8_t *const values = lds + kImage;  // a code to a byte
   const KvAppendArgs &a = ra.append;
-  const uint32_t head = blockIdx.y, tid = threadIdx.x;
-  const KvSlot slot = kv_find_slot(a.seqs, blockIdx.x, 1, 32, 2, each_slots);
-  if (slot.seq >= a.seqs.batch) {
-    return;
-  }
-  const uint32_t length = kv_length(a.seqs, a.pool.shift, slot.seq);
-  const int64_t origin = int64_t(length) - slot.rows.count;  // place of the first row
+  const uint32_t head = blockIdx.x % a.pool.heads, tid = threadIdx.x;
+  const KvSlot slot = kv_find_slot(a.seqs, blockIdx.x / a.pool.heads, 1, 32, 2, each_slots);
   Span s;
-  s.base = (origin >> 5) * 32 + int64_t(slot.local) * 32;
-  s.lo = origin > s.base ? uint32_t(origin - s.base) : 0u;
-  s.hi = uint32_t(min(max(int64_t(length) - s.base, int64_t(0)), int64_t(32)));
-  s.row0 = int64_t(slot.rows.first) + (s.base - origin);
-  if (s.lo >= s.hi) {
+  if (slot.seq >= a.seqs.batch ||
+      !span_of<32>(slot, kv_length(a.seqs, a.pool.shift, slot.seq), &s)) {
     return;
   }
   // Places before the first token have no block, but queries.
@@ -341,29 +377,14 @@ __global__ __launch_bounds__(kThreads) void append4_kernel(KvRotateArgs ra, uint
   const Bf16x16 raw_value = load16(a.v + head * a.v_head + row * a.v_row + c * 16, a.vec);
   float k[16], v[16];
   if constexpr (ROTATE) {
-    Rotation<D> rotation(ra, s, head, id >= 0);
-    SpanTurns<D> *const turns = reinterpret_cast<SpanTurns<D> *>(lds);
-    span_turns<D>(ra.rotary, s, turns);
-    __syncthreads();
-    const Turns8 mine = load_turns<D>(*turns, ra.rotary, rotation.lot);
-    __syncthreads();
-    if (id >= 0 && rotation.lot.head == 0) {
-      rotate_key<D>(rotated, rotation.key, ra.rotary, mine, rotation.lot, rotation.k_runs);
-    }
-    rotation.queries(mine);
+    KeyImage<D, 32> *const rotated = reinterpret_cast<KeyImage<D, 32> *>(lds);
+    Rotation<D, 32>(ra, s, head, id >= 0)
+        .run(reinterpret_cast<SpanTurns<D, 32> *>(lds), id >= 0 ? rotated : nullptr);
     if (id < 0) {
       return;
     }
-    __syncthreads();
     if (live) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4 w = *reinterpret_cast<const f32x4 *>(&rotated->x[t][c * 16 + 4 * j]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          k[4 * j + e] = w[e];
-        }
-      }
+      read_row<D, 32>(*rotated, t, c, k);
     }
   } else {
     if (id < 0) {
@@ -431,95 +452,54 @@ __global__ __launch_bounds__(kThreads) void append4_kernel(KvRotateArgs ra, uint
 // ------------------------------------------------------- append, 8 bits, rotated
 
 // One workgroup stores the new tokens of one block and head, as append_kernel
-// does; keys come rotated from LDS, 32 tokens at a time.
+// does, with keys that come rotated from LDS, and rotates the queries of its
+// group: a thread has one unit of 16 dims of the block.
 template <int D, uint32_t bt>
-__global__ __launch_bounds__(kThreads) void append8_rotary_kernel(KvRotateArgs ra,
-                                                                  uint32_t each_slots) {
-  constexpr uint32_t kUnits = D / 16, kSpans = bt / 32;
-  constexpr uint32_t kEach = (32 * kUnits + kThreads - 1) / kThreads;  // of a thread and span
+__global__ __launch_bounds__((kSpanThreads<D, bt>)) void append8_rotary_kernel(
+    KvRotateArgs ra, uint32_t each_slots) {
+  constexpr uint32_t kUnits = D / 16, kAll = kSpanThreads<D, bt>;
   // Turns, and when all threads have theirs, rotated keys; at the end values.
-  constexpr uint32_t kFirst = sizeof(SpanTurns<D>) > sizeof(KeyImage<D>) ? sizeof(SpanTurns<D>)
-                                                                         : sizeof(KeyImage<D>);
-  __shared__ __align__(16) uint8_t lds[kFirst > bt * D ? kFirst : bt * D];
-  SpanTurns<D> *const turns = reinterpret_cast<SpanTurns<D> *>(lds);
-  KeyImage<D> *const rotated = reinterpret_cast<KeyImage<D> *>(lds);
-  uint8_t *const image = lds;
+  extern __shared__ __align__(16) uint8_t append8_lds[];
+  KeyImage<D, bt> *const rotated = reinterpret_cast<KeyImage<D, bt> *>(append8_lds);
   const KvAppendArgs &a = ra.append;
-  const uint32_t head = blockIdx.y, tid = threadIdx.x;
-  const KvSlot slot = kv_find_slot(a.seqs, blockIdx.x, 1, bt, 2, each_slots);
-  if (slot.seq >= a.seqs.batch) {
+  const uint32_t head = blockIdx.x % a.pool.heads, tid = threadIdx.x;
+  const KvSlot slot = kv_find_slot(a.seqs, blockIdx.x / a.pool.heads, 1, bt, 2, each_slots);
+  Span s;
+  if (slot.seq >= a.seqs.batch ||
+      !span_of<bt>(slot, kv_length(a.seqs, a.pool.shift, slot.seq), &s)) {
     return;
   }
-  const uint32_t length = kv_length(a.seqs, a.pool.shift, slot.seq);
-  const int64_t origin = int64_t(length) - slot.rows.count;
-  const int64_t base = (origin >> a.pool.shift) * bt + int64_t(slot.local) * bt;
-  const uint32_t lo = origin > base ? uint32_t(origin - base) : 0u;
-  const uint32_t hi = uint32_t(min(max(int64_t(length) - base, int64_t(0)), int64_t(bt)));
-  if (lo >= hi) {
-    return;
-  }
-  const int64_t row0 = int64_t(slot.rows.first) + (base - origin);
-  const int32_t id = base < 0 ? -1
-                              : kv_block(a.seqs.tables + slot.seq * a.seqs.stride, a.seqs,
-                                         a.pool.blocks, uint32_t(base) >> a.pool.shift);
+  const int32_t id = s.base < 0 ? -1
+                                : kv_block(a.seqs.tables + slot.seq * a.seqs.stride, a.seqs,
+                                           a.pool.blocks, uint32_t(s.base) >> a.pool.shift);
   const uint64_t unit = uint64_t(id < 0 ? 0 : id) * a.pool.heads + head;
   const int ek0 = a.pool.exps[unit * 2], ev0 = a.pool.exps[unit * 2 + 1];
-  // Unit r of this thread in a span: token t of the span, dims 16c .. 16c + 15.
-  const auto token = [&](uint32_t r) { return (tid + r * kThreads) / kUnits; };
-  const uint32_t c = tid % kUnits;
-  float x[kSpans * kEach][16];
-  Bf16x16 y[kSpans * kEach];
-  uint32_t ak = 0, av = 0;
-#pragma unroll
-  for (uint32_t p = 0; p < kSpans; ++p) {
-    Span s;
-    s.base = base + 32 * p;
-    s.row0 = row0 + 32 * p;
-    s.lo = lo > 32 * p ? min(lo - 32 * p, 32u) : 0u;
-    s.hi = hi > 32 * p ? min(hi - 32 * p, 32u) : 0u;
-    s.lo = min(s.lo, s.hi);
-    if (s.lo < s.hi) {  // the same for all threads
-      Rotation<D> rotation(ra, s, head, id >= 0);
-      span_turns<D>(ra.rotary, s, turns);
-      __syncthreads();
-      const Turns8 mine = load_turns<D>(*turns, ra.rotary, rotation.lot);
-      __syncthreads();
-      if (id >= 0 && rotation.lot.head == 0) {
-        rotate_key<D>(rotated, rotation.key, ra.rotary, mine, rotation.lot, rotation.k_runs);
-      }
-      rotation.queries(mine);
-      __syncthreads();
-    }
-#pragma unroll
-    for (uint32_t r = 0; r < kEach; ++r) {
-      const uint32_t t = token(r), i = p * kEach + r;
-      y[i] = Bf16x16{};
-      const bool live = id >= 0 && t >= s.lo && t < s.hi;
-      if (live) {
-        y[i] = load16(a.v + head * a.v_head + uint64_t(s.row0 + t) * a.v_row + c * 16, a.vec);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4 w =
-            *reinterpret_cast<const f32x4 *>(&rotated->x[live ? t : 0][c * 16 + 4 * j]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[i][4 * j + e] = live ? w[e] : 0.f;
-          const uint32_t m = f32_bits(x[i][4 * j + e]) & 0x7fffffffu;
-          ak = max(ak, m < 0x7f800000u ? m : 0u);  // infinities and NaN do not count
-        }
-      }
-    }
-    __syncthreads();
+  // This thread's unit: token t, dims 16c .. 16c + 15.
+  const uint32_t t = s.lo + tid / kUnits, c = tid % kUnits;
+  const bool live = t < s.hi && id >= 0;
+  Bf16x16 y[1] = {};
+  if (live) {
+    y[0] = load16(a.v + head * a.v_head + uint64_t(s.row0 + t) * a.v_row + c * 16, a.vec);
   }
+  Rotation<D, bt>(ra, s, head, id >= 0)
+      .run(reinterpret_cast<SpanTurns<D, bt> *>(append8_lds), id >= 0 ? rotated : nullptr);
   if (id < 0) {
     return;
   }
-  av = largest_magnitude(y);
-  block_umax2(ak, av);
+  float x[16];
+  uint32_t ak = 0, av = largest_magnitude(y);
+  if (live) {
+    read_row<D, bt>(*rotated, t, c, x);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {  // infinities and NaN do not count
+      const uint32_t m = f32_bits(x[i]) & 0x7fffffffu;
+      ak = max(ak, m < 0x7f800000u ? m : 0u);
+    }
+  }
+  block_umax2<kAll>(ak, av);
   int ek = exponent_for_f32(ak), ev = exponent_for(av);
   float fk = 1.f, fv = 1.f;  // factor of the codes that were there
-  if (lo > 0) {
+  if (s.lo > 0) {
     ek = max(ek, ek0);
     ev = max(ev, ev0);
     fk = exp2_int(max(ek0 - ek, -126));
@@ -531,21 +511,17 @@ __global__ __launch_bounds__(kThreads) void append8_rotary_kernel(KvRotateArgs r
   }
   uint8_t *kc = a.pool.codes + unit * (uint64_t(2 * D) << a.pool.shift);
   uint8_t *vc = kc + (uint64_t(D) << a.pool.shift);
-  rescale_keys<D>(kc, lo, fk);
-#pragma unroll
-  for (uint32_t i = 0; i < kSpans * kEach; ++i) {
-    const uint32_t t = 32 * (i / kEach) + token(i % kEach);
-    if (token(i % kEach) < 32 && t >= lo && t < hi) {
-      *reinterpret_cast<u32x4 *>(kc + kv_key_unit<D>(t, c)) = encode16(x[i], ek);
-      place_value<D>(image, t, c, encode16(y[i], ev));
-    }
+  rescale_keys<D, kAll>(kc, s.lo, fk);
+  if (live) {
+    *reinterpret_cast<u32x4 *>(kc + kv_key_unit<D>(t, c)) = encode16(x, ek);
+    place_value<D>(append8_lds, t, c, encode16(y[0], ev));
   }
   __syncthreads();
-  store_values<D>(image, vc, lo, hi, fv);
+  store_values<D, kAll>(append8_lds, vc, s.lo, s.hi, fv);
   if (a.pool.weights != nullptr) {
-    for (uint32_t t = lo + tid; t < hi; t += kThreads) {
-      a.pool.weights[(unit << a.pool.shift) + t] =
-          a.weights != nullptr ? a.weights[uint64_t(row0 + t) * a.pool.heads + head] : 0.f;
+    for (uint32_t i = s.lo + tid; i < s.hi; i += kAll) {
+      a.pool.weights[(unit << a.pool.shift) + i] =
+          a.weights != nullptr ? a.weights[uint64_t(s.row0 + i) * a.pool.heads + head] : 0.f;
     }
   }
 }
@@ -733,11 +709,13 @@ __global__ __launch_bounds__(kThreads) void evict4_move_kernel(KvEvictArgs a) {
 
 }  // namespace
 
+// Workgroups: the heads of a span lie side by side, so that whole rows are on
+// their way at a time.
 hipError_t launch_kv4_append(const KvRotateArgs &a, uint32_t dim, hipStream_t s) {
   const KvSeqs &q = a.append.seqs;
   // n rows touch at most (n + 30) / 32 + 1 chunks.
   const uint32_t each = q.each == 0 ? 1 : (q.each + 30) / 32 + 1;
-  const dim3 grid(uint32_t(kv_slots(q, 1, 32, 2, each)), a.append.pool.heads);
+  const uint32_t grid = uint32_t(kv_slots(q, 1, 32, 2, each)) * a.append.pool.heads;
   const auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(a, each); };
   if (a.rotary.dims != 0) {
     launch(dim == 64 ? append4_kernel<64, true> : append4_kernel<128, true>);
@@ -747,22 +725,29 @@ hipError_t launch_kv4_append(const KvRotateArgs &a, uint32_t dim, hipStream_t s)
   return hipGetLastError();
 }
 
-hipError_t launch_kv8_append_rotary(const KvRotateArgs &a, uint32_t dim, hipStream_t s) {
+template <int D, uint32_t bt>
+static hipError_t launch_append8(const KvRotateArgs &a, hipStream_t s) {
   const KvSeqs &q = a.append.seqs;
-  const uint32_t bt = 1u << a.append.pool.shift;
   const uint32_t each = q.each == 0 ? 1 : (q.each + bt - 2) / bt + 1;
-  const dim3 grid(uint32_t(kv_slots(q, 1, bt, 2, each)), a.append.pool.heads);
-  const auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(a, each); };
-  if (dim == 64) {
-    launch(bt == 32   ? append8_rotary_kernel<64, 32>
-           : bt == 64 ? append8_rotary_kernel<64, 64>
-                      : append8_rotary_kernel<64, 128>);
-  } else {
-    launch(bt == 32   ? append8_rotary_kernel<128, 32>
-           : bt == 64 ? append8_rotary_kernel<128, 64>
-                      : append8_rotary_kernel<128, 128>);
+  const uint32_t grid = uint32_t(kv_slots(q, 1, bt, 2, each)) * a.append.pool.heads;
+  constexpr size_t lds = larger(larger(sizeof(SpanTurns<D, bt>), sizeof(KeyImage<D, bt>)), bt * D);
+  const auto kernel = append8_rotary_kernel<D, bt>;
+  const hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kernel), lds);
+  if (e != hipSuccess) {
+    return e;
   }
+  kernel<<<grid, kSpanThreads<D, bt>, lds, s>>>(a, each);
   return hipGetLastError();
+}
+hipError_t launch_kv8_append_rotary(const KvRotateArgs &a, uint32_t dim, hipStream_t s) {
+  const uint32_t bt = 1u << a.append.pool.shift;
+  const auto launch = dim == 64 ? (bt == 32   ? launch_append8<64, 32>
+                                   : bt == 64 ? launch_append8<64, 64>
+                                              : launch_append8<64, 128>)
+                                : (bt == 32   ? launch_append8<128, 32>
+                                   : bt == 64 ? launch_append8<128, 64>
+                                              : launch_append8<128, 128>);
+  return launch(a, s);
 }
 
 hipError_t launch_kv4_gather(const KvGatherArgs &a, uint32_t dim, hipStream_t s) {
