@@ -167,9 +167,9 @@ __device__ __forceinline__ RawPairs load_pairs(const uint16_t *row, const KvRota
   RawPairs p;
   if (runs) {
     const PairDims d = pair_dims(8 * u, r.dims, r.interleaved);
-    p.a = *reinterpret_cast<const u32x4 *>(row + d.first);
-    p.b = *reinterpret_cast<const u32x4 *>(
-        row + (side_by_side(r, u, runs) ? d.first + 8 : d.second));
+    p.a = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(row + d.first));
+    p.b = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(
+        row + (side_by_side(r, u, runs) ? d.first + 8 : d.second)));
   } else {
 #pragma unroll
     for (uint32_t i = 0; i < 8; i += 2) {
@@ -210,7 +210,9 @@ __device__ __forceinline__ Turns8 load_turns(const SpanTurns<D, T> &turns, const
   return v;
 }
 
-// A query's eight pairs, rotated in f32, to their place.
+// A query's eight pairs, rotated in f32, to their place.  Rows of q are read
+// once, and their results next by another kernel: both pass the caches by (14006
+// tokens of 32 and 8 heads: 64 us, through them 75).
 __device__ __forceinline__ void rotate_query(uint16_t *row, const RawPairs &p, const KvRotary &r,
                                              const Turns8 &v, uint32_t u, bool runs) {
   const bool side = side_by_side(r, u, runs);
@@ -231,8 +233,8 @@ __device__ __forceinline__ void rotate_query(uint16_t *row, const RawPairs &p, c
       a[i] = side ? f32x2_to_bf16x2(x[i], y[i]) : f32x2_to_bf16x2(x[2 * i], x[2 * i + 1]);
       b[i] = side ? f32x2_to_bf16x2(x[4 + i], y[4 + i]) : f32x2_to_bf16x2(y[2 * i], y[2 * i + 1]);
     }
-    *reinterpret_cast<u32x4 *>(row + d.first) = a;
-    *reinterpret_cast<u32x4 *>(row + (side ? d.first + 8 : d.second)) = b;
+    __builtin_nontemporal_store(a, reinterpret_cast<u32x4 *>(row + d.first));
+    __builtin_nontemporal_store(b, reinterpret_cast<u32x4 *>(row + (side ? d.first + 8 : d.second)));
   } else {
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
@@ -375,6 +377,24 @@ __global__ __launch_bounds__(kThreads) void append4_kernel(KvRotateArgs ra, uint
   const bool live = t < s.hi && id >= 0;
   const uint64_t row = uint64_t(s.row0 + (live ? t : s.lo));
   const Bf16x16 raw_value = load16(a.v + head * a.v_head + row * a.v_row + c * 16, a.vec);
+  const uint32_t in_block = uint32_t(s.base) & ((1u << a.pool.shift) - 1);
+  const uint64_t unit = uint64_t(id < 0 ? 0 : id) * a.pool.heads + head;
+  uint8_t *const chunk = kv4_chunk<D>(a.pool, unit, in_block);
+  // At the end a thread has two dwords of a lane's four: dims d and d + 16 of the
+  // eight tokens of group g.  What they hold is on its way from here.
+  const uint32_t g = tid / (D / 2), d = tid % (D / 2) / 16 * 32 + tid % 16;
+  u32x2 *const value_at =
+      reinterpret_cast<u32x2 *>(chunk + Chunk::kSide + kv4_value_dword(g % 4, d));
+  uint32_t fresh = 0;  // nibbles of new tokens
+#pragma unroll
+  for (uint32_t j = 0; j < 8; ++j) {
+    const uint32_t of = 4 * g + j % 4 + 16 * (j / 4);
+    fresh |= g < 4 && of >= s.lo && of < s.hi ? 15u << (4 * j) : 0u;
+  }
+  u32x2 held = {0u, 0u};
+  if (fresh != 0 && fresh != ~0u) {
+    held = *value_at;
+  }
   float k[16], v[16];
   if constexpr (ROTATE) {
     KeyImage<D, 32> *const rotated = reinterpret_cast<KeyImage<D, 32> *>(lds);
@@ -392,9 +412,6 @@ __global__ __launch_bounds__(kThreads) void append4_kernel(KvRotateArgs ra, uint
     }
     unpack16(load16(a.k + head * a.k_head + row * a.k_row + c * 16, a.vec), k);
   }
-  const uint32_t in_block = uint32_t(s.base) & ((1u << a.pool.shift) - 1);
-  const uint64_t unit = uint64_t(id) * a.pool.heads + head;
-  uint8_t *chunk = kv4_chunk<D>(a.pool, unit, in_block);
   if (live) {
     unpack16(raw_value, v);
     const uint32_t e = key_exp4(largest16<2>(k));
@@ -418,28 +435,16 @@ __global__ __launch_bounds__(kThreads) void append4_kernel(KvRotateArgs ra, uint
     }
   }
   __syncthreads();
-  // Two dwords of a lane's four to a thread: dims d and d + 16 of eight tokens.
-  for (uint32_t i = tid; i < 2 * D; i += kThreads) {
-    const uint32_t g = i / (D / 2), d = i % (D / 2) / 16 * 32 + i % 16;
-    uint32_t fresh = 0;
-    u32x2 w = {0u, 0u};
+  if (fresh != 0) {
+    u32x2 w = {held.x & ~fresh, held.y & ~fresh};
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j) {
-      const uint32_t of = 4 * g + j % 4 + 16 * (j / 4);
-      const bool is_new = of >= s.lo && of < s.hi;
-      const uint8_t *from = values + of * kPitch + d;
+      const uint8_t *from = values + (4 * g + j % 4 + 16 * (j / 4)) * kPitch + d;
+      const bool is_new = (fresh >> (4 * j) & 1u) != 0;
       w.x |= (is_new ? from[0] : 0u) << (4 * j);
       w.y |= (is_new ? from[16] : 0u) << (4 * j);
-      fresh |= is_new ? 15u << (4 * j) : 0u;
     }
-    if (fresh != 0) {
-      u32x2 *at = reinterpret_cast<u32x2 *>(chunk + Chunk::kSide + kv4_value_dword(g, d));
-      if (fresh != ~0u) {
-        const u32x2 old = *at;
-        w = u32x2{w.x | (old.x & ~fresh), w.y | (old.y & ~fresh)};
-      }
-      *at = w;
-    }
+    *value_at = w;
   }
   if (a.pool.weights != nullptr) {
     for (uint32_t i = s.lo + tid; i < s.hi; i += kThreads) {
