@@ -5,6 +5,8 @@
 
 #include "ullm/hip.h"
 #include "ullm/kv_cache.h"
+#include "ullm/kv_cache4.h"
+#include "ullm/kv_rotary.h"
 #include "ullm/linear.h"
 #include "ullm/weights_io.h"
 

@@ -284,6 +284,12 @@ ullm::KvAppendArgs append_args(const D *d) {
   return a;
 }
 
+ullm_status_t check_append_grid(uint64_t threads, ullm_error_sink_t *sink) {
+  return threads <= UINT32_MAX ? ULLM_STATUS_OK
+                               : write_error(sink, ULLM_STATUS_UNSUPPORTED,
+                                             "too many spans of rows x kv_heads for one launch");
+}
+
 ullm::KvAttendArgs attend_args(const ullm_kv_cache_attend_desc_t *d) {
   const ullm_kv_cache_t *c = d->cache;
   const Strides q = strides_of(d->q_row_stride, d->q_head_stride, d->heads, c->head_dim);
@@ -468,15 +474,21 @@ extern "C" ULLM_HIP_API ullm_status_t ullm_kv_cache_query(const ullm_kv_cache_t 
 extern "C" ULLM_HIP_API ullm_status_t ullm_kv_cache_append(
     const ullm_kv_cache_append_desc_t *desc, ullm_error_sink_t *error_sink) {
   ULLM_ENTRY(error_sink, "cache append", {
-    const ullm_status_t st = validate_append(desc, error_sink);
+    ullm_status_t st = validate_append(desc, error_sink);
     if (st != ULLM_STATUS_OK || no_work(desc->seqs)) {
       return st;
     }
     const ullm_kv_cache_t *c = desc->cache;
+    const ullm::KvAppendArgs a = append_args(desc);
+    if (four_bits(c)) {
+      st = check_append_grid(ullm::kv4_append_threads(a), error_sink);
+      if (st != ULLM_STATUS_OK) {
+        return st;
+      }
+    }
     DeviceScope scope(c->device);
     HIP_TRY(error_sink, "hipSetDevice", scope.error());
     const hipStream_t stream = static_cast<hipStream_t>(desc->stream);
-    const ullm::KvAppendArgs a = append_args(desc);
     if (four_bits(c)) {
       ullm::KvRotateArgs r{};
       r.append = a;
@@ -491,19 +503,26 @@ extern "C" ULLM_HIP_API ullm_status_t ullm_kv_cache_append(
 extern "C" ULLM_HIP_API ullm_status_t ullm_kv_cache_append_rotary(
     const ullm_kv_cache_append_rotary_desc_t *desc, ullm_error_sink_t *error_sink) {
   ULLM_ENTRY(error_sink, "cache append_rotary", {
-    const ullm_status_t st = validate_append_rotary(desc, error_sink);
+    ullm_status_t st = validate_append_rotary(desc, error_sink);
     if (st != ULLM_STATUS_OK || no_work(desc->seqs)) {
       return st;
     }
     const ullm_kv_cache_t *c = desc->cache;
+    ullm::KvRotateArgs a{};
+    a.append = append_args(desc);
+    st = check_append_grid(four_bits(c)
+                               ? ullm::kv4_append_threads(a.append)
+                               : ullm::kv8_append_rotary_threads(a.append, c->head_dim),
+                           error_sink);
+    if (st != ULLM_STATUS_OK) {
+      return st;
+    }
     DeviceScope scope(c->device);
     HIP_TRY(error_sink, "hipSetDevice", scope.error());
     const Strides q = strides_of(desc->q_row_stride, desc->q_head_stride, desc->heads,
                                  c->head_dim);
     const Strides o = strides_of(desc->q_out_row_stride, desc->q_out_head_stride, desc->heads,
                                  c->head_dim);
-    ullm::KvRotateArgs a{};
-    a.append = append_args(desc);
     a.rotary.inv_freq = desc->inv_freq;
     a.rotary.positions = desc->positions;
     a.rotary.position_stride =

@@ -103,6 +103,9 @@ struct KvRotateArgs {
 // Into a cache of 4 bits, rotated if rotary.dims != 0; into one of 8, rotated.
 hipError_t launch_kv4_append(const KvRotateArgs &a, uint32_t dim, hipStream_t s);
 hipError_t launch_kv8_append_rotary(const KvRotateArgs &a, uint32_t dim, hipStream_t s);
+// Threads of these launches, which count them in 32 bits.
+uint64_t kv4_append_threads(const KvAppendArgs &a);
+uint64_t kv8_append_rotary_threads(const KvAppendArgs &a, uint32_t dim);
 hipError_t launch_kv4_gather(const KvGatherArgs &a, uint32_t dim, hipStream_t s);
 hipError_t launch_kv4_evict(const KvEvictArgs &a, uint32_t dim, hipStream_t s);
 KvAttendPlan plan_kv4_attend(const KvAttendArgs &a, uint32_t dim);

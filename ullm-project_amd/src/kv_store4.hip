@@ -714,13 +714,24 @@ __global__ __launch_bounds__(kThreads) void evict4_move_kernel(KvEvictArgs a) {
 
 }  // namespace
 
+// Slots that n rows of every sequence need: they touch at most (n + t - 2) / t + 1
+// spans of t tokens.
+static uint32_t each_slots(const KvSeqs &q, uint32_t t) {
+  return q.each == 0 ? 1 : (q.each + t - 2) / t + 1;
+}
 // Workgroups: the heads of a span lie side by side, so that whole rows are on
 // their way at a time.
+static uint64_t append_grid(const KvAppendArgs &a, uint32_t t) {
+  return kv_slots(a.seqs, 1, t, 2, each_slots(a.seqs, t)) * a.pool.heads;
+}
+uint64_t kv4_append_threads(const KvAppendArgs &a) { return append_grid(a, 32) * kThreads; }
+uint64_t kv8_append_rotary_threads(const KvAppendArgs &a, uint32_t dim) {
+  const uint32_t bt = 1u << a.pool.shift;
+  return append_grid(a, bt) * larger(bt * (dim / 16), kThreads);
+}
+
 hipError_t launch_kv4_append(const KvRotateArgs &a, uint32_t dim, hipStream_t s) {
-  const KvSeqs &q = a.append.seqs;
-  // n rows touch at most (n + 30) / 32 + 1 chunks.
-  const uint32_t each = q.each == 0 ? 1 : (q.each + 30) / 32 + 1;
-  const uint32_t grid = uint32_t(kv_slots(q, 1, 32, 2, each)) * a.append.pool.heads;
+  const uint32_t each = each_slots(a.append.seqs, 32), grid = uint32_t(append_grid(a.append, 32));
   const auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(a, each); };
   if (a.rotary.dims != 0) {
     launch(dim == 64 ? append4_kernel<64, true> : append4_kernel<128, true>);
@@ -732,9 +743,7 @@ hipError_t launch_kv4_append(const KvRotateArgs &a, uint32_t dim, hipStream_t s)
 
 template <int D, uint32_t bt>
 static hipError_t launch_append8(const KvRotateArgs &a, hipStream_t s) {
-  const KvSeqs &q = a.append.seqs;
-  const uint32_t each = q.each == 0 ? 1 : (q.each + bt - 2) / bt + 1;
-  const uint32_t grid = uint32_t(kv_slots(q, 1, bt, 2, each)) * a.append.pool.heads;
+  const uint32_t each = each_slots(a.append.seqs, bt), grid = uint32_t(append_grid(a.append, bt));
   constexpr size_t lds = larger(larger(sizeof(SpanTurns<D, bt>), sizeof(KeyImage<D, bt>)), bt * D);
   const auto kernel = append8_rotary_kernel<D, bt>;
   const hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kernel), lds);
@@ -760,7 +769,7 @@ hipError_t launch_kv4_gather(const KvGatherArgs &a, uint32_t dim, hipStream_t s)
     launch_kv_gather_weights(a, s);
     return hipGetLastError();
   }
-  const uint32_t each = a.seqs.each == 0 ? 1 : (a.seqs.each + 30) / 32 + 1;
+  const uint32_t each = each_slots(a.seqs, 32);
   const dim3 grid(uint32_t(kv_slots(a.seqs, 1, 32, 2, each)), a.pool.heads);
   if (dim == 64) {
     gather4_kernel<64><<<grid, kThreads, 0, s>>>(a, each);
