@@ -7,8 +7,8 @@ it, so fixed stand-ins keep the chain well-defined and bounded:
 
   * attention output, by default the q slice (first 4096 columns) of the qkv
     output, read in place as a strided view (x_row_stride = 6144).  With
-    context=N it is attention over an 8-bit key/value cache of up to N tokens
-    for each sequence instead: prompt() takes the sequences' first rows,
+    context=N it is attention over a key/value cache (8 bits; kv_bits=4 for 4)
+    of up to N tokens for each sequence instead: prompt() takes the sequences' first rows,
     step() one more each, and with evict_to=T evict() cuts each sequence to
     the T tokens per head that received most of the weight.  A call that a
     sequence has no room for (N in whole blocks) raises ValueError; steps
@@ -16,7 +16,11 @@ it, so fixed stand-ins keep the chain well-defined and bounded:
     and values are the strided thirds of the qkv output.  Scores are not
     scaled (scale = 1 instead of 1 / sqrt(128)): those of unit normal rows
     are then far apart, and the output of a row stays near unit RMS however
-    many tokens it sees, as the missing norms would have it;
+    many tokens it sees, as the missing norms would have it.  With rope_base=B
+    pair j of a head's dims d and d + head_dim / 2 is rotated by its token's
+    position times B ** (-2j / head_dim) as the rows are stored, the queries in
+    place.  A position counts the tokens that its sequence has been given: it
+    stays right where evict() has taken tokens before it away;
   * MLP activation, by default the pass-through stand-in: the gate half
     (first 14336 columns) of the gate_up output, read in place
     (x_row_stride = 28672).  With swiglu=True it is the real SwiGLU gate
@@ -77,7 +81,8 @@ class DecodeStack:
 
     def __init__(self, uh, torch, device, batch=8, layers=LAYERS, hidden=HIDDEN,
                  qkv=QKV, ffn=FFN, vocab=VOCAB, seed=0, weights=None,
-                 swiglu=False, context=0, head_dim=128, block_tokens=64, evict_to=0):
+                 swiglu=False, context=0, head_dim=128, block_tokens=64, evict_to=0,
+                 kv_bits=8, rope_base=0.0):
         self.uh, self.torch, self.dev = uh, torch, device
         self.m, self.layers = batch, layers
         self.hidden, self.qkv, self.ffn, self.vocab = hidden, qkv, ffn, vocab
@@ -124,10 +129,12 @@ class DecodeStack:
 
         self.caches = []
         self.evict_to = evict_to
+        if rope_base < 0 or not context and (rope_base or kv_bits != 8):
+            raise ValueError("rope_base must not be negative; it and kv_bits need a context")
         if context:
-            self._make_caches(context, head_dim, block_tokens)
+            self._make_caches(context, head_dim, block_tokens, kv_bits, rope_base)
 
-    def _make_caches(self, context, dim, block_tokens):
+    def _make_caches(self, context, dim, block_tokens, kv_bits, rope_base):
         """One cache per layer; all share the tables, of which sequence b has
         row b, and the blocks that evict() moves tokens into."""
         torch = self.torch
@@ -145,9 +152,16 @@ class DecodeStack:
         self.caches = [self.uh.KvCache(ids.numel(), self.kv_heads, dim,
                                        block_tokens=block_tokens,
                                        track_weights=self.evict_to > 0,
-                                       device=torch.device(self.dev).index or 0)
+                                       device=torch.device(self.dev).index or 0,
+                                       bits=kv_bits)
                        for _ in range(self.layers)]
         self.attn = torch.empty((self.m, self.hidden), dtype=torch.bfloat16, device=self.dev)
+        self.inv_freq = None
+        if rope_base:
+            pairs = torch.arange(0, dim, 2, dtype=torch.float64, device=self.dev)
+            self.inv_freq = (float(rope_base) ** (-pairs / dim)).float()
+        # Tokens that each sequence has been given, the evicted ones too.
+        self.given = torch.zeros((self.m,), dtype=torch.int32, device=self.dev)
 
     def _grow(self, counts):
         """Count new tokens of the sequences: the kernels take a length past
@@ -164,7 +178,7 @@ class DecodeStack:
         if self.caches:
             self._grow([steps] * self.m)
 
-    def _attention(self, layer, qkv, out, starts, stream):
+    def _attention(self, layer, qkv, out, starts, positions, stream):
         """Store the rows' keys and values, attend from their queries."""
         if not self.caches:
             return qkv[:, :self.hidden]
@@ -173,18 +187,35 @@ class DecodeStack:
         v0 = k0 + self.kv_heads * dim
         heads = [qkv[:, a:b].view(rows, -1, dim) for a, b in
                  ((0, k0), (k0, v0), (v0, v0 + self.kv_heads * dim))]
-        cache.append(heads[1], heads[2], self.lengths, self.tables, starts=starts, stream=stream)
+        if self.inv_freq is None:
+            cache.append(heads[1], heads[2], self.lengths, self.tables, starts=starts,
+                         stream=stream)
+        else:
+            cache.append_rotary(*heads, self.lengths, self.tables, self.inv_freq, starts=starts,
+                                positions=positions, out=heads[0], stream=stream)
         cache.attend(heads[0], self.lengths, self.tables, starts=starts,
                      out=out.view(rows, -1, dim), scale=1.0,
                      accumulate=self.evict_to > 0, stream=stream)
         return out
 
-    def _layers(self, h0, h, qkv_out, attn, o_out, act, starts, stream):
+    def _positions(self, ends, rows):
+        """Positions of the rows of a call: of sequence b up to ends[b], or one
+        row of each."""
+        if not self.caches or self.inv_freq is None:
+            return None
+        if ends is None:
+            return self.given - 1
+        torch = self.torch
+        of = torch.arange(rows, dtype=torch.int32, device=self.dev)
+        owner = torch.searchsorted(ends, of, right=True)
+        return of + (self.given - ends)[owner]
+
+    def _layers(self, h0, h, qkv_out, attn, o_out, act, starts, positions, stream):
         for i, ws in enumerate(self.weights):
             ws["qkv"].forward(h0 if i == 0 else h, qkv_out, alpha=self.alpha_h,
                               stream=stream)
-            ws["o"].forward(self._attention(i, qkv_out, attn, starts, stream), o_out,
-                            alpha=self.alpha_h, stream=stream)
+            ws["o"].forward(self._attention(i, qkv_out, attn, starts, positions, stream),
+                            o_out, alpha=self.alpha_h, stream=stream)
             ws["gate_up"].forward(o_out, act, alpha=self.alpha_h, stream=stream)
             ws["down"].forward(act[:, :self.ffn], h, alpha=self.alpha_f, stream=stream)
 
@@ -196,8 +227,9 @@ class DecodeStack:
             if not self.torch.cuda.is_current_stream_capturing():
                 self._grow([1] * self.m)
             self.lengths.add_(1)
+            self.given.add_(1)
         self._layers(self.h0, self.h, self.qkv_out, self.attn if self.caches else None,
-                     self.o_out, self.act, None, stream)
+                     self.o_out, self.act, None, self._positions(None, self.m), stream)
         self.lm_head.forward(self.h, self.logits, alpha=self.alpha_h, stream=stream)
         return self.logits
 
@@ -213,10 +245,11 @@ class DecodeStack:
         ends = n.cumsum(0, dtype=torch.int32)
         starts = torch.cat([torch.zeros_like(ends[:1]), ends])
         self.lengths.add_(n)
+        self.given.add_(n)
         x, qkv, attn, o, act = (torch.empty((rows, c), dtype=torch.bfloat16, device=self.dev)
                                 for c in (self.hidden, self.qkv, self.hidden, self.hidden,
                                           self.act.shape[1]))
-        self._layers(h, x, qkv, attn, o, act, starts, None)
+        self._layers(h, x, qkv, attn, o, act, starts, self._positions(ends, rows), None)
         self.h.copy_(x[(ends - 1).long()])
         self.lm_head.forward(self.h, self.logits, alpha=self.alpha_h)
         return self.logits
