@@ -107,6 +107,28 @@ def test_appends_refuse_more_workgroups_than_a_launch_has(calls, uh, bits):
         assert st == uh.Status.UNSUPPORTED and "spans" in s.text()
 
 
+@pytest.mark.parametrize("name", ["attend", "attend_plan"])
+def test_the_scale_of_scores(calls, name):
+    for scale in (1e30, -1e30, 3e38):
+        st, text = calls.call(name, scale=scale)
+        assert st == "INVALID_ARGUMENT" and "scale" in text
+        assert calls.call(name, cache="eight", scale=1e30)[0] == "OK"
+    for scale in (6e29, -6e29, 0.0, 1e-38):
+        assert calls.call(name, scale=scale)[0] == "OK"
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("rows", [2, 200])
+def test_scales_of_scores_at_their_ends(uh, gpu, rows):
+    """Scores of 0 whatever the scale, and scores that are all alike."""
+    p = Pair(uh, gpu, [300], heads=2, bt=64, seed=22, spare=WIDE // 64)
+    size = torch.exp2(torch.randint(-6, 7, (300, 1, 1), device=gpu).float())
+    p.append([300], v=(p.random(300, 2).float() * size).bfloat16())
+    for scale in (6e29, -6e29, 0.0, 1e-38):
+        q = p.random(rows, 8)
+        p.check_attend([rows], 8, q=torch.zeros_like(q) if scale else q, scale=scale)
+
+
 # --------------------------------------------------------------------- plans
 
 @pytest.mark.parametrize("counts,heads,lengths,few,parts", [

@@ -43,6 +43,8 @@ ullm_status_t lookup_cache(const ullm_kv_cache_t *c, ullm_error_sink_t *sink) {
   return ULLM_STATUS_OK;
 }
 
+bool four_bits(const ullm_kv_cache_t *c) { return (c->flags & ULLM_KV_CACHE_4_BITS) != 0; }
+
 ullm_status_t fail(ullm_error_sink_t *sink, const char *message) {
   return write_error(sink, ULLM_STATUS_INVALID_ARGUMENT, message);
 }
@@ -92,8 +94,6 @@ ullm_status_t validate_seqs(const ullm_kv_cache_t *c, const ullm_kv_sequences_t 
   }
   return ULLM_STATUS_OK;
 }
-
-bool four_bits(const ullm_kv_cache_t *c) { return (c->flags & ULLM_KV_CACHE_4_BITS) != 0; }
 
 bool no_work(const ullm_kv_sequences_t &s) { return s.batch == 0 || s.rows == 0; }
 
@@ -247,6 +247,10 @@ ullm_status_t validate_attend(const ullm_kv_cache_attend_desc_t *d, ullm_error_s
   }
   if (!std::isfinite(log2_scale(d->scale))) {
     return fail(sink, "scale must be finite, and in units of log2 too");
+  }
+  // Scales of values enter the scores in units of this one.
+  if (four_bits(c) && std::fabs(log2_scale(d->scale)) > 0x1p100f) {
+    return fail(sink, "scale must not pass 2^99 with a cache of 4 bits");
   }
   for (const uint64_t s :
        {d->q_row_stride, d->q_head_stride, d->out_row_stride, d->out_head_stride}) {

@@ -107,15 +107,6 @@ __device__ __forceinline__ float largest_log2(uint32_t scales) {
   const uint32_t most = min(max(scales & 0xffffu, scales >> 16), uint32_t(kScaleMostBits));
   return __builtin_amdgcn_logf(fmaxf(f16_to_f32(uint16_t(most)), kScaleLeast));
 }
-// Whether one of eight scales is NaN.
-__device__ __forceinline__ bool any_nan(u32x4 scales) {
-  uint32_t w = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    w |= (scales[i] & 0x7fff7fffu) + 0x03ff03ffu;  // past infinity: a carry into the sign
-  }
-  return (w & 0x80008000u) != 0;
-}
 // log2 of a scale in a word's lower or upper half.  Also of what has none: the
 // zero of a token that was never written, NaN; their tokens have a score and a
 // share of the sum like any other.
@@ -318,17 +309,35 @@ struct Many4 {
   static constexpr uint32_t kSlot = kCodes + 1024, kLds = kStages * 2 * kSlot;
 };
 
+// Scales.  Token t's scale s_t enters where the matrix instructions take it for
+// nothing: a score starts as log2(s_t) / scale, so that its power is p' = p * s_t at
+// once and the largest of what the row has is the reference; the sum takes p' / s_t.
+// A wave makes both numbers for a step, a token to a lane, and reads them back as
+// the 16 of each lane's results.  (Against the product p * s in f16, with the
+// reference checked by a bound: 13 instructions fewer of 160 for 32 x 32, prompts of
+// 4096 and 3001 tokens of 32 and 8 heads 248 us against 262.)
+//
+// What bounds it: 16 matrix instructions of 32 cycles and 148 others of 4 and more
+// for 32 rows x 32 tokens, at the clock that they leave the card: 990 TFLOP/s in long
+// parts (1024 rows at 140000 tokens, 2.37 ms), 800 to 920 where tiles are few or end
+// early.  The next chunk's scores beside this one's powers, in two waves to a SIMD:
+// level in parts, 9 % slower in prompts.  A fourth wave with 64 dims: level.
+//
 // LONG: a part may have more blocks than LDS holds entries of, which are then
-// replaced on the way.
+// replaced on the way; two waves to a SIMD then have their registers (1 % faster
+// than three that spill).
 template <int D, bool LONG>
-__global__ __launch_bounds__(kWaves * kWave, 3) void many_rows4_kernel(KvAttendArgs a, Scratch x,
-                                                                       uint32_t each_slots) {
+__global__ __launch_bounds__(kWaves * kWave, LONG ? 2 : 3) void many_rows4_kernel(
+    KvAttendArgs a, Scratch x, uint32_t each_slots) {
   using Chunk = Kv4Chunk<D>;
   constexpr uint32_t kSlot = Many4<D>::kSlot;
   extern __shared__ __align__(1024) uint8_t many_ring4[];
   const auto ring = [](uint32_t stage) { return many_ring4 + stage * 2 * kSlot; };
   // Where a block's chunks start; one out of the pool has the first one's, plus 1.
   __shared__ uint64_t entries[kManyBlocks];
+  // Of a wave and the 64 tokens of a step: log2(scale) in units of scores, and
+  // 1 / scale.
+  __shared__ __align__(16) float tables[kWaves][2][64];
   const uint32_t kvh = blockIdx.x % a.pool.heads;
   const uint32_t rest = blockIdx.x / a.pool.heads, slots = gridDim.x / a.pool.heads / x.parts;
   const uint32_t part = rest % x.parts;
@@ -436,7 +445,13 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows4_kernel(KvAttendA
   const uint32_t exp_at = opaque_u32(Chunk::kExps + kv4_exp_byte(tok, D / 2 * h));
   const uint32_t value_at =
       opaque_u32(Chunk::kSide + kv4_value_dword(h, D / 2 * (i / 16) + i % 16));
-  const uint32_t scale_at = opaque_u32(Chunk::kScales + 16 * h);
+  const float per_score = 1.0f / a.scale_log2;
+  const uint32_t table_at = opaque_u32(wave * 512 + 32 * h);
+  // Four entries, of the tokens of elements e .. e + 3 in chunk u of the step.
+  const auto token_table = [&](uint32_t side, uint32_t u, uint32_t e) {
+    return *reinterpret_cast<const f32x4 *>(reinterpret_cast<const uint8_t *>(tables) + table_at +
+                                            256 * side + 128 * u + 64 * (e / 8) + 4 * (e % 8));
+  };
   for (uint32_t step = 0; step < steps; ++step) {
     wait_copies<0>();
     step_barrier();
@@ -451,6 +466,18 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows4_kernel(KvAttendA
         __syncthreads();
       }
       next = start_step(grp0, ring((step + 1) % kStages));
+    }
+    {  // each lane's token of the step's 64
+      const float scale = f16_to_f32(*reinterpret_cast<const uint16_t *>(
+          stage + lane / 32 * kSlot + Chunk::kScales + 2 * (lane % 32)));
+      // Of a token that was never written, 0, as of the least; of NaN the score is
+      // NaN, and the reciprocal beside a weight of 0 still a number.
+      const float sure = fmaxf(scale, kScaleLeast);
+      float *const to = &tables[wave][0][lane];
+      to[0] = __builtin_amdgcn_logf(sure) * per_score + (scale - scale);
+      to[64] = __builtin_amdgcn_rcpf(sure);
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
     }
 #pragma unroll
     for (uint32_t u = 0; u < 2; ++u) {
@@ -474,16 +501,20 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows4_kernel(KvAttendA
         keys[0] = u32x4{w0.x, w0.y, w1.x, w1.y};
         power[0] = bits_f32(uint32_t(chunk[exp_at]) << 23);
       }
+      f32x16 s;
+#pragma unroll
+      for (uint32_t e = 0; e < 16; e += 4) {
+        const f32x4 w = token_table(0, u, e);
+        s[e] = w[0], s[e + 1] = w[1], s[e + 2] = w[2], s[e + 3] = w[3];
+      }
       __builtin_amdgcn_sched_barrier(0);
-      f32x16 s = f32x16{};
 #pragma unroll
       for (uint32_t c = 0; c < D / 16; ++c) {
         s = mfma32_bf16(codes4_to_bf16(keys[c / 4][c % 4], power[c / 4]), q[c], s);
       }
-      u32x4 scales[2], values[2];
+      u32x4 values[2];
 #pragma unroll
       for (uint32_t c = 0; c < 2; ++c) {
-        scales[c] = *reinterpret_cast<const u32x4 *>(chunk + scale_at + c * 32);
         if constexpr (D == 128) {
           values[c] = *reinterpret_cast<const u32x4 *>(chunk + value_at + c * 512);
         } else {
@@ -493,21 +524,11 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows4_kernel(KvAttendA
       }
       const uint32_t gone = absent >> u << 31;
       if (((grp - whole.first) | gone) >= whole.count) {
-        const auto seen = [&](int e) {
-          const int32_t at =
-              int32_t(grp * 32) + int32_t((e / 4 % 2) * 16 + e / 8 * 8 + 4 * h + e % 4);
-          return gone == 0 && at <= pos && at > oldest;
-        };
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          s[e] = seen(e) ? s[e] : -INFINITY;
-        }
-        if (__any(any_nan(scales[0]) || any_nan(scales[1]))) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const uint32_t w = scales[e / 8][e % 8 / 2];
-            scales[e / 8][e % 8 / 2] = seen(e) ? w : w & (e % 2 == 0 ? 0xffff0000u : 0x0000ffffu);
-          }
+          const int32_t at =
+              int32_t(grp * 32) + int32_t((e / 4 % 2) * 16 + e / 8 * 8 + 4 * h + e % 4);
+          s[e] = gone == 0 && at <= pos && at > oldest ? s[e] : -INFINITY;
         }
       }
       float top = s[0];
@@ -515,20 +536,11 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows4_kernel(KvAttendA
       for (int e = 1; e < 16; ++e) {
         top = fmaxf(top, s[e]);
       }
-      const uint32_t most = max_scales(max_scales(max_scales(scales[0].x, scales[0].y),
-                                            max_scales(scales[0].z, scales[0].w)),
-                                    max_scales(max_scales(scales[1].x, scales[1].y),
-                                            max_scales(scales[1].z, scales[1].w)));
-      if (__any(__builtin_fmaf(top, a.scale_log2, largest_log2(most)) > limit)) {
-        float now = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          now = fmaxf(now, __builtin_fmaf(s[e], a.scale_log2,
-                                          scale_log2_of(scales[e / 8][e % 8 / 2], e % 2)));
-        }
+      top *= a.scale_log2;
+      if (__any(top > limit)) {
         const auto both =
-            __builtin_amdgcn_permlane32_swap(f32_bits(now), f32_bits(now), false, false);
-        now = fmaxf(m, fmaxf(bits_f32(both[0]), bits_f32(both[1])));
+            __builtin_amdgcn_permlane32_swap(f32_bits(top), f32_bits(top), false, false);
+        const float now = fmaxf(m, fmaxf(bits_f32(both[0]), bits_f32(both[1])));
         const float keep = now == -INFINITY ? 1.f : exp2_fast(m - now);
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
@@ -542,12 +554,16 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows4_kernel(KvAttendA
       u32x4 p[2];
       float sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        const float p0 = exp2_fast(__builtin_fmaf(s[e], a.scale_log2, bias));
-        const float p1 = exp2_fast(__builtin_fmaf(s[e + 1], a.scale_log2, bias));
-        sum += p0;
-        sum += p1;
-        p[e / 8][e % 8 / 2] = scaled_weights(p0, p1, scales[e / 8][e % 8 / 2]);
+      for (int e = 0; e < 16; e += 4) {
+        const f32x4 per = token_table(1, u, e);
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+          const float p0 = exp2_fast(__builtin_fmaf(s[e + j], a.scale_log2, bias));
+          const float p1 = exp2_fast(__builtin_fmaf(s[e + j + 1], a.scale_log2, bias));
+          sum = __builtin_fmaf(p0, per[j], sum);
+          sum = __builtin_fmaf(p1, per[j + 1], sum);
+          p[e / 8][e % 8 / 2 + j / 2] = f32x2_to_f16x2(p0, p1);
+        }
       }
       l += sum;
 #pragma unroll
@@ -556,9 +572,6 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void many_rows4_kernel(KvAttendA
 #pragma unroll
         for (uint32_t n = 0; n < D / 32; ++n) {
           o[n] = mfma32_f16(codes4_to_f16(values[c][n]), b, o[n]);
-          if (n % 2 == 1) {
-            __builtin_amdgcn_sched_barrier(0);
-          }
         }
       }
     }
