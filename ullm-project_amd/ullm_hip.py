@@ -889,28 +889,40 @@ class KvCache:
         ``pair_axes`` (uint8 [pairs]) for the axis of each pair."""
         heads, dim, here = self.kv_heads, self.head_dim, self.device
         torch = _torch_module or _torch()
-        for t in (q, k, v, lengths, tables, inv_freq, starts, positions, pair_axes, out, weights):
-            if t is not None and t.get_device() != here:
-                raise self._elsewhere()
+        if k.get_device() != here or v.get_device() != here or lengths.get_device() != here \
+                or tables.get_device() != here or inv_freq.get_device() != here \
+                or q is not None and q.get_device() != here \
+                or out is not None and out.get_device() != here \
+                or starts is not None and starts.get_device() != here \
+                or positions is not None and positions.get_device() != here \
+                or pair_axes is not None and pair_axes.get_device() != here \
+                or weights is not None and weights.get_device() != here:
+            raise self._elsewhere()
         rows, k_row, k_head = _strides3(k, "k", heads, dim)
         v_rows, v_row, v_head = _strides3(v, "v", heads, dim)
         if v_rows != rows:
             raise ValueError("k and v must have the same number of rows")
-        if weights is not None and (weights.shape != (rows, heads)
-                                    or weights.dtype is not torch.float32
-                                    or not weights.is_contiguous()):
+        if weights is None:
+            at_weights = 0
+        elif weights.shape != (rows, heads) or weights.dtype is not torch.float32 \
+                or not weights.is_contiguous():
             raise ValueError("weights must be a contiguous float32 [rows][kv_heads] tensor")
-        if len(inv_freq.shape) != 1 or inv_freq.dtype is not torch.float32 \
+        else:
+            at_weights = weights.data_ptr()
+        if inv_freq.dim() != 1 or inv_freq.dtype is not torch.float32 \
                 or not inv_freq.is_contiguous():
             raise ValueError("inv_freq must be a contiguous float32 [pairs] tensor")
-        pairs, axes, at_axes = inv_freq.shape[0], 1, 0
-        if pair_axes is not None:
-            if pair_axes.shape != (pairs,) or pair_axes.dtype is not torch.uint8 \
-                    or not pair_axes.is_contiguous():
-                raise ValueError("pair_axes must be a contiguous uint8 [pairs] tensor")
+        pairs, axes, position_stride = inv_freq.numel(), 1, 0
+        if pair_axes is None:
+            at_axes = 0
+        elif pair_axes.shape != (pairs,) or pair_axes.dtype is not torch.uint8 \
+                or not pair_axes.is_contiguous():
+            raise ValueError("pair_axes must be a contiguous uint8 [pairs] tensor")
+        else:
             at_axes = pair_axes.data_ptr()
-        at_positions, position_stride = 0, 0
-        if positions is not None:
+        if positions is None:
+            at_positions = 0
+        else:
             shape = positions.shape
             if positions.dtype is not torch.int32 or len(shape) not in (1, 2) \
                     or shape[-1] != rows or (rows > 1 and positions.stride(-1) != 1):
@@ -924,31 +936,31 @@ class KvCache:
         if q is None:
             if out is not None:
                 raise ValueError("out needs q")
-            q_fields = (0,) * 6
-            q_heads = 0
+            q_at = q_row = q_head = out_at = out_row = out_head = q_heads = 0
         else:
-            if len(q.shape) != 3:
-                raise ValueError(f"q must be bfloat16 [rows][heads][{dim}]")
-            q_heads = q.shape[1]
+            shape = q.shape
+            if len(shape) != 3 or shape[1] == 0:
+                raise ValueError(f"q must be bfloat16 [rows][heads][{dim}], with heads")
+            q_heads = shape[1]
             q_rows, q_row, q_head = _strides3(q, "q", q_heads, dim)
-            if out is None:
-                out = torch.empty_like(q) if q.is_contiguous() else \
-                    q.new_empty((rows, q_heads, dim))
-                out_rows, out_row, out_head = rows, 0, 0
-            else:
+            if out is q:
+                out_rows, out_row, out_head = rows, q_row, q_head
+            elif out is not None:
                 out_rows, out_row, out_head = _strides3(out, "out", q_heads, dim)
+            else:
+                # empty_like keeps the order of q's dims, so it is for contiguous ones.
+                out = torch.empty_like(q) if q.is_contiguous() else \
+                    q.new_empty((q_rows, q_heads, dim))
+                out_rows, out_row, out_head = rows, 0, 0
             if q_rows != rows or out_rows != rows:
                 raise ValueError("q, k, v and out must have the same number of rows")
-            if q_heads == 0:
-                raise ValueError("q must have heads")
-            q_fields = (q.data_ptr(), q_row, q_head, out.data_ptr(), out_row, out_head)
+            q_at, out_at = q.data_ptr(), out.data_ptr()
         _packed(KvAppendRotaryDesc).call(
             lib().ullm_kv_cache_append_rotary,
-            self.handle or 0, *self._seqs(lengths, tables, rows, starts), *q_fields,
-            k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head,
-            0 if weights is None else weights.data_ptr(), inv_freq.data_ptr(), at_positions,
-            position_stride, at_axes, q_heads, 2 * pairs, axes,
-            KV_ROTARY_INTERLEAVED if interleaved else 0, _stream(stream) or 0)
+            self.handle or 0, *self._seqs(lengths, tables, rows, starts), q_at, q_row, q_head,
+            out_at, out_row, out_head, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head,
+            at_weights, inv_freq.data_ptr(), at_positions, position_stride, at_axes, q_heads,
+            2 * pairs, axes, KV_ROTARY_INTERLEAVED if interleaved else 0, _stream(stream) or 0)
         return out
 
     def _gatherable(self, lengths, tables, rows, starts):
