@@ -17,7 +17,7 @@
  * each pair's axis.
  *
  * Angles are reduced to a turn, and their cosines and sines taken, in 64 bits:
- * position 2^31 - 1 is as exact as position 1.  Queries are then rotated in f32
+ * position 2^31 - 1 is as exact as position 1 (for frequencies up to 2^16).  Queries are then rotated in f32
  * and rounded to bf16.  Keys are rotated in 64 bits and rounded once, to their
  * codes (in caches of 8 and of 4 bits), so that a key between two codes does not
  * depend on the last bits of an f32.
