@@ -137,6 +137,16 @@ template <int D, uint32_t T>
 struct SpanTurns {
   Turn at[T][8][D / 16];
 };
+// That of a token's pair.
+__device__ __forceinline__ Turn turn_of_pair(const KvRotary &r, const Span &s, uint32_t t,
+                                             uint32_t j) {
+  const float f = r.inv_freq[j];
+  const uint32_t axis = r.pair_axes == nullptr ? 0u : min(uint32_t(r.pair_axes[j]), r.axes - 1);
+  return turn_of(r.positions == nullptr ? int32_t(s.base + t)
+                                        : r.positions[axis * r.position_stride +
+                                                      uint64_t(s.row0 + t)],
+                 f);
+}
 template <int D, uint32_t T>
 __device__ __forceinline__ void span_turns(const KvRotary &r, const Span &s,
                                            SpanTurns<D, T> *turns) {
@@ -144,12 +154,8 @@ __device__ __forceinline__ void span_turns(const KvRotary &r, const Span &s,
   if (j >= r.dims / 2) {
     return;
   }
-  const float f = r.inv_freq[j];
-  const uint32_t axis = r.pair_axes == nullptr ? 0u : min(uint32_t(r.pair_axes[j]), r.axes - 1);
-  const int32_t *at = r.positions + axis * r.position_stride;
   for (uint32_t t = s.lo + threadIdx.x / (D / 2); t < s.hi; t += kSpanThreads<D, T> / (D / 2)) {
-    turns->at[t][j % 8][j / 8] =
-        turn_of(r.positions == nullptr ? int32_t(s.base + t) : at[s.row0 + t], f);
+    turns->at[t][j % 8][j / 8] = turn_of_pair(r, s, t, j);
   }
 }
 
@@ -327,6 +333,69 @@ struct Rotation {
     __syncthreads();
   }
 };
+// The same of a span so short that each pair of a row has a thread: a thread makes
+// its turn itself and rotates one pair of each row (the key's first, if there are
+// `keys`, then the queries').  A token then takes a tenth of the instructions in a
+// row that a thread with eight pairs has: what a single token waits for.
+template <int D, uint32_t T>
+__device__ __forceinline__ bool few_pairs(const Span &s) {
+  return (s.hi - s.lo) * (D / 2) <= kSpanThreads<D, T>;
+}
+template <int D, uint32_t T>
+__device__ __forceinline__ void rotate_pairs(const KvRotateArgs &a, const Span &s, uint32_t head,
+                                             KeyImage<D, T> *keys) {
+  const uint32_t n = (s.hi - s.lo) * (D / 2), step = kSpanThreads<D, T> / n;
+  const uint32_t lot = threadIdx.x / n, i = threadIdx.x % n;
+  const uint32_t t = s.lo + i / (D / 2), j = i % (D / 2);
+  uint32_t m = lot < step ? lot : kNoHead;  // row 0: the key
+  if (keys == nullptr && m == 0) {
+    m = step;
+  }
+  const PairDims d = pair_dims(j, a.rotary.dims, a.rotary.interleaved);
+  const uint64_t row = uint64_t(s.row0 + t);
+  uint32_t x = 0, y = 0;
+  const auto load = [&] {
+    if (m <= a.group) {
+      const uint16_t *from = m == 0 ? a.append.k + row * a.append.k_row + head * a.append.k_head
+                                    : a.q + row * a.q_row +
+                                          (uint64_t(head) * a.group + m - 1) * a.q_head;
+      x = from[d.first];
+      y = from[d.second];
+    }
+  };
+  load();
+  const bool live = j < a.rotary.dims / 2;
+  Turn w = {1.0, 0.0};
+  if (live) {
+    w = turn_of_pair(a.rotary, s, t, j);
+  }
+  const float c = float(w.c), sn = float(w.s);
+  while (m <= a.group) {
+    const float u = bits_f32(x << 16), v = bits_f32(y << 16);
+    if (m == 0) {
+      keys->x[t][d.first] = live ? to_odd(fma(double(u), w.c, -(double(v) * w.s))) : u;
+      keys->x[t][d.second] = live ? to_odd(fma(double(v), w.c, double(u) * w.s)) : v;
+    } else {
+      uint16_t *to = a.q_out + row * a.out_row + (uint64_t(head) * a.group + m - 1) * a.out_head;
+      to[d.first] = f32_to_bf16(live ? __builtin_fmaf(u, c, -(v * sn)) : u);
+      to[d.second] = f32_to_bf16(live ? __builtin_fmaf(v, c, u * sn) : v);
+    }
+    m += step;
+    load();
+  }
+  __syncthreads();
+}
+// A span's queries to memory, and its keys (if it has any) to an image in `lds`.
+template <int D, uint32_t T>
+__device__ __forceinline__ void rotate_span(const KvRotateArgs &a, const Span &s, uint32_t head,
+                                            uint8_t *lds, bool has_keys) {
+  KeyImage<D, T> *const keys = has_keys ? reinterpret_cast<KeyImage<D, T> *>(lds) : nullptr;
+  if (few_pairs<D, T>(s)) {
+    rotate_pairs<D, T>(a, s, head, keys);
+  } else {
+    Rotation<D, T>(a, s, head, has_keys).run(reinterpret_cast<SpanTurns<D, T> *>(lds), keys);
+  }
+}
 // Sixteen elements of a rotated row.
 template <int D, uint32_t T>
 __device__ __forceinline__ void read_row(const KeyImage<D, T> &keys, uint32_t t, uint32_t c,
@@ -398,8 +467,7 @@ __global__ __launch_bounds__(kThreads) void append4_kernel(KvRotateArgs ra, uint
   float k[16], v[16];
   if constexpr (ROTATE) {
     KeyImage<D, 32> *const rotated = reinterpret_cast<KeyImage<D, 32> *>(lds);
-    Rotation<D, 32>(ra, s, head, id >= 0)
-        .run(reinterpret_cast<SpanTurns<D, 32> *>(lds), id >= 0 ? rotated : nullptr);
+    rotate_span<D, 32>(ra, s, head, lds, id >= 0);
     if (id < 0) {
       return;
     }
@@ -486,8 +554,7 @@ __global__ __launch_bounds__((kSpanThreads<D, bt>)) void append8_rotary_kernel(
   if (live) {
     y[0] = load16(a.v + head * a.v_head + uint64_t(s.row0 + t) * a.v_row + c * 16, a.vec);
   }
-  Rotation<D, bt>(ra, s, head, id >= 0)
-      .run(reinterpret_cast<SpanTurns<D, bt> *>(append8_lds), id >= 0 ? rotated : nullptr);
+  rotate_span<D, bt>(ra, s, head, append8_lds, id >= 0);
   if (id < 0) {
     return;
   }
