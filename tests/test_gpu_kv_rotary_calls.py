@@ -29,6 +29,35 @@ def test_rows_of_no_sequence_are_left_alone(uh, gpu, bits):
 
 
 @pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dim,bt", [(64, 32), (64, 128), (128, 32), (128, 64), (128, 128)])
+def test_the_same_number_of_rows_each(uh, gpu, bits, dim, bt):
+    """Without starts: on both sides of where each pair of a sequence's rows has a
+    thread of its own, across the ends of chunks and blocks, before the first
+    token and in places of no block, against the same call with starts."""
+    lengths = [0, 1, 3, 33, bt, bt + 2, 200]
+    p, twin = (pair(bits, uh, gpu, lengths, heads=2, dim=dim, bt=bt, seed=6, spare=1)
+               for _ in range(2))
+    p.tables[6, 0] = twin.tables[6, 0] = -1
+    f = freqs(gpu, dim // 2)
+    for i, each in enumerate((1, 2, 4, 5, 8, 9, 16)):
+        now = [n + i for n in lengths]
+        q, k, v = p.random(7 * each, 6), p.random(7 * each, 2), p.random(7 * each, 2)
+        at = p.rs.integers(0, 10 ** 6, (2, 7 * each))
+        axes = np.arange(dim // 2) % 2
+        kw = dict(positions=at, axes=axes, interleaved=True) if i % 2 else {}
+        want = check(twin, [each] * 7, 6, f, lengths=now, q=q, k=k, v=v, stored=False, **kw)
+        got = p.cache.append_rotary(
+            q, k, v, p.dev(now), p.dev(p.tables), f, interleaved=bool(i % 2),
+            positions=p.dev(at) if i % 2 else None,
+            pair_axes=p.dev(axes, torch.uint8) if i % 2 else None)
+        assert torch.equal(got, want), each
+        twin.check_stored(lengths=now)
+        for a, b in zip(*(c.cache.gather(c.dev(now), c.dev(c.tables), sum(now),
+                                         starts=c.starts(now)) for c in (p, twin))):
+            assert torch.equal(a, b), each
+
+
+@pytest.mark.parametrize("bits", [4, 8])
 def test_lengths_past_the_tables(uh, gpu, bits):
     """They are taken as the tables' end, places too."""
     p = pair(bits, uh, gpu, [64, 128], heads=1, dim=64, bt=64, seed=2, spare=0)

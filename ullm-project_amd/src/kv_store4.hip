@@ -121,14 +121,14 @@ constexpr uint32_t kSpanThreads = T * (D / 16) > kThreads ? T * (D / 16) : kThre
 // `head` + step and so on; none where `head` is kNoHead.
 constexpr uint32_t kNoHead = ~0u;
 struct Lot {
-  uint32_t t, u, head, step;
+  uint32_t t, row, u, head, step;  // row: t counted from lo
 };
 template <int D, uint32_t T>
 __device__ __forceinline__ Lot lot_of(const Span &s) {
   constexpr uint32_t kUnits = D / 16;
   const uint32_t n = (s.hi - s.lo) * kUnits, step = kSpanThreads<D, T> / n;
   const uint32_t head = threadIdx.x / n, i = threadIdx.x % n;
-  return {s.lo + i / kUnits, i % kUnits, head < step ? head : kNoHead, step};
+  return {s.lo + i / kUnits, i / kUnits, i % kUnits, head < step ? head : kNoHead, step};
 }
 
 // Cosines and sines of a span: pair j of token t is at [t][j % 8][j / 8], where
@@ -251,7 +251,7 @@ __device__ __forceinline__ void rotate_query(uint16_t *row, const RawPairs &p, c
   }
 }
 
-// Rows of rotated keys in LDS.
+// Rows of a span's rotated keys in LDS, its first new token's first.
 template <int D, uint32_t T>
 struct KeyImage {
   alignas(16) float x[T][D + 4];
@@ -268,8 +268,8 @@ __device__ __forceinline__ void rotate_key(KeyImage<D, T> *to, const RawPairs &p
     const PairXY e = raw_pair(p, side, i);
     const double x = e.x, y = e.y, c = v.w[i].c, s = v.w[i].s;
     const bool live = (v.live >> i & 1u) != 0;
-    to->x[lot.t][d.first] = live ? to_odd(fma(x, c, -(y * s))) : e.x;
-    to->x[lot.t][d.second] = live ? to_odd(fma(y, c, x * s)) : e.y;
+    to->x[lot.row][d.first] = live ? to_odd(fma(x, c, -(y * s))) : e.x;
+    to->x[lot.row][d.second] = live ? to_odd(fma(y, c, x * s)) : e.y;
   }
 }
 
@@ -337,22 +337,20 @@ struct Rotation {
 // its turn itself and rotates one pair of each row (the key's first, if there are
 // `keys`, then the queries').  A token then takes a tenth of the instructions in a
 // row that a thread with eight pairs has: what a single token waits for.
-template <int D, uint32_t T>
-__device__ __forceinline__ bool few_pairs(const Span &s) {
-  return (s.hi - s.lo) * (D / 2) <= kSpanThreads<D, T>;
-}
-template <int D, uint32_t T>
+template <int D, uint32_t THREADS>
+constexpr uint32_t kFewTokens = THREADS / (D / 2);  // most tokens of such a span
+template <int D, uint32_t THREADS, uint32_t T>
 __device__ __forceinline__ void rotate_pairs(const KvRotateArgs &a, const Span &s, uint32_t head,
                                              KeyImage<D, T> *keys) {
-  const uint32_t n = (s.hi - s.lo) * (D / 2), step = kSpanThreads<D, T> / n;
+  const uint32_t n = (s.hi - s.lo) * (D / 2), step = THREADS / n;
   const uint32_t lot = threadIdx.x / n, i = threadIdx.x % n;
-  const uint32_t t = s.lo + i / (D / 2), j = i % (D / 2);
+  const uint32_t t = i / (D / 2), j = i % (D / 2);  // the span's token t, pair j
   uint32_t m = lot < step ? lot : kNoHead;  // row 0: the key
   if (keys == nullptr && m == 0) {
     m = step;
   }
   const PairDims d = pair_dims(j, a.rotary.dims, a.rotary.interleaved);
-  const uint64_t row = uint64_t(s.row0 + t);
+  const uint64_t row = uint64_t(s.row0 + s.lo + t);
   uint32_t x = 0, y = 0;
   const auto load = [&] {
     if (m <= a.group) {
@@ -367,7 +365,7 @@ __device__ __forceinline__ void rotate_pairs(const KvRotateArgs &a, const Span &
   const bool live = j < a.rotary.dims / 2;
   Turn w = {1.0, 0.0};
   if (live) {
-    w = turn_of_pair(a.rotary, s, t, j);
+    w = turn_of_pair(a.rotary, s, s.lo + t, j);
   }
   const float c = float(w.c), sn = float(w.s);
   while (m <= a.group) {
@@ -390,19 +388,19 @@ template <int D, uint32_t T>
 __device__ __forceinline__ void rotate_span(const KvRotateArgs &a, const Span &s, uint32_t head,
                                             uint8_t *lds, bool has_keys) {
   KeyImage<D, T> *const keys = has_keys ? reinterpret_cast<KeyImage<D, T> *>(lds) : nullptr;
-  if (few_pairs<D, T>(s)) {
-    rotate_pairs<D, T>(a, s, head, keys);
+  if (s.hi - s.lo <= kFewTokens<D, kSpanThreads<D, T>>) {
+    rotate_pairs<D, kSpanThreads<D, T>>(a, s, head, keys);
   } else {
     Rotation<D, T>(a, s, head, has_keys).run(reinterpret_cast<SpanTurns<D, T> *>(lds), keys);
   }
 }
 // Sixteen elements of a rotated row.
 template <int D, uint32_t T>
-__device__ __forceinline__ void read_row(const KeyImage<D, T> &keys, uint32_t t, uint32_t c,
+__device__ __forceinline__ void read_row(const KeyImage<D, T> &keys, uint32_t row, uint32_t c,
                                          float (&k)[16]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const f32x4 w = *reinterpret_cast<const f32x4 *>(&keys.x[t][c * 16 + 4 * j]);
+    const f32x4 w = *reinterpret_cast<const f32x4 *>(&keys.x[row][c * 16 + 4 * j]);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       k[4 * j + e] = w[e];
@@ -410,6 +408,9 @@ __device__ __forceinline__ void read_row(const KeyImage<D, T> &keys, uint32_t t,
   }
 }
 constexpr size_t larger(size_t a, size_t b) { return a > b ? a : b; }
+
+// What an append rotates: nothing, spans of any size, or such as kFewTokens names.
+enum Turning { kTurnNone, kTurnAny, kTurnFew };
 
 // --------------------------------------------------------------- append, 4 bits
 
@@ -419,15 +420,16 @@ constexpr size_t larger(size_t a, size_t b) { return a > b ? a : b; }
 // from LDS, to their codes and memory; values' codes are brought into dwords of
 // eight tokens in LDS.  A dword that new tokens share with earlier ones is read
 // and written by this workgroup alone.
-template <int D, bool ROTATE>
+template <int D, Turning MODE>
 __global__ __launch_bounds__(kThreads) void append4_kernel(KvRotateArgs ra, uint32_t each_slots) {
   using Chunk = Kv4Chunk<D>;
+  using Image = KeyImage<D, MODE == kTurnFew ? kFewTokens<D, kThreads> : 32>;
   constexpr uint32_t kUnits = D / 16, kPitch = D + 16;
   static_assert(kSpanThreads<D, 32> == kThreads, "a thread for each unit");
   // Turns, and when all threads have theirs, keys and values.
-  constexpr uint32_t kImage = ROTATE ? sizeof(KeyImage<D, 32>) : 0;
+  constexpr uint32_t kImage = MODE != kTurnNone ? sizeof(Image) : 0;
   __shared__ __align__(16) uint8_t
-      lds[larger(ROTATE ? sizeof(SpanTurns<D, 32>) : 0, kImage + 32 * kPitch)];
+      lds[larger(MODE == kTurnAny ? sizeof(SpanTurns<D, 32>) : 0, kImage + 32 * kPitch)];
   uint8_t *const values = lds + kImage;  // a code to a byte
   const KvAppendArgs &a = ra.append;
   const uint32_t head = blockIdx.x % a.pool.heads, tid = threadIdx.x;
@@ -465,14 +467,18 @@ __global__ __launch_bounds__(kThreads) void append4_kernel(KvRotateArgs ra, uint
     held = *value_at;
   }
   float k[16], v[16];
-  if constexpr (ROTATE) {
-    KeyImage<D, 32> *const rotated = reinterpret_cast<KeyImage<D, 32> *>(lds);
-    rotate_span<D, 32>(ra, s, head, lds, id >= 0);
+  if constexpr (MODE != kTurnNone) {
+    Image *const rotated = reinterpret_cast<Image *>(lds);
+    if constexpr (MODE == kTurnFew) {
+      rotate_pairs<D, kThreads>(ra, s, head, id >= 0 ? rotated : nullptr);
+    } else {
+      rotate_span<D, 32>(ra, s, head, lds, id >= 0);
+    }
     if (id < 0) {
       return;
     }
     if (live) {
-      read_row<D, 32>(*rotated, t, c, k);
+      read_row(*rotated, t - s.lo, c, k);
     }
   } else {
     if (id < 0) {
@@ -527,13 +533,21 @@ __global__ __launch_bounds__(kThreads) void append4_kernel(KvRotateArgs ra, uint
 // One workgroup stores the new tokens of one block and head, as append_kernel
 // does, with keys that come rotated from LDS, and rotates the queries of its
 // group: a thread has one unit of 16 dims of the block.
-template <int D, uint32_t bt>
-__global__ __launch_bounds__((kSpanThreads<D, bt>)) void append8_rotary_kernel(
+template <int D, uint32_t bt, bool FEW>
+struct Append8 {
+  static constexpr uint32_t kAll = FEW ? kThreads : kSpanThreads<D, bt>;
+  using Image = KeyImage<D, FEW ? kFewTokens<D, kThreads> : bt>;
+  static constexpr size_t kLds =
+      larger(larger(FEW ? 0 : sizeof(SpanTurns<D, bt>), sizeof(Image)), bt * D);
+};
+template <int D, uint32_t bt, bool FEW>
+__global__ __launch_bounds__((Append8<D, bt, FEW>::kAll)) void append8_rotary_kernel(
     KvRotateArgs ra, uint32_t each_slots) {
-  constexpr uint32_t kUnits = D / 16, kAll = kSpanThreads<D, bt>;
+  using Image = typename Append8<D, bt, FEW>::Image;
+  constexpr uint32_t kUnits = D / 16, kAll = Append8<D, bt, FEW>::kAll;
   // Turns, and when all threads have theirs, rotated keys; at the end values.
   extern __shared__ __align__(16) uint8_t append8_lds[];
-  KeyImage<D, bt> *const rotated = reinterpret_cast<KeyImage<D, bt> *>(append8_lds);
+  Image *const rotated = reinterpret_cast<Image *>(append8_lds);
   const KvAppendArgs &a = ra.append;
   const uint32_t head = blockIdx.x % a.pool.heads, tid = threadIdx.x;
   const KvSlot slot = kv_find_slot(a.seqs, blockIdx.x / a.pool.heads, 1, bt, 2, each_slots);
@@ -554,14 +568,18 @@ __global__ __launch_bounds__((kSpanThreads<D, bt>)) void append8_rotary_kernel(
   if (live) {
     y[0] = load16(a.v + head * a.v_head + uint64_t(s.row0 + t) * a.v_row + c * 16, a.vec);
   }
-  rotate_span<D, bt>(ra, s, head, append8_lds, id >= 0);
+  if constexpr (FEW) {
+    rotate_pairs<D, kThreads>(ra, s, head, id >= 0 ? rotated : nullptr);
+  } else {
+    rotate_span<D, bt>(ra, s, head, append8_lds, id >= 0);
+  }
   if (id < 0) {
     return;
   }
   float x[16];
   uint32_t ak = 0, av = largest_magnitude(y);
   if (live) {
-    read_row<D, bt>(*rotated, t, c, x);
+    read_row(*rotated, t - s.lo, c, x);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {  // infinities and NaN do not count
       const uint32_t m = f32_bits(x[i]) & 0x7fffffffu;
@@ -792,43 +810,59 @@ static uint64_t append_grid(const KvAppendArgs &a, uint32_t t) {
   return kv_slots(a.seqs, 1, t, 2, each_slots(a.seqs, t)) * a.pool.heads;
 }
 uint64_t kv4_append_threads(const KvAppendArgs &a) { return append_grid(a, 32) * kThreads; }
+// Whether a workgroup of kThreads has a thread for each pair of the rows that a
+// sequence appends.  A kernel for such calls alone has half the registers and less
+// LDS, so that more of it runs at once (32 and 8 heads of 128; 256 sequences of one
+// token: 9.7 us against 11.2 in 4 bits, 10.6 against 18.6 in 8; 400 of four 28
+// against 39, 30 against 66; a single one: level).
+static bool few_each(const KvSeqs &q, uint32_t dim) {
+  return q.each != 0 && q.each <= kThreads / (dim / 2);
+}
 uint64_t kv8_append_rotary_threads(const KvAppendArgs &a, uint32_t dim) {
   const uint32_t bt = 1u << a.pool.shift;
-  return append_grid(a, bt) * larger(bt * (dim / 16), kThreads);
+  return append_grid(a, bt) *
+         (few_each(a.seqs, dim) ? kThreads : larger(bt * (dim / 16), kThreads));
 }
 
 hipError_t launch_kv4_append(const KvRotateArgs &a, uint32_t dim, hipStream_t s) {
   const uint32_t each = each_slots(a.append.seqs, 32), grid = uint32_t(append_grid(a.append, 32));
   const auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(a, each); };
-  if (a.rotary.dims != 0) {
-    launch(dim == 64 ? append4_kernel<64, true> : append4_kernel<128, true>);
+  if (a.rotary.dims == 0) {
+    launch(dim == 64 ? append4_kernel<64, kTurnNone> : append4_kernel<128, kTurnNone>);
+  } else if (few_each(a.append.seqs, dim)) {
+    launch(dim == 64 ? append4_kernel<64, kTurnFew> : append4_kernel<128, kTurnFew>);
   } else {
-    launch(dim == 64 ? append4_kernel<64, false> : append4_kernel<128, false>);
+    launch(dim == 64 ? append4_kernel<64, kTurnAny> : append4_kernel<128, kTurnAny>);
   }
   return hipGetLastError();
 }
 
-template <int D, uint32_t bt>
+template <int D, uint32_t bt, bool FEW>
 static hipError_t launch_append8(const KvRotateArgs &a, hipStream_t s) {
+  using Form = Append8<D, bt, FEW>;
   const uint32_t each = each_slots(a.append.seqs, bt), grid = uint32_t(append_grid(a.append, bt));
-  constexpr size_t lds = larger(larger(sizeof(SpanTurns<D, bt>), sizeof(KeyImage<D, bt>)), bt * D);
-  const auto kernel = append8_rotary_kernel<D, bt>;
-  const hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kernel), lds);
+  const auto kernel = append8_rotary_kernel<D, bt, FEW>;
+  const hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kernel), Form::kLds);
   if (e != hipSuccess) {
     return e;
   }
-  kernel<<<grid, kSpanThreads<D, bt>, lds, s>>>(a, each);
+  kernel<<<grid, Form::kAll, Form::kLds, s>>>(a, each);
   return hipGetLastError();
 }
+template <int D, uint32_t bt>
+static hipError_t launch_append8(const KvRotateArgs &a, hipStream_t s) {
+  return few_each(a.append.seqs, D) ? launch_append8<D, bt, true>(a, s)
+                                    : launch_append8<D, bt, false>(a, s);
+}
 hipError_t launch_kv8_append_rotary(const KvRotateArgs &a, uint32_t dim, hipStream_t s) {
-  const uint32_t bt = 1u << a.append.pool.shift;
-  const auto launch = dim == 64 ? (bt == 32   ? launch_append8<64, 32>
-                                   : bt == 64 ? launch_append8<64, 64>
-                                              : launch_append8<64, 128>)
-                                : (bt == 32   ? launch_append8<128, 32>
-                                   : bt == 64 ? launch_append8<128, 64>
-                                              : launch_append8<128, 128>);
-  return launch(a, s);
+  switch (dim + a.append.pool.shift) {
+    case 64 + 5: return launch_append8<64, 32>(a, s);
+    case 64 + 6: return launch_append8<64, 64>(a, s);
+    case 64 + 7: return launch_append8<64, 128>(a, s);
+    case 128 + 5: return launch_append8<128, 32>(a, s);
+    case 128 + 6: return launch_append8<128, 64>(a, s);
+    default: return launch_append8<128, 128>(a, s);
+  }
 }
 
 hipError_t launch_kv4_gather(const KvGatherArgs &a, uint32_t dim, hipStream_t s) {
