@@ -131,12 +131,16 @@ __device__ __forceinline__ Lot lot_of(const Span &s) {
   return {s.lo + i / kUnits, i / kUnits, i % kUnits, head < step ? head : kNoHead, step};
 }
 
-// Cosines and sines of a span: pair j of token t is at [t][j % 8][j / 8], where
-// the threads that read a pair each lie side by side.
+// Cosines and sines of a span, those of token t from t * D / 2 on: where pair 8u + i
+// is there keeps both the threads that write a token's pairs in order and those that
+// read pair i of eight apart, some tokens at a time, on banks of their own.
 template <int D, uint32_t T>
 struct SpanTurns {
-  Turn at[T][8][D / 16];
+  Turn at[T][D / 2];
 };
+__device__ __forceinline__ uint32_t turn_slot(uint32_t t, uint32_t u, uint32_t i) {
+  return 8 * (u ^ (t & 1)) + (i ^ (u & 7) ^ 2 * (t & 2));
+}
 // That of a token's pair.
 __device__ __forceinline__ Turn turn_of_pair(const KvRotary &r, const Span &s, uint32_t t,
                                              uint32_t j) {
@@ -155,7 +159,7 @@ __device__ __forceinline__ void span_turns(const KvRotary &r, const Span &s,
     return;
   }
   for (uint32_t t = s.lo + threadIdx.x / (D / 2); t < s.hi; t += kSpanThreads<D, T> / (D / 2)) {
-    turns->at[t][j % 8][j / 8] = turn_of_pair(r, s, t, j);
+    turns->at[t][turn_slot(t, j / 8, j % 8)] = turn_of_pair(r, s, t, j);
   }
 }
 
@@ -211,7 +215,7 @@ __device__ __forceinline__ Turns8 load_turns(const SpanTurns<D, T> &turns, const
   v.live = first >= pairs ? 0u : pairs - first >= 8 ? 0xffu : (1u << (pairs - first)) - 1;
 #pragma unroll
   for (uint32_t i = 0; i < 8; ++i) {
-    v.w[i] = turns.at[lot.t][i][lot.u];
+    v.w[i] = turns.at[lot.t][turn_slot(lot.t, lot.u, i)];
   }
   return v;
 }
@@ -262,14 +266,31 @@ __device__ __forceinline__ void rotate_key(KeyImage<D, T> *to, const RawPairs &p
                                            const KvRotary &r, const Turns8 &v, const Lot &lot,
                                            bool runs) {
   const bool side = side_by_side(r, lot.u, runs);
+  float a[8], b[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const PairDims d = pair_dims(8 * lot.u + uint32_t(i), r.dims, r.interleaved);
     const PairXY e = raw_pair(p, side, i);
     const double x = e.x, y = e.y, c = v.w[i].c, s = v.w[i].s;
     const bool live = (v.live >> i & 1u) != 0;
-    to->x[lot.row][d.first] = live ? to_odd(fma(x, c, -(y * s))) : e.x;
-    to->x[lot.row][d.second] = live ? to_odd(fma(y, c, x * s)) : e.y;
+    a[i] = live ? to_odd(fma(x, c, -(y * s))) : e.x;
+    b[i] = live ? to_odd(fma(y, c, x * s)) : e.y;
+  }
+  float *const row = to->x[lot.row];
+  if (runs) {
+    const PairDims d = pair_dims(8 * lot.u, r.dims, r.interleaved);
+    f32x4 *const near = reinterpret_cast<f32x4 *>(row + d.first);
+    f32x4 *const far = reinterpret_cast<f32x4 *>(row + (side ? d.first + 8 : d.second));
+    near[0] = side ? f32x4{a[0], b[0], a[1], b[1]} : f32x4{a[0], a[1], a[2], a[3]};
+    near[1] = side ? f32x4{a[2], b[2], a[3], b[3]} : f32x4{a[4], a[5], a[6], a[7]};
+    far[0] = side ? f32x4{a[4], b[4], a[5], b[5]} : f32x4{b[0], b[1], b[2], b[3]};
+    far[1] = side ? f32x4{a[6], b[6], a[7], b[7]} : f32x4{b[4], b[5], b[6], b[7]};
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      const PairDims d = pair_dims(8 * lot.u + i, r.dims, r.interleaved);
+      row[d.first] = a[i];
+      row[d.second] = b[i];
+    }
   }
 }
 
@@ -496,13 +517,14 @@ __global__ __launch_bounds__(kThreads) void append4_kernel(KvRotateArgs ra, uint
     const uint32_t top = largest16<kUnits>(v);
     const float scale = value_scale4(bits_f32(top));
     const u32x2 w = encode4_scaled(v, scale);
-    uint8_t *to = values + t * kPitch + c * 16;
+    u32x4 bytes;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {  // four codes of w to four bytes
       const uint32_t h = w[j / 2] >> (16 * (j % 2)) & 0xffffu;
       const uint32_t b = (h | h << 8) & 0x00ff00ffu;
-      reinterpret_cast<uint32_t *>(to)[j] = (b | b << 4) & 0x0f0f0f0fu;
+      bytes[j] = (b | b << 4) & 0x0f0f0f0fu;
     }
+    *reinterpret_cast<u32x4 *>(values + t * kPitch + c * 16) = bytes;
     if (c == 0) {
       *reinterpret_cast<uint16_t *>(chunk + Chunk::kScales + kv4_scale_byte(t)) =
           top >= 0x7f800000u ? uint16_t(0x7e00) : f32_to_f16(scale);
