@@ -12,14 +12,14 @@
 // over a reference M that follows the largest of score + log2(s) (not of the
 // score alone), so that the largest p' is near 2^kOff: what a token adds to the
 // result decides how exactly it enters, whatever the scales of the others.  M is
-// left alone while (largest score) + log2(largest s) of a lane's tokens, which no
-// sum passes, stays within kSlack of it; else it moves to the largest sum.  With
-// scales from 2^-19 to 2^16 the p of a row's sum stay within 2^-28 and 2^34 of
-// what they would be over the largest score, far inside f32.
+// left alone while the largest sum (few rows: (largest score) + log2(largest s) of a
+// lane's tokens, which no sum passes) stays within kSlack of it; else it moves to the
+// largest.  With scales from 2^-19 to 2^16 the p of a row's sum stay within 2^-28 and
+// 2^34 of what they would be over the largest score, far inside f32.
 //
 // NaN.  Codes are finite, NaN is in a key's exponent or a value's scale, so that
 // it can reach a row only through its score or its weight: tokens that a row
-// does not see have score -infinity and scale 0 put in their place.
+// does not see have score -infinity (few rows: and scale 0) put in their place.
 #include <algorithm>
 
 #include "kv_attend.hpp"
@@ -204,6 +204,13 @@ __device__ __forceinline__ void attend_group4(RowState4<D> &st, Group4<D> &x, co
 // One workgroup owns a part of the tokens of a tile of 16 rows of one
 // key/value head, as few_rows_kernel does: its waves take the 32-token chunks
 // in turn, each with a softmax of its own, and join them at the end.
+//
+// What bounds it: the read.  131072 tokens of 8 heads of 128 (140 MB) 24 to 25 us;
+// the loads alone, nothing computed, 24.8, 5.7 TB/s with the start and the end of a
+// launch that is short for it; 16 sequences of up to 8192 22.5, 128 of 4000 88 (6.2
+// TB/s).  Two chunks on their way to a wave 31, two workgroups to a compute unit
+// 27, loads through the caches 27.  333 tokens, 5.7: launch, three loads that
+// wait for each other, the join of the waves.
 template <int D, int W, bool NT, bool SCORES>
 __global__ __launch_bounds__(W * kWave, 3) void few_rows4_kernel(KvAttendArgs a, Scratch x,
                                                               uint32_t each_slots) {
@@ -314,10 +321,10 @@ struct Many4 {
 // once and the largest of what the row has is the reference; the sum takes p' / s_t.
 // A wave makes both numbers for a step, a token to a lane, and reads them back as
 // the 16 of each lane's results.  (Against the product p * s in f16, with the
-// reference checked by a bound: 13 instructions fewer of 160 for 32 x 32, prompts of
+// reference checked by a bound: 14 instructions fewer of 158 for 32 x 32, prompts of
 // 4096 and 3001 tokens of 32 and 8 heads 248 us against 262.)
 //
-// What bounds it: 16 matrix instructions of 32 cycles and 148 others of 4 and more
+// What bounds it: 16 matrix instructions of 32 cycles and 144 others of 4 and more
 // for 32 rows x 32 tokens, at the clock that they leave the card: 990 TFLOP/s in long
 // parts (1024 rows at 140000 tokens, 2.37 ms), 800 to 920 where tiles are few or end
 // early.  The next chunk's scores beside this one's powers, in two waves to a SIMD:
@@ -635,7 +642,9 @@ KvAttendPlan plan_kv4_attend(const KvAttendArgs &a, uint32_t dim) {
   // A wave has half the bytes on their way that it has with 8 bits: eight waves
   // where a workgroup has a compute unit to itself, for 128 dims too (131072
   // tokens of 8 heads: 25.5 us, four waves 31.9; 16 sequences of up to 8192
-  // 22.6, 30.6).
+  // 22.6, 30.6).  Beyond that level: 40 sequences of 4000 35.0 against 35.6, 64 43.4
+  // against 41.4, 128 87.9 against 88.7; 160 with 14 and 2 heads of 64 25.3 against
+  // 29.0, 256 of 1000 11.6 against 11.3.
   p.waves = p.grid <= device_cu_count() ? 8 : 4;
   return p;
 }
