@@ -129,6 +129,17 @@ def test_scales_of_scores_at_their_ends(uh, gpu, rows):
         p.check_attend([rows], 8, q=torch.zeros_like(q) if scale else q, scale=scale)
 
 
+@pytest.mark.parametrize("rows", [2, 200])
+@pytest.mark.parametrize("size", [2.0 ** -14, 1.0, 2.0 ** 12])
+def test_log_sums_of_small_and_large_values(uh, gpu, rows, size):
+    """The values' scales are in the references of the powers, not in the log-sum."""
+    p = Pair(uh, gpu, [300, 200], heads=2, bt=64, seed=23, spare=WIDE // 64)
+    p.append([300, 200], v=p.random(500, 2, std=size))
+    for scale in (None, 0.0, -0.2):
+        p.check_attend([rows, 1], 8, scale=scale)
+        p.check_attend([1, 1], 4, scale=scale)
+
+
 # --------------------------------------------------------------------- plans
 
 @pytest.mark.parametrize("counts,heads,lengths,few,parts", [

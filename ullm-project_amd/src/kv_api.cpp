@@ -318,6 +318,7 @@ ullm::KvAttendArgs attend_args(const ullm_kv_cache_attend_desc_t *d) {
   a.scale_log2 = std::max(std::fabs(log2_scale(d->scale)), 0x1p-120f);
   a.q_sign = d->scale < 0.f ? 0x80008000u : 0u;
   a.accumulate = (d->flags & ULLM_KV_ATTEND_ACCUMULATE) != 0;
+  a.whole_refs = four_bits(c);
   return a;
 }
 

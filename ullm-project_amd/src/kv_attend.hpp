@@ -218,7 +218,13 @@ __device__ __forceinline__ void store_stats(const KvAttendArgs &a, const Scratch
                                             uint32_t head, float top, float sum) {
   const uint64_t at = row * a.heads + head;
   if (a.lse != nullptr) {
-    a.lse[at] = sum == 0.f ? -INFINITY : (top + (log2f(sum) - float(kOff))) * kLn2;
+    // A whole reference and the sum's exponent cancel exactly where the log-sum is
+    // small and they are not (values of small or large scales).
+    const float log2_sum =
+        a.whole_refs ? (top + float(__builtin_amdgcn_frexp_expf(sum) - kOff)) +
+                           log2f(__builtin_amdgcn_frexp_mantf(sum))
+                     : top + (log2f(sum) - float(kOff));
+    a.lse[at] = sum == 0.f ? -INFINITY : log2_sum * kLn2;
   }
   if (x.stats != nullptr) {
     x.stats[stats_at(a, head / a.group, row) + head % a.group] = RowStats{(top == -INFINITY ? 0.f : top) - float(kOff),

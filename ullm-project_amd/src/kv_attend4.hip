@@ -14,7 +14,8 @@
 // result decides how exactly it enters, whatever the scales of the others.  M is
 // left alone while the largest sum (few rows: (largest score) + log2(largest s) of a
 // lane's tokens, which no sum passes) stays within kSlack of it; else it moves to the
-// largest.  With scales from 2^-19 to 2^16 the p of a row's sum stay within 2^-28 and
+// largest, rounded down to a whole number: what is added to a score before its power
+// is then exact, and so is what earlier sums are multiplied by.  With scales from 2^-19 to 2^16 the p of a row's sum stay within 2^-28 and
 // 2^34 of what they would be over the largest score, far inside f32.
 //
 // NaN.  Codes are finite, NaN is in a key's exponent or a value's scale, so that
@@ -169,7 +170,7 @@ __device__ __forceinline__ void attend_group4(RowState4<D> &st, Group4<D> &x, co
     for (int i = 0; i < 8; ++i) {
       now = fmaxf(now, s[i / 4][i % 4] + scale_log2_of(x.scales[i / 2], i % 2));
     }
-    now = fmaxf(st.m, max_groups(now));
+    now = fmaxf(st.m, floorf(max_groups(now)));
     const float keep = now == -INFINITY ? 1.f : exp2_fast(st.m - now);
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {
@@ -547,7 +548,7 @@ __global__ __launch_bounds__(kWaves * kWave, LONG ? 2 : 3) void many_rows4_kerne
       if (__any(top > limit)) {
         const auto both =
             __builtin_amdgcn_permlane32_swap(f32_bits(top), f32_bits(top), false, false);
-        const float now = fmaxf(m, fmaxf(bits_f32(both[0]), bits_f32(both[1])));
+        const float now = fmaxf(m, floorf(fmaxf(bits_f32(both[0]), bits_f32(both[1]))));
         const float keep = now == -INFINITY ? 1.f : exp2_fast(m - now);
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {

@@ -93,6 +93,7 @@ struct KvAttendArgs {
   float scale_log2;  // |scale| * log2(e), not 0
   uint32_t q_sign;   // 0x80008000 if the scale is negative: two queries' signs
   bool accumulate;
+  bool whole_refs;   // references of the rows' powers are whole numbers
 };
 struct KvAttendPlan {
   uint32_t kernel = 0, row_tile = 0, parts = 1, part_tokens = 0;
