@@ -121,23 +121,25 @@ def test_the_scale_of_scores(calls, name):
 @pytest.mark.parametrize("rows", [2, 200])
 def test_scales_of_scores_at_their_ends(uh, gpu, rows):
     """Scores of 0 whatever the scale, and scores that are all alike."""
-    p = Pair(uh, gpu, [300], heads=2, bt=64, seed=22, spare=WIDE // 64)
+    p = Pair(uh, gpu, [300], heads=8, bt=64, seed=22, spare=WIDE // 64)
     size = torch.exp2(torch.randint(-6, 7, (300, 1, 1), device=gpu).float())
-    p.append([300], v=(p.random(300, 2).float() * size).bfloat16())
+    p.append([300], v=(p.random(300, 8).float() * size).bfloat16())
     for scale in (6e29, -6e29, 0.0, 1e-38):
-        q = p.random(rows, 8)
-        p.check_attend([rows], 8, q=torch.zeros_like(q) if scale else q, scale=scale)
+        q = p.random(rows, 32)
+        p.check_attend([rows], 32, q=torch.zeros_like(q) if scale else q, scale=scale,
+                       kernel=uh.KV_KERNEL_FEW_ROWS if rows == 2 else uh.KV_KERNEL_MANY_ROWS)
 
 
 @pytest.mark.parametrize("rows", [2, 200])
 @pytest.mark.parametrize("size", [2.0 ** -14, 1.0, 2.0 ** 12])
 def test_log_sums_of_small_and_large_values(uh, gpu, rows, size):
     """The values' scales are in the references of the powers, not in the log-sum."""
-    p = Pair(uh, gpu, [300, 200], heads=2, bt=64, seed=23, spare=WIDE // 64)
-    p.append([300, 200], v=p.random(500, 2, std=size))
+    p = Pair(uh, gpu, [300, 200], heads=8, bt=64, seed=23, spare=WIDE // 64)
+    p.append([300, 200], v=p.random(500, 8, std=size))
     for scale in (None, 0.0, -0.2):
-        p.check_attend([rows, 1], 8, scale=scale)
-        p.check_attend([1, 1], 4, scale=scale)
+        p.check_attend([rows, 1], 32, scale=scale, kernel=uh.KV_KERNEL_FEW_ROWS if rows == 2
+                       else uh.KV_KERNEL_MANY_ROWS)
+        p.check_attend([1, 1], 16, scale=scale)
 
 
 # --------------------------------------------------------------------- plans
@@ -146,9 +148,13 @@ def test_log_sums_of_small_and_large_values(uh, gpu, rows, size):
     ([1], 8, [333], True, 1),
     ([1], 8, [5000], True, 2),
     ([16], 8, [5000], True, 2),
-    ([17], 8, [5000], False, 2),
+    ([17], 8, [5000], True, 2),               # all small tiles run at once
     ([150, 12], 8, [400, 90], True, 1),
-    ([150], 8, [5000], False, 2),
+    ([150], 8, [5000], True, 2),
+    ([400], 8, [5000], False, 2),
+    # (51 + 3 tiles) x 2 heads x 2 parts: 216 run at once; (68 + 4) x 2 x 2 do not.
+    ([17, 17, 17], 32, [5000, 4200, 90], True, 2),
+    ([17, 17, 17, 17], 32, [5000, 4200, 90, 400], False, 2),
     ([1500, 700], 16, [1500, 700], False, 1)])
 def test_plans_and_their_results(uh, gpu, counts, heads, lengths, few, parts):
     p = Pair(uh, gpu, lengths, heads=2, seed=sum(counts))
@@ -177,9 +183,9 @@ def test_tiles_of_many_sequences(uh, gpu):
 @pytest.mark.parametrize("counts", [[1, 300, 0, 129, 40], [300, 1], [0, 0, 500], [128, 128]])
 def test_tiles_of_ragged_prompts(uh, gpu, counts):
     lengths = [n + 7 * i for i, n in enumerate(counts)]
-    p = Pair(uh, gpu, lengths, heads=2, seed=5, spare=WIDE // 64)
+    p = Pair(uh, gpu, lengths, heads=8, seed=5, spare=WIDE // 64)
     p.fill()
-    p.check_attend(counts, 4, kernel=uh.KV_KERNEL_MANY_ROWS, accumulate=True)
+    p.check_attend(counts, 16, kernel=uh.KV_KERNEL_MANY_ROWS, accumulate=True)
 
 
 @pytest.mark.parametrize("case", [
@@ -199,7 +205,8 @@ def test_with_wide_tables(uh, gpu, monkeypatch, case):
     init, attend, kernels = Pair.__init__, uh.KvCache.attend, set()
 
     def wide(self, uh, gpu, lengths, bt=64, spare=0, **kw):
-        init(self, uh, gpu, lengths, bt=bt, spare=spare + WIDE // bt, **kw)
+        # 64 parts of small tiles at least: more than run at once.
+        init(self, uh, gpu, lengths, bt=bt, spare=spare + 64 * 64, **kw)
 
     def watched(self, q, lengths, tables, out=None, lse=None, workspace=None, **kw):
         kernels.add(self.attend_plan(q, lengths, tables, **kw).kernel)
@@ -222,11 +229,11 @@ def test_windows_of_large_tiles(uh, gpu, dim, group, rows, window):
 
 def test_large_scores_of_large_tiles(uh, gpu):
     """Maxima that grow all along, scores of both signs, scales of all kinds."""
-    p = Pair(uh, gpu, [900], heads=2, seed=12, spare=WIDE // 64)
+    p = Pair(uh, gpu, [900], heads=8, seed=12, spare=WIDE // 64)
     ramp = torch.arange(900, device=gpu).view(900, 1, 1) / 60
-    p.append([900], k=p.random(900, 2).float().mul(ramp).bfloat16())
+    p.append([900], k=p.random(900, 8).float().mul(ramp).bfloat16())
     for scale in (None, 1.0, -0.3, 0.0, 1e-30, 50.0):
-        p.check_attend([120], 8, scale=scale, kernel=uh.KV_KERNEL_MANY_ROWS)
+        p.check_attend([150], 32, scale=scale, kernel=uh.KV_KERNEL_MANY_ROWS)
 
 
 @pytest.mark.parametrize("nan", [False, True])

@@ -988,28 +988,33 @@ constexpr uint32_t kFewMost = 64, kFewTilesOfUnit = 4, kFewTokens = 4096;
 // 61 and 111).
 constexpr uint64_t kMostScores = uint64_t(1) << 31;
 
+static uint64_t tiles_of(const KvAttendArgs &a, uint32_t rows) {
+  return kv_slots(a.seqs, a.group, rows, 1, each_tiles(a, rows)) * a.pool.heads;
+}
+// The most tokens that a tile's rows see, from the start of a 32-token group.
+static uint64_t span_of(const KvAttendArgs &a, uint32_t rows) {
+  const uint64_t all = uint64_t(a.seqs.max_blocks) << a.pool.shift;
+  return a.window == 0 ? all : std::min<uint64_t>(all, uint64_t(a.window) + rows / a.group + 32);
+}
+
 KvAttendPlan plan_kv_attend(const KvAttendArgs &a, uint32_t dim) {
+  const bool many =
+      uint64_t(a.seqs.rows) * a.group > uint64_t(kFewMost) * a.seqs.batch &&
+      (tiles_of(a, kRows) > uint64_t(kFewTilesOfUnit) * uint64_t(device_cu_count()) ||
+       span_of(a, kRows) > kFewTokens);
+  return plan_kv_tiles(a, dim, many);
+}
+
+KvAttendPlan plan_kv_tiles(const KvAttendArgs &a, uint32_t dim, bool many) {
   KvAttendPlan p;
   if (a.seqs.rows == 0 || a.seqs.batch == 0) {
     return p;
   }
   const uint32_t cus = device_cu_count();
   const uint64_t rows_of_head = uint64_t(a.seqs.rows) * a.group;
-  const auto tiles_of = [&](uint32_t rows) {
-    return kv_slots(a.seqs, a.group, rows, 1, each_tiles(a, rows)) * a.pool.heads;
-  };
-  // The most tokens that a tile's rows see, from the start of a 32-token group.
-  const auto span_of = [&](uint32_t rows) {
-    const uint64_t all = uint64_t(a.seqs.max_blocks) << a.pool.shift;
-    return a.window == 0 ? all
-                         : std::min<uint64_t>(all, uint64_t(a.window) + rows / a.group + 32);
-  };
-  const bool many = rows_of_head > uint64_t(kFewMost) * a.seqs.batch &&
-                    (tiles_of(kRows) > uint64_t(kFewTilesOfUnit) * cus ||
-                     span_of(kRows) > kFewTokens);
   p.kernel = many ? ULLM_KV_KERNEL_MANY_ROWS : ULLM_KV_KERNEL_FEW_ROWS;
   p.row_tile = many ? kManyRows : kRows;
-  const uint64_t tiles = tiles_of(p.row_tile), span = span_of(p.row_tile);
+  const uint64_t tiles = tiles_of(a, p.row_tile), span = span_of(a, p.row_tile);
   const uint64_t split = tiles < cus ? (!many ? 1 : dim == 64 ? 3 : 2) * cus / tiles
                          : many && span > kPartLong && tiles < 2 * cus ? 2
                                                                        : 1;

@@ -640,6 +640,17 @@ struct WeightKeys4 {
 
 KvAttendPlan plan_kv4_attend(const KvAttendArgs &a, uint32_t dim) {
   KvAttendPlan p = plan_kv_attend(a, dim);
+  // Small tiles also for more rows than with 8 bits, where all their workgroups run
+  // at once (us with the join, small tiles against large ones: 32 heads over 8, 17
+  // queries at 16000 tokens 20 / 26, 32 26 / 29; 14 over 2 of 64 dims, 10 queries 10 /
+  // 19, 64 20 / 24; 2 over 2, 400 queries 22 / 30), and not past that (17 queries at
+  // 30000 38 / 34, 8 times 32 at 8000 70 / 59).
+  if (p.kernel == ULLM_KV_KERNEL_MANY_ROWS) {
+    const KvAttendPlan few = plan_kv_tiles(a, dim, false);
+    if (few.grid <= uint64_t(device_cu_count())) {
+      p = few;
+    }
+  }
   // A wave has half the bytes on their way that it has with 8 bits: eight waves
   // where a workgroup has a compute unit to itself, for 128 dims too (131072
   // tokens of 8 heads: 25.5 us, four waves 31.9; 16 sequences of up to 8192

@@ -110,6 +110,8 @@ hipError_t launch_kv_evict(const KvEvictArgs &a, uint32_t dim, hipStream_t s);
 void launch_kv_evict_select(const KvEvictArgs &a, hipStream_t s);
 void launch_kv_gather_weights(const KvGatherArgs &a, hipStream_t s);
 KvAttendPlan plan_kv_attend(const KvAttendArgs &a, uint32_t dim);
+// With large tiles (many rows) or small ones.
+KvAttendPlan plan_kv_tiles(const KvAttendArgs &a, uint32_t dim, bool many);
 hipError_t launch_kv_attend(const KvAttendArgs &a, uint32_t dim, const KvAttendPlan &p,
                             void *workspace, hipStream_t s);
 
