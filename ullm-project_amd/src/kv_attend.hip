@@ -1051,7 +1051,14 @@ void launch_join_parts(const KvAttendArgs &a, uint32_t dim, const KvAttendPlan &
   const auto launch = [&](auto kernel, uint32_t waves) {
     kernel<<<grid, waves * kWave, 0, s>>>(a, x, p.row_tile, rows, each);
   };
-  if (p.parts > 2 * kJoinAhead) {
+  // Eight waves to a row take many parts sooner, until the rows fill the units by
+  // themselves (us, eight against one: 544 rows of 32 parts 5.6 / 10.5, 448 of 32 at
+  // 64 dims 6.0 / 16; 1056 rows 7.7 / 7.2, 7126 of 13 parts at 64 dims 24 / 8).  The
+  // 8-bit cache keeps eight, and with them the order of its sums.
+  const bool wide = p.parts > 2 * kJoinAhead &&
+                    (!a.whole_refs ||
+                     uint64_t(a.seqs.rows) * a.heads <= 4 * uint64_t(device_cu_count()));
+  if (wide) {
     launch(dim == 64 ? join_parts_kernel<64, 8> : join_parts_kernel<128, 8>, 8);
   } else {
     launch(dim == 64 ? join_parts_kernel<64, 1> : join_parts_kernel<128, 1>, 1);
