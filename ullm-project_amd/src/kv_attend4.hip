@@ -206,10 +206,9 @@ __device__ __forceinline__ void attend_group4(RowState4<D> &st, Group4<D> &x, co
 // key/value head, as few_rows_kernel does: its waves take the 32-token chunks
 // in turn, each with a softmax of its own, and join them at the end.
 //
-// What bounds it: the read.  131072 tokens of 8 heads of 128 (140 MB) 24 to 25 us;
-// the loads alone, nothing computed, 24.8, 5.7 TB/s with the start and the end of a
-// launch that is short for it; 16 sequences of up to 8192 22.5, 128 of 4000 88 (6.2
-// TB/s).  Two chunks on their way to a wave 31, two workgroups to a compute unit
+// What bounds it: the read, and some 5.7 us of start and end.  131072 tokens of 8
+// heads of 128 (140 MB) 24 to 25 us, the loads alone, nothing computed, 24.8; 16
+// sequences of 4000 14.4, of 8000 23; 128 of 4000 88 (6.2 TB/s).  Two chunks on their way to a wave 31, two workgroups to a compute unit
 // 27, loads through the caches 27.  333 tokens, 5.7: launch, three loads that
 // wait for each other, the join of the waves.
 template <int D, int W, bool NT, bool SCORES>
