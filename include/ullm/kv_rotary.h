@@ -17,10 +17,10 @@
  * each pair's axis.
  *
  * Angles are reduced to a turn, and their cosines and sines taken, in 64 bits:
- * position 2^31 - 1 is as exact as position 1 (for frequencies up to 2^16).  Queries are then rotated in f32
- * and rounded to bf16.  Keys are rotated in 64 bits and rounded once, to their
- * codes (in caches of 8 and of 4 bits), so that a key between two codes does not
- * depend on the last bits of an f32.
+ * position 2^31 - 1 is as exact as position 1 (for frequencies up to 2^16).
+ * Queries are then rotated in f32 and rounded to bf16.  Keys are rotated in 64
+ * bits and rounded once, to their codes (in caches of 8 and of 4 bits), so that a
+ * key between two codes does not depend on the last bits of an f32.
  *
  * Every row that a sequence owns has its queries rotated, rows that name no
  * token among them (their place is negative); rows that no sequence owns are

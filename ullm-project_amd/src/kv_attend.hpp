@@ -309,7 +309,8 @@ struct JoinLds {
   float m[W][kRows], l[W][kRows];
 };
 template <int D, int W>
-__device__ __forceinline__ void join_waves(JoinLds<D, W> &lds, const KvAttendArgs &a, const Scratch &x, const Tile &t,
+__device__ __forceinline__ void join_waves(JoinLds<D, W> &lds, const KvAttendArgs &a,
+                                           const Scratch &x, const Tile &t,
                                            uint32_t kvh, uint32_t part, uint32_t parts, float m,
                                            float lane_sum, const f32x4 (&o)[D / 16],
                                            float power) {

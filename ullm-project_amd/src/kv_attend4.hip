@@ -15,8 +15,9 @@
 // left alone while the largest sum (few rows: (largest score) + log2(largest s) of a
 // lane's tokens, which no sum passes) stays within kSlack of it; else it moves to the
 // largest, rounded down to a whole number: what is added to a score before its power
-// is then exact, and so is what earlier sums are multiplied by.  With scales from 2^-19 to 2^16 the p of a row's sum stay within 2^-28 and
-// 2^34 of what they would be over the largest score, far inside f32.
+// is then exact, and so is what earlier sums are multiplied by.  With scales from
+// 2^-19 to 2^16 the p of a row's sum stay within 2^-28 and 2^34 of what they would be
+// over the largest score, far inside f32.
 //
 // NaN.  Codes are finite, NaN is in a key's exponent or a value's scale, so that
 // it can reach a row only through its score or its weight: tokens that a row
@@ -208,9 +209,10 @@ __device__ __forceinline__ void attend_group4(RowState4<D> &st, Group4<D> &x, co
 //
 // What bounds it: the read, and some 5.7 us of start and end.  131072 tokens of 8
 // heads of 128 (140 MB) 24 to 25 us, the loads alone, nothing computed, 24.8; 16
-// sequences of 4000 14.4, of 8000 23; 128 of 4000 88 (6.2 TB/s).  Two chunks on their way to a wave 31, two workgroups to a compute unit
-// 27, loads through the caches 27.  333 tokens, 5.7: launch, three loads that
-// wait for each other, the join of the waves.
+// sequences of 4000 14.4, of 8000 23; 128 of 4000 88 (6.2 TB/s).  Two chunks on their
+// way to a wave 31 (of 131072 tokens), two workgroups to a compute unit 27, loads
+// through the caches 27.  333 tokens, 5.7: launch, three loads that wait for each
+// other, the join of the waves.
 template <int D, int W, bool NT, bool SCORES>
 __global__ __launch_bounds__(W * kWave, 3) void few_rows4_kernel(KvAttendArgs a, Scratch x,
                                                               uint32_t each_slots) {

@@ -261,7 +261,8 @@ __device__ __forceinline__ void rotate_query(uint16_t *row, const RawPairs &p, c
       b[i] = side ? f32x2_to_bf16x2(x[4 + i], y[4 + i]) : f32x2_to_bf16x2(y[2 * i], y[2 * i + 1]);
     }
     __builtin_nontemporal_store(a, reinterpret_cast<u32x4 *>(row + d.first));
-    __builtin_nontemporal_store(b, reinterpret_cast<u32x4 *>(row + (side ? d.first + 8 : d.second)));
+    __builtin_nontemporal_store(
+        b, reinterpret_cast<u32x4 *>(row + (side ? d.first + 8 : d.second)));
   } else {
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
