@@ -895,9 +895,11 @@ static hipError_t launch_append8(const KvRotateArgs &a, hipStream_t s) {
   using Form = Append8<D, bt, FEW>;
   const uint32_t each = each_slots(a.append.seqs, bt), grid = uint32_t(append_grid(a.append, bt));
   const auto kernel = append8_rotary_kernel<D, bt, FEW>;
-  const hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kernel), Form::kLds);
-  if (e != hipSuccess) {
-    return e;
+  if constexpr (Form::kLds > 32768) {
+    const hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kernel), Form::kLds);
+    if (e != hipSuccess) {
+      return e;
+    }
   }
   kernel<<<grid, Form::kAll, Form::kLds, s>>>(a, each);
   return hipGetLastError();
