@@ -980,6 +980,7 @@ constexpr uint32_t kPartLeast = 512, kPartLong = 8192;
 // 28; past that 8 times 128 at 1000 39 / 30, 32 at 30000 42 / 37.  64 times 16
 // at 4000 tokens: 157 / 164, 64 times 24 206 / 167.
 constexpr uint32_t kFewMost = 64, kFewTilesOfUnit = 4, kFewTokens = 4096;
+constexpr uint32_t kWholeTokens = 2048;  // many rows in 4 bits (plan_kv_tiles)
 // Stored scores cost 8 bytes for each row and token, a second pass over the keys
 // `dim` bytes for each token.  Scores have a place for each token of the tables,
 // in use or not: past kMostScores bytes, under a hundredth of the memory, the
@@ -1015,7 +1016,14 @@ KvAttendPlan plan_kv_tiles(const KvAttendArgs &a, uint32_t dim, bool many) {
   p.kernel = many ? ULLM_KV_KERNEL_MANY_ROWS : ULLM_KV_KERNEL_FEW_ROWS;
   p.row_tile = many ? kManyRows : kRows;
   const uint64_t tiles = tiles_of(a, p.row_tile), span = span_of(a, p.row_tile);
-  const uint64_t split = tiles < cus ? (!many ? 1 : dim == 64 ? 3 : 2) * cus / tiles
+  // In 4 bits many rows that fill half the units stay whole where tokens are few: the
+  // join costs them more (28 heads over 4 of 64 dims, whole against split: twice 500
+  // queries at 1000 tokens 26 / 37 us, three times 300 at 2000 46 / 49, twice 500 at
+  // 4000 87 / 73; 32 over 8 of 128, three times 300 at 1000 32 / 48, 600 at 2000 52 /
+  // 49).  In 8 bits they are split, and their sums keep that order.
+  const bool whole = many && a.whole_refs && span <= kWholeTokens && 2 * tiles >= cus;
+  const uint64_t split = whole        ? 1
+                         : tiles < cus ? (!many ? 1 : dim == 64 ? 3 : 2) * cus / tiles
                          : many && span > kPartLong && tiles < 2 * cus ? 2
                                                                        : 1;
   const uint64_t part = std::max<uint64_t>((span + split - 1) / split, kPartLeast);
