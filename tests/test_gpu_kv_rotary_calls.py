@@ -58,6 +58,21 @@ def test_the_same_number_of_rows_each(uh, gpu, bits, dim, bt):
 
 
 @pytest.mark.parametrize("bits", [4, 8])
+def test_no_rows(uh, gpu, bits):
+    """Tensors without rows have no address."""
+    p = pair(bits, uh, gpu, [50, 60], heads=2, bt=32, seed=7)
+    p.fill()
+    q, k = p.random(0, 4), p.random(0, 2)
+    for positions in (None, np.zeros((1, 0)), np.zeros((3, 0))):
+        got = p.cache.append_rotary(
+            q, k, k, p.dev(p.lengths), p.dev(p.tables), freqs(gpu, 64), starts=p.dev([0, 0, 0]),
+            positions=None if positions is None else p.dev(positions),
+            pair_axes=p.dev(np.arange(64) % 3, torch.uint8))
+        assert got.shape == (0, 4, 128)
+    p.check_stored()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
 def test_lengths_past_the_tables(uh, gpu, bits):
     """They are taken as the tables' end, places too."""
     p = pair(bits, uh, gpu, [64, 128], heads=1, dim=64, bt=64, seed=2, spare=0)

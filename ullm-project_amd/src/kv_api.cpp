@@ -185,9 +185,6 @@ ullm_status_t validate_append_rotary(const ullm_kv_cache_append_rotary_desc_t *d
   if (d->axes == 0 || d->axes > 4) {
     return fail(sink, "axes must be 1 to 4");
   }
-  if (d->positions == nullptr && d->axes != 1) {
-    return fail(sink, "more than one axis needs positions");
-  }
   if (d->position_stride != 0 && d->position_stride < d->seqs.rows && d->axes > 1) {
     return fail(sink, "position_stride is smaller than rows");
   }
@@ -207,6 +204,9 @@ ullm_status_t validate_append_rotary(const ullm_kv_cache_append_rotary_desc_t *d
   }
   if (no_work(d->seqs)) {
     return ULLM_STATUS_OK;
+  }
+  if (d->positions == nullptr && d->axes != 1) {
+    return fail(sink, "more than one axis needs positions");
   }
   if (d->k == nullptr || d->v == nullptr || d->inv_freq == nullptr) {
     return fail(sink, "k, v or inv_freq pointer is null");
