@@ -224,6 +224,11 @@ struct Turns8 {
   Turn w[8];
   uint32_t live;
 };
+// The same in f32, for queries.
+struct QueryTurns8 {
+  float c[8], s[8];
+  uint32_t live;
+};
 template <int D, uint32_t T>
 __device__ __forceinline__ Turns8 load_turns(const SpanTurns<D, T> &turns, const KvRotary &r,
                                              const Lot &lot) {
@@ -241,13 +246,13 @@ __device__ __forceinline__ Turns8 load_turns(const SpanTurns<D, T> &turns, const
 // once, and their results next by another kernel: both pass the caches by (14006
 // tokens of 32 and 8 heads: 64 us, through them 75).
 __device__ __forceinline__ void rotate_query(uint16_t *row, const RawPairs &p, const KvRotary &r,
-                                             const Turns8 &v, uint32_t u, bool runs) {
+                                             const QueryTurns8 &v, uint32_t u, bool runs) {
   const bool side = side_by_side(r, u, runs);
   float x[8], y[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const PairXY e = raw_pair(p, side, i);
-    const float c = float(v.w[i].c), s = float(v.w[i].s);
+    const float c = v.c[i], s = v.s[i];
     const bool live = (v.live >> i & 1u) != 0;
     x[i] = live ? __builtin_fmaf(e.x, c, -(e.y * s)) : e.x;
     y[i] = live ? __builtin_fmaf(e.y, c, e.x * s) : e.y;
@@ -312,26 +317,28 @@ __device__ __forceinline__ void rotate_key(KeyImage<D, T> *to, const RawPairs &p
   }
 }
 
-// The rotation of a span: the first loads of keys and queries are on their way
-// before their turns are known.  More than two heads ahead cost the registers of
-// a fourth wave (14006 tokens of 32 and 8 heads: four ahead 82 us, two 78; with
-// queries in 64 bits 78, in 32 76; heads of a span side by side in the grid 72).
-constexpr uint32_t kAheadHeads = 2;
-template <int D, uint32_t T>
+// The rotation of a span: the first loads of keys and of AHEAD heads of queries are
+// on their way before their turns are known.  (14006 tokens of 32 and 8 heads, an
+// earlier state: queries in 64 bits 78 us, in 32 76; heads of a span side by side in
+// the grid 72.)
+template <int D, uint32_t T, uint32_t AHEAD>
 struct Rotation {
   const KvRotateArgs &a;
   const Span &s;
   uint32_t head;  // key/value head
   Lot lot;
   bool k_runs, q_runs;
-  RawPairs key, query[kAheadHeads];
+  RawPairs key, query[AHEAD];
 
   __device__ __forceinline__ Rotation(const KvRotateArgs &args, const Span &span, uint32_t kvh,
-                                      bool keys)
+                                      bool keys, bool any)
       : a(args), s(span), head(kvh), lot(lot_of<D, T>(span)) {
     const bool runs = a.rotary.interleaved || a.rotary.dims % 16 == 0;
     k_runs = runs && a.append.vec;
     q_runs = runs && a.q_vec;
+    if (!any) {
+      return;
+    }
     if (keys && lot.head == 0) {
       key = load_pairs(a.append.k + row() * a.append.k_row + head * a.append.k_head, a.rotary,
                        lot.u, k_runs);
@@ -342,7 +349,7 @@ struct Rotation {
   __device__ __forceinline__ uint64_t query_head(uint32_t h) const { return head * a.group + h; }
   __device__ __forceinline__ void load_queries(uint32_t h) {
 #pragma unroll
-    for (uint32_t i = 0; i < kAheadHeads; ++i, h += lot.step) {
+    for (uint32_t i = 0; i < AHEAD; ++i, h += lot.step) {
       if (lot.head != kNoHead && h < a.group) {
         query[i] = load_pairs(a.q + row() * a.q_row + query_head(h) * a.q_head, a.rotary, lot.u,
                               q_runs);
@@ -350,8 +357,8 @@ struct Rotation {
     }
   }
   // Turns by way of `turns` in LDS; keys (if the span has any) to `keys`, which may
-  // lie in the same place, queries to memory.
-  __device__ __forceinline__ void run(SpanTurns<D, T> *turns, KeyImage<D, T> *keys) {
+  // lie in the same place.
+  __device__ __forceinline__ QueryTurns8 turn_keys(SpanTurns<D, T> *turns, KeyImage<D, T> *keys) {
     span_turns<D, T>(a.rotary, s, turns);
     __syncthreads();
     const Turns8 v = load_turns<D, T>(*turns, a.rotary, lot);
@@ -359,9 +366,20 @@ struct Rotation {
     if (keys != nullptr && lot.head == 0) {
       rotate_key<D, T>(keys, key, a.rotary, v, lot, k_runs);
     }
+    __syncthreads();
+    QueryTurns8 q;
+    q.live = v.live;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      q.c[i] = float(v.w[i].c);
+      q.s[i] = float(v.w[i].s);
+    }
+    return q;
+  }
+  __device__ __forceinline__ void turn_queries(const QueryTurns8 &v) {
     for (uint32_t h = lot.head; lot.head != kNoHead && h < a.group;) {
 #pragma unroll
-      for (uint32_t i = 0; i < kAheadHeads; ++i, h += lot.step) {
+      for (uint32_t i = 0; i < AHEAD; ++i, h += lot.step) {
         if (h < a.group) {
           rotate_query(a.q_out + row() * a.out_row + query_head(h) * a.out_head, query[i],
                        a.rotary, v, lot.u, q_runs);
@@ -369,7 +387,6 @@ struct Rotation {
       }
       load_queries(h);
     }
-    __syncthreads();
   }
 };
 // The same of a span so short that each pair of a row has a thread: a thread makes
@@ -423,15 +440,32 @@ __device__ __forceinline__ void rotate_pairs(const KvRotateArgs &a, const Span &
   }
   __syncthreads();
 }
-// A span's queries to memory, and its keys (if it has any) to an image in `lds`.
-template <int D, uint32_t T>
+// A span's keys (if it has any) to an image in `lds` that `store` takes them from,
+// and its queries to memory: before that or after it, as the caller's workgroups are
+// served best.  In 4 bits two heads ahead and before (14006 tokens of 32 and 8 heads
+// with the gather 76 us, 7300 of 28 and 4 of 64 dims with positions of three axes 24;
+// after it 77 and 26, four heads ahead and after it 79 and 24); in 8, whose exponents
+// cost more barriers, four and after (82 us; two and before 86, two and after 84).
+template <int D, uint32_t T, uint32_t AHEAD, bool AFTER, typename F>
 __device__ __forceinline__ void rotate_span(const KvRotateArgs &a, const Span &s, uint32_t head,
-                                            uint8_t *lds, bool has_keys) {
+                                            uint8_t *lds, bool has_keys, F store) {
   KeyImage<D, T> *const keys = has_keys ? reinterpret_cast<KeyImage<D, T> *>(lds) : nullptr;
-  if (s.hi - s.lo <= kFewTokens<D, kSpanThreads<D, T>>) {
+  const bool few = s.hi - s.lo <= kFewTokens<D, kSpanThreads<D, T>>;
+  Rotation<D, T, AHEAD> r(a, s, head, has_keys, !few);
+  QueryTurns8 v{};
+  if (few) {
     rotate_pairs<D, kSpanThreads<D, T>>(a, s, head, keys);
   } else {
-    Rotation<D, T>(a, s, head, has_keys).run(reinterpret_cast<SpanTurns<D, T> *>(lds), keys);
+    v = r.turn_keys(reinterpret_cast<SpanTurns<D, T> *>(lds), keys);
+  }
+  if (!AFTER && !few) {
+    r.turn_queries(v);
+  }
+  if (has_keys) {
+    store();
+  }
+  if (AFTER && !few) {
+    r.turn_queries(v);
   }
 }
 // Sixteen elements of a rotated row.
@@ -511,65 +545,63 @@ __global__ __launch_bounds__(kThreads) void append4_kernel(KvRotateArgs ra, uint
   if (fresh != 0 && fresh != ~0u) {
     held = *value_at;
   }
-  float k[16], v[16];
-  if constexpr (MODE != kTurnNone) {
-    Image *const rotated = reinterpret_cast<Image *>(lds);
-    if constexpr (MODE == kTurnFew) {
-      rotate_pairs<D, kThreads>(ra, s, head, id >= 0 ? rotated : nullptr);
-    } else {
-      rotate_span<D, 32>(ra, s, head, lds, id >= 0);
-    }
-    if (id < 0) {
-      return;
+  const auto store = [&] {
+    float k[16], v[16];
+    if constexpr (MODE == kTurnNone) {
+      unpack16(load16(a.k + head * a.k_head + row * a.k_row + c * 16, a.vec), k);
+    } else if (live) {
+      read_row(*reinterpret_cast<const Image *>(lds), t - s.lo, c, k);
     }
     if (live) {
-      read_row(*rotated, t - s.lo, c, k);
+      unpack16(raw_value, v);
+      const uint32_t e = key_exp4(largest16<2>(k));
+      *reinterpret_cast<u32x2 *>(chunk + kv4_key_byte<D>(t, c * 16)) = encode4(k, exp4_power(e));
+      if (c % 2 == 0) {
+        chunk[Chunk::kExps + kv4_exp_byte(t, c * 16)] = uint8_t(e);
+      }
+      const uint32_t top = largest16<kUnits>(v);
+      const float scale = value_scale4(bits_f32(top));
+      const u32x2 w = encode4_scaled(v, scale);
+      u32x4 bytes;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {  // four codes of w to four bytes
+        const uint32_t h = w[j / 2] >> (16 * (j % 2)) & 0xffffu;
+        const uint32_t b = (h | h << 8) & 0x00ff00ffu;
+        bytes[j] = (b | b << 4) & 0x0f0f0f0fu;
+      }
+      *reinterpret_cast<u32x4 *>(values + t * kPitch + c * 16) = bytes;
+      if (c == 0) {
+        *reinterpret_cast<uint16_t *>(chunk + Chunk::kScales + kv4_scale_byte(t)) =
+            top >= 0x7f800000u ? uint16_t(0x7e00) : f32_to_f16(scale);
+      }
     }
+    __syncthreads();
+    if (fresh != 0) {
+      u32x2 w = {held.x & ~fresh, held.y & ~fresh};
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) {
+        const uint8_t *from = values + (4 * g + j % 4 + 16 * (j / 4)) * kPitch + d;
+        const bool is_new = (fresh >> (4 * j) & 1u) != 0;
+        w.x |= (is_new ? from[0] : 0u) << (4 * j);
+        w.y |= (is_new ? from[16] : 0u) << (4 * j);
+      }
+      *value_at = w;
+    }
+    if (a.pool.weights != nullptr) {
+      for (uint32_t i = s.lo + tid; i < s.hi; i += kThreads) {
+        a.pool.weights[(unit << a.pool.shift) + in_block + i] =
+            a.weights != nullptr ? a.weights[uint64_t(s.row0 + i) * a.pool.heads + head] : 0.f;
+      }
+    }
+  };
+  if constexpr (MODE == kTurnAny) {
+    rotate_span<D, 32, 2, false>(ra, s, head, lds, id >= 0, store);
   } else {
-    if (id < 0) {
-      return;
+    if constexpr (MODE == kTurnFew) {
+      rotate_pairs<D, kThreads>(ra, s, head, id >= 0 ? reinterpret_cast<Image *>(lds) : nullptr);
     }
-    unpack16(load16(a.k + head * a.k_head + row * a.k_row + c * 16, a.vec), k);
-  }
-  if (live) {
-    unpack16(raw_value, v);
-    const uint32_t e = key_exp4(largest16<2>(k));
-    *reinterpret_cast<u32x2 *>(chunk + kv4_key_byte<D>(t, c * 16)) = encode4(k, exp4_power(e));
-    if (c % 2 == 0) {
-      chunk[Chunk::kExps + kv4_exp_byte(t, c * 16)] = uint8_t(e);
-    }
-    const uint32_t top = largest16<kUnits>(v);
-    const float scale = value_scale4(bits_f32(top));
-    const u32x2 w = encode4_scaled(v, scale);
-    u32x4 bytes;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {  // four codes of w to four bytes
-      const uint32_t h = w[j / 2] >> (16 * (j % 2)) & 0xffffu;
-      const uint32_t b = (h | h << 8) & 0x00ff00ffu;
-      bytes[j] = (b | b << 4) & 0x0f0f0f0fu;
-    }
-    *reinterpret_cast<u32x4 *>(values + t * kPitch + c * 16) = bytes;
-    if (c == 0) {
-      *reinterpret_cast<uint16_t *>(chunk + Chunk::kScales + kv4_scale_byte(t)) =
-          top >= 0x7f800000u ? uint16_t(0x7e00) : f32_to_f16(scale);
-    }
-  }
-  __syncthreads();
-  if (fresh != 0) {
-    u32x2 w = {held.x & ~fresh, held.y & ~fresh};
-#pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) {
-      const uint8_t *from = values + (4 * g + j % 4 + 16 * (j / 4)) * kPitch + d;
-      const bool is_new = (fresh >> (4 * j) & 1u) != 0;
-      w.x |= (is_new ? from[0] : 0u) << (4 * j);
-      w.y |= (is_new ? from[16] : 0u) << (4 * j);
-    }
-    *value_at = w;
-  }
-  if (a.pool.weights != nullptr) {
-    for (uint32_t i = s.lo + tid; i < s.hi; i += kThreads) {
-      a.pool.weights[(unit << a.pool.shift) + in_block + i] =
-          a.weights != nullptr ? a.weights[uint64_t(s.row0 + i) * a.pool.heads + head] : 0.f;
+    if (id >= 0) {
+      store();
     }
   }
 }
@@ -580,7 +612,7 @@ __global__ __launch_bounds__(kThreads) void append4_kernel(KvRotateArgs ra, uint
 // does, with keys that come rotated from LDS, and rotates the queries of its
 // group: a thread has one unit of 16 dims of the block.  Bound as append4_kernel is,
 // with fewer workgroups at once (turns of a whole block in LDS): 14006 tokens of 32
-// and 8 heads 74 us, 4.3 TB/s; one token 5.4.
+// and 8 heads 70 us, 4.5 TB/s; one token 5.4.
 template <int D, uint32_t bt, bool FEW>
 struct Append8 {
   static constexpr uint32_t kAll = FEW ? kThreads : kSpanThreads<D, bt>;
@@ -616,51 +648,53 @@ __global__ __launch_bounds__((Append8<D, bt, FEW>::kAll)) void append8_rotary_ke
   if (live) {
     y[0] = load16(a.v + head * a.v_head + uint64_t(s.row0 + t) * a.v_row + c * 16, a.vec);
   }
+  const auto store = [&] {
+    float x[16];
+    uint32_t ak = 0, av = largest_magnitude(y);
+    if (live) {
+      read_row(*rotated, t - s.lo, c, x);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {  // infinities and NaN do not count
+        const uint32_t m = f32_bits(x[i]) & 0x7fffffffu;
+        ak = max(ak, m < 0x7f800000u ? m : 0u);
+      }
+    }
+    block_umax2<kAll>(ak, av);
+    int ek = exponent_for_f32(ak), ev = exponent_for(av);
+    float fk = 1.f, fv = 1.f;  // factor of the codes that were there
+    if (s.lo > 0) {
+      ek = max(ek, ek0);
+      ev = max(ev, ev0);
+      fk = exp2_int(max(ek0 - ek, -126));
+      fv = exp2_int(max(ev0 - ev, -126));
+    }
+    if (tid == 0) {  // all have read the old ones
+      a.pool.exps[unit * 2] = int8_t(ek);
+      a.pool.exps[unit * 2 + 1] = int8_t(ev);
+    }
+    uint8_t *kc = a.pool.codes + unit * (uint64_t(2 * D) << a.pool.shift);
+    uint8_t *vc = kc + (uint64_t(D) << a.pool.shift);
+    rescale_keys<D, kAll>(kc, s.lo, fk);
+    if (live) {
+      *reinterpret_cast<u32x4 *>(kc + kv_key_unit<D>(t, c)) = encode16(x, ek);
+      place_value<D>(append8_lds, t, c, encode16(y[0], ev));
+    }
+    __syncthreads();
+    store_values<D, kAll>(append8_lds, vc, s.lo, s.hi, fv);
+    if (a.pool.weights != nullptr) {
+      for (uint32_t i = s.lo + tid; i < s.hi; i += kAll) {
+        a.pool.weights[(unit << a.pool.shift) + i] =
+            a.weights != nullptr ? a.weights[uint64_t(s.row0 + i) * a.pool.heads + head] : 0.f;
+      }
+    }
+  };
   if constexpr (FEW) {
     rotate_pairs<D, kThreads>(ra, s, head, id >= 0 ? rotated : nullptr);
+    if (id >= 0) {
+      store();
+    }
   } else {
-    rotate_span<D, bt>(ra, s, head, append8_lds, id >= 0);
-  }
-  if (id < 0) {
-    return;
-  }
-  float x[16];
-  uint32_t ak = 0, av = largest_magnitude(y);
-  if (live) {
-    read_row(*rotated, t - s.lo, c, x);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {  // infinities and NaN do not count
-      const uint32_t m = f32_bits(x[i]) & 0x7fffffffu;
-      ak = max(ak, m < 0x7f800000u ? m : 0u);
-    }
-  }
-  block_umax2<kAll>(ak, av);
-  int ek = exponent_for_f32(ak), ev = exponent_for(av);
-  float fk = 1.f, fv = 1.f;  // factor of the codes that were there
-  if (s.lo > 0) {
-    ek = max(ek, ek0);
-    ev = max(ev, ev0);
-    fk = exp2_int(max(ek0 - ek, -126));
-    fv = exp2_int(max(ev0 - ev, -126));
-  }
-  if (tid == 0) {  // all have read the old ones
-    a.pool.exps[unit * 2] = int8_t(ek);
-    a.pool.exps[unit * 2 + 1] = int8_t(ev);
-  }
-  uint8_t *kc = a.pool.codes + unit * (uint64_t(2 * D) << a.pool.shift);
-  uint8_t *vc = kc + (uint64_t(D) << a.pool.shift);
-  rescale_keys<D, kAll>(kc, s.lo, fk);
-  if (live) {
-    *reinterpret_cast<u32x4 *>(kc + kv_key_unit<D>(t, c)) = encode16(x, ek);
-    place_value<D>(append8_lds, t, c, encode16(y[0], ev));
-  }
-  __syncthreads();
-  store_values<D, kAll>(append8_lds, vc, s.lo, s.hi, fv);
-  if (a.pool.weights != nullptr) {
-    for (uint32_t i = s.lo + tid; i < s.hi; i += kAll) {
-      a.pool.weights[(unit << a.pool.shift) + i] =
-          a.weights != nullptr ? a.weights[uint64_t(s.row0 + i) * a.pool.heads + head] : 0.f;
-    }
+    rotate_span<D, bt, 4, true>(ra, s, head, append8_lds, id >= 0, store);
   }
 }
 
