@@ -19,9 +19,12 @@
 // 2^-19 to 2^16 the p of a row's sum stay within 2^-28 and 2^34 of what they would be
 // over the largest score, far inside f32.
 //
-// NaN.  Codes are finite, NaN is in a key's exponent or a value's scale, so that
-// it can reach a row only through its score or its weight: tokens that a row
-// does not see have score -infinity (few rows: and scale 0) put in their place.
+// NaN.  Codes are finite, NaN is in a key's exponent or a value's scale.  A key's
+// reaches a row through its score, and -infinity takes the place of the scores that
+// a row does not see.  A value's makes the row's result NaN, but neither its log-sum
+// nor the weights that its tokens receive, which are of scores alone: with few rows
+// it enters the operand p' (scale 0 takes the place of hidden ones), with many a
+// flag of the row.
 #include <algorithm>
 
 #include "kv_attend.hpp"
@@ -322,9 +325,11 @@ struct Many4 {
 // nothing: a score starts as log2(s_t) / scale, so that its power is p' = p * s_t at
 // once and the largest of what the row has is the reference; the sum takes p' / s_t.
 // A wave makes both numbers for a step, a token to a lane, and reads them back as
-// the 16 of each lane's results.  (Against the product p * s in f16, with the
-// reference checked by a bound: 14 instructions fewer of 158 for 32 x 32, prompts of
-// 4096 and 3001 tokens of 32 and 8 heads 248 us against 262.)
+// the 16 of each lane's results.  A scale of NaN counts as the least there; that
+// there was one is noted, and which rows see it found at the end.
+// (Against the product p * s in f16, with the reference checked by a bound: 14
+// instructions fewer of 158 for 32 x 32, prompts of 4096 and 3001 tokens of 32 and 8
+// heads 248 us against 262.)
 //
 // What bounds it: 16 matrix instructions of 32 cycles and 144 others of 4 and more
 // for 32 rows x 32 tokens, at the clock that they leave the card: 990 TFLOP/s in long
@@ -394,7 +399,9 @@ __global__ __launch_bounds__(kWaves * kWave, LONG ? 2 : 3) void many_rows4_kerne
   };
   hold_blocks();
   // bias: what a scaled score becomes a power of two with.
+  // dirty: not 0 if a value of NaN was met, in a token that some row sees or not.
   float m = -INFINITY, l = 0.f, limit = -INFINITY, bias = float(kOff);
+  uint64_t dirty = 0;
   f32x16 o[D / 32];
 #pragma unroll
   for (int c = 0; c < D / 32; ++c) {
@@ -479,11 +486,11 @@ __global__ __launch_bounds__(kWaves * kWave, LONG ? 2 : 3) void many_rows4_kerne
     {  // each lane's token of the step's 64
       const float scale = f16_to_f32(*reinterpret_cast<const uint16_t *>(
           stage + lane / 32 * kSlot + Chunk::kScales + 2 * (lane % 32)));
-      // Of a token that was never written, 0, as of the least; of NaN the score is
-      // NaN, and the reciprocal beside a weight of 0 still a number.
+      dirty |= __ballot(scale != scale);
+      // Of a token that was never written, 0, and of NaN as of the least.
       const float sure = fmaxf(scale, kScaleLeast);
       float *const to = &tables[wave][0][lane];
-      to[0] = __builtin_amdgcn_logf(sure) * per_score + (scale - scale);
+      to[0] = __builtin_amdgcn_logf(sure) * per_score;
       to[64] = __builtin_amdgcn_rcpf(sure);
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
@@ -587,7 +594,34 @@ __global__ __launch_bounds__(kWaves * kWave, LONG ? 2 : 3) void many_rows4_kerne
   }
   wait_copies<0>();  // none may land after the workgroup has gone
 
-  const uint32_t mine = 32 * wave + i, rr = t.r0 + min(mine, last);
+  // Whether the lane's row sees a value of NaN: the scales once more, a chunk to a
+  // lane (rare; in the loop the question alone cost 2 %).
+  bool spoilt = false;
+  for (uint32_t grp0 = from; dirty != 0 && grp0 < to; grp0 += kWave) {
+    const uint32_t grp = grp0 + lane;
+    const int32_t id =
+        grp < to ? kv_block(table, a.seqs, a.pool.blocks, grp * 32 >> a.pool.shift) : -1;
+    uint32_t bad = 0;  // bit n: scale n is NaN
+    if (id >= 0) {
+      const uint8_t *chunk =
+          kv4_chunk<D>(a.pool, uint64_t(id) * a.pool.heads + kvh, grp * 32 & in_mask);
+      const uint16_t *scales = reinterpret_cast<const uint16_t *>(chunk + Chunk::kScales);
+      for (uint32_t n = 0; n < 32; ++n) {
+        bad |= (scales[n] & 0x7fffu) > 0x7c00u ? 1u << n : 0u;
+      }
+    }
+    for (uint64_t with = __ballot(bad != 0); with != 0; with &= with - 1) {
+      const uint32_t of = uint32_t(__builtin_ctzll(with));
+      uint32_t rest = uint32_t(__builtin_amdgcn_readlane(int(bad), int(of)));
+      for (; rest != 0; rest &= rest - 1) {
+        const uint32_t n = uint32_t(__builtin_ctz(rest));
+        const int32_t at = int32_t((grp0 + of) * 32 + n / 8 * 4 + n % 4 + n % 8 / 4 * 16);
+        spoilt = spoilt || (at <= pos && at > oldest);
+      }
+    }
+  }
+  // (The row once more: kept through the loop it would cost it registers.)
+  const uint32_t mine = opaque_u32(32 * wave + i), rr = t.r0 + min(mine, last);
   RowSink out;
   out.row = t.first_row + rr / a.group;
   out.head = kvh * a.group + rr % a.group;
@@ -596,7 +630,7 @@ __global__ __launch_bounds__(kWaves * kWave, LONG ? 2 : 3) void many_rows4_kerne
   out.slot = (out.row * a.heads + out.head) * x.parts + part;
   const auto half = __builtin_amdgcn_permlane32_swap(f32_bits(l), f32_bits(l), false, false);
   const float total = bits_f32(half[0]) + bits_f32(half[1]);
-  const float join = total == 0.f ? 0.f : 1.0f / total;
+  const float join = spoilt ? __builtin_nanf("") : total == 0.f ? 0.f : 1.0f / total;
 #pragma unroll
   for (int n = 0; n < D / 32; ++n) {
 #pragma unroll
