@@ -28,6 +28,8 @@
  * Attention as in ullm/kv_cache.h.  A token's weight times its scale enters
  * the product with the values in f16: with a relative error of 2^-11, and where
  * it is below 2^-25 of the row's largest, with an absolute one of 2^-36 of that.
+ * A value of NaN makes the results of the queries that see it NaN, not their
+ * lse nor the weights that tokens receive from them.
  * The scale of the scores must not pass 2^99.
  *
  * Evict moves codes and scales as they are.

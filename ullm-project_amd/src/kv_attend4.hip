@@ -23,8 +23,8 @@
 // reaches a row through its score, and -infinity takes the place of the scores that
 // a row does not see.  A value's makes the row's result NaN, but neither its log-sum
 // nor the weights that its tokens receive, which are of scores alone: with few rows
-// it enters the operand p' (scale 0 takes the place of hidden ones), with many a
-// flag of the row.
+// it enters the operand p' (scale 0 takes the place of hidden ones), with many the
+// quotient at the end.
 #include <algorithm>
 
 #include "kv_attend.hpp"
@@ -595,7 +595,7 @@ __global__ __launch_bounds__(kWaves * kWave, LONG ? 2 : 3) void many_rows4_kerne
   wait_copies<0>();  // none may land after the workgroup has gone
 
   // Whether the lane's row sees a value of NaN: the scales once more, a chunk to a
-  // lane (rare; in the loop the question alone cost 2 %).
+  // lane (rare; the same question in the loop cost prompts 2 % without any NaN).
   bool spoilt = false;
   for (uint32_t grp0 = from; dirty != 0 && grp0 < to; grp0 += kWave) {
     const uint32_t grp = grp0 + lane;
