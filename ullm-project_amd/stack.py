@@ -156,12 +156,12 @@ class DecodeStack:
                                        bits=kv_bits)
                        for _ in range(self.layers)]
         self.attn = torch.empty((self.m, self.hidden), dtype=torch.bfloat16, device=self.dev)
-        self.inv_freq = None
+        self.inv_freq = self.given = None
         if rope_base:
             pairs = torch.arange(0, dim, 2, dtype=torch.float64, device=self.dev)
             self.inv_freq = (float(rope_base) ** (-pairs / dim)).float()
-        # Tokens that each sequence has been given, the evicted ones too.
-        self.given = torch.zeros((self.m,), dtype=torch.int32, device=self.dev)
+            # Tokens that each sequence has been given, the evicted ones too.
+            self.given = torch.zeros((self.m,), dtype=torch.int32, device=self.dev)
 
     def _grow(self, counts):
         """Count new tokens of the sequences: the kernels take a length past
@@ -198,11 +198,12 @@ class DecodeStack:
                      accumulate=self.evict_to > 0, stream=stream)
         return out
 
-    def _positions(self, ends, rows):
-        """Positions of the rows of a call: of sequence b up to ends[b], or one
-        row of each."""
-        if not self.caches or self.inv_freq is None:
+    def _positions(self, counts, ends, rows):
+        """Positions of the rows of a call, whose counts join `given`: of sequence b
+        up to ends[b], or (ends None) one row of each."""
+        if not self.caches or self.given is None:
             return None
+        self.given.add_(counts)
         if ends is None:
             return self.given - 1
         torch = self.torch
@@ -227,9 +228,8 @@ class DecodeStack:
             if not self.torch.cuda.is_current_stream_capturing():
                 self._grow([1] * self.m)
             self.lengths.add_(1)
-            self.given.add_(1)
         self._layers(self.h0, self.h, self.qkv_out, self.attn if self.caches else None,
-                     self.o_out, self.act, None, self._positions(None, self.m), stream)
+                     self.o_out, self.act, None, self._positions(1, None, self.m), stream)
         self.lm_head.forward(self.h, self.logits, alpha=self.alpha_h, stream=stream)
         return self.logits
 
@@ -245,11 +245,10 @@ class DecodeStack:
         ends = n.cumsum(0, dtype=torch.int32)
         starts = torch.cat([torch.zeros_like(ends[:1]), ends])
         self.lengths.add_(n)
-        self.given.add_(n)
         x, qkv, attn, o, act = (torch.empty((rows, c), dtype=torch.bfloat16, device=self.dev)
                                 for c in (self.hidden, self.qkv, self.hidden, self.hidden,
                                           self.act.shape[1]))
-        self._layers(h, x, qkv, attn, o, act, starts, self._positions(ends, rows), None)
+        self._layers(h, x, qkv, attn, o, act, starts, self._positions(n, ends, rows), None)
         self.h.copy_(x[(ends - 1).long()])
         self.lm_head.forward(self.h, self.logits, alpha=self.alpha_h)
         return self.logits
