@@ -30,7 +30,7 @@
  * it is below 2^-25 of the row's largest, with an absolute one of 2^-36 of that.
  * A value of NaN makes the results of the queries that see it NaN, not their
  * lse nor the weights that tokens receive from them.
- * The scale of the scores must not pass 2^99.
+ * The scale of the scores must not pass 2^100 / log2(e), 2^100 in units of log2.
  *
  * Evict moves codes and scales as they are.
  */

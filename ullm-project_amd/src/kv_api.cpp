@@ -250,7 +250,7 @@ ullm_status_t validate_attend(const ullm_kv_cache_attend_desc_t *d, ullm_error_s
   }
   // Scales of values enter the scores in units of this one.
   if (four_bits(c) && std::fabs(log2_scale(d->scale)) > 0x1p100f) {
-    return fail(sink, "scale must not pass 2^99 with a cache of 4 bits");
+    return fail(sink, "scale * log2(e) must not pass 2^100 with a cache of 4 bits");
   }
   for (const uint64_t s :
        {d->q_row_stride, d->q_head_stride, d->out_row_stride, d->out_head_stride}) {
