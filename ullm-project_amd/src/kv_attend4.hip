@@ -325,8 +325,10 @@ struct Many4 {
 // nothing: a score starts as log2(s_t) / scale, so that its power is p' = p * s_t at
 // once and the largest of what the row has is the reference; the sum takes p' / s_t.
 // A wave makes both numbers for a step, a token to a lane, and reads them back as
-// the 16 of each lane's results.  A scale of NaN counts as the least there; that
-// there was one is noted, and which rows see it found at the end.
+// the 16 of each lane's results.  A large score rounds log2(s_t) with its own last
+// bits: tokens of equal keys and different scales then get weights as far apart.  A
+// scale of NaN counts as the least; that there was one is noted, and which rows see
+// it found at the end.
 // (Against the product p * s in f16, with the reference checked by a bound: 14
 // instructions fewer of 158 for 32 x 32, prompts of 4096 and 3001 tokens of 32 and 8
 // heads 248 us against 262.)
