@@ -1020,7 +1020,8 @@ KvAttendPlan plan_kv_tiles(const KvAttendArgs &a, uint32_t dim, bool many) {
   // join costs them more (28 heads over 4 of 64 dims, whole against split: twice 500
   // queries at 1000 tokens 26 / 37 us, three times 300 at 2000 46 / 49, twice 500 at
   // 4000 87 / 73; 32 over 8 of 128, three times 300 at 1000 32 / 48, 600 at 2000 52 /
-  // 49).  In 8 bits they are split, and their sums keep that order.
+  // 49: for both head sizes the end lies near 2000, a little before it with 128).  In 8
+  // bits they are split, and their sums keep that order.
   const bool whole = many && a.whole_refs && span <= kWholeTokens && 2 * tiles >= cus;
   const uint64_t split = whole        ? 1
                          : tiles < cus ? (!many ? 1 : dim == 64 ? 3 : 2) * cus / tiles

@@ -612,7 +612,8 @@ __global__ __launch_bounds__(kThreads) void append4_kernel(KvRotateArgs ra, uint
 // does, with keys that come rotated from LDS, and rotates the queries of its
 // group: a thread has one unit of 16 dims of the block.  Bound as append4_kernel is,
 // with fewer workgroups at once (turns of a whole block in LDS): 14006 tokens of 32
-// and 8 heads 70 us, 4.5 TB/s; one token 5.4.
+// and 8 heads 70 us in blocks of 32, 69 to 75 of 64 (4.5 TB/s), 88 of 128 (one
+// workgroup to a compute unit); one token 5.4.
 template <int D, uint32_t bt, bool FEW>
 struct Append8 {
   static constexpr uint32_t kAll = FEW ? kThreads : kSpanThreads<D, bt>;
