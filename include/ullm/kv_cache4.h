@@ -29,9 +29,9 @@
  * the product with the values in f16: with a relative error of 2^-11, and where
  * it is below 2^-25 of the row's largest, with an absolute one of 2^-36 of that.
  * Calls of many rows (ULLM_KV_KERNEL_MANY_ROWS) add log2 of the value's scale to
- * the score, in f32: tokens of equal keys and values of different scales then
- * have weights that are equal within the rounding of scores (2^-20 of a sum of
- * magnitudes), else to the last bit.
+ * the score, in f32: tokens of equal keys and values of different scales have
+ * weights that are equal within the rounding of such a sum (2^-20 of its
+ * magnitudes) there.
  * A value of NaN makes the results of the queries that see it NaN, not their
  * lse nor the weights that tokens receive from them.
  * The scale of the scores must not pass 2^100 / log2(e), 2^100 in units of log2.

@@ -212,11 +212,11 @@ __device__ __forceinline__ void attend_group4(RowState4<D> &st, Group4<D> &x, co
 //
 // What bounds it: the read, and some 5.7 us of start and end.  131072 tokens of 8
 // heads of 128 (140 MB) 24 to 25 us, the loads alone, nothing computed, 24.8; 16
-// sequences of 4000 14.4, of 8000 23; 128 of 4000 88 (6.2 TB/s).  Out of memory alone
-// (caches of 1.2 GB in turn) 24.8, 15.6, 25 and 90: 7.4 TB/s beyond the 5.7.  Two chunks on their
-// way to a wave 31 (of 131072 tokens), two workgroups to a compute unit 27, loads
-// through the caches 27.  333 tokens, 5.7: launch, three loads that wait for each
-// other, the join of the waves.
+// sequences of 4000 14.4, of 8000 23; 128 of 4000 88 (6.2 TB/s).  With caches of 1.2
+// GB in turn, so that none is found in the card's last cache, 24.8, 15.6, 25 and 90:
+// 7.4 TB/s beyond the 5.7.  Two chunks on their way to a wave 31 (of 131072 tokens),
+// two workgroups to a compute unit 27, loads through the caches 27.  333 tokens, 5.7:
+// launch, three loads that wait for each other, the join of the waves.
 template <int D, int W, bool NT, bool SCORES>
 __global__ __launch_bounds__(W * kWave, 3) void few_rows4_kernel(KvAttendArgs a, Scratch x,
                                                               uint32_t each_slots) {
@@ -329,10 +329,9 @@ struct Many4 {
 // the 16 of each lane's results.  A large score rounds log2(s_t) with its own last
 // bits: tokens of equal keys and different scales then get weights as far apart.  A
 // scale of NaN counts as the least; that there was one is noted, and which rows see
-// it found at the end.
-// (Against the product p * s in f16, with the reference checked by a bound: 14
-// instructions fewer of 158 for 32 x 32, prompts of 4096 and 3001 tokens of 32 and 8
-// heads 5 % less time; 218 us now, in a row of such launches.)
+// it found at the end.  (Against the product p * s in f16, with the reference checked
+// by a bound: 14 instructions fewer of 158 for 32 x 32, prompts of 4096 and 3001
+// tokens of 32 and 8 heads 5 % less time; 218 us now, in a row of such launches.)
 //
 // What bounds it: 16 matrix instructions of 32 cycles and 144 others of 4 and more
 // for 32 rows x 32 tokens, at the clock that they leave the card: 990 TFLOP/s in long
